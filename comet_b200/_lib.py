@@ -102,6 +102,15 @@ for _w in ("i64", "i32"):
         "_mlir_ciface_comet_b200_masked_count_csr_f64_" + _w: (c_double, _CI_CSR * 3),
         "_mlir_ciface_comet_b200_sddmm_csr_f64_" + _w: (None, [c_void_p] + _CI_CSR + [c_void_p, c_void_p]),
     })
+# rows of logits beside a CSR matrix, per type of the logits
+for _t in ("bf16", "f16", "f32"):
+    SIGNATURES.update({
+        "comet_b200_dev_top_entries_%s_i64" % _t: (c_int32, [c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 6),
+        "comet_b200_dev_distill_loss_%s_i64" % _t: (c_int32, [c_int64, c_int64] + [c_void_p] * 3 + [c_int32] + [c_void_p] * 3 +
+                                                    [c_int64, c_void_p, c_int64] + [c_void_p] * 4),
+        "comet_b200_dev_balance_loss_%s_i64" % _t: (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32,
+                                                    c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 4),
+    })
 SIGNATURES["comet_b200_ciface_free"] = (None, [c_void_p])
 
 # the host entry points exist once per index width

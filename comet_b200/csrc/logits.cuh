@@ -1,0 +1,174 @@
+// Shared by the operators on rows of logits (top.cu, distill.cu, balance.cu): the three element types, 16-byte vectors of
+// them, and sums and maxima over a CTA.  Arithmetic is in f32 whatever the type; a result is rounded once, when it is stored.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cb200 {
+
+static const double LOG2E_D = 1.4426950408889634;
+
+#ifdef __CUDACC__
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float MINUS_INF = -__builtin_huge_valf();
+
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ float from_float(float v) { return v; }
+
+// a NaN among the operands is the result
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 16 bytes of elements
+template <typename T>
+struct Granule;
+template <>
+struct Granule<float> {
+    static constexpr int N = 4;
+    uint4 w;
+    __device__ __forceinline__ void unpack(float (&v)[4]) const
+    {
+        v[0] = __uint_as_float(w.x);
+        v[1] = __uint_as_float(w.y);
+        v[2] = __uint_as_float(w.z);
+        v[3] = __uint_as_float(w.w);
+    }
+    __device__ __forceinline__ void pack(const float (&v)[4])
+    {
+        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <>
+struct Granule<__nv_bfloat16> {
+    static constexpr int N = 8;
+    uint4 w;
+    __device__ __forceinline__ void unpack(float (&v)[8]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&v)[8])
+    {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *(const uint32_t *)&p;
+        }
+        w = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+};
+template <>
+struct Granule<__half> {
+    static constexpr int N = 8;
+    uint4 w;
+    __device__ __forceinline__ void unpack(float (&v)[8]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*(const __half2 *)&u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&v)[8])
+    {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *(const uint32_t *)&p;
+        }
+        w = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+};
+
+// the largest element of a granule; NaN if one is
+__device__ __forceinline__ float granule_max(const Granule<float> &g)
+{
+    float v[4];
+    g.unpack(v);
+    return max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
+}
+template <typename T, typename T2>
+__device__ __forceinline__ float granule_max16(const uint4 &w)
+{
+    const T2 a = __hmax2_nan(__hmax2_nan(*(const T2 *)&w.x, *(const T2 *)&w.y), __hmax2_nan(*(const T2 *)&w.z, *(const T2 *)&w.w));
+    return to_float(__hmax_nan(a.x, a.y));
+}
+__device__ __forceinline__ float granule_max(const Granule<__nv_bfloat16> &g) { return granule_max16<__nv_bfloat16, __nv_bfloat162>(g.w); }
+__device__ __forceinline__ float granule_max(const Granule<__half> &g) { return granule_max16<__half, __half2>(g.w); }
+
+// 2^v, correct to two units in the last place; results below 2^-126 are 0
+__device__ __forceinline__ float exp2_fast(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// N values per thread to their sums (or maxima) over the CTA, in every thread.  `room` holds N * WARPS floats and is free
+// again after the next barrier.  Every thread adds in the same order: all have the same bits.
+template <int N, int WARPS, bool MAX>
+__device__ __forceinline__ void cta_reduce(float (&v)[N], float *room)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) room[i * WARPS + (threadIdx.x >> 5)] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float s = room[i * WARPS];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) s = MAX ? max_nan(s, room[i * WARPS + w]) : s + room[i * WARPS + w];
+        v[i] = s;
+    }
+}
+
+// One of the counters by which the last CTA of a launch finds out that it is the last.  Each goes back to 0 by itself
+// (atomicInc), a call takes the next one of 1024, so calls on two streams do not meet.
+__device__ __forceinline__ bool last_of(unsigned *counter, unsigned ctas)
+{
+    __threadfence();
+    return atomicInc(counter, ctas - 1) == ctas - 1;
+}
+#endif
+
+unsigned *next_counter();      // device address (top.cu); null, with the error kept, if there is no device
+
+}  // namespace cb200

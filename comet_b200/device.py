@@ -154,3 +154,130 @@ def masked_pair_count(A, B, M, row_lo=0, row_hi=None, out=None):
           A.pos.data_ptr(), A.crd.data_ptr(), B.pos.data_ptr(), B.crd.data_ptr(), M.pos.data_ptr(), M.crd.data_ptr(),
           out.data_ptr(), _stream())
     return out
+
+
+# Rows of logits beside a CSR matrix.  The logits are CUDA matrices with unit column stride, in bf16, f16 or f32; the
+# results are new tensors, and every call is asynchronous on the current stream.
+_LOGITS = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_numbers = {}
+
+
+def _floats(*v):
+    """The address of host doubles, and what keeps them alive (the calls take integers and addresses)."""
+    got = _numbers.get(v)
+    if got is None:
+        if len(_numbers) >= 256:
+            _numbers.clear()
+        a = (ctypes.c_double * len(v))(*v)
+        got = _numbers[v] = (ctypes.addressof(a), a)
+    return got
+
+
+def _check_logits(what, X):
+    if not (isinstance(X, torch.Tensor) and X.is_cuda and X.dim() == 2 and (X.stride(1) == 1 or X.shape[1] == 1) and X.dtype in _LOGITS):
+        raise ValueError(what + ": the logits must be a CUDA matrix of bfloat16, float16 or float32 with unit column stride")
+    if X.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(what + ": the logits must be on the current device")
+    if X.shape[1] < 1:
+        raise ValueError(what + ": the logits have no columns")
+    ld = X.stride(0) if X.shape[0] > 1 else X.shape[1]
+    if ld < X.shape[1]:
+        raise ValueError(what + ": rows of the logits must not overlap")
+    return ld
+
+
+def _check_beside(what, S, X):
+    """S: a CSR matrix of X's shape with int64 indices."""
+    if S.row_ids is not None:
+        raise ValueError(what + ": the sparse operand must be CSR (a row that stores nothing is empty there)")
+    if (S.nrows, S.ncols) != tuple(X.shape) or S.pos.shape[0] != S.nrows + 1:
+        raise ValueError(what + ": the sparse operand and the logits must have the same shape")
+    _check_like(what, X, S.pos, torch.int64, S.nrows + 1)
+    _check_like(what, X, S.crd, torch.int64, S.nnz)
+
+
+def _check_like(what, X, v, dtype, n):
+    if not (v.dtype == dtype and v.dim() == 1 and v.shape[0] == n and v.device == X.device and v.is_contiguous()):
+        raise ValueError("%s: expected %d contiguous values of %s on the logits' device" % (what, n, dtype))
+
+
+def _gradient(what, X, ld, grad):
+    """(gradient, its row stride): new, none, or the caller's (the logits themselves, say)."""
+    if grad is None or grad is False:
+        return None, 0
+    if grad is True:
+        return torch.empty(X.shape, dtype=X.dtype, device=X.device), X.shape[1]
+    if grad.dtype != X.dtype or grad.shape != X.shape or grad.device != X.device:
+        raise ValueError(what + ": the gradient must have the logits' shape, type and device")
+    return grad, _check_logits(what, grad)
+
+
+def top_entries(X, k, temperature=1.0, lse=False):
+    """The k largest entries of each row of X (1 <= k <= 1024) as a DeviceCSR with float32 values, columns ascending; of equal entries the lower
+    column, NaN above all numbers.  Returns (matrix, the log of the sum of each row's exp(X / temperature), or None)."""
+    ld = _check_logits("top_entries", X)
+    n, k = X.shape[0], int(k)
+    if not 1 <= k <= min(1024, X.shape[1]):
+        raise ValueError("top_entries: k must be between 1 and 1024, and at most the number of columns")
+    new = X.new_empty
+    pos, crd, val = new(n + 1, dtype=torch.int64), new(n * k, dtype=torch.int64), new(n * k, dtype=torch.float32)
+    sums = new(n, dtype=torch.float32) if lse else None
+    options = _floats(float(temperature))
+    _call("comet_b200_dev_top_entries_%s_i64" % _LOGITS[X.dtype], n, X.shape[1], X.data_ptr(), ld, k, options[0], pos.data_ptr(), crd.data_ptr(),
+          val.data_ptr(), _p(sums), _stream())
+    return DeviceCSR(n, X.shape[1], pos, crd, val), sums
+
+
+def distill_loss(S, X, temperature=1.0, lse=None, weight=None, scale=1.0, grad=True):
+    """Distillation from a teacher's top logits: S holds them (DeviceCSR of X's shape, float32 or float64 values, columns of a row ascending), X the
+    student's.  With q = softmax(X / temperature) and p = exp(S / temperature) over the sum of the row's entries, a row's loss is
+    sum p (log p - log q) over the entries.  lse: the log of the sum of exp(teacher / temperature) over the teacher's whole rows, as top_entries gives
+    it; p is then a part of the whole row, and all that is not stored counts as one outcome.  Rows that store nothing, or whose weight is 0, are
+    left out.  One entry in each row: the cross entropy with that column.
+
+    Returns (scale * sum of weight * rows, rows, its gradient).  grad: True (a new tensor), False (none), or a tensor to write it to, such as X."""
+    ld = _check_logits("distill_loss", X)
+    _check_beside("distill_loss", S, X)
+    n = S.nrows
+    if S.val.dtype not in (torch.float32, torch.float64):
+        raise ValueError("distill_loss: the teacher's values must be float32 or float64")
+    _check_like("distill_loss", X, S.val, S.val.dtype, S.nnz)
+    if lse is not None:
+        _check_like("distill_loss", X, lse, torch.float32, n)
+    if weight is not None:
+        _check_like("distill_loss", X, weight, torch.float32, n)
+    out, ldg = _gradient("distill_loss", X, ld, grad)
+    rows, loss = X.new_empty(n, dtype=torch.float32), X.new_empty((), dtype=torch.float32)
+    options = _floats(float(temperature), float(scale))
+    _call("comet_b200_dev_distill_loss_%s_i64" % _LOGITS[X.dtype], n, S.ncols, S.pos.data_ptr(), S.crd.data_ptr(), S.val.data_ptr(),
+          S.val.element_size(), _p(lse), _p(weight), X.data_ptr(), ld, _p(out), ldg, options[0], rows.data_ptr(), loss.data_ptr(), _stream())
+    return loss, rows, out
+
+
+def balance_loss(S, R, seq=None, mask=None, scores="softmax", scale=1.0, grad=True):
+    """Balance loss of a router: S (DeviceCSR of R's shape, at most 1024 columns; its values are not looked at) says which experts take which tokens, R
+    holds the router's logits.  seq: int64 bounds of the sequences, from 0 to the number of rows (None: one); mask: bool, rows that count (rows that store
+    nothing do not).  The loss is scale * the mean over sequences with such rows of E * sum_e f_e P_e, f_e the share of the sequence's entries in column e and
+    P_e the mean over its rows of p_e, with p = softmax(R) or, for scores="sigmoid", sigmoid(R) over the row's sum.
+
+    Returns (loss, counts[sequences, E] as int64, gradient with respect to R).  grad: True (a new tensor), False (none), or a tensor to write it to."""
+    ld = _check_logits("balance_loss", R)
+    _check_beside("balance_loss", S, R)
+    if scores not in ("softmax", "sigmoid"):
+        raise ValueError("balance_loss: scores must be 'softmax' or 'sigmoid'")
+    if S.ncols > 1024:
+        raise ValueError("balance_loss: at most 1024 experts")
+    nseq = 1
+    if seq is not None:
+        if seq.dim() != 1 or seq.shape[0] < 2:
+            raise ValueError("balance_loss: seq holds the bounds of one sequence or more")
+        nseq = seq.shape[0] - 1
+        _check_like("balance_loss", R, seq, torch.int64, nseq + 1)
+    if mask is not None:
+        _check_like("balance_loss", R, mask, torch.bool, S.nrows)
+    out, ldg = _gradient("balance_loss", R, ld, grad)
+    counts, loss = R.new_empty((nseq, S.ncols), dtype=torch.int64), R.new_empty((), dtype=torch.float32)
+    options = _floats(float(scale))
+    _call("comet_b200_dev_balance_loss_%s_i64" % _LOGITS[R.dtype], S.nrows, S.ncols, S.pos.data_ptr(), S.crd.data_ptr(), nseq, _p(seq), _p(mask),
+          int(scores == "sigmoid"), R.data_ptr(), ld, _p(out), ldg, options[0], counts.data_ptr(), loss.data_ptr(), _stream())
+    return loss, counts, out

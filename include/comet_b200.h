@@ -612,6 +612,71 @@ COMET_B200_EXPORT int32_t comet_b200_dev_masked_spgemm_count_f64_i64(
     const int64_t *apos, const int64_t *acrd, const int64_t *bpos, const int64_t *bcrd,
     const int64_t *mpos, const int64_t *mcrd, int64_t *count_dev, void *stream);
 
+/* ---- rows of logits beside a CSR matrix ------------------------------------------------------------------------------- */
+/* Dense operands are row-major with unit column stride, in bf16, f16 or f32 (the suffix); arithmetic is in f32 and a result  */
+/* is rounded once.  Any row stride and any address that is a multiple of the element's size will do.  The floating options */
+/* are read from host memory during the call.  Refused (non-zero status): no columns, a leading dimension below the number   */
+/* of columns, a temperature that is not positive, and what each entry point names.                                          */
+
+/* The k largest entries (1 <= k <= 1024, k <= ncols < 2^30) of each row of x as a CSR matrix: pos[nrows+1], crd and val
+   [nrows*k], columns ascending.  Of equal entries the lower column is taken; NaN is above all numbers, -0 equals 0, and
+   -inf is an entry like any other.  lse (may be NULL): lse[nrows] = log(sum_j exp(x_j / *temperature)) of the whole row,
+   -inf for a row of -inf. */
+COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_bf16_i64(
+    int64_t nrows, int64_t ncols, const void *x, int64_t ldx, int64_t k, const double *temperature, int64_t *pos,
+    int64_t *crd, float *val, float *lse, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f16_i64(
+    int64_t nrows, int64_t ncols, const void *x, int64_t ldx, int64_t k, const double *temperature, int64_t *pos,
+    int64_t *crd, float *val, float *lse, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f32_i64(
+    int64_t nrows, int64_t ncols, const void *x, int64_t ldx, int64_t k, const double *temperature, int64_t *pos,
+    int64_t *crd, float *val, float *lse, void *stream);
+
+/* Distillation from a teacher's top logits.  pos/crd/val: the teacher's logits (val_bytes = 4: float, 8: double), a CSR
+   matrix of x's shape; x: the student's logits.  temperature_scale: {temperature, scale}.  q = softmax(x / temperature);
+   p = exp(val / temperature) over the sum of the row's entries, or, with lse (the log of the sum of the teacher's whole
+   row at this temperature, as top_entries gives it), p = exp(val / temperature - lse) and all that is not stored is one
+   outcome of probability left = max(0, 1 - sum p).
+     rows[t] = sum p (log p - log q)  [+ left (log left - log q_left)]
+     loss    = scale * sum_t weight[t] * rows[t]                            (weight may be NULL: all 1)
+     grad    = d loss / d x, in x's type; may be x itself (same ldx), or NULL: no gradient.
+   A row that stores nothing, or nothing but -inf, or whose weight is 0, has a loss and a gradient of 0, and its logits are
+   not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf.  Columns of a row ascend; repeated ones are next to each other, and their p
+   add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
+   bits). */
+COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_bf16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *val, int32_t val_bytes, const
+    float *lse, const float *weight, const void *x, int64_t ldx, void *grad, int64_t ldg, const double
+    *temperature_scale, float *rows, float *loss, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_f16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *val, int32_t val_bytes, const
+    float *lse, const float *weight, const void *x, int64_t ldx, void *grad, int64_t ldg, const double
+    *temperature_scale, float *rows, float *loss, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_f32_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *val, int32_t val_bytes, const
+    float *lse, const float *weight, const void *x, int64_t ldx, void *grad, int64_t ldg, const double
+    *temperature_scale, float *rows, float *loss, void *stream);
+
+/* Balance loss of a router.  pos/crd: which experts (columns, at most 1024) take which tokens (rows); r: the router's
+   logits.  seq[nseq+1], ascending from 0 to nrows: the rows of each sequence (NULL with nseq = 1: all rows are one).  A row
+   is active if it stores something and its mask is not 0 (mask may be NULL).  With N_s active rows and K_s entries in them,
+     counts[s][e] = entries of active rows in column e,   p = softmax(r), or sigmoid(r) / sum sigmoid(r) if sigmoid != 0
+     loss = *scale * mean over sequences with active rows of  ncols * sum_e (counts[s][e] / K_s) * (mean over active rows of p_e)
+     grad = d loss / d r (the counts have no gradient), in r's type, 0 in rows that are not active; may be r itself, or NULL.
+   A row whose logits are all -inf counts, and has p = 0.  A column outside the matrix makes the loss NaN. */
+COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_bf16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, int64_t nseq, const int64_t *seq, const
+    uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
+    int64_t *counts, float *loss, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_f16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, int64_t nseq, const int64_t *seq, const
+    uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
+    int64_t *counts, float *loss, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_f32_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, int64_t nseq, const int64_t *seq, const
+    uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
+    int64_t *counts, float *loss, void *stream);
+
 /* Measurement aid (no counterpart in the reference): the bare gather SpMM / SDDMM are built around.  For
    each of the nnz column indices the k-double row b[crd[p], :] is read and folded into a sum; out
    (device, at least 8 * ctas_per_sm * SM-count doubles) receives one partial sum per warp.  fold_rows > 0
