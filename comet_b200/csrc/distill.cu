@@ -34,33 +34,6 @@ struct DistillArgs {
     unsigned *counter;
 };
 
-__device__ __forceinline__ void copy_granule(void *to, const void *from)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ unsigned cluster_size()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ unsigned cluster_rank()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void store_peer(float *mine, unsigned rank, float v)
-{
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
-}
-
 // what a CTA tells the others of its row: the maximum of its part, sums of 2^((x - maximum) c) of elements that are not
 // stored and of those that are, of p's weights and of p's weights times (x - maximum) c
 struct Told {
@@ -103,7 +76,7 @@ distill_kernel(const DistillArgs a)
             if (i == 0 || i == n - 1)              // elements before and behind the row
                 for (int k = 0; k < N; k++)
                     if (col0 + i * N + k < 0 || col0 + i * N + k >= a.ncols) elem[i * N + k] = from_float<T>(MINUS_INF);
-            m[0] = max_nan(m[0], granule_max(*(const Granule<T> *)(part + i)));
+            m[0] = max_nan(m[0], to_float(granule_max(*(const Granule<T> *)(part + i))));
         }
     }
     cta_reduce<2, DW, true>(m, room2);
@@ -257,21 +230,7 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
     const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);
-    auto kernel = distill_kernel<T, TV, REST, GRAD>;
-    if (smem > 40 * 1024) CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ranks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.nrows * ranks));
-    cfg.blockDim = dim3(DT);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
-    return 0;
+    return launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a);
 }
 
 template <typename T, typename TV>

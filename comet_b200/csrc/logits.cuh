@@ -111,13 +111,13 @@ __device__ __forceinline__ float granule_max(const Granule<float> &g)
     return max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
 }
 template <typename T, typename T2>
-__device__ __forceinline__ float granule_max16(const uint4 &w)
+__device__ __forceinline__ T granule_max16(const uint4 &w)
 {
     const T2 a = __hmax2_nan(__hmax2_nan(*(const T2 *)&w.x, *(const T2 *)&w.y), __hmax2_nan(*(const T2 *)&w.z, *(const T2 *)&w.w));
-    return to_float(__hmax_nan(a.x, a.y));
+    return __hmax_nan(a.x, a.y);
 }
-__device__ __forceinline__ float granule_max(const Granule<__nv_bfloat16> &g) { return granule_max16<__nv_bfloat16, __nv_bfloat162>(g.w); }
-__device__ __forceinline__ float granule_max(const Granule<__half> &g) { return granule_max16<__half, __half2>(g.w); }
+__device__ __forceinline__ __nv_bfloat16 granule_max(const Granule<__nv_bfloat16> &g) { return granule_max16<__nv_bfloat16, __nv_bfloat162>(g.w); }
+__device__ __forceinline__ __half granule_max(const Granule<__half> &g) { return granule_max16<__half, __half2>(g.w); }
 
 // 2^v, correct to two units in the last place; results below 2^-126 are 0
 __device__ __forceinline__ float exp2_fast(float v)
@@ -160,12 +160,82 @@ __device__ __forceinline__ void cta_reduce(float (&v)[N], float *room)
     }
 }
 
+__device__ __forceinline__ void copy_granule(void *to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ unsigned cluster_size()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+template <typename V>
+__device__ __forceinline__ uint32_t peer_address(const V *mine, unsigned rank)
+{
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void store_peer(float *mine, unsigned rank, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_address(mine, rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ float peer_load(const float *mine, unsigned rank)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(mine, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int peer_load(const int *mine, unsigned rank)
+{
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(peer_address(mine, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long peer_load(const unsigned long long *mine, unsigned rank)
+{
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_address(mine, rank)) : "memory");
+    return v;
+}
+
 // One of the counters by which the last CTA of a launch finds out that it is the last.  Each goes back to 0 by itself
 // (atomicInc), a call takes the next one of 1024, so calls on two streams do not meet.
 __device__ __forceinline__ bool last_of(unsigned *counter, unsigned ctas)
 {
     __threadfence();
     return atomicInc(counter, ctas - 1) == ctas - 1;
+}
+
+// `ctas` CTAs in clusters of `ranks`
+template <typename... P, typename... A>
+inline int launch_cluster(void (*kernel)(P...), unsigned ctas, int ranks, int threads, size_t smem, cudaStream_t st, A... args)
+{
+    if (smem > 16 * 1024) CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+    return 0;
 }
 #endif
 
