@@ -76,7 +76,7 @@ distill_kernel(const DistillArgs a)
             if (i == 0 || i == n - 1)              // elements before and behind the row
                 for (int k = 0; k < N; k++)
                     if (col0 + i * N + k < 0 || col0 + i * N + k >= a.ncols) elem[i * N + k] = from_float<T>(MINUS_INF);
-            m[0] = max_nan(m[0], to_float(granule_max(*(const Granule<T> *)(part + i))));
+            m[0] = max_nan(m[0], to_float(largest(((const Granule<T> *)(part + i))->most())));
         }
     }
     cta_reduce<2, DW, true>(m, room2);

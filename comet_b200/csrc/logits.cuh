@@ -26,11 +26,35 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ float from_float(float v) { return v; }
 
+typedef unsigned long long u64_pair;
+
 // a NaN among the operands is the result
 __device__ __forceinline__ float max_nan(float a, float b)
 {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(u64_pair *)&r) : "l"(*(const u64_pair *)&a), "l"(*(const u64_pair *)&b));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(u64_pair *)&r) : "l"(*(const u64_pair *)&a), "l"(*(const u64_pair *)&b));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(*(u64_pair *)&r)
+        : "l"(*(const u64_pair *)&a), "l"(*(const u64_pair *)&b), "l"(*(const u64_pair *)&c));
     return r;
 }
 
@@ -41,6 +65,22 @@ template <>
 struct Granule<float> {
     static constexpr int N = 4;
     uint4 w;
+    __device__ __forceinline__ void unpack(float2 (&v)[2]) const
+    {
+        v[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+        v[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+    }
+    typedef float Most;                            // a granule's largest element, for 16-bit types of the even and of the odd ones
+    __device__ __forceinline__ Most most() const
+    {
+        return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+    // a bit per element that is not smaller than `than` (a NaN never is, nor is anything smaller than one)
+    __device__ __forceinline__ unsigned at_least(float than) const
+    {
+        return (__uint_as_float(w.x) < than ? 0u : 1u) | (__uint_as_float(w.y) < than ? 0u : 2u) | (__uint_as_float(w.z) < than ? 0u : 4u) |
+               (__uint_as_float(w.w) < than ? 0u : 8u);
+    }
     __device__ __forceinline__ void unpack(float (&v)[4]) const
     {
         v[0] = __uint_as_float(w.x);
@@ -53,10 +93,30 @@ struct Granule<float> {
         w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
 };
+// a bit per element that is not smaller than `than`
+template <typename T2>
+__device__ __forceinline__ unsigned at_least16(const uint4 &w, T2 than)
+{
+    const unsigned v = (__hgeu2_mask(*(const T2 *)&w.x, than) & 0x00020001u) | (__hgeu2_mask(*(const T2 *)&w.y, than) & 0x00080004u) |
+                       (__hgeu2_mask(*(const T2 *)&w.z, than) & 0x00200010u) | (__hgeu2_mask(*(const T2 *)&w.w, than) & 0x00800040u);
+    return (v | v >> 16) & 0xffu;
+}
 template <>
 struct Granule<__nv_bfloat16> {
     static constexpr int N = 8;
     uint4 w;
+    __device__ __forceinline__ void unpack(float2 (&v)[4]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    }
+    typedef __nv_bfloat162 Most;
+    __device__ __forceinline__ Most most() const
+    {
+        return __hmax2_nan(__hmax2_nan(*(const Most *)&w.x, *(const Most *)&w.y), __hmax2_nan(*(const Most *)&w.z, *(const Most *)&w.w));
+    }
+    __device__ __forceinline__ unsigned at_least(__nv_bfloat16 than) const { return at_least16<__nv_bfloat162>(w, {than, than}); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -81,6 +141,18 @@ template <>
 struct Granule<__half> {
     static constexpr int N = 8;
     uint4 w;
+    __device__ __forceinline__ void unpack(float2 (&v)[4]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __half22float2(*(const __half2 *)&u[i]);
+    }
+    typedef __half2 Most;
+    __device__ __forceinline__ Most most() const
+    {
+        return __hmax2_nan(__hmax2_nan(*(const Most *)&w.x, *(const Most *)&w.y), __hmax2_nan(*(const Most *)&w.z, *(const Most *)&w.w));
+    }
+    __device__ __forceinline__ unsigned at_least(__half than) const { return at_least16<__half2>(w, {than, than}); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -103,21 +175,17 @@ struct Granule<__half> {
     }
 };
 
-// the largest element of a granule; NaN if one is
-__device__ __forceinline__ float granule_max(const Granule<float> &g)
-{
-    float v[4];
-    g.unpack(v);
-    return max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
-}
-template <typename T, typename T2>
-__device__ __forceinline__ T granule_max16(const uint4 &w)
-{
-    const T2 a = __hmax2_nan(__hmax2_nan(*(const T2 *)&w.x, *(const T2 *)&w.y), __hmax2_nan(*(const T2 *)&w.z, *(const T2 *)&w.w));
-    return __hmax_nan(a.x, a.y);
-}
-__device__ __forceinline__ __nv_bfloat16 granule_max(const Granule<__nv_bfloat16> &g) { return granule_max16<__nv_bfloat16, __nv_bfloat162>(g.w); }
-__device__ __forceinline__ __half granule_max(const Granule<__half> &g) { return granule_max16<__half, __half2>(g.w); }
+// largest elements: NaN if one is
+__device__ __forceinline__ float most_of(float a, float b) { return max_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 most_of(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __half2 most_of(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ float largest(float a) { return a; }
+__device__ __forceinline__ __nv_bfloat16 largest(__nv_bfloat162 a) { return __hmax_nan(a.x, a.y); }
+__device__ __forceinline__ __half largest(__half2 a) { return __hmax_nan(a.x, a.y); }
+// one of the elements is not smaller
+__device__ __forceinline__ bool reaches(float a, float than) { return !(a < than); }
+__device__ __forceinline__ bool reaches(__nv_bfloat162 a, __nv_bfloat16 than) { return __hgeu2_mask(a, {than, than}) != 0; }
+__device__ __forceinline__ bool reaches(__half2 a, __half than) { return __hgeu2_mask(a, {than, than}) != 0; }
 
 // 2^v, correct to two units in the last place; results below 2^-126 are 0
 __device__ __forceinline__ float exp2_fast(float v)

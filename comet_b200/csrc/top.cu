@@ -3,7 +3,7 @@
 //
 // An entry is compared as 64 bits: its value in an order-preserving code, then the complement of its column, so no two are
 // equal and the k largest are always the same k.
-// A CTA streams its row, or its part of it, once.  The first 512 groups of 16 bytes have a largest entry each, and of those comes a bound
+// A CTA streams its row, or its part of it, once.  The first 1024 groups of 16 bytes have a largest entry each, and of those comes a bound
 // that k entries reach, so few entries of the rest pass it; they are candidates, in shared memory.  When they become many, the
 // k largest are kept and the k-th of them is the new bound.
 #include <atomic>
@@ -35,7 +35,7 @@ unsigned *next_counter()
     return p + turn++ % 1024;
 }
 
-static const int TT = 256, TW = TT / 32, TU = 2, STAGES = 4, MOST_K = 1024, ROOM = 2048, MOST_RANKS = 8;
+static const int TT = 256, TW = TT / 32, TU = 4, STAGES = 3, MOST_K = 1024, ROOM = 2048, MOST_RANKS = 8;
 
 typedef unsigned long long u64;
 
@@ -44,46 +44,78 @@ template <typename T>
 struct Order;
 template <>
 struct Order<float> {
-    static constexpr int BITS = 32;
+    static constexpr int BITS = 32, DIGIT = 16;    // DIGIT: 256 digits of the histogram cover a factor of four or so of the value
     static __device__ __forceinline__ uint32_t key(float v)
     {
         const uint32_t u = __float_as_uint(v + 0.0f);
         return v != v ? 0xffffffffu : u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
     }
+    static __device__ __forceinline__ float code(uint32_t k) { return value(k); }
     static __device__ __forceinline__ float value(uint32_t k)
     {
         return __uint_as_float(k == 0xffffffffu ? 0x7fffffffu : k ^ ((int32_t)k < 0 ? 0x80000000u : 0xffffffffu));
     }
 };
-template <typename T>
+template <typename T, int D>
 struct Order16 {
-    static constexpr int BITS = 16;
+    static constexpr int BITS = 16, DIGIT = D;
     static __device__ __forceinline__ uint32_t key(T v)
     {
         const uint32_t u = *(const uint16_t *)&v;
         if (__hisnan(v)) return 0xffffu;
         return u == 0x8000u ? 0x8000u : u ^ (u & 0x8000u ? 0xffffu : 0x8000u);
     }
-    static __device__ __forceinline__ float value(uint32_t k)
+    static __device__ __forceinline__ T code(uint32_t k)
     {
         const uint16_t u = (uint16_t)(k == 0xffffu ? 0x7fffu : k ^ (k & 0x8000u ? 0x8000u : 0xffffu));
-        return to_float(*(const T *)&u);
+        return *(const T *)&u;
     }
+    static __device__ __forceinline__ float value(uint32_t k) { return to_float(code(k)); }
 };
 template <>
-struct Order<__nv_bfloat16> : Order16<__nv_bfloat16> {};
+struct Order<__nv_bfloat16> : Order16<__nv_bfloat16, 0> {};
 template <>
-struct Order<__half> : Order16<__half> {};
+struct Order<__half> : Order16<__half, 3> {};
 
 struct TopShared {
     u64 cand[ROOM];
     int hist[256];
     int digit, left, exact;
     int count;
+    uint32_t base, bound;          // keys that k entries reach: the first, and the best so far
     float room[2 * TW], m, s;
     u64 ends[2 * TW];
     uint32_t least[TW];
 };
+
+// Of 256 counts: the highest digit from which on there are at least `want`, how many are above it, and its own; by one warp, in one lane.
+__device__ __forceinline__ bool highest_digit(const volatile int *hist, int want, int &digit, int &above, int &own)
+{
+    const int lane = threadIdx.x & 31;
+    int each[8], sum = 0;                          // lane l: the eight digits from 255 - 8 l down
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += each[i] = hist[255 - 8 * lane - i];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    before -= sum;
+    if (before >= want || want > before + sum) return false;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (!done && want <= before + each[i]) {
+            done = true;
+            digit = 255 - 8 * lane - i;
+            above = before;
+            own = each[i];
+        }
+        before += each[i];
+    }
+    return true;
+}
 
 // The least number that exactly k of cand[0..n) reach; 0 if n <= k.  The digits of 8 bits begin where the entries begin to differ
 // (they lie between a bound and the largest, so their first bits are alike), and end where a digit tells the k from the rest.
@@ -120,29 +152,12 @@ __device__ u64 kth_largest(TopShared &sh, int n, int k)
             if (v >> width == found) atomicAdd(&sh.hist[(int)v & ((1 << width) - 1)], 1);
         }
         __syncthreads();
-        if (tid < 32) {                            // lane l: the eight digits from 255 - 8 l down
-            int own[8], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) sum += own[i] = sh.hist[255 - 8 * tid - i];
-            int before = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, before, o);
-                if (tid >= o) before += v;
-            }
-            before -= sum;
-            if (before < left && left <= before + sum) {
-                bool done = false;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (!done && left <= before + own[i]) {
-                        done = true;
-                        sh.digit = 255 - 8 * tid - i;
-                        sh.left = left - before;
-                        sh.exact = left - before == own[i];
-                    }
-                    before += own[i];
-                }
+        if (tid < 32) {
+            int digit, above, own;
+            if (highest_digit(sh.hist, left, digit, above, own)) {
+                sh.digit = digit;
+                sh.left = left - above;
+                sh.exact = left - above == own;
             }
         }
         __syncthreads();
@@ -159,13 +174,17 @@ __device__ u64 kth_largest(TopShared &sh, int n, int k)
 // The k largest of cand[0..n) to the front, in any order, and count = min(n, k); returns the least number that only they reach.
 __device__ u64 keep_largest(TopShared &sh, int n, int k)
 {
+    const int tid = threadIdx.x;
+    if (n <= k) {
+        __syncthreads();
+        return 0;
+    }
     const u64 least = kth_largest(sh, n, k);
     u64 mine[ROOM / TT];
 #pragma unroll
-    for (int i = 0; i < ROOM / TT; i++) mine[i] = threadIdx.x + i * TT < n ? sh.cand[threadIdx.x + i * TT] : 0;
+    for (int i = 0; i < ROOM / TT; i++) mine[i] = tid + i * TT < n ? sh.cand[tid + i * TT] : 0;
     __syncthreads();
-    if (n <= k) return 0;
-    if (threadIdx.x == 0) sh.count = 0;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ROOM / TT; i++)
@@ -174,137 +193,298 @@ __device__ u64 keep_largest(TopShared &sh, int n, int k)
     return least;
 }
 
-// Long rows, or many entries of them: a cluster of CTAs per row, each streams a part of it through a ring of stages in shared memory
-// (a thread copies 16 bytes and reads the same 16, so the ring needs no barriers).
-template <typename T, bool LSE>
-__global__ void __launch_bounds__(TT)
-top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_t ldx, int k, int colbits, float c, float inv, int64_t *__restrict__ pos,
-           int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse)
-{
-    constexpr int N = Granule<T>::N;
-    extern __shared__ uint4 ring[];                // STAGES * TU * TT
-    __shared__ TopShared sh;
-    const int tid = threadIdx.x;
-    const unsigned rank = cluster_rank(), ranks = cluster_size();
-    const int64_t t = blockIdx.x / ranks;
-    const T *x = xs + t * ldx;
-    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T), all = (off + ncols + N - 1) / N;
-    const int begin = min((int)rank * slice, all), end = min(begin + slice, all);
-    const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15);
-    const int limit = min(max(4 * k, 512), ROOM);  // more candidates than this are cut to k
-    if (tid == 0) sh.count = 0;
-    auto fetch = [&](int step) {
+// A thread's way through a row, or a CTA's part of one: a ring of stages in shared memory, of which it copies and reads the same 16
+// bytes each time, so the ring needs no barriers.
+template <typename T>
+struct Way {
+    static constexpr int N = Granule<T>::N;
+    uint4 *ring;                                   // STAGES * TU * TT
+    const uint4 *from;                             // the row's granule 0
+    int begin, end, all, off, ncols;               // the part, the row's granules, elements before the row, its columns
+    const uint4 *next;
+    int left, put, at;
+
+    __device__ __forceinline__ int steps() const { return (end - begin + TU * TT - 1) / (TU * TT); }
+    __device__ __forceinline__ void fetch()
+    {
 #pragma unroll
-        for (int u = 0; u < TU; u++) {
-            const int i = begin + (step * TU + u) * TT + tid;
-            if (i < end) copy_granule(ring + ((step % STAGES) * TU + u) * TT + tid, from + i);
-        }
+        for (int u = 0; u < TU; u++)
+            if (u * TT < left) copy_granule(ring + (put * TU + u) * TT + threadIdx.x, next + u * TT);
         asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+        next += TU * TT;
+        left -= TU * TT;
+        put = put == STAGES - 1 ? 0 : put + 1;
+    }
+    __device__ __forceinline__ void start()
+    {
+        next = from + begin + threadIdx.x;
+        left = end - begin - (int)threadIdx.x;
+        put = at = 0;
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) fetch(i);
-    __syncthreads();
-    u64 bound = 0;                                 // an entry has to be larger
-    uint32_t boundkey = 0;
-    float m = MINUS_INF, s = 0.0f;
-    const int steps = (end - begin + TU * TT - 1) / (TU * TT);
-    for (int step = 0; step < steps; step++) {
-        fetch(step + STAGES - 1);
+        for (int i = 0; i < STAGES - 1; i++) fetch();
+    }
+    // the thread's granules of a step, TT apart; -inf where there is no row
+    __device__ __forceinline__ Granule<T> *stage(int step)
+    {
+        fetch();
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        Granule<T> g[TU];
-        uint32_t gk[TU];
+        Granule<T> *mine = (Granule<T> *)(ring + at * TU * TT + threadIdx.x);
+        at = at == STAGES - 1 ? 0 : at + 1;
+        const int first = begin + step * TU * TT;
+        if (first == 0 || first + TU * TT > min(end, all - 1)) {
 #pragma unroll
-        for (int u = 0; u < TU; u++) {
-            const int i = begin + (step * TU + u) * TT + tid;
-            if (i < end) g[u].w = ring[((step % STAGES) * TU + u) * TT + tid];
-            if (i == 0 || i >= all - 1 || i >= end) {          // entries before and behind the row
+            for (int u = 0; u < TU; u++) {
+                const int i = first + threadIdx.x + u * TT;
+                if (i == 0 || i >= all - 1 || i >= end) {
+                    T *v = (T *)&mine[u * TT];
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (i >= end || i * N + e < off || i * N + e >= off + ncols) v[e] = from_float<T>(MINUS_INF);
+                }
+            }
+        }
+        return mine;
+    }
+    __device__ __forceinline__ int column(int step, int u, int e) const { return (begin + (step * TU + u) * TT + (int)threadIdx.x) * N + e - off; }
+};
+
+// A thread's sum of exp(x / temperature): its maximum, that times c, and two sums of 2^(x c - mc).
+struct LogSum {
+    float m, mc;
+    float2 s;
+    template <typename T>
+    __device__ __forceinline__ void add(const Granule<T> (&g)[TU], typename Granule<T>::Most most, float c)
+    {
+        constexpr int N = Granule<T>::N;
+        const float nm = max_nan(m, to_float(largest(most)));
+        if (nm != m) {
+            const float f = exp2_fast((m - nm) * c);
+            s.x *= f;
+            s.y *= f;
+            m = nm;
+            mc = m == MINUS_INF ? 0.0f : m * c;
+        }
+        if (fabsf(mc) < 1e30f) {
+#pragma unroll
+            for (int u = 0; u < TU; u++) {
+                float2 v[N / 2];
+                g[u].unpack(v);
+#pragma unroll
+                for (int e = 0; e < N / 2; e++) {
+                    const float2 d = fma2(v[e], make_float2(c, c), make_float2(-mc, -mc));
+                    s = add2(s, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+                }
+            }
+        } else {                                   // m * c may be beyond f32 where x - m is not; and NaN, and infinity
+#pragma unroll
+            for (int u = 0; u < TU; u++) {
                 float v[N];
                 g[u].unpack(v);
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (i >= end || i * N + e < off || i * N + e >= off + ncols) v[e] = MINUS_INF;
-                g[u].pack(v);
+                for (int e = 0; e < N; e++) s.x += exp2_fast((v[e] - m) * c);
             }
-            const T gm = granule_max(g[u]);
-            gk[u] = Order<T>::key(gm);
-            if (LSE) {
-                const float nm = max_nan(m, to_float(gm));
-                if (nm != m) {
-                    s *= exp2_fast((m - nm) * c);
-                    m = nm;
-                }
-                if (m != MINUS_INF) {
-                    float v[N];
-                    g[u].unpack(v);
+        }
+    }
+};
+
+// The first step's bound, by all threads: each warp finds the ceil(k / 8)-th largest of its 128 granules' largest entries, and k entries
+// reach the least of those eight keys.
+template <typename T>
+__device__ __forceinline__ uint32_t first_bound(TopShared &sh, const typename Granule<T>::Most (&gm)[TU], int k)
+{
+    const int want = (k + TW - 1) / TW;
+    uint32_t key = 0, gk[TU];
 #pragma unroll
-                    for (int e = 0; e < N; e++) s += exp2_fast((v[e] - m) * c);
-                }
-            }
+    for (int u = 0; u < TU; u++) gk[u] = Order<T>::key(largest(gm[u]));
+    for (int bit = Order<T>::BITS - 1; bit >= 0; bit--) {
+        const uint32_t more = key | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < TU; u++) n += __popc(__ballot_sync(0xffffffffu, gk[u] >= more));
+        if (n >= want) key = more;
+        if (n == want) break;
+    }
+    if ((threadIdx.x & 31) == 0) sh.least[threadIdx.x >> 5] = key;
+    __syncthreads();
+    key = sh.least[0];
+#pragma unroll
+    for (int i = 1; i < TW; i++) key = min(key, sh.least[i]);
+    return key;
+}
+
+// Candidates without barriers.  Each one is counted in a histogram of keys above the first bound, and every 64th makes its warp
+// look for the highest digit that k entries reach: the other warps' bound from their next step on.  It only rises, and holds
+// whenever it is read.  count > ROOM afterwards: the row is one (in order, or of few values) that has to be taken step by step.
+template <typename T, bool LSE>
+__device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, int colbits, float c, LogSum &sum)
+{
+    constexpr int N = Granule<T>::N, DIGIT = Order<T>::DIGIT;
+    const u64 low = (1ull << colbits) - 1;
+    volatile uint32_t *bound = &sh.bound;
+    const int steps = way.steps();
+    uint32_t base = 0;
+    bool over = false;
+    way.start();
+    for (int step = 0; step < steps; step++) {
+        const Granule<T> *mine = way.stage(step);
+        Granule<T> g[TU];
+        typename Granule<T>::Most gm[TU];
+#pragma unroll
+        for (int u = 0; u < TU; u++) {
+            g[u] = mine[u * TT];
+            gm[u] = g[u].most();
         }
         if (step == 0) {
-            // Each warp finds the ceil(k / 8)-th largest of its 64 groups' largest entries; k entries reach the least of those eight.
-            const int want = (k + TW - 1) / TW;
-            uint32_t key = 0;
-            if (want <= 32 * TU)
-                for (int bit = Order<T>::BITS - 1; bit >= 0; bit--) {
-                    const uint32_t more = key | 1u << bit;
-                    int n = 0;
-#pragma unroll
-                    for (int u = 0; u < TU; u++) n += __popc(__ballot_sync(0xffffffffu, gk[u] >= more));
-                    if (n >= want) key = more;
-                    if (n == want) break;
-                }
-            if ((tid & 31) == 0) sh.least[tid >> 5] = key;
+            base = first_bound<T>(sh, gm, k);
+            if (threadIdx.x == 0) sh.base = *bound = base;
             __syncthreads();
-            boundkey = sh.least[0];
-#pragma unroll
-            for (int i = 1; i < TW; i++) boundkey = min(boundkey, sh.least[i]);
-            bound = (u64)boundkey << colbits;
         }
+        if (LSE) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
+        if (over) continue;
+        const T least = Order<T>::code(*bound);
         unsigned pending = 0;
-        bool full = false;
-        auto look = [&](bool put) {
 #pragma unroll
-            for (int u = 0; u < TU; u++) {
-                if (put ? !(pending >> (u * N) & ((1u << N) - 1)) : gk[u] < boundkey) continue;
-                const T *v = (const T *)&g[u].w;
+        for (int u = 0; u < TU; u++)
+            if (reaches(gm[u], least)) pending |= g[u].at_least(least) << (u * N);
+        if (!__any_sync(0xffffffffu, pending != 0)) continue;
+        bool look = false;
+        while (pending) {
+            const int b = __ffs(pending) - 1, u = b / N, e = b % N, col = way.column(step, u, e);
+            pending &= pending - 1;
+            if (col < 0 || col >= way.ncols) continue;
+            const uint32_t key = Order<T>::key(((const T *)&mine[u * TT])[e]);
+            if (key < base) continue;              // nothing is smaller than a bound that is NaN
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < ROOM) sh.cand[at] = (u64)key << colbits | (low - (unsigned)col);
+            atomicAdd(&sh.hist[min((key - base) >> DIGIT, 255u)], 1);
+            look |= at % 64 == 63;
+        }
+        if (__any_sync(0xffffffffu, look)) {
+            int digit, above, own;
+            if (highest_digit(sh.hist, k, digit, above, own)) atomicMax((unsigned *)bound, base + ((uint32_t)digit << DIGIT));
+            __syncwarp();
+            over = __any_sync(0xffffffffu, *(volatile int *)&sh.count > ROOM);         // the same in every lane
+            if (!LSE && over) break;
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+}
+
+// Candidates step by step: when they become many, the k largest are kept and the k-th of them is the new bound.  Holds for
+// every row and k.  Leaves the k largest.
+template <typename T, bool LSE>
+__device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, int colbits, float c, LogSum &sum)
+{
+    constexpr int N = Granule<T>::N;
+    const u64 low = (1ull << colbits) - 1;
+    const int steps = way.steps(), limit = min(max(2 * k, 256), ROOM);
+    u64 bound = 0;                                 // an entry has to be larger
+    T least_value = Order<T>::code(0xffffffffu);   // the bound's value; NaN: all are larger
+    if (threadIdx.x == 0) sh.count = 0;
+    way.start();
+    for (int step = 0; step < steps; step++) {
+        const Granule<T> *mine = way.stage(step);
+        Granule<T> g[TU];
+        typename Granule<T>::Most gm[TU];
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int col = (begin + (step * TU + u) * TT + tid) * N + e - off;
-                    const u64 it = (u64)Order<T>::key(v[e]) << colbits | (u64)((1u << colbits) - 1 - (unsigned)col);
-                    const unsigned bit = 1u << (u * N + e);
-                    if (!put) {
-                        if (it > bound && col >= 0 && col < ncols) pending |= bit;
-                    } else if (pending & bit) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        full |= at >= limit - 1;
-                        if (at < ROOM) {
-                            sh.cand[at] = it;
-                            pending &= ~bit;
-                        }
-                    }
+        for (int u = 0; u < TU; u++) {
+            g[u] = mine[u * TT];
+            gm[u] = g[u].most();
+        }
+        if (step == 0) {
+            const uint32_t key = first_bound<T>(sh, gm, k);
+            bound = (u64)key << colbits;
+            least_value = Order<T>::code(key);
+        }
+        if (LSE) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
+        unsigned pending = 0;
+#pragma unroll
+        for (int u = 0; u < TU; u++) pending |= g[u].at_least(least_value) << (u * N);
+        for (;;) {
+            bool full = false;
+            unsigned without = 0;                  // entries that found no room
+            while (pending) {
+                const int b = __ffs(pending) - 1, u = b / N, e = b % N, col = way.column(step, u, e);
+                pending &= pending - 1;
+                const u64 it = (u64)Order<T>::key(((const T *)&mine[u * TT])[e]) << colbits | (low - (unsigned)col);
+                if (it > bound && col >= 0 && col < way.ncols) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    full |= at >= limit - 1;
+                    if (at < ROOM) sh.cand[at] = it;
+                    else without |= 1u << b;
                 }
             }
-        };
-        look(false);
-        for (;;) {
-            if (pending) look(true);
-            if (!__syncthreads_or(full || pending != 0)) break;
+            if (!__syncthreads_or(full)) break;
             const u64 least = keep_largest(sh, min(sh.count, ROOM), k);
-            if (least > bound + 1) bound = least - 1;
-            boundkey = (uint32_t)(bound >> colbits);
-            full = false;
-            if (pending) {                         // of those that found no room, the ones that are still large enough
-                const unsigned without = pending;
-                pending = 0;
-                look(false);
-                pending &= without;
+            if (least > bound + 1) {
+                bound = least - 1;
+                least_value = Order<T>::code((uint32_t)(bound >> colbits));
             }
+            pending = without;
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     keep_largest(sh, sh.count, k);
+}
+
+// Long rows, or many entries of them: a CTA, or a cluster of them, per row.
+template <typename T, bool LSE, bool FREE>
+__global__ void __launch_bounds__(TT, 3)
+top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_t ldx, int k, int colbits, float c, float inv, int64_t *__restrict__ pos,
+           int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse)
+{
+    extern __shared__ uint4 ring[];
+    __shared__ TopShared sh;
+    const int tid = threadIdx.x;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    const int64_t t = blockIdx.x / ranks;
+    const T *x = xs + t * ldx;
+    Way<T> way;
+    way.ring = ring;
+    way.from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15);
+    way.off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+    way.ncols = ncols;
+    way.all = (way.off + ncols + Way<T>::N - 1) / Way<T>::N;
+    way.begin = min((int)rank * slice, way.all);
+    way.end = min(way.begin + slice, way.all);
+    LogSum sum = {MINUS_INF, 0.0f, make_float2(0.0f, 0.0f)};
+    const u64 low = (1ull << colbits) - 1;
+    if (FREE) {
+        sh.hist[tid] = 0;
+        if (tid == 0) {
+            sh.count = 0;
+            sh.base = sh.bound = 0;
+        }
+        __syncthreads();
+        stream_free<T, LSE>(sh, way, k, colbits, c, sum);
+        const int n = sh.count;
+        __syncthreads();                           // all have read it
+        if (n > ROOM) {
+            stream_stepwise<T, false>(sh, way, k, colbits, c, sum);
+        } else if (n > k) {                        // those that do not reach the last bound go
+            if (tid < 32) {
+                int digit, above, own;
+                if (highest_digit(sh.hist, k, digit, above, own)) sh.bound = sh.base + ((uint32_t)digit << Order<T>::DIGIT);
+            }
+            u64 mine[ROOM / TT];
+#pragma unroll
+            for (int i = 0; i < ROOM / TT; i++) mine[i] = tid + i * TT < n ? sh.cand[tid + i * TT] : 0;
+            __syncthreads();
+            const u64 least = (u64)sh.bound << colbits;
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ROOM / TT; i++)
+                if (mine[i] > least) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
+            __syncthreads();
+            if (sh.count > ROOM / MOST_RANKS) keep_largest(sh, sh.count, k);
+        }
+    } else {
+        stream_stepwise<T, LSE>(sh, way, k, colbits, c, sum);
+    }
+    float m = sum.m, s = sum.s.x + sum.s.y;
     if (LSE) {
         float r[1] = {m}, q[1];
         cta_reduce<1, TW, true>(r, sh.room);
@@ -321,20 +501,22 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        if (rank == 0)
-            for (unsigned r = 1; r < ranks; r++) {             // the others' candidates, as many as fit at a time
+        if (rank == 0) {
+            const int most = max(k, ROOM / MOST_RANKS);        // candidates of a CTA
+            for (unsigned r = 1; r < ranks; r++) {
                 const int n = peer_load(&sh.count, r), have = sh.count;
                 for (int i = tid; i < n; i += TT) sh.cand[have + i] = peer_load(&sh.cand[i], r);
                 __syncthreads();
                 if (tid == 0) sh.count = have + n;
                 __syncthreads();
-                if (sh.count > ROOM - k || r == ranks - 1) keep_largest(sh, sh.count, k);
+                if (sh.count > ROOM - most) keep_largest(sh, sh.count, k);
                 if (LSE) {
                     const float om = peer_load(&sh.m, r), os = peer_load(&sh.s, r), nm = max_nan(m, om);
                     s = (m == MINUS_INF ? 0.0f : s * exp2_fast((m - nm) * c)) + (om == MINUS_INF ? 0.0f : os * exp2_fast((om - nm) * c));
                     m = nm;
                 }
             }
+        }
         __syncwarp();
         cluster_arrive();
         cluster_wait();
@@ -345,14 +527,25 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         pos[t] = t * k;
         if (t == nrows - 1) pos[nrows] = nrows * k;
     }
+    int n = sh.count;
+    if (n > TT && n > k) {
+        keep_largest(sh, n, k);
+        n = k;
+    }
     // by column, ascending: the complement of the column, descending
-    const u64 low = (1ull << colbits) - 1;
-    if (k <= TT) {
-        u64 it = 0;
-        int at = 0;
-        if (tid < k) {
-            it = sh.cand[tid];
-            for (int i = 0; i < k; i++) at += (sh.cand[i] & low) > (it & low);
+    if (n <= TT) {
+        u64 it = tid < n ? sh.cand[tid] : 0;
+        if (n > k) {
+            int above = 0;
+            for (int i = 0; i < n; i++) above += sh.cand[i] > it;
+            __syncthreads();
+            if (above >= k) it = 0;
+            if (tid < n) sh.cand[tid] = it;
+            __syncthreads();
+        }
+        if (it) {
+            int at = 0;
+            for (int i = 0; i < n; i++) at += (sh.cand[i] & low) > (it & low);
             crd[t * k + at] = (int64_t)(low - (it & low));
             val[t * k + at] = Order<T>::value((uint32_t)(it >> colbits));
         }
@@ -360,12 +553,12 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
     }
     int p = 1;
     while (p < k) p *= 2;
+    u64 *v = sh.cand + MOST_K;
     for (int i = tid; i < p; i += TT) {
         const u64 it = i < k ? sh.cand[i] : 0;
-        sh.cand[MOST_K + i] = i < k ? (low - (it & low)) << 32 | it >> colbits : ~0ull;
+        v[i] = i < k ? (low - (it & low)) << 32 | it >> colbits : ~0ull;
     }
     __syncthreads();
-    u64 *v = sh.cand + MOST_K;
     for (int size = 2; size <= p; size *= 2)
         for (int step = size / 2; step > 0; step /= 2) {
             for (int i = tid; i < p / 2; i += TT) {
@@ -491,7 +684,9 @@ static int launch_long(const TopCall &a)
     while ((1 << colbits) <= a.ncols) colbits++;
     const size_t smem = (size_t)STAGES * TU * TT * 16;
     if (a.nrows * ranks > 0x7fffffffLL) return fail("top_entries: more than 2^31 rows");
-    return launch_cluster(top_kernel<T, LSE>, (unsigned)(a.nrows * ranks), ranks, TT, smem, a.st, a.nrows, a.ncols, (int)ceil_div(all, ranks),
+    // beyond 256 entries the candidates of a row without barriers would not fit their room
+    auto kernel = a.k <= 256 ? top_kernel<T, LSE, true> : top_kernel<T, LSE, false>;
+    return launch_cluster(kernel, (unsigned)(a.nrows * ranks), ranks, TT, smem, a.st, a.nrows, a.ncols, (int)ceil_div(all, ranks),
                           (const T *)a.x, a.ldx, a.k, colbits, a.c, a.inv, a.pos, a.crd, a.val, a.lse);
 }
 
