@@ -7,16 +7,51 @@
 // g = f - 1 / E, taken from whole numbers: for balanced experts the difference f_e - sum f p would lose its digits otherwise.
 // sigmoid(r) / sum is softmax(log sigmoid(r)), which holds where every sigmoid underflows.
 //
-// Bound: HBM, R and its gradient; small batches: the launches.
+// Small batches: one cluster counts, exchanges its counts through shared memory and takes the rows, in one launch.  Otherwise a
+// kernel counts and a second one, whose start overlaps with it, takes the rows.
+// A group of lanes takes a row, 16 bytes a lane or a few times that: a lane's columns are the same in every row, so their g stay in
+// registers while the sequence lasts.
+//
+// Bound: HBM, R and its gradient; small batches: the launch.
 #include "logits.cuh"
 #include "stream.cuh"
 
 namespace cb200 {
 
-static const int BT = 256, MOST_EXPERTS = 1024;
+static const int BT = 256, BW = BT / 32, MOST_EXPERTS = 1024;
+static const int64_t SMALL_ELEMENTS = 65536;       // logits of the one-launch kernel
+static const int SMALL_COUNTS = 2048;              // sequences times (experts + 2) that the one-launch kernel holds
+static const int KEPT_COUNTS = 16384;              // and that are counted in memory that every call leaves at 0
 
-// What the counts leave for the main kernel, in SLOT_MISC: {sequences with active rows, -}, then {active rows, entries} per sequence.
 typedef unsigned long long u64;
+static __device__ u64 g_kept[KEPT_COUNTS + 2];
+
+// What the counting leaves: counts[sequence][expert], and {active rows, entries} per sequence; in `all`: sequences with active rows, and
+// whether a column was outside.
+struct Tally {
+    u64 *counts, *rows, *all;
+};
+
+struct BalanceArgs {
+    int64_t nrows;
+    int ncols;
+    const int64_t *pos, *crd;
+    int64_t nseq;
+    const int64_t *seq;
+    const uint8_t *mask;
+    const void *r;
+    int64_t ldr;
+    void *grad;
+    int64_t ldg;
+    float scale;
+    bool whole;                  // rows of R and of the gradient begin at 16 bytes and are a whole number of them
+    Tally tally;
+    bool kept;                   // the tally is g_kept
+    int64_t *counts;
+    double *partial;
+    float *loss;
+    unsigned *counter;
+};
 
 __device__ __forceinline__ int64_t sequence_of(const int64_t *seq, int64_t nseq, int64_t row)
 {
@@ -29,125 +64,362 @@ __device__ __forceinline__ int64_t sequence_of(const int64_t *seq, int64_t nseq,
     return lo;
 }
 
-__global__ void __launch_bounds__(BT)
-balance_count_kernel(int64_t nrows, int ncols, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, int64_t nseq,
-                     const int64_t *__restrict__ seq, const uint8_t *__restrict__ mask, u64 *__restrict__ counts, u64 *__restrict__ info)
+// Counts rows [r0, r1) by one warp, 32 at a time: hit(sequence, column) for each entry of an active row, rows(sequence, active, entries)
+// for sums over lanes of one sequence, by one lane.  Where all 32 rows store the same number, their entries are read side by side.
+template <typename Hit, typename Rows, typename Bad>
+__device__ __forceinline__ void count_rows(const BalanceArgs &a, int64_t r0, int64_t r1, Hit hit, Rows rows, Bad bad)
 {
-    for (int64_t t = (int64_t)blockIdx.x * BT + threadIdx.x; t < nrows; t += (int64_t)gridDim.x * BT) {
-        const int64_t lo = pos[t], hi = pos[t + 1];
-        if (lo >= hi || (mask && !mask[t])) continue;
-        const int64_t s = seq ? sequence_of(seq, nseq, t) : 0;
-        for (int64_t e = lo; e < hi; e++) {
-            const int64_t j = crd[e];
-            if (j >= 0 && j < ncols) atomicAdd(&counts[s * ncols + j], 1ull);
-            else atomicExch(&info[1], 1ull);
+    const int lane = threadIdx.x & 31;
+    for (int64_t b = r0; b < r1; b += 32) {
+        const int64_t t = b + lane;
+        int64_t lo = 0, hi = 0, s = 0;
+        if (t < r1) {
+            lo = a.pos[t];
+            hi = a.pos[t + 1];
+            if (a.seq) s = sequence_of(a.seq, a.nseq, t);
         }
-        if (atomicAdd(&info[2 + 2 * s], 1ull) == 0) atomicAdd(&info[0], 1ull);
-        atomicAdd(&info[3 + 2 * s], (u64)(hi - lo));
+        const bool active = hi > lo && (!a.mask || a.mask[t]);
+        const unsigned on = __ballot_sync(0xffffffffu, active);
+        if (!on) continue;
+        const int64_t lo0 = __shfl_sync(0xffffffffu, (long long)lo, 0), s0 = __shfl_sync(0xffffffffu, (long long)s, __ffs(on) - 1);
+        const int n = (int)min(hi - lo, (int64_t)0x7fffffff), n0 = __shfl_sync(0xffffffffu, n, 0);
+        const bool one = __all_sync(0xffffffffu, s == s0 || !active);
+        if (one && n0 > 0 && n0 <= 64 && __all_sync(0xffffffffu, t >= r1 || n == n0)) {
+            const int many = 32 * n0;
+            for (int i = lane; i < many; i += 32) {
+                if (!(on >> (i / n0) & 1)) continue;
+                const int64_t j = a.crd[lo0 + i];
+                if (j >= 0 && j < a.ncols) hit(s0, (int)j);
+                else bad();
+            }
+        } else if (active) {
+            for (int64_t e = lo; e < hi; e++) {
+                const int64_t j = a.crd[e];
+                if (j >= 0 && j < a.ncols) hit(s, (int)j);
+                else bad();
+            }
+        }
+        if (one) {
+            int64_t sum = active ? hi - lo : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, (long long)sum, o);
+            if (lane == 0) rows(s0, __popc(on), sum);
+        } else if (active) {
+            rows(s, 1, hi - lo);
+        }
     }
 }
 
-struct BalanceArgs {
-    int64_t nrows;
-    int ncols;
-    const int64_t *pos;
-    int64_t nseq;
-    const int64_t *seq;
-    const uint8_t *mask;
-    const void *r;
-    int64_t ldr;
-    void *grad;
-    int64_t ldg;
-    float scale;
-    const u64 *counts, *info;
-    double *partial;
-    float *loss;
-    unsigned *counter;
-};
+// Rows [r0, r1) of a warp, G lanes and Q times 16 bytes a lane each.  Returns the lane's part of the loss.
+template <typename T, int G, int Q, bool SIGMOID>
+__device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &tally, int64_t r0, int64_t r1)
+{
+    constexpr int N = Granule<T>::N, AT_ONCE = 32 / G;
+    const int lane = threadIdx.x & 31, l = lane % G;
+    const float sequences = (float)tally.all[0], share = 1.0f / (float)a.ncols;
+    int64_t s_end = -1;                            // the row at which the lane's sequence ends
+    float g[Q * N], by = 0.0f;
+    double sum = 0.0;
+    for (int64_t b = r0; b < r1; b += AT_ONCE) {
+        const int64_t t = b + lane / G;
+        const bool there = t < r1;
+        const T *r = (const T *)a.r + t * a.ldr;
+        Granule<T> x[Q];
+        if (there) {
+            if (a.whole) {
+#pragma unroll
+                for (int q = 0; q < Q; q++)
+                    if ((q * G + l) * N < a.ncols) x[q].w = __ldg((const uint4 *)r + q * G + l);
+            } else {
+#pragma unroll
+                for (int q = 0; q < Q; q++)
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if ((q * G + l) * N + e < a.ncols) ((T *)&x[q].w)[e] = r[(q * G + l) * N + e];
+            }
+        }
+        const bool active = there && a.pos[t] < a.pos[t + 1] && (!a.mask || a.mask[t]);
+        if (there && t >= s_end) {
+            int64_t s = 0;
+            s_end = a.nrows;
+            if (a.seq) {
+                s = sequence_of(a.seq, a.nseq, t);
+                if (s + 1 < a.nseq) s_end = a.seq[s + 1];
+            }
+            const int64_t entries = (int64_t)tally.rows[2 * s + 1];
+            by = a.scale * (float)a.ncols / (sequences * (float)tally.rows[2 * s]);
+            const float unit = (float)(1.0 / ((double)entries * a.ncols));
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int col = (q * G + l) * N + e;
+                    g[q * N + e] = col < a.ncols ? (float)((int64_t)tally.counts[s * a.ncols + col] * a.ncols - entries) * unit : 0.0f;
+                }
+        }
+        float v[Q * N], slope[SIGMOID ? Q * N : 1];
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            float u[N];
+            x[q].unpack(u);
+#pragma unroll
+            for (int e = 0; e < N; e++) v[q * N + e] = active && (q * G + l) * N + e < a.ncols ? u[e] : MINUS_INF;
+        }
+        float p = 0.0f, gp = 0.0f;
+        auto add_up = [&]() {
+            p = gp = 0.0f;
+#pragma unroll
+            for (int i = 0; i < Q * N; i++) {
+                p += v[i];
+                gp = fmaf(v[i], g[i], gp);
+            }
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) {
+                p += __shfl_xor_sync(0xffffffffu, p, o);
+                gp += __shfl_xor_sync(0xffffffffu, gp, o);
+            }
+        };
+        auto maximum = [&]() {
+            float m = v[0];
+#pragma unroll
+            for (int i = 1; i < Q * N; i++) m = max_nan(m, v[i]);
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            return m == MINUS_INF ? 0.0f : m;      // exp(-inf - 0) = 0: a row of -inf has no scores
+        };
+        if (SIGMOID) {
+            float low[Q * N];
+#pragma unroll
+            for (int i = 0; i < Q * N; i++) {
+                low[i] = v[i];
+                float d = exp2_fast(v[i] * -LOG2E);
+                d = d > 1e38f ? 1e38f : d;
+                v[i] = __fdividef(1.0f, 1.0f + d);
+                slope[i] = d * v[i];
+            }
+            add_up();
+            if (__any_sync(0xffffffffu, active && p < 1e-30f)) {         // sigmoids below f32's range, or none: their shares by e^(r - max) / (1 + e^r)
+#pragma unroll
+                for (int i = 0; i < Q * N; i++) v[i] = low[i];
+                const float m = fminf(maximum(), 0.0f);
+#pragma unroll
+                for (int i = 0; i < Q * N; i++) {
+                    const float d = exp2_fast(low[i] * LOG2E);
+                    slope[i] = __fdividef(1.0f, 1.0f + (d > 1e38f ? 1e38f : d));
+                    v[i] = low[i] > 60.0f ? exp2_fast(-m * LOG2E) : exp2_fast((low[i] - m) * LOG2E) * slope[i];
+                }
+                add_up();
+            }
+        } else {
+            const float m = maximum();
+#pragma unroll
+            for (int i = 0; i < Q * N; i++) v[i] = exp2_fast((v[i] - m) * LOG2E);
+            add_up();
+        }
+        const float inv = p == 0.0f ? 0.0f : 1.0f / p;
+        gp *= inv;
+        if (l == 0 && active && p != 0.0f) sum += (double)(by * (share + gp));
+        if (a.grad && there) {
+            T *grad = (T *)a.grad + t * a.ldg;
+            const float f = active ? by * inv : 0.0f;
+#pragma unroll
+            for (int i = 0; i < Q * N; i++) v[i] = active ? f * v[i] * (g[i] - gp) * (SIGMOID ? slope[i] : 1.0f) : 0.0f;
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                float u[N];
+#pragma unroll
+                for (int e = 0; e < N; e++) u[e] = v[q * N + e];
+                if (a.whole) {
+                    x[q].pack(u);
+                    if ((q * G + l) * N < a.ncols) ((uint4 *)grad)[q * G + l] = x[q].w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if ((q * G + l) * N + e < a.ncols) grad[(q * G + l) * N + e] = from_float<T>(u[e]);
+                }
+            }
+        }
+    }
+    return sum;
+}
 
-// A warp per row, a lane's experts 32 apart.
-template <typename T, int R, bool SIGMOID>
+// The CTA's sum, in thread 0, in a fixed order.
+__device__ __forceinline__ double cta_sum(double v, double *room)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 1; i < BW; i++) v += room[i];
+    return v;
+}
+
+// All of a small batch by one cluster.
+template <typename T, int G, int Q, bool SIGMOID>
+__global__ void __launch_bounds__(BT)
+balance_small_kernel(const BalanceArgs a)
+{
+    __shared__ int hits[SMALL_COUNTS + 1];         // counts, {rows, entries} per sequence, a column outside
+    __shared__ u64 total[SMALL_COUNTS + 2];
+    __shared__ double room[BW], parts[MOST_CLUSTER];
+    const int tid = threadIdx.x, many = (int)a.nseq * a.ncols, words = many + 2 * (int)a.nseq + 1;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    for (int i = tid; i < words; i += BT) hits[i] = 0;
+    if (tid == 0) total[words] = 0;
+    __syncthreads();
+    const int64_t warps = (int64_t)ranks * BW, w = (int64_t)rank * BW + (tid >> 5);
+    const int64_t per = (a.nrows + warps * 32 - 1) / (warps * 32) * 32, r0 = min(w * per, a.nrows), r1 = min(r0 + per, a.nrows);
+    count_rows(a, r0, r1, [&](int64_t s, int j) { atomicAdd(&hits[(int)s * a.ncols + j], 1); },
+               [&](int64_t s, int n, int64_t e) {
+                   atomicAdd(&hits[many + 2 * (int)s], n);
+                   atomicAdd(&hits[many + 2 * (int)s + 1], (int)e);
+               },
+               [&]() { hits[words - 1] = 1; });
+    if (ranks > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    for (int i = tid; i < words; i += BT) {
+        u64 n = 0;
+        for (unsigned k = 0; k < ranks; k++) n += (u64)(ranks > 1 ? peer_load(&hits[i], k) : hits[i]);
+        total[i] = n;
+        if (rank == 0 && i < many) a.counts[i] = (int64_t)n;
+        if (i >= many && i < words - 1 && (i - many) % 2 == 0 && n) atomicAdd(&total[words], 1ull);
+    }
+    __syncthreads();
+    const Tally tally = {total, total + many, total + words};
+    const int64_t each = (a.nrows + warps - 1) / warps, q0 = min(w * each, a.nrows), q1 = min(q0 + each, a.nrows);
+    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID>(a, tally, q0, q1), room);
+    if (ranks > 1) {
+        if (tid == 0) store_peer(&parts[rank], 0, sum);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    } else if (tid == 0) {
+        parts[0] = sum;
+    }
+    if (rank != 0 || tid != 0) return;
+    double loss = 0.0;
+    for (unsigned k = 0; k < ranks; k++) loss += parts[k];
+    *a.loss = total[words - 1] ? __int_as_float(0x7fffffff) : (float)loss;
+}
+
+// Counts of a larger batch: a CTA's rows of one sequence in shared memory first.
+__global__ void __launch_bounds__(BT)
+balance_count_kernel(const BalanceArgs a, int64_t per)
+{
+    __shared__ int hits[MOST_EXPERTS];
+    let_next_start();
+    const int64_t c0 = (int64_t)blockIdx.x * per, c1 = min(c0 + per, a.nrows);
+    const int64_t s0 = a.seq && c0 < a.nrows ? sequence_of(a.seq, a.nseq, c0) : 0;
+    for (int i = threadIdx.x; i < a.ncols; i += BT) hits[i] = 0;
+    __syncthreads();
+    wait_for_previous();                           // the call before has left the tally at 0
+    const int64_t each = (per / BW + 31) / 32 * 32, r0 = min(c0 + (threadIdx.x >> 5) * each, c1), r1 = min(r0 + each, c1);
+    const Tally &y = a.tally;
+    count_rows(a, r0, r1,
+               [&](int64_t s, int j) {
+                   if (s == s0) atomicAdd(&hits[j], 1);
+                   else atomicAdd(&y.counts[s * a.ncols + j], 1ull);
+               },
+               [&](int64_t s, int n, int64_t e) {
+                   if (atomicAdd(&y.rows[2 * s], (u64)n) == 0) atomicAdd(&y.all[0], 1ull);
+                   atomicAdd(&y.rows[2 * s + 1], (u64)e);
+               },
+               [&]() { y.all[1] = 1; });
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.ncols; i += BT)
+        if (hits[i]) atomicAdd(&y.counts[s0 * a.ncols + i], (u64)hits[i]);
+}
+
+template <typename T, int G, int Q, bool SIGMOID>
 __global__ void __launch_bounds__(BT)
 balance_kernel(const BalanceArgs a)
 {
-    const int lane = threadIdx.x & 31;
-    const float sequences = (float)a.info[0];
-    double sum = 0.0;
-    for (int64_t t = ((int64_t)blockIdx.x * BT + threadIdx.x) >> 5; t < a.nrows; t += ((int64_t)gridDim.x * BT) >> 5) {
-        const T *r = (const T *)a.r + t * a.ldr;
-        T *grad = a.grad ? (T *)a.grad + t * a.ldg : nullptr;
-        if (a.pos[t] >= a.pos[t + 1] || (a.mask && !a.mask[t])) {
-            if (grad)
-                for (int e = lane; e < a.ncols; e += 32) grad[e] = from_float<T>(0.0f);
-            continue;
-        }
-        const int64_t s = a.seq ? sequence_of(a.seq, a.nseq, t) : 0;
-        const float rows = (float)a.info[2 + 2 * s], by = a.scale * (float)a.ncols / (sequences * rows);
-        const u64 entries = a.info[3 + 2 * s];
-        const float unit = (float)(1.0 / ((double)entries * a.ncols));
-        float u[R], slope[R], m = MINUS_INF;
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            const int e = lane + 32 * i;
-            u[i] = e < a.ncols ? to_float(r[e]) : MINUS_INF;
-            slope[i] = 1.0f;
-            if (SIGMOID) {
-                const float d = expf(-fabsf(u[i])), l = fminf(u[i], 0.0f) - log1pf(d);
-                slope[i] = u[i] > 0.0f ? d / (1.0f + d) : 1.0f / (1.0f + d);       // 1 - sigmoid
-                u[i] = u[i] == MINUS_INF ? MINUS_INF : l;
-            }
-            m = max_nan(m, u[i]);
-        }
-        m = warp_max(m);
-        float p = 0.0f, gp = 0.0f, g[R];
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            const int e = lane + 32 * i;
-            g[i] = e < a.ncols ? (float)((int64_t)a.counts[s * a.ncols + e] * a.ncols - (int64_t)entries) * unit : 0.0f;
-            u[i] = m == MINUS_INF ? 0.0f : exp2_fast((u[i] - m) * LOG2E);
-            p += u[i];
-            gp += u[i] * g[i];
-        }
-        p = warp_sum(p);
-        gp = warp_sum(gp);
-        const float inv = p == 0.0f ? 0.0f : 1.0f / p;
-        gp *= inv;
-        if (grad)
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int e = lane + 32 * i;
-                if (e < a.ncols) grad[e] = from_float<T>(by * (u[i] * inv) * (g[i] - gp) * slope[i]);
-            }
-        if (p != 0.0f) sum += (double)by * (1.0f / (float)a.ncols + gp);
-    }
-    __shared__ double sums[BT / 32];
+    __shared__ double room[BW];
     __shared__ bool last;
-    if (lane == 0) sums[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < BT / 32; i++) sum += sums[i];
+    const int tid = threadIdx.x;
+    const int64_t warps = (int64_t)gridDim.x * BW, w = (int64_t)blockIdx.x * BW + (tid >> 5);
+    const int64_t each = (a.nrows + warps - 1) / warps, r0 = min(w * each, a.nrows), r1 = min(r0 + each, a.nrows);
+    wait_for_previous();
+    const int64_t many = a.nseq * a.ncols;
+    if (a.kept)
+        for (int64_t i = (int64_t)blockIdx.x * BT + tid; i < many; i += (int64_t)gridDim.x * BT) a.counts[i] = (int64_t)a.tally.counts[i];
+    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID>(a, a.tally, r0, r1), room);
+    if (tid == 0) {
         a.partial[blockIdx.x] = sum;
         last = last_of(a.counter, gridDim.x);
     }
     __syncthreads();
-    if (!last || threadIdx.x >= 32) return;
+    if (!last) return;
     __threadfence();
-    sum = 0.0;
-    for (int i = lane; i < (int)gridDim.x; i += 32) sum += __ldcg(a.partial + i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) *a.loss = a.info[1] ? __int_as_float(0x7fffffff) : (float)sum;
+    double all = 0.0;
+    for (int i = tid; i < (int)gridDim.x; i += BT) all += __ldcg(a.partial + i);
+    all = cta_sum(all, room);
+    if (tid == 0) *a.loss = a.tally.all[1] ? __int_as_float(0x7fffffff) : (float)all;
+    if (a.kept) {
+        __syncthreads();
+        for (int i = tid; i < (int)many; i += BT) a.tally.counts[i] = 0;
+        for (int i = tid; i < 2 * (int)a.nseq; i += BT) a.tally.rows[i] = 0;
+        if (tid < 2) a.tally.all[tid] = 0;
+    }
 }
 
-template <typename T, bool SIGMOID>
-static void launch_balance(const BalanceArgs &a, unsigned grid, cudaStream_t st)
+template <typename T, int G, int Q, bool SIGMOID>
+static int launch_balance(BalanceArgs a, cudaStream_t st)
 {
-    if (a.ncols <= 32) balance_kernel<T, 1, SIGMOID><<<grid, BT, 0, st>>>(a);
-    else if (a.ncols <= 64) balance_kernel<T, 2, SIGMOID><<<grid, BT, 0, st>>>(a);
-    else if (a.ncols <= 128) balance_kernel<T, 4, SIGMOID><<<grid, BT, 0, st>>>(a);
-    else if (a.ncols <= 256) balance_kernel<T, 8, SIGMOID><<<grid, BT, 0, st>>>(a);
-    else if (a.ncols <= 512) balance_kernel<T, 16, SIGMOID><<<grid, BT, 0, st>>>(a);
-    else balance_kernel<T, 32, SIGMOID><<<grid, BT, 0, st>>>(a);
+    const int64_t many = a.nseq * a.ncols, words = many + 2 * a.nseq;
+    if (words <= SMALL_COUNTS && a.nrows * a.ncols <= SMALL_ELEMENTS && a.nrows * 4 < SMALL_ELEMENTS) {
+        int ranks = 1;
+        while (ranks < MOST_CLUSTER && a.nrows * a.ncols > (int64_t)ranks * 4096) ranks *= 2;
+        return launch_cluster(balance_small_kernel<T, G, Q, SIGMOID>, (unsigned)ranks, ranks, BT, 0, st, a);
+    }
+    constexpr int AT_ONCE = BW * 32 / G;
+    const int64_t most = (int64_t)sm_count() * 8;
+    const int64_t grid = max((int64_t)1, min(most, ceil_div(a.nrows, AT_ONCE * 2)));
+    void *room = nullptr;
+    a.kept = words <= KEPT_COUNTS;
+    CB_TRY(scratch(SLOT_MISC, (size_t)most * sizeof(double) + (a.kept ? 0 : (size_t)(2 + 2 * a.nseq) * sizeof(u64)), &room));
+    a.partial = (double *)room;
+    if (a.kept) {
+        u64 *kept = nullptr;
+        CB_CUDA(cudaGetSymbolAddress((void **)&kept, g_kept));
+        a.tally = {kept, kept + many, kept + many + 2 * a.nseq};
+    } else {
+        u64 *info = (u64 *)(a.partial + most);
+        a.tally = {(u64 *)a.counts, info, info + 2 * a.nseq};
+        CB_CUDA(cudaMemsetAsync(a.counts, 0, (size_t)many * sizeof(int64_t), st));
+        CB_CUDA(cudaMemsetAsync(info, 0, (size_t)(2 + 2 * a.nseq) * sizeof(u64), st));
+    }
+    const int64_t per = max((int64_t)BT, ceil_div(ceil_div(a.nrows, most), BT) * BT);
+    if (a.nrows > 0) balance_count_kernel<<<(unsigned)ceil_div(a.nrows, per), BT, 0, st>>>(a, per);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_behind(balance_kernel<T, G, Q, SIGMOID>, dim3((unsigned)grid), BT, 0, st, a);
+    if (e != cudaSuccess) {
+        if (a.kept) cudaMemsetAsync(a.tally.counts, 0, sizeof(g_kept), st);       // what was counted is not the next call's
+        return fail("balance_loss: launch failed: %s", cudaGetErrorString(e));
+    }
+    return 0;
+}
+
+// G lanes x Q granules of N elements just cover the experts
+template <typename T, bool SIGMOID>
+static int dispatch_balance(const BalanceArgs &a, cudaStream_t st)
+{
+    const int granules = (a.ncols + Granule<T>::N - 1) / Granule<T>::N;
+    if (granules <= 1) return launch_balance<T, 1, 1, SIGMOID>(a, st);
+    if (granules <= 2) return launch_balance<T, 2, 1, SIGMOID>(a, st);
+    if (granules <= 4) return launch_balance<T, 4, 1, SIGMOID>(a, st);
+    if (granules <= 8) return launch_balance<T, 8, 1, SIGMOID>(a, st);
+    if (granules <= 16) return launch_balance<T, 16, 1, SIGMOID>(a, st);
+    if (granules <= 32) return launch_balance<T, 32, 1, SIGMOID>(a, st);
+    if (granules <= 64) return launch_balance<T, 32, 2, SIGMOID>(a, st);
+    if (granules <= 128) return launch_balance<T, 32, 4, SIGMOID>(a, st);
+    return launch_balance<T, 32, 1024 / (32 * Granule<T>::N), SIGMOID>(a, st);
 }
 
 template <typename T>
@@ -162,26 +434,12 @@ static int balance_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
     if (ldr < ncols || (grad && ldg < ncols)) return fail("balance_loss: leading dimension smaller than the number of columns");
     if (nseq < 1 || (nseq > 1 && !seq)) return fail("balance_loss: %lld sequences without their bounds", (long long)nseq);
     if ((uintptr_t)r % sizeof(T) || (uintptr_t)grad % sizeof(T)) return fail("balance_loss: an address that is not a multiple of the element's size");
-    const int64_t most = (int64_t)sm_count() * 8;
-    int64_t grid = ceil_div(nrows, BT / 32);
-    if (grid > most) grid = most;
-    if (grid < 1) grid = 1;
-    void *room = nullptr;
-    CB_TRY(scratch(SLOT_MISC, (size_t)(2 + 2 * nseq) * sizeof(u64) + (size_t)most * sizeof(double), &room));
-    u64 *info = (u64 *)room;
-    BalanceArgs a = {nrows, (int)ncols, pos, nseq, seq, mask, r, ldr, grad, ldg, (float)*scale, (const u64 *)counts, info, (double *)(info + 2 + 2 * nseq),
-                     loss, next_counter()};
+    const int64_t size = (int64_t)sizeof(T);
+    const bool whole = ncols * size % 16 == 0 && ((uintptr_t)r | (uintptr_t)grad) % 16 == 0 && ldr * size % 16 == 0 && ldg * size % 16 == 0;
+    const BalanceArgs a = {nrows, (int)ncols, pos, crd, nseq, seq, mask, r, ldr, grad, ldg, (float)*scale, whole, {}, false, counts, nullptr, loss,
+                           next_counter()};
     if (!a.counter) return 1;
-    CB_CUDA(cudaMemsetAsync(counts, 0, (size_t)(nseq * ncols) * sizeof(int64_t), st));
-    CB_CUDA(cudaMemsetAsync(info, 0, (size_t)(2 + 2 * nseq) * sizeof(u64), st));
-    int64_t blocks = ceil_div(nrows, BT);
-    if (blocks > most) blocks = most;
-    if (blocks > 0) balance_count_kernel<<<(unsigned)blocks, BT, 0, st>>>(nrows, (int)ncols, pos, crd, nseq, seq, mask, (u64 *)counts, info);
-    CB_LAUNCH_CHECK();
-    if (sigmoid) launch_balance<T, true>(a, (unsigned)grid, st);
-    else launch_balance<T, false>(a, (unsigned)grid, st);
-    CB_LAUNCH_CHECK();
-    return 0;
+    return sigmoid ? dispatch_balance<T, true>(a, st) : dispatch_balance<T, false>(a, st);
 }
 
 }  // namespace cb200

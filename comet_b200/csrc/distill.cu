@@ -16,7 +16,6 @@
 namespace cb200 {
 
 static const int DT = 256, DW = DT / 32;
-static const int MAX_CLUSTER = 8;
 static const int MOST_SLICE = 192 * 1024;          // bytes of a row in one CTA
 
 struct DistillArgs {
@@ -47,7 +46,7 @@ distill_kernel(const DistillArgs a)
     constexpr int N = Granule<T>::N;
     extern __shared__ uint4 dyn[];
     __shared__ float room[6 * DW], room2[2 * DW];
-    __shared__ Told told[MAX_CLUSTER];
+    __shared__ Told told[MOST_CLUSTER];
     __shared__ bool last;
     const int tid = threadIdx.x;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
@@ -226,7 +225,7 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     constexpr int N = Granule<T>::N;
     const int all = (a.ncols + 2 * N - 2) / N;     // granules of a row, wherever it starts
     int ranks = 1;
-    while (ranks < MAX_CLUSTER && (ceil_div(all, ranks) * 16 > 32 * 1024 || (a.nrows * ranks < sm_count() * 2 && all / ranks >= 512))) ranks *= 2;
+    while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > 32 * 1024 || (a.nrows * ranks < sm_count() * 2 && all / ranks >= 512))) ranks *= 2;
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
     const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);
@@ -252,9 +251,9 @@ static int distill_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
     if (ldx < ncols || (grad && ldg < ncols)) return fail("distill_loss: leading dimension smaller than the number of columns");
     if (!(temperature > 0.0) || temperature > 1e30) return fail("distill_loss: temperature %g is not a positive number", temperature);
     if (val_bytes != 4 && val_bytes != 8) return fail("distill_loss: the teacher's values have 4 or 8 bytes");
-    if (ncols > (int64_t)MAX_CLUSTER * MOST_SLICE / (int64_t)sizeof(T) - 64)
+    if (ncols > (int64_t)MOST_CLUSTER * MOST_SLICE / (int64_t)sizeof(T) - 64)
         return fail("distill_loss: rows of %lld columns do not fit the shared memory of eight SMs", (long long)ncols);
-    if (nrows > 0x7fffffffLL / MAX_CLUSTER) return fail("distill_loss: more than 2^28 rows");
+    if (nrows > 0x7fffffffLL / MOST_CLUSTER) return fail("distill_loss: more than 2^28 rows");
     if ((uintptr_t)x % sizeof(T) || (uintptr_t)grad % sizeof(T)) return fail("distill_loss: an address that is not a multiple of the element's size");
     if (nrows == 0) {
         CB_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));

@@ -8,6 +8,7 @@
 
 namespace cb200 {
 
+static const int MOST_CLUSTER = 8;                  // CTAs of a cluster that every device takes
 static const double LOG2E_D = 1.4426950408889634;
 
 #ifdef __CUDACC__
@@ -258,6 +259,10 @@ __device__ __forceinline__ uint32_t peer_address(const V *mine, unsigned rank)
 __device__ __forceinline__ void store_peer(float *mine, unsigned rank, float v)
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_address(mine, rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ void store_peer(double *mine, unsigned rank, double v)
+{
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(peer_address(mine, rank)), "d"(v) : "memory");
 }
 __device__ __forceinline__ float peer_load(const float *mine, unsigned rank)
 {

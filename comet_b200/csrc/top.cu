@@ -35,7 +35,7 @@ unsigned *next_counter()
     return p + turn++ % 1024;
 }
 
-static const int TT = 256, TW = TT / 32, TU = 4, STAGES = 3, MOST_K = 1024, ROOM = 2048, MOST_RANKS = 8;
+static const int TT = 256, TW = TT / 32, TU = 4, STAGES = 3, MOST_K = 1024, ROOM = 2048;
 
 typedef unsigned long long u64;
 
@@ -479,7 +479,7 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
             for (int i = 0; i < ROOM / TT; i++)
                 if (mine[i] > least) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
             __syncthreads();
-            if (sh.count > ROOM / MOST_RANKS) keep_largest(sh, sh.count, k);
+            if (sh.count > ROOM / MOST_CLUSTER) keep_largest(sh, sh.count, k);
         }
     } else {
         stream_stepwise<T, LSE>(sh, way, k, colbits, c, sum);
@@ -502,7 +502,7 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         cluster_arrive();
         cluster_wait();
         if (rank == 0) {
-            const int most = max(k, ROOM / MOST_RANKS);        // candidates of a CTA
+            const int most = max(k, ROOM / MOST_CLUSTER);        // candidates of a CTA
             for (unsigned r = 1; r < ranks; r++) {
                 const int n = peer_load(&sh.count, r), have = sh.count;
                 for (int i = tid; i < n; i += TT) sh.cand[have + i] = peer_load(&sh.cand[i], r);
@@ -680,7 +680,7 @@ static int launch_long(const TopCall &a)
     constexpr int N = Granule<T>::N;
     const int all = (a.ncols + 2 * N - 2) / N;     // granules of a row, wherever it starts
     int ranks = 1, colbits = 1;
-    while (ranks < MOST_RANKS && a.nrows * ranks <= sm_count() && all / ranks >= 2 * TU * TT) ranks *= 2;
+    while (ranks < MOST_CLUSTER && a.nrows * ranks <= sm_count() && all / ranks >= 2 * TU * TT) ranks *= 2;
     while ((1 << colbits) <= a.ncols) colbits++;
     const size_t smem = (size_t)STAGES * TU * TT * 16;
     if (a.nrows * ranks > 0x7fffffffLL) return fail("top_entries: more than 2^31 rows");
