@@ -12,11 +12,13 @@
 //
 // Bound: HBM, the bytes of X and of the gradient.
 #include "logits.cuh"
+#include "stream.cuh"
 
 namespace cb200 {
 
 static const int DT = 256, DW = DT / 32;
-static const int MOST_SLICE = 192 * 1024;          // bytes of a row in one CTA
+static const int SLICE = 64 * 1024;                // bytes of a row that a CTA gets if the cluster is not larger for it
+static const int MOST_SLICE = 192 * 1024;          // and at most
 
 struct DistillArgs {
     int64_t nrows;
@@ -30,7 +32,7 @@ struct DistillArgs {
     int64_t ldg;
     float c, by, scale;          // log2(e) / temperature, scale / temperature
     float *rows, *loss;
-    unsigned *counter;
+    unsigned *counter;           // null: another kernel adds the rows up
 };
 
 // what a CTA tells the others of its row: the maximum of its part, sums of 2^((x - maximum) c) of elements that are not
@@ -39,50 +41,139 @@ struct Told {
     float m, others, stored, p, pu;
 };
 
+// (x - m) c.  As x c - m c it is one operation, and the rounding of m c is a factor that all of a row's terms and their sum
+// have alike; m c may be beyond f32 where the difference is not.
+struct Exponent {
+    float c, m, mc;
+    bool near;
+    __device__ __forceinline__ Exponent(float most, float c_) : c(c_), m(most == MINUS_INF ? 0.0f : most)
+    {
+        mc = m * c;
+        near = fabsf(mc) < 1e30f;
+    }
+    __device__ __forceinline__ float of(float x) const { return near ? fmaf(x, c, -mc) : (x - m) * c; }
+    __device__ __forceinline__ float2 of(float2 x) const { return fma2(x, make_float2(c, c), make_float2(-mc, -mc)); }      // near
+    __device__ __forceinline__ float to(const Exponent &o) const { return near && o.near ? mc - o.mc : (m - o.m) * c; }
+};
+
+template <int N>
+__device__ __forceinline__ float sum_of(const float (&v)[N])
+{
+    float s = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) s += v[i];
+    return s;
+}
+
+// scale * the sum of weight * rows, by one warp or more, in a fixed order; the result in thread 0
+template <int THREADS>
+__device__ __forceinline__ void add_rows(const DistillArgs &a, double *room)
+{
+    double sum = 0.0;
+    for (int64_t r = threadIdx.x; r < a.nrows; r += THREADS) {
+        const float w = a.weight ? a.weight[r] : 1.0f;
+        if (w != 0.0f) sum += (double)w * __ldcg(a.rows + r);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (THREADS > 32) {
+        if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 1; i < THREADS / 32; i++) sum += room[i];
+    }
+    if (threadIdx.x == 0) *a.loss = (float)(sum * a.scale);
+}
+
+__global__ void __launch_bounds__(1024)
+distill_sum_kernel(const DistillArgs a)
+{
+    __shared__ double room[32];
+    wait_for_previous();
+    add_rows<1024>(a, room);
+}
+
 template <typename T, typename TV, bool REST, bool GRAD>
 __global__ void __launch_bounds__(DT)
 distill_kernel(const DistillArgs a)
 {
     constexpr int N = Granule<T>::N;
     extern __shared__ uint4 dyn[];
-    __shared__ float room[6 * DW], room2[2 * DW];
+    __shared__ float most[DW], zmost[DW], sums[6][DW];
     __shared__ Told told[MOST_CLUSTER];
-    __shared__ bool last;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     const int64_t t = blockIdx.x / ranks, lo = a.pos[t], hi = a.pos[t + 1];
     const float w = a.weight ? a.weight[t] : 1.0f;
     const T *x = (const T *)a.x + t * a.ldx;
+    T *g = GRAD ? (T *)a.grad + t * a.ldg : nullptr;
     const TV *z = (const TV *)a.val;
     // the row's granules, and this CTA's; element e of them is column e - off + first * N
     const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
     const int all = (off + a.ncols + N - 1) / N, first = min((int)rank * a.slice, all), n = min(a.slice, all - first);
     const int col0 = first * N - off;              // the column of this CTA's element 0; negative if that lies before the row
-    uint4 *part = dyn;
+    Granule<T> *part = (Granule<T> *)dyn;
     uint32_t *bits = (uint32_t *)(dyn + a.slice);  // a bit per element: stored
-    T *elem = (T *)part;
+    T *elem = (T *)dyn;
+    const bool entries = lo + warp * 32 < hi;      // the warp has some of the row's
 
-    float m[2] = {MINUS_INF, MINUS_INF};
-    cluster_arrive();
+    float zm = MINUS_INF;
     if (lo < hi && w != 0.0f) {
+        if (ranks > 1) cluster_arrive();
         const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15) + first;
         for (int i = tid; i < n; i += DT) copy_granule(part + i, from + i);
         if (REST)
             for (int i = tid; i < (n * N + 31) / 32; i += DT) bits[i] = 0;
-        for (int64_t e = lo + tid; e < hi; e += DT) m[1] = max_nan(m[1], (float)z[e]);
+        for (int64_t e = lo + tid; e < hi; e += DT) zm = max_nan(zm, (float)z[e]);
+        if (entries) zm = warp_max(zm);
         wait_copies();
-        for (int i = tid; i < n; i += DT) {
-            if (i == 0 || i == n - 1)              // elements before and behind the row
-                for (int k = 0; k < N; k++)
-                    if (col0 + i * N + k < 0 || col0 + i * N + k >= a.ncols) elem[i * N + k] = from_float<T>(MINUS_INF);
-            m[0] = max_nan(m[0], to_float(largest(((const Granule<T> *)(part + i))->most())));
+        float m = MINUS_INF;
+        if (tid < n) {
+#pragma unroll
+            for (int side = 0; side < 2; side++) { // elements before and behind the row
+                const int i = side ? n - 1 : 0;
+                if (tid == i % DT && (col0 + i * N < 0 || col0 + i * N + N > a.ncols))
+                    for (int k = 0; k < N; k++)
+                        if (col0 + i * N + k < 0 || col0 + i * N + k >= a.ncols) elem[i * N + k] = from_float<T>(MINUS_INF);
+            }
+            typename Granule<T>::Most mm = part[tid].most();
+#pragma unroll 4
+            for (int i = tid + DT; i < n; i += DT) mm = most_of(mm, part[i].most());
+            m = to_float(largest(mm));
         }
+        m = warp_max(m);
+        if (lane == 0) {
+            most[warp] = m;
+            zmost[warp] = entries ? zm : MINUS_INF;
+        }
+        __syncthreads();
+        zm = zmost[0];
+#pragma unroll
+        for (int i = 1; i < DW; i++) zm = max_nan(zm, zmost[i]);
     }
-    cta_reduce<2, DW, true>(m, room2);
-    const bool counts = m[1] != MINUS_INF;         // the row stores something, and its weight is not 0
-    float s[6] = {0, 0, 0, 0, 0, 0};
-    const float mx = m[0] == MINUS_INF ? 0.0f : m[0];
-    if (counts) {
+    if (zm == MINUS_INF) {                         // the row does not count
+        if (GRAD) {
+            uint4 *to = (uint4 *)((uintptr_t)g & ~(uintptr_t)15) + first;
+            const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+            for (int i = tid; i < n; i += DT) {
+                const int col = col0 + i * N;
+                if (alike && col >= 0 && col + N <= a.ncols) {
+                    to[i] = make_uint4(0, 0, 0, 0);
+                } else {
+                    for (int k = 0; k < N; k++)
+                        if (col + k >= 0 && col + k < a.ncols) g[col + k] = from_float<T>(0.0f);
+                }
+            }
+        }
+        __syncwarp();
+        if (lo < hi && w != 0.0f && ranks > 1) cluster_wait();
+        if (rank != 0 || warp != 0) return;
+        if (lane == 0) a.rows[t] = 0.0f;
+    } else {
+        float m = most[0];
+#pragma unroll
+        for (int i = 1; i < DW; i++) m = max_nan(m, most[i]);
+        const Exponent u(m, a.c);
         if (REST) {
             for (int64_t e = lo + tid; e < hi; e += DT) {
                 const int64_t j = a.crd[e] - col0;
@@ -90,133 +181,152 @@ distill_kernel(const DistillArgs a)
             }
             __syncthreads();
         }
-        for (int i = tid; i < n; i += DT) {
-            float v[N];
-            ((const Granule<T> *)(part + i))->unpack(v);
-            unsigned skip = 0;
-            if (REST) skip = N == 8 ? ((const uint8_t *)bits)[i] : ((const uint8_t *)bits)[i >> 1] >> ((i & 1) * 4);
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float q = exp2_fast((v[k] - mx) * a.c);
-                if (!REST || !(skip >> k & 1)) s[0] += q;
-            }
-        }
-        const float zref = REST ? a.lse[t] * LOG2E : m[1];
-        for (int64_t e = lo + tid; e < hi; e += DT) {
-            const int64_t col = a.crd[e], j = col - col0;
-            const float lz = REST ? fmaf((float)z[e], a.c, -zref) : ((float)z[e] - zref) * a.c, p = exp2_fast(lz);
-            s[1] += p;
-            if (!(p <= 0.0f)) s[2] += p * lz;
-            if (col < 0 || col >= a.ncols) s[5] = __int_as_float(0x7fffffff);
-            if (j >= 0 && j < (int64_t)n * N && col >= 0 && col < a.ncols) {
-                const float u = (to_float(elem[j]) - mx) * a.c;
-                s[3] += p;
-                if (!(p <= 0.0f)) s[4] += p * u;
-                if (REST && (e == lo || a.crd[e - 1] != col)) s[5] += exp2_fast(u);
-            }
-        }
-    }
-    cta_reduce<6, DW, false>(s, room);
-    cluster_wait();                                // the others are there
-    if (tid < (int)ranks) {
-        Told *to = &told[rank];
-        store_peer(&to->m, tid, m[0]);
-        store_peer(&to->others, tid, s[0]);
-        store_peer(&to->stored, tid, s[5]);
-        store_peer(&to->p, tid, s[3]);
-        store_peer(&to->pu, tid, s[4]);
-    }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-
-    float top = MINUS_INF, others = 0.0f, stored = 0.0f, pu = 0.0f;
-    for (unsigned r = 0; r < ranks; r++) top = max_nan(top, told[r].m);
-    if (top == MINUS_INF) top = 0.0f;
-    for (unsigned r = 0; r < ranks; r++) {
-        const Told &o = told[r];
-        const float d = ((o.m == MINUS_INF ? 0.0f : o.m) - top) * a.c, f = exp2_fast(d);
-        if (o.others != 0.0f) others += o.others * f;
-        if (o.stored != 0.0f) stored += o.stored * f;
-        if (o.p != 0.0f) pu += o.pu + o.p * d;
-    }
-    const float total = others + stored, l2 = total == 0.0f ? 0.0f : log2f(total);     // 0: every logit is -inf, and so is q's log
-    const float left = REST ? fmaxf(0.0f, 1.0f - s[1]) : 0.0f, inv = REST ? 1.0f : 1.0f / s[1];
-    const float by = w * a.by;
-    T *g = GRAD ? (T *)a.grad + t * a.ldg : nullptr;
-    if (GRAD) {
-        const float of = counts ? (left > 0.0f && others > 0.0f ? by * (1.0f - left * (total / others)) : by) : 0.0f;
-        const bool whole = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
-        uint4 *to = (uint4 *)((uintptr_t)g & ~(uintptr_t)15) + first;
-        if (whole) {
+        float2 s2 = make_float2(0.0f, 0.0f);
+        if (u.near) {
+#pragma unroll 4
             for (int i = tid; i < n; i += DT) {
-                Granule<T> o;
-                float v[N];
-                if (counts) {
-                    ((const Granule<T> *)(part + i))->unpack(v);
+                float2 v[N / 2];
+                part[i].unpack(v);
 #pragma unroll
-                    for (int k = 0; k < N; k++) v[k] = of * exp2_fast(fmaf(v[k] - top, a.c, -l2));
-                } else {
-#pragma unroll
-                    for (int k = 0; k < N; k++) v[k] = 0.0f;
+                for (int k = 0; k < N / 2; k++) {
+                    v[k] = u.of(v[k]);
+                    v[k] = make_float2(exp2_fast(v[k].x), exp2_fast(v[k].y));
                 }
-                const int col = col0 + i * N;
-                if (col >= 0 && col + N <= a.ncols) {
-                    o.pack(v);
-                    to[i] = o.w;
-                } else {
+                if (REST) {
+                    const unsigned skip = N == 8 ? ((const uint8_t *)bits)[i] : ((const uint8_t *)bits)[i >> 1] >> ((i & 1) * 4) & 15;
+                    if (skip)
 #pragma unroll
-                    for (int k = 0; k < N; k++)
-                        if (col + k >= 0 && col + k < a.ncols) g[col + k] = from_float<T>(v[k]);
+                        for (int k = 0; k < N / 2; k++) {
+                            if (skip >> (2 * k) & 1) v[k].x = 0.0f;
+                            if (skip >> (2 * k + 1) & 1) v[k].y = 0.0f;
+                        }
                 }
+#pragma unroll
+                for (int k = 0; k < N / 2; k++) s2 = add2(s2, v[k]);
             }
         } else {
             for (int i = tid; i < n * N; i += DT)
-                if (col0 + i >= 0 && col0 + i < a.ncols)
-                    g[col0 + i] = from_float<T>(counts ? of * exp2_fast(fmaf(to_float(elem[i]) - top, a.c, -l2)) : 0.0f);
+                if (!REST || !(bits[i >> 5] >> (i & 31) & 1)) s2.x += exp2_fast(u.of(to_float(elem[i])));
+        }
+        s2.x = warp_sum(s2.x + s2.y);
+        // of the entries: p's weights, times their log2; in this part: weights, times (x - m) c, and stored columns' 2^((x - m) c)
+        float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        const float zref = REST ? a.lse[t] * LOG2E : zm;
+        auto log_p = [&](int64_t e) { return REST ? fmaf((float)z[e], a.c, -zref) : ((float)z[e] - zref) * a.c; };
+        if (entries) {
+            for (int64_t e = lo + tid; e < hi; e += DT) {
+                const int64_t col = a.crd[e], j = col - col0;
+                const float lp = log_p(e), p = exp2_fast(lp);
+                s[0] += p;
+                if (!(p <= 0.0f)) s[1] += p * lp;
+                if (col < 0 || col >= a.ncols) {
+                    s[1] = __int_as_float(0x7fffffff);
+                } else if (j >= 0 && j < (int64_t)n * N) {
+                    const float v = u.of(to_float(elem[j]));
+                    s[2] += p;
+                    if (!(p <= 0.0f)) s[3] += p * v;
+                    if (REST && (e == lo || a.crd[e - 1] != col)) s[4] += exp2_fast(v);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 5; i++) s[i] = warp_sum(s[i]);
+        }
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < 5; i++) sums[i][warp] = s[i];
+            sums[5][warp] = s2.x;
         }
         __syncthreads();
-        if (counts) {
-            const float zref = REST ? a.lse[t] * LOG2E : m[1];
+        if (ranks > 1) cluster_wait();             // the others are there
+        if (warp == 0 && lane < (int)ranks) {
+            const float others = sum_of(sums[5]), stored = sum_of(sums[4]), p = sum_of(sums[2]), pu = sum_of(sums[3]);
+            if (ranks > 1) {
+                Told *to = &told[rank];
+                store_peer(&to->m, lane, m);
+                store_peer(&to->others, lane, others);
+                store_peer(&to->stored, lane, stored);
+                store_peer(&to->p, lane, p);
+                store_peer(&to->pu, lane, pu);
+            } else {
+                told[0] = {m, others, stored, p, pu};
+            }
+        }
+        if (ranks > 1) {
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+        } else {
+            __syncthreads();
+        }
+        if (!GRAD && (rank != 0 || warp != 0)) return;
+        // the row's: a lane per CTA
+        const Told &o = told[lane & (MOST_CLUSTER - 1)];
+        const bool there = (lane & (MOST_CLUSTER - 1)) < (int)ranks;
+        const Exponent top(warp_max(there ? o.m : MINUS_INF), a.c);
+        const float d = there ? Exponent(o.m, a.c).to(top) : 0.0f, f = exp2_fast(d);
+        float others = there && o.others != 0.0f ? o.others * f : 0.0f, stored = there && o.stored != 0.0f ? o.stored * f : 0.0f;
+        float pu = there && o.p != 0.0f ? o.pu + o.p * d : 0.0f;
+#pragma unroll
+        for (int i = 1; i < MOST_CLUSTER; i *= 2) {
+            others += __shfl_xor_sync(0xffffffffu, others, i);
+            stored += __shfl_xor_sync(0xffffffffu, stored, i);
+            pu += __shfl_xor_sync(0xffffffffu, pu, i);
+        }
+        const float total = REST ? others + stored : others, p = sum_of(sums[0]);
+        const float left = REST ? fmaxf(0.0f, 1.0f - p) : 0.0f;
+        if (GRAD) {
+            const float by = w * a.by, part_of = total == 0.0f ? 0.0f : by / total;     // total 0: every logit is -inf
+            const float of = left > 0.0f && others > 0.0f ? part_of * (1.0f - left * (total / others)) : part_of;
+            const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+            if (alike && top.near) {
+                uint4 *to = (uint4 *)((uintptr_t)g & ~(uintptr_t)15) + first;
+#pragma unroll 4
+                for (int i = tid; i < n; i += DT) {
+                    float2 v[N / 2];
+                    part[i].unpack(v);
+#pragma unroll
+                    for (int k = 0; k < N / 2; k++) {
+                        v[k] = top.of(v[k]);
+                        v[k] = mul2(make_float2(exp2_fast(v[k].x), exp2_fast(v[k].y)), make_float2(of, of));
+                    }
+                    Granule<T> out;
+                    out.pack(v);
+                    const int col = col0 + i * N;
+                    if (col >= 0 && col + N <= a.ncols) {
+                        to[i] = out.w;
+                    } else {
+                        for (int k = 0; k < N; k++)
+                            if (col + k >= 0 && col + k < a.ncols) g[col + k] = ((const T *)&out)[k];
+                    }
+                }
+            } else {
+                for (int i = tid; i < n * N; i += DT)
+                    if (col0 + i >= 0 && col0 + i < a.ncols) g[col0 + i] = from_float<T>(of * exp2_fast(top.of(to_float(elem[i]))));
+            }
+            __syncthreads();
+            const float inv = REST ? 1.0f : 1.0f / p;
             for (int64_t e = lo + tid; e < hi; e += DT) {
                 const int64_t col = a.crd[e], j = col - col0;
                 if (j < 0 || j >= (int64_t)n * N || col < 0 || col >= a.ncols || (e > lo && a.crd[e - 1] == col)) continue;
-                float p = 0.0f;                    // repeated columns are next to each other: their sum
-                for (int64_t f = e; f < hi && a.crd[f] == col; f++)
-                    p += exp2_fast(REST ? fmaf((float)z[f], a.c, -zref) : ((float)z[f] - zref) * a.c);
-                g[col] = from_float<T>(by * (exp2_fast(fmaf(to_float(elem[j]) - top, a.c, -l2)) - p * inv));
+                float pj = 0.0f;                   // repeated columns are next to each other: their sum
+                for (int64_t i = e; i < hi && a.crd[i] == col; i++) pj += exp2_fast(log_p(i));
+                g[col] = from_float<T>(part_of * exp2_fast(top.of(to_float(elem[j]))) - by * (pj * inv));
             }
+            if (rank != 0 || warp != 0) return;
+        }
+        const float l2 = total == 0.0f ? 0.0f : log2f(total), plogp = sum_of(sums[1]);
+        if (lane == 0) {
+            const float loss = REST ? plogp - pu + p * l2 + (left > 0.0f ? left * (log2f(left) - log2f(others) + l2) : 0.0f)
+                                    : (plogp - pu) / p - log2f(p) + l2;
+            a.rows[t] = loss * LN2;
         }
     }
-    if (rank != 0) return;
-    if (tid == 0) {
-        float loss = 0.0f;
-        if (counts) {
-            if (REST)
-                loss = s[2] - pu + s[1] * l2 + (left > 0.0f ? left * (log2f(left) - log2f(others) + l2) : 0.0f);
-            else
-                loss = (s[2] - pu) * inv - log2f(s[1]) + l2;
-        }
-        a.rows[t] = loss * LN2;
-        last = last_of(a.counter, (unsigned)a.nrows);
-    }
-    __syncthreads();
-    if (!last) return;
+    if (!a.counter) return;
+    unsigned last = 0;
+    if (lane == 0) last = last_of(a.counter, (unsigned)a.nrows);
+    if (!__shfl_sync(0xffffffffu, last, 0)) return;
     __threadfence();
-    __shared__ double sums[DW];
-    double sum = 0.0;
-    for (int64_t r = tid; r < a.nrows; r += DT) {
-        const float wr = a.weight ? a.weight[r] : 1.0f;
-        if (wr != 0.0f) sum += (double)wr * __ldcg(a.rows + r);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((tid & 31) == 0) sums[tid >> 5] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < DW; i++) sum += sums[i];
-        *a.loss = (float)(sum * a.scale);
-    }
+    add_rows<32>(a, nullptr);
 }
 
 template <typename T, typename TV, bool REST, bool GRAD>
@@ -225,11 +335,15 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     constexpr int N = Granule<T>::N;
     const int all = (a.ncols + 2 * N - 2) / N;     // granules of a row, wherever it starts
     int ranks = 1;
-    while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > 32 * 1024 || (a.nrows * ranks < sm_count() * 2 && all / ranks >= 512))) ranks *= 2;
+    while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > SLICE || (a.nrows * ranks < sm_count() && all / ranks >= 2 * DT))) ranks *= 2;
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
     const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);
-    return launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a);
+    const bool few = a.nrows <= 256;               // the last row's warp adds them up
+    if (!few) a.counter = nullptr;
+    CB_TRY(launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a));
+    if (!few) CB_CUDA(launch_behind(distill_sum_kernel, dim3(1), 1024, 0, st, a));
+    return 0;
 }
 
 template <typename T, typename TV>

@@ -89,6 +89,10 @@ struct Granule<float> {
         v[2] = __uint_as_float(w.z);
         v[3] = __uint_as_float(w.w);
     }
+    __device__ __forceinline__ void pack(const float2 (&v)[2])
+    {
+        w = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+    }
     __device__ __forceinline__ void pack(const float (&v)[4])
     {
         w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
@@ -127,6 +131,16 @@ struct Granule<__nv_bfloat16> {
             v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
     }
+    __device__ __forceinline__ void pack(const float2 (&v)[4])
+    {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v[i].x, v[i].y);
+            u[i] = *(const uint32_t *)&p;
+        }
+        w = make_uint4(u[0], u[1], u[2], u[3]);
+    }
     __device__ __forceinline__ void pack(const float (&v)[8])
     {
         uint32_t u[4];
@@ -163,6 +177,16 @@ struct Granule<__half> {
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
         }
+    }
+    __device__ __forceinline__ void pack(const float2 (&v)[4])
+    {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 p = __floats2half2_rn(v[i].x, v[i].y);
+            u[i] = *(const uint32_t *)&p;
+        }
+        w = make_uint4(u[0], u[1], u[2], u[3]);
     }
     __device__ __forceinline__ void pack(const float (&v)[8])
     {
@@ -204,9 +228,9 @@ __device__ __forceinline__ float warp_sum(float v)
 }
 __device__ __forceinline__ float warp_max(float v)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
 // N values per thread to their sums (or maxima) over the CTA, in every thread.  `room` holds N * WARPS floats and is free

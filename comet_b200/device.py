@@ -159,6 +159,8 @@ def masked_pair_count(A, B, M, row_lo=0, row_hi=None, out=None):
 # Rows of logits beside a CSR matrix.  The logits are CUDA matrices with unit column stride, in bf16, f16 or f32; the
 # results are new tensors, and every call is asynchronous on the current stream.
 _LOGITS = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_TOP, _DISTILL, _BALANCE = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _LOGITS.items()}
+                            for op in ("top_entries", "distill_loss", "balance_loss"))
 _numbers = {}
 
 
@@ -174,58 +176,63 @@ def _floats(*v):
 
 
 def _check_logits(what, X):
-    if not (isinstance(X, torch.Tensor) and X.is_cuda and X.dim() == 2 and (X.stride(1) == 1 or X.shape[1] == 1) and X.dtype in _LOGITS):
-        raise ValueError(what + ": the logits must be a CUDA matrix of bfloat16, float16 or float32 with unit column stride")
+    """(rows, columns, row stride) of a matrix of logits.  The checks are few: they are most of a small call's time on the host."""
+    if not (isinstance(X, torch.Tensor) and X.is_cuda and X.dtype in _LOGITS):
+        raise ValueError(what + ": the logits must be a CUDA matrix of bfloat16, float16 or float32")
+    shape, stride = X.shape, X.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] != 1):
+        raise ValueError(what + ": the logits must be a matrix with unit column stride")
     if X.get_device() != torch._C._cuda_getDevice():
         raise ValueError(what + ": the logits must be on the current device")
-    if X.shape[1] < 1:
+    n, m = shape
+    if m < 1:
         raise ValueError(what + ": the logits have no columns")
-    ld = X.stride(0) if X.shape[0] > 1 else X.shape[1]
-    if ld < X.shape[1]:
+    ld = stride[0] if n > 1 else m
+    if ld < m:
         raise ValueError(what + ": rows of the logits must not overlap")
-    return ld
+    return n, m, ld
 
 
-def _check_beside(what, S, X):
-    """S: a CSR matrix of X's shape with int64 indices."""
+def _check_vector(what, v, dtype, n):
+    if v.dtype is not dtype or v.shape != (n,) or not v.is_contiguous() or v.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("%s: expected %d contiguous values of %s on the logits' device" % (what, n, dtype))
+    return v.data_ptr()
+
+
+def _check_beside(what, S, n, m):
+    """Addresses of pos and crd of a CSR matrix of the logits' shape, with int64 indices."""
     if S.row_ids is not None:
         raise ValueError(what + ": the sparse operand must be CSR (a row that stores nothing is empty there)")
-    if (S.nrows, S.ncols) != tuple(X.shape) or S.pos.shape[0] != S.nrows + 1:
+    if S.nrows != n or S.ncols != m:
         raise ValueError(what + ": the sparse operand and the logits must have the same shape")
-    _check_like(what, X, S.pos, torch.int64, S.nrows + 1)
-    _check_like(what, X, S.crd, torch.int64, S.nnz)
+    return _check_vector(what, S.pos, torch.int64, n + 1), _check_vector(what, S.crd, torch.int64, S.nnz)
 
 
-def _check_like(what, X, v, dtype, n):
-    if not (v.dtype == dtype and v.dim() == 1 and v.shape[0] == n and v.device == X.device and v.is_contiguous()):
-        raise ValueError("%s: expected %d contiguous values of %s on the logits' device" % (what, n, dtype))
-
-
-def _gradient(what, X, ld, grad):
-    """(gradient, its row stride): new, none, or the caller's (the logits themselves, say)."""
-    if grad is None or grad is False:
-        return None, 0
+def _gradient(what, X, shape, grad):
+    """(gradient, its address, its row stride): new, none, or the caller's (the logits themselves, say)."""
     if grad is True:
-        return torch.empty(X.shape, dtype=X.dtype, device=X.device), X.shape[1]
-    if grad.dtype != X.dtype or grad.shape != X.shape or grad.device != X.device:
+        grad = X.new_empty(shape)
+        return grad, grad.data_ptr(), shape[1]
+    if grad is None or grad is False:
+        return None, 0, 0
+    if grad.dtype is not X.dtype or grad.shape != shape:
         raise ValueError(what + ": the gradient must have the logits' shape, type and device")
-    return grad, _check_logits(what, grad)
+    return grad, grad.data_ptr(), _check_logits(what, grad)[2]
 
 
 def top_entries(X, k, temperature=1.0, lse=False):
     """The k largest entries of each row of X (1 <= k <= 1024) as a DeviceCSR with float32 values, columns ascending; of equal entries the lower
     column, NaN above all numbers.  Returns (matrix, the log of the sum of each row's exp(X / temperature), or None)."""
-    ld = _check_logits("top_entries", X)
-    n, k = X.shape[0], int(k)
-    if not 1 <= k <= min(1024, X.shape[1]):
+    n, m, ld = _check_logits("top_entries", X)
+    k = int(k)
+    if not 1 <= k <= min(1024, m):
         raise ValueError("top_entries: k must be between 1 and 1024, and at most the number of columns")
     new = X.new_empty
     pos, crd, val = new(n + 1, dtype=torch.int64), new(n * k, dtype=torch.int64), new(n * k, dtype=torch.float32)
     sums = new(n, dtype=torch.float32) if lse else None
     options = _floats(float(temperature))
-    _call("comet_b200_dev_top_entries_%s_i64" % _LOGITS[X.dtype], n, X.shape[1], X.data_ptr(), ld, k, options[0], pos.data_ptr(), crd.data_ptr(),
-          val.data_ptr(), _p(sums), _stream())
-    return DeviceCSR(n, X.shape[1], pos, crd, val), sums
+    _call(_TOP[X.dtype], n, m, X.data_ptr(), ld, k, options[0], pos.data_ptr(), crd.data_ptr(), val.data_ptr(), _p(sums), _stream())
+    return DeviceCSR(n, m, pos, crd, val), sums
 
 
 def distill_loss(S, X, temperature=1.0, lse=None, weight=None, scale=1.0, grad=True):
@@ -236,21 +243,16 @@ def distill_loss(S, X, temperature=1.0, lse=None, weight=None, scale=1.0, grad=T
     left out.  One entry in each row: the cross entropy with that column.
 
     Returns (scale * sum of weight * rows, rows, its gradient).  grad: True (a new tensor), False (none), or a tensor to write it to, such as X."""
-    ld = _check_logits("distill_loss", X)
-    _check_beside("distill_loss", S, X)
-    n = S.nrows
-    if S.val.dtype not in (torch.float32, torch.float64):
-        raise ValueError("distill_loss: the teacher's values must be float32 or float64")
-    _check_like("distill_loss", X, S.val, S.val.dtype, S.nnz)
-    if lse is not None:
-        _check_like("distill_loss", X, lse, torch.float32, n)
-    if weight is not None:
-        _check_like("distill_loss", X, weight, torch.float32, n)
-    out, ldg = _gradient("distill_loss", X, ld, grad)
+    n, m, ld = shape = _check_logits("distill_loss", X)
+    pos, crd = _check_beside("distill_loss", S, n, m)
+    width = 4 if S.val.dtype is torch.float32 else 8
+    val = _check_vector("distill_loss", S.val, torch.float32 if width == 4 else torch.float64, S.nnz)
+    sums = 0 if lse is None else _check_vector("distill_loss", lse, torch.float32, n)
+    weights = 0 if weight is None else _check_vector("distill_loss", weight, torch.float32, n)
+    out, to, ldg = _gradient("distill_loss", X, shape[:2], grad)
     rows, loss = X.new_empty(n, dtype=torch.float32), X.new_empty((), dtype=torch.float32)
     options = _floats(float(temperature), float(scale))
-    _call("comet_b200_dev_distill_loss_%s_i64" % _LOGITS[X.dtype], n, S.ncols, S.pos.data_ptr(), S.crd.data_ptr(), S.val.data_ptr(),
-          S.val.element_size(), _p(lse), _p(weight), X.data_ptr(), ld, _p(out), ldg, options[0], rows.data_ptr(), loss.data_ptr(), _stream())
+    _call(_DISTILL[X.dtype], n, m, pos, crd, val, width, sums, weights, X.data_ptr(), ld, to, ldg, options[0], rows.data_ptr(), loss.data_ptr(), _stream())
     return loss, rows, out
 
 
@@ -261,23 +263,22 @@ def balance_loss(S, R, seq=None, mask=None, scores="softmax", scale=1.0, grad=Tr
     P_e the mean over its rows of p_e, with p = softmax(R) or, for scores="sigmoid", sigmoid(R) over the row's sum.
 
     Returns (loss, counts[sequences, E] as int64, gradient with respect to R).  grad: True (a new tensor), False (none), or a tensor to write it to."""
-    ld = _check_logits("balance_loss", R)
-    _check_beside("balance_loss", S, R)
+    n, m, ld = shape = _check_logits("balance_loss", R)
+    pos, crd = _check_beside("balance_loss", S, n, m)
     if scores not in ("softmax", "sigmoid"):
         raise ValueError("balance_loss: scores must be 'softmax' or 'sigmoid'")
-    if S.ncols > 1024:
+    if m > 1024:
         raise ValueError("balance_loss: at most 1024 experts")
-    nseq = 1
+    nseq, bounds = 1, 0
     if seq is not None:
-        if seq.dim() != 1 or seq.shape[0] < 2:
+        nseq = seq.numel() - 1
+        if nseq < 1:
             raise ValueError("balance_loss: seq holds the bounds of one sequence or more")
-        nseq = seq.shape[0] - 1
-        _check_like("balance_loss", R, seq, torch.int64, nseq + 1)
-    if mask is not None:
-        _check_like("balance_loss", R, mask, torch.bool, S.nrows)
-    out, ldg = _gradient("balance_loss", R, ld, grad)
-    counts, loss = R.new_empty((nseq, S.ncols), dtype=torch.int64), R.new_empty((), dtype=torch.float32)
+        bounds = _check_vector("balance_loss", seq, torch.int64, nseq + 1)
+    on = 0 if mask is None else _check_vector("balance_loss", mask, torch.bool, n)
+    out, to, ldg = _gradient("balance_loss", R, shape[:2], grad)
+    counts, loss = R.new_empty((nseq, m), dtype=torch.int64), R.new_empty((), dtype=torch.float32)
     options = _floats(float(scale))
-    _call("comet_b200_dev_balance_loss_%s_i64" % _LOGITS[R.dtype], S.nrows, S.ncols, S.pos.data_ptr(), S.crd.data_ptr(), nseq, _p(seq), _p(mask),
-          int(scores == "sigmoid"), R.data_ptr(), ld, _p(out), ldg, options[0], counts.data_ptr(), loss.data_ptr(), _stream())
+    _call(_BALANCE[R.dtype], n, m, pos, crd, nseq, bounds, on, int(scores == "sigmoid"), R.data_ptr(), ld, to, ldg, options[0], counts.data_ptr(),
+          loss.data_ptr(), _stream())
     return loss, counts, out
