@@ -11,7 +11,8 @@
 // a row have to tell each other are five floats, written into each other's shared memory.
 //
 // Bound: HBM, the bytes of X and of the gradient.
-#include "distill.cuh"
+#include "logits.cuh"
+#include "stream.cuh"
 
 namespace cb200 {
 
@@ -19,10 +20,40 @@ static const int DT = 256, DW = DT / 32;
 static const int SLICE = 64 * 1024;                // bytes of a row that a CTA gets if the cluster is not larger for it
 static const int MOST_SLICE = 192 * 1024;          // and at most
 
+struct DistillArgs {
+    int64_t nrows;
+    int ncols, slice;            // granules per CTA
+    const int64_t *pos, *crd;
+    const void *val;
+    const float *lse, *weight;
+    const void *x;
+    int64_t ldx;
+    void *grad;
+    int64_t ldg;
+    float c, by, scale;          // log2(e) / temperature, scale / temperature
+    float *rows, *loss;
+    unsigned *counter;           // null: another kernel adds the rows up
+};
+
 // what a CTA tells the others of its row: the maximum of its part, sums of 2^((x - maximum) c) of elements that are not
 // stored and of those that are, of p's weights and of p's weights times (x - maximum) c
 struct Told {
     float m, others, stored, p, pu;
+};
+
+// (x - m) c.  As x c - m c it is one operation, and the rounding of m c is a factor that all of a row's terms and their sum
+// have alike; m c may be beyond f32 where the difference is not.
+struct Exponent {
+    float c, m, mc;
+    bool near;
+    __device__ __forceinline__ Exponent(float most, float c_) : c(c_), m(most == MINUS_INF ? 0.0f : most)
+    {
+        mc = m * c;
+        near = fabsf(mc) < 1e30f;
+    }
+    __device__ __forceinline__ float of(float x) const { return near ? fmaf(x, c, -mc) : (x - m) * c; }
+    __device__ __forceinline__ float2 of(float2 x) const { return fma2(x, make_float2(c, c), make_float2(-mc, -mc)); }      // near
+    __device__ __forceinline__ float to(const Exponent &o) const { return near && o.near ? mc - o.mc : (m - o.m) * c; }
 };
 
 template <int N>
@@ -32,6 +63,34 @@ __device__ __forceinline__ float sum_of(const float (&v)[N])
 #pragma unroll
     for (int i = 1; i < N; i++) s += v[i];
     return s;
+}
+
+// scale * the sum of weight * rows, by one warp or more, in a fixed order; the result in thread 0
+template <int THREADS>
+__device__ __forceinline__ void add_rows(const DistillArgs &a, double *room)
+{
+    double sum = 0.0;
+    for (int64_t r = threadIdx.x; r < a.nrows; r += THREADS) {
+        const float w = a.weight ? a.weight[r] : 1.0f;
+        if (w != 0.0f) sum += (double)w * __ldcg(a.rows + r);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (THREADS > 32) {
+        if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 1; i < THREADS / 32; i++) sum += room[i];
+    }
+    if (threadIdx.x == 0) *a.loss = (float)(sum * a.scale);
+}
+
+__global__ void __launch_bounds__(1024)
+distill_sum_kernel(const DistillArgs a)
+{
+    __shared__ double room[32];
+    wait_for_previous();
+    add_rows<1024>(a, room);
 }
 
 template <typename T, typename TV, bool REST, bool GRAD>
@@ -280,7 +339,11 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
     const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);
-    return launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a);
+    const bool few = a.nrows <= 256;               // the last row's warp adds them up
+    if (!few) a.counter = nullptr;
+    CB_TRY(launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a));
+    if (!few) CB_CUDA(launch_behind(distill_sum_kernel, dim3(1), 1024, 0, st, a));
+    return 0;
 }
 
 template <typename T, typename TV>
@@ -302,7 +365,9 @@ static int distill_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
     if (ldx < ncols || (grad && ldg < ncols)) return fail("distill_loss: leading dimension smaller than the number of columns");
     if (!(temperature > 0.0) || temperature > 1e30) return fail("distill_loss: temperature %g is not a positive number", temperature);
     if (val_bytes != 4 && val_bytes != 8) return fail("distill_loss: the teacher's values have 4 or 8 bytes");
-    if (ncols > 1 << 20) return fail("distill_loss: %lld columns; at most 2^20", (long long)ncols);
+    if (ncols > (int64_t)MOST_CLUSTER * MOST_SLICE / (int64_t)sizeof(T) - 64)
+        return fail("distill_loss: rows of %lld columns do not fit the shared memory of eight SMs", (long long)ncols);
+    if (nrows > 0x7fffffffLL / MOST_CLUSTER) return fail("distill_loss: more than 2^28 rows");
     if ((uintptr_t)x % sizeof(T) || (uintptr_t)grad % sizeof(T)) return fail("distill_loss: an address that is not a multiple of the element's size");
     if (nrows == 0) {
         CB_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
@@ -311,8 +376,6 @@ static int distill_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
     DistillArgs a = {nrows, (int)ncols, 0, pos, crd, val, lse, weight, x, ldx, grad, ldg, (float)((double)LOG2E_D / temperature),
                      (float)(scale / temperature), (float)scale, rows, loss, next_counter()};
     if (!a.counter) return 1;
-    // A CTA per row from half as many rows as SMs; fewer rows are spread over clusters, if eight SMs can hold them.
-    if (nrows * 2 > sm_count() || ncols * (int64_t)sizeof(T) > (int64_t)MOST_CLUSTER * MOST_SLICE - 64) return distill_by_rows<T>(a, val_bytes, st);
     return val_bytes == 4 ? launch_distill<T, float>(a, st) : launch_distill<T, double>(a, st);
 }
 

@@ -66,7 +66,6 @@ template <>
 struct Granule<float> {
     static constexpr int N = 4;
     uint4 w;
-    static __device__ __forceinline__ Granule least() { return {make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[2]) const
     {
         v[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
@@ -111,7 +110,6 @@ template <>
 struct Granule<__nv_bfloat16> {
     static constexpr int N = 8;
     uint4 w;
-    static __device__ __forceinline__ Granule least() { return {make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[4]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -158,7 +156,6 @@ template <>
 struct Granule<__half> {
     static constexpr int N = 8;
     uint4 w;
-    static __device__ __forceinline__ Granule least() { return {make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[4]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
