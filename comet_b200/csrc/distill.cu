@@ -16,8 +16,8 @@
 
 namespace cb200 {
 
-static const int DT = 256, DW = DT / 32;
-static const int SLICE = 64 * 1024;                // bytes of a row that a CTA gets if the cluster is not larger for it
+static const int DT = 128, DW = DT / 32;
+static const int SLICE = 48 * 1024;                // bytes of a row that a CTA gets if eight of them can take the row at that
 static const int MOST_SLICE = 192 * 1024;          // and at most
 
 struct DistillArgs {
@@ -335,7 +335,7 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     constexpr int N = Granule<T>::N;
     const int all = (a.ncols + 2 * N - 2) / N;     // granules of a row, wherever it starts
     int ranks = 1;
-    while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > SLICE || (a.nrows * ranks < sm_count() && all / ranks >= 2 * DT))) ranks *= 2;
+    while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > SLICE + 64 || (a.nrows * ranks < sm_count() && all / ranks >= 2 * DT))) ranks *= 2;
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
     const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);

@@ -121,7 +121,9 @@ def check_distill(S, pos, crd, val, x, x64, kind, tau=1.0, lse=None, weight=None
     return grad
 
 
-SHAPES = [(1, 1, 1), (1, 2, 1), (2, 7, 3), (3, 17, 4), (40, 33, 5), (7, 1000, 8), (5, 4099, 33), (300, 1025, 6), (2, 50021, 64), (3, 131072, 16), (1, 20000, 700)]
+SHAPES = [(1, 1, 1), (1, 2, 1), (2, 7, 3), (3, 17, 4), (40, 33, 5), (7, 1000, 8), (5, 4099, 33), (300, 1025, 6), (2, 50021, 64), (3, 131072, 16), (1, 20000, 700),
+          # many rows, and rows of several CTAs; more entries than a CTA has threads; the longest rows
+          (1300, 9, 4), (700, 700, 700), (600, 4096, 9), (200, 24001, 200), (160, 60007, 300), (90, 140001, 64), (1, 390000, 8)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
