@@ -110,8 +110,16 @@ __device__ __forceinline__ void count_rows(const BalanceArgs &a, int64_t r0, int
     }
 }
 
-// Rows [r0, r1) of a warp, G lanes and Q times 16 bytes a lane each.  Returns the lane's part of the loss.
-template <typename T, int G, int Q, bool SIGMOID>
+// A row as a lane has it ahead of time.
+template <int Q>
+struct NextRow {
+    uint4 x[Q];
+    bool active;
+};
+
+// Rows [r0, r1) of a warp, G lanes and Q times 16 bytes a lane each; the next rows are on their way while these are computed.  WHOLE: every granule is
+// 16 aligned bytes of one row.  Returns the lane's part of the loss.
+template <typename T, int G, int Q, bool SIGMOID, bool WHOLE>
 __device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &tally, int64_t r0, int64_t r1)
 {
     constexpr int N = Granule<T>::N, AT_ONCE = 32 / G;
@@ -120,25 +128,48 @@ __device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &t
     int64_t s_end = -1;                            // the row at which the lane's sequence ends
     float g[Q * N], by = 0.0f;
     double sum = 0.0;
+    auto has = [&](int q, int e) { return (q * G + l) * N + e < a.ncols; };
+    auto fetch = [&](int64_t t) {
+        NextRow<Q> n;
+        n.active = false;
+        if (t < r1) {
+            const T *r = (const T *)a.r + t * a.ldr;
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                if (WHOLE) {
+                    if (has(q, 0)) n.x[q] = __ldg((const uint4 *)r + q * G + l);
+                } else {
+                    T *v = (T *)&n.x[q];
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[e] = has(q, e) ? r[(q * G + l) * N + e] : from_float<T>(MINUS_INF);
+                }
+            }
+            n.active = a.pos[t] < a.pos[t + 1] && (!a.mask || a.mask[t]);
+        }
+        return n;
+    };
+    NextRow<Q> next = fetch(r0 + lane / G);
     for (int64_t b = r0; b < r1; b += AT_ONCE) {
         const int64_t t = b + lane / G;
         const bool there = t < r1;
-        const T *r = (const T *)a.r + t * a.ldr;
-        Granule<T> x[Q];
-        if (there) {
-            if (a.whole) {
+        const NextRow<Q> now = next;
+        next = fetch(t + AT_ONCE);
+        const bool active = now.active;
+        T *grad = a.grad ? (T *)a.grad + t * a.ldg : nullptr;
+        if (!__any_sync(0xffffffffu, active)) {    // nothing but zeros
+            if (grad && there)
 #pragma unroll
-                for (int q = 0; q < Q; q++)
-                    if ((q * G + l) * N < a.ncols) x[q].w = __ldg((const uint4 *)r + q * G + l);
-            } else {
+                for (int q = 0; q < Q; q++) {
+                    if (WHOLE) {
+                        if (has(q, 0)) ((uint4 *)grad)[q * G + l] = make_uint4(0, 0, 0, 0);
+                    } else {
 #pragma unroll
-                for (int q = 0; q < Q; q++)
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if ((q * G + l) * N + e < a.ncols) ((T *)&x[q].w)[e] = r[(q * G + l) * N + e];
-            }
+                        for (int e = 0; e < N; e++)
+                            if (has(q, e)) grad[(q * G + l) * N + e] = from_float<T>(0.0f);
+                    }
+                }
+            continue;
         }
-        const bool active = there && a.pos[t] < a.pos[t + 1] && (!a.mask || a.mask[t]);
         if (there && t >= s_end) {
             int64_t s = 0;
             s_end = a.nrows;
@@ -152,19 +183,23 @@ __device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &t
 #pragma unroll
             for (int q = 0; q < Q; q++)
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int col = (q * G + l) * N + e;
-                    g[q * N + e] = col < a.ncols ? (float)((int64_t)tally.counts[s * a.ncols + col] * a.ncols - entries) * unit : 0.0f;
-                }
+                for (int e = 0; e < N; e++)
+                    g[q * N + e] = has(q, e) ? (float)((int64_t)tally.counts[s * a.ncols + (q * G + l) * N + e] * a.ncols - entries) * unit : 0.0f;
         }
         float v[Q * N], slope[SIGMOID ? Q * N : 1];
+        // the lane's logits; -inf where there is no column
+        auto logits = [&](float (&u)[Q * N]) {
 #pragma unroll
-        for (int q = 0; q < Q; q++) {
-            float u[N];
-            x[q].unpack(u);
+            for (int q = 0; q < Q; q++) {
+                Granule<T> x;
+                x.w = now.x[q];
+                if (WHOLE && !has(q, 0)) x = Granule<T>::least();
+                float each[N];
+                x.unpack(each);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[q * N + e] = active && (q * G + l) * N + e < a.ncols ? u[e] : MINUS_INF;
-        }
+                for (int e = 0; e < N; e++) u[q * N + e] = each[e];
+            }
+        };
         float p = 0.0f, gp = 0.0f;
         auto add_up = [&]() {
             p = gp = 0.0f;
@@ -179,63 +214,66 @@ __device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &t
                 gp += __shfl_xor_sync(0xffffffffu, gp, o);
             }
         };
-        auto maximum = [&]() {
-            float m = v[0];
+        auto maximum = [&](const float (&u)[Q * N]) {
+            float m = u[0];
 #pragma unroll
-            for (int i = 1; i < Q * N; i++) m = max_nan(m, v[i]);
+            for (int i = 1; i < Q * N; i++) m = max_nan(m, u[i]);
+            if (G == 32) m = warp_max(m);
+            else
 #pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                for (int o = G / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
             return m == MINUS_INF ? 0.0f : m;      // exp(-inf - 0) = 0: a row of -inf has no scores
         };
+        logits(v);
         if (SIGMOID) {
-            float low[Q * N];
 #pragma unroll
             for (int i = 0; i < Q * N; i++) {
-                low[i] = v[i];
-                float d = exp2_fast(v[i] * -LOG2E);
-                d = d > 1e38f ? 1e38f : d;
-                v[i] = __fdividef(1.0f, 1.0f + d);
+                const float d = min_nan(exp2_fast(v[i] * -LOG2E), 1e38f);
+                v[i] = reciprocal(1.0f + d);
                 slope[i] = d * v[i];
             }
             add_up();
-            if (__any_sync(0xffffffffu, active && p < 1e-30f)) {         // sigmoids below f32's range, or none: their shares by e^(r - max) / (1 + e^r)
-#pragma unroll
-                for (int i = 0; i < Q * N; i++) v[i] = low[i];
-                const float m = fminf(maximum(), 0.0f);
+            if (__any_sync(0xffffffffu, active && p < 1e-30f)) {               // sigmoids below f32's range, or none: their shares by e^(r - max) / (1 + e^r)
+                float low[Q * N];
+                logits(low);
+                const float m = fminf(maximum(low), 0.0f);
 #pragma unroll
                 for (int i = 0; i < Q * N; i++) {
-                    const float d = exp2_fast(low[i] * LOG2E);
-                    slope[i] = __fdividef(1.0f, 1.0f + (d > 1e38f ? 1e38f : d));
+                    slope[i] = reciprocal(1.0f + min_nan(exp2_fast(low[i] * LOG2E), 1e38f));
                     v[i] = low[i] > 60.0f ? exp2_fast(-m * LOG2E) : exp2_fast((low[i] - m) * LOG2E) * slope[i];
                 }
                 add_up();
             }
         } else {
-            const float m = maximum();
+            const float m = maximum(v);
 #pragma unroll
             for (int i = 0; i < Q * N; i++) v[i] = exp2_fast((v[i] - m) * LOG2E);
             add_up();
         }
-        const float inv = p == 0.0f ? 0.0f : 1.0f / p;
+        const float inv = p == 0.0f ? 0.0f : reciprocal(p);
         gp *= inv;
         if (l == 0 && active && p != 0.0f) sum += (double)(by * (share + gp));
-        if (a.grad && there) {
-            T *grad = (T *)a.grad + t * a.ldg;
-            const float f = active ? by * inv : 0.0f;
+        if (grad && there) {
+            const float f = by * inv;
 #pragma unroll
-            for (int i = 0; i < Q * N; i++) v[i] = active ? f * v[i] * (g[i] - gp) * (SIGMOID ? slope[i] : 1.0f) : 0.0f;
+            for (int i = 0; i < Q * N; i++) {
+                v[i] = f * v[i] * (g[i] - gp);
+                if (SIGMOID) v[i] *= slope[i];
+                if (G < 32 && !active) v[i] = 0.0f;            // its logits may be anything
+            }
 #pragma unroll
             for (int q = 0; q < Q; q++) {
                 float u[N];
 #pragma unroll
                 for (int e = 0; e < N; e++) u[e] = v[q * N + e];
-                if (a.whole) {
-                    x[q].pack(u);
-                    if ((q * G + l) * N < a.ncols) ((uint4 *)grad)[q * G + l] = x[q].w;
+                if (WHOLE) {
+                    Granule<T> x;
+                    x.pack(u);
+                    if (has(q, 0)) ((uint4 *)grad)[q * G + l] = x.w;
                 } else {
 #pragma unroll
                     for (int e = 0; e < N; e++)
-                        if ((q * G + l) * N + e < a.ncols) grad[(q * G + l) * N + e] = from_float<T>(u[e]);
+                        if (has(q, e)) grad[(q * G + l) * N + e] = from_float<T>(u[e]);
                 }
             }
         }
@@ -256,7 +294,7 @@ __device__ __forceinline__ double cta_sum(double v, double *room)
 }
 
 // All of a small batch by one cluster.
-template <typename T, int G, int Q, bool SIGMOID>
+template <typename T, int G, int Q, bool SIGMOID, bool WHOLE>
 __global__ void __launch_bounds__(BT)
 balance_small_kernel(const BalanceArgs a)
 {
@@ -293,7 +331,7 @@ balance_small_kernel(const BalanceArgs a)
     __syncthreads();
     const Tally tally = {total, total + many, total + words};
     const int64_t each = (a.nrows + warps - 1) / warps, q0 = min(w * each, a.nrows), q1 = min(q0 + each, a.nrows);
-    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID>(a, tally, q0, q1), room);
+    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID, WHOLE>(a, tally, q0, q1), room);
     if (ranks > 1) {
         if (tid == 0) store_peer(&parts[rank], 0, sum);
         __syncwarp();
@@ -336,7 +374,7 @@ balance_count_kernel(const BalanceArgs a, int64_t per)
         if (hits[i]) atomicAdd(&y.counts[s0 * a.ncols + i], (u64)hits[i]);
 }
 
-template <typename T, int G, int Q, bool SIGMOID>
+template <typename T, int G, int Q, bool SIGMOID, bool WHOLE>
 __global__ void __launch_bounds__(BT)
 balance_kernel(const BalanceArgs a)
 {
@@ -349,7 +387,7 @@ balance_kernel(const BalanceArgs a)
     const int64_t many = a.nseq * a.ncols;
     if (a.kept)
         for (int64_t i = (int64_t)blockIdx.x * BT + tid; i < many; i += (int64_t)gridDim.x * BT) a.counts[i] = (int64_t)a.tally.counts[i];
-    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID>(a, a.tally, r0, r1), room);
+    const double sum = cta_sum(take_rows<T, G, Q, SIGMOID, WHOLE>(a, a.tally, r0, r1), room);
     if (tid == 0) {
         a.partial[blockIdx.x] = sum;
         last = last_of(a.counter, gridDim.x);
@@ -369,14 +407,14 @@ balance_kernel(const BalanceArgs a)
     }
 }
 
-template <typename T, int G, int Q, bool SIGMOID>
+template <typename T, int G, int Q, bool SIGMOID, bool WHOLE>
 static int launch_balance(BalanceArgs a, cudaStream_t st)
 {
     const int64_t many = a.nseq * a.ncols, words = many + 2 * a.nseq;
     if (words <= SMALL_COUNTS && a.nrows * a.ncols <= SMALL_ELEMENTS && a.nrows * 4 < SMALL_ELEMENTS) {
         int ranks = 1;
         while (ranks < MOST_CLUSTER && a.nrows * a.ncols > (int64_t)ranks * 4096) ranks *= 2;
-        return launch_cluster(balance_small_kernel<T, G, Q, SIGMOID>, (unsigned)ranks, ranks, BT, 0, st, a);
+        return launch_cluster(balance_small_kernel<T, G, Q, SIGMOID, WHOLE>, (unsigned)ranks, ranks, BT, 0, st, a);
     }
     constexpr int AT_ONCE = BW * 32 / G;
     const int64_t most = (int64_t)sm_count() * 8;
@@ -398,12 +436,18 @@ static int launch_balance(BalanceArgs a, cudaStream_t st)
     const int64_t per = max((int64_t)BT, ceil_div(ceil_div(a.nrows, most), BT) * BT);
     if (a.nrows > 0) balance_count_kernel<<<(unsigned)ceil_div(a.nrows, per), BT, 0, st>>>(a, per);
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = launch_behind(balance_kernel<T, G, Q, SIGMOID>, dim3((unsigned)grid), BT, 0, st, a);
+    if (e == cudaSuccess) e = launch_behind(balance_kernel<T, G, Q, SIGMOID, WHOLE>, dim3((unsigned)grid), BT, 0, st, a);
     if (e != cudaSuccess) {
         if (a.kept) cudaMemsetAsync(a.tally.counts, 0, sizeof(g_kept), st);       // what was counted is not the next call's
         return fail("balance_loss: launch failed: %s", cudaGetErrorString(e));
     }
     return 0;
+}
+
+template <typename T, int G, int Q, bool SIGMOID>
+static int launch_balance(const BalanceArgs &a, cudaStream_t st)
+{
+    return a.whole ? launch_balance<T, G, Q, SIGMOID, true>(a, st) : launch_balance<T, G, Q, SIGMOID, false>(a, st);
 }
 
 // G lanes x Q granules of N elements just cover the experts

@@ -27,6 +27,19 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ float from_float(float v) { return v; }
 
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 1 / v, correct to one unit in the last place; 0 from 2^126 on
+__device__ __forceinline__ float reciprocal(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 typedef unsigned long long u64_pair;
 
 // a NaN among the operands is the result
@@ -66,6 +79,7 @@ template <>
 struct Granule<float> {
     static constexpr int N = 4;
     uint4 w;
+    static __device__ __forceinline__ Granule least() { return {make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[2]) const
     {
         v[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
@@ -110,6 +124,7 @@ template <>
 struct Granule<__nv_bfloat16> {
     static constexpr int N = 8;
     uint4 w;
+    static __device__ __forceinline__ Granule least() { return {make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[4]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -156,6 +171,7 @@ template <>
 struct Granule<__half> {
     static constexpr int N = 8;
     uint4 w;
+    static __device__ __forceinline__ Granule least() { return {make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u)}; }          // -inf
     __device__ __forceinline__ void unpack(float2 (&v)[4]) const
     {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -260,6 +276,7 @@ __device__ __forceinline__ void copy_granule(void *to, const void *from)
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ unsigned cluster_size()
 {
