@@ -86,11 +86,23 @@ __device__ __forceinline__ void count_rows(const BalanceArgs &a, int64_t r0, int
         const bool one = __all_sync(0xffffffffu, s == s0 || !active);
         if (one && n0 > 0 && n0 <= 64 && __all_sync(0xffffffffu, t >= r1 || n == n0)) {
             const int many = 32 * n0;
-            for (int i = lane; i < many; i += 32) {
-                if (!(on >> (i / n0) & 1)) continue;
-                const int64_t j = a.crd[lo0 + i];
-                if (j >= 0 && j < a.ncols) hit(s0, (int)j);
-                else bad();
+            for (int i0 = lane; i0 < many; i0 += 32 * 8) {     // eight at a time on their way
+                int64_t j[8];
+                unsigned have = 0;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int i = i0 + 32 * k;
+                    if (i < many && on >> (i / n0) & 1) {
+                        j[k] = a.crd[lo0 + i];
+                        have |= 1u << k;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (have >> k & 1) {
+                        if (j[k] >= 0 && j[k] < a.ncols) hit(s0, (int)j[k]);
+                        else bad();
+                    }
             }
         } else if (active) {
             for (int64_t e = lo; e < hi; e++) {
@@ -374,8 +386,12 @@ balance_count_kernel(const BalanceArgs a, int64_t per)
         if (hits[i]) atomicAdd(&y.counts[s0 * a.ncols + i], (u64)hits[i]);
 }
 
+// CTAs on an SM: as many as a lane's values leave registers for
+template <typename T, int Q>
+constexpr int balance_ctas() { return Q * Granule<T>::N <= 8 ? 4 : Q * Granule<T>::N <= 16 ? 2 : 1; }
+
 template <typename T, int G, int Q, bool SIGMOID, bool WHOLE>
-__global__ void __launch_bounds__(BT)
+__global__ void __launch_bounds__(BT, balance_ctas<T, Q>())
 balance_kernel(const BalanceArgs a)
 {
     __shared__ double room[BW];
@@ -418,7 +434,7 @@ static int launch_balance(BalanceArgs a, cudaStream_t st)
     }
     constexpr int AT_ONCE = BW * 32 / G;
     const int64_t most = (int64_t)sm_count() * 8;
-    const int64_t grid = max((int64_t)1, min(most, ceil_div(a.nrows, AT_ONCE * 2)));
+    const int64_t grid = max((int64_t)1, min((int64_t)sm_count() * balance_ctas<T, Q>(), ceil_div(a.nrows, AT_ONCE * 2)));
     void *room = nullptr;
     a.kept = words <= KEPT_COUNTS;
     CB_TRY(scratch(SLOT_MISC, (size_t)most * sizeof(double) + (a.kept ? 0 : (size_t)(2 + 2 * a.nseq) * sizeof(u64)), &room));

@@ -65,6 +65,15 @@ struct Order16 {
         if (__hisnan(v)) return 0xffffu;
         return u == 0x8000u ? 0x8000u : u ^ (u & 0x8000u ? 0xffffu : 0x8000u);
     }
+    // two at a time
+    template <typename T2>
+    static __device__ __forceinline__ uint32_t keys(uint32_t u)
+    {
+        const T2 v = *(const T2 *)&u, zero = {from_float<T>(0.0f), from_float<T>(0.0f)};
+        const T2 same = __hadd2(v, zero);          // -0 is 0
+        const uint32_t w = *(const uint32_t *)&same, minus = ((w & 0x80008000u) >> 15) * 0xffffu;
+        return (w ^ (minus | 0x80008000u)) | __hneu2_mask(v, v);
+    }
     static __device__ __forceinline__ T code(uint32_t k)
     {
         const uint16_t u = (uint16_t)(k == 0xffffu ? 0x7fffu : k ^ (k & 0x8000u ? 0x8000u : 0xffffu));
@@ -73,9 +82,13 @@ struct Order16 {
     static __device__ __forceinline__ float value(uint32_t k) { return to_float(code(k)); }
 };
 template <>
-struct Order<__nv_bfloat16> : Order16<__nv_bfloat16, 0> {};
+struct Order<__nv_bfloat16> : Order16<__nv_bfloat16, 0> {
+    static __device__ __forceinline__ uint32_t keys2(uint32_t u) { return keys<__nv_bfloat162>(u); }
+};
 template <>
-struct Order<__half> : Order16<__half, 3> {};
+struct Order<__half> : Order16<__half, 3> {
+    static __device__ __forceinline__ uint32_t keys2(uint32_t u) { return keys<__half2>(u); }
+};
 
 struct TopShared {
     u64 cand[ROOM];
@@ -639,11 +652,21 @@ top_short_kernel(int64_t nrows, int ncols, const T *__restrict__ xs, int64_t ldx
         for (int r = 0; r < R; r++) part.v[r] = lane * R + r < ncols ? x[lane * R + r] : from_float<T>(MINUS_INF);
     }
     Short<T> own[R];
+    if constexpr (ONE && R > 1) {
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        own[r].set(part.v[r], lane * R + r);
-        if (lane * R + r >= ncols) own[r].none();
+        for (int r = 0; r < R; r += 2) {
+            const uint32_t keys = Order<T>::keys2(((const uint32_t *)&part)[r / 2]), col = lane * R + r;
+            own[r].word = keys << 16 | (0xffffu - col);
+            own[r + 1].word = (keys & 0xffff0000u) | (0xfffeu - col);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; r++) own[r].set(part.v[r], lane * R + r);
     }
+    if (lane * R + R > ncols)
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (lane * R + r >= ncols) own[r].none();
 #pragma unroll
     for (int p = 1; p < R; p *= 2)
 #pragma unroll
