@@ -121,7 +121,17 @@ distill_kernel(const DistillArgs a)
     if (lo < hi && w != 0.0f) {
         if (ranks > 1) cluster_arrive_relaxed();   // only to say that it is there
         const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15) + first;
-        for (int i = tid; i < n; i += DT) copy_granule(part + i, from + i);
+        {
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(part);
+            int i = tid;
+            for (; i + 3 * DT < n; i += 4 * DT) {
+                copy_far<0>(to + i * 16, from + i);
+                copy_far<DT * 16>(to + i * 16, from + i);
+                copy_far<DT * 32>(to + i * 16, from + i);
+                copy_far<DT * 48>(to + i * 16, from + i);
+            }
+            for (; i < n; i += DT) copy_far<0>(to + i * 16, from + i);
+        }
         if (REST)
             for (int i = tid; i < (n * N + 31) / 32; i += DT) bits[i] = 0;
         for (int64_t e = lo + tid; e < hi; e += DT) zm = max_nan(zm, (float)z[e]);
@@ -275,10 +285,26 @@ distill_kernel(const DistillArgs a)
         const float total = REST ? others + stored : others, p = sum_of(sums[0]);
         const float left = REST ? fmaxf(0.0f, 1.0f - p) : 0.0f;
         if (GRAD) {
-            const float by = w * a.by, part_of = total == 0.0f ? 0.0f : by / total;     // total 0: every logit is -inf
+            const float by = w * a.by, part_of = total == 0.0f ? 0.0f : __fdividef(by, total);      // total 0: every logit is -inf
             const float of = left > 0.0f && others > 0.0f ? part_of * (1.0f - left * (total / others)) : part_of;
             const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
-            if (alike && top.near) {
+            if (alike && top.near && col0 >= 0 && col0 + n * N <= a.ncols) {            // no granule that is not all the row's
+                uint4 *to = (uint4 *)((uintptr_t)g & ~(uintptr_t)15) + first;
+                const float2 of2 = make_float2(of, of);
+#pragma unroll 4
+                for (int i = tid; i < n; i += DT) {
+                    float2 v[N / 2];
+                    part[i].unpack(v);
+#pragma unroll
+                    for (int k = 0; k < N / 2; k++) {
+                        v[k] = top.of(v[k]);
+                        v[k] = mul2(make_float2(exp2_fast(v[k].x), exp2_fast(v[k].y)), of2);
+                    }
+                    Granule<T> out;
+                    out.pack(v);
+                    to[i] = out.w;
+                }
+            } else if (alike && top.near) {
                 uint4 *to = (uint4 *)((uintptr_t)g & ~(uintptr_t)15) + first;
 #pragma unroll 4
                 for (int i = tid; i < n; i += DT) {
@@ -304,7 +330,7 @@ distill_kernel(const DistillArgs a)
                     if (col0 + i >= 0 && col0 + i < a.ncols) g[col0 + i] = from_float<T>(of * exp2_fast(top.of(to_float(elem[i]))));
             }
             __syncthreads();
-            const float inv = REST ? 1.0f : 1.0f / p;
+            const float inv = REST ? 1.0f : __fdividef(1.0f, p);
             for (int64_t e = lo + tid; e < hi; e += DT) {
                 const int64_t col = a.crd[e], j = col - col0;
                 if (j < 0 || j >= (int64_t)n * N || col < 0 || col >= a.ncols || (e > lo && a.crd[e - 1] == col)) continue;

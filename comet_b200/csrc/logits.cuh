@@ -273,6 +273,12 @@ __device__ __forceinline__ void copy_granule(void *to, const void *from)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
+// 16 bytes, from and to BYTES behind the addresses
+template <int BYTES>
+__device__ __forceinline__ void copy_far(uint32_t to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %2], 16;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }

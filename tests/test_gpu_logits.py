@@ -570,3 +570,17 @@ def test_refusals():
     with pytest.raises(ValueError, match="experts"):
         device.balance_loss(S, wide[:, :1025])
     assert float(device.top_entries(x, 2)[0].val.sum()) == 0           # and the library goes on
+
+
+def test_a_routed_student_learns():
+    """The example: its first loss is that of even odds over the vocabulary against the teacher's list, and it falls."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "distill_routed_student.py")
+    spec = importlib.util.spec_from_file_location("distill_routed_student", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    history, counts = example.train(steps=40)
+    assert sum(counts) == 512 * 2
+    losses = [loss for loss, _ in history]
+    assert all(math.isfinite(v) for v in losses) and sum(losses[-5:]) < sum(losses[:5])
