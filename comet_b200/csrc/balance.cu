@@ -5,14 +5,16 @@
 //   d loss / d r_e = scale E / (sequences N) * p_e (f_e - sum_j f_j p_j)          [times (1 - sigmoid(r_e))]
 // The counts are all that the gradient needs of other rows, so they come first and R is read once.  f is used as
 // g = f - 1 / E, taken from whole numbers: for balanced experts the difference f_e - sum f p would lose its digits otherwise.
-// sigmoid(r) / sum is softmax(log sigmoid(r)), which holds where every sigmoid underflows.
+// Where every sigmoid of a row underflows, their shares are those of e^(r - max) / (1 + e^r).
 //
 // Small batches: one cluster counts, exchanges its counts through shared memory and takes the rows, in one launch.  Otherwise a
 // kernel counts and a second one, whose start overlaps with it, takes the rows.
 // A group of lanes takes a row, 16 bytes a lane or a few times that: a lane's columns are the same in every row, so their g stay in
 // registers while the sequence lasts.
 //
-// Bound: HBM, R and its gradient; small batches: the launch.
+// Bound: HBM, R and its gradient; small batches: the launch.  65536 x 256 bf16 in 32 sequences, sigmoid: 40 us, 11 by the bytes; counting 5, rows 34,
+// which are 276 instructions a row.  16384 x 64 f32: 16.6 us, most of it the two launches and their chains of loads.  128 x 8: 4.6 us on
+// the device, 14 a call.  With the counters cleared by the driver and a warp per row whatever its length: 155, 47 and 23.
 #include "logits.cuh"
 #include "stream.cuh"
 

@@ -2,6 +2,9 @@
 torch CUDA tensors.  torch supplies device memory and streams only; every
 computation is done by the kernels of ``libcomet_b200``.
 
+Beside the sparse operations: the largest entries of rows of logits as a CSR matrix, and two losses of such a matrix beside
+logits (``top_entries``, ``distill_loss``, ``balance_loss``).
+
 Used by the benchmark (inputs already in HBM when the clock starts), by the
 multi-GPU sharding layer and by the device-level parity tests.
 """

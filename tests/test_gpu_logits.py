@@ -573,7 +573,7 @@ def test_refusals():
 
 
 def test_a_routed_student_learns():
-    """The example: its first loss is that of even odds over the vocabulary against the teacher's list, and it falls."""
+    """The example: its distillation loss falls to less than half."""
     import importlib.util
     import os
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "distill_routed_student.py")
@@ -583,4 +583,4 @@ def test_a_routed_student_learns():
     history, counts = example.train(steps=40)
     assert sum(counts) == 512 * 2
     losses = [loss for loss, _ in history]
-    assert all(math.isfinite(v) for v in losses) and sum(losses[-5:]) < sum(losses[:5])
+    assert all(math.isfinite(v) for v in losses) and losses[-1] < losses[0] / 2
