@@ -21,7 +21,9 @@
 namespace cb200 {
 
 static const int BT = 256, BW = BT / 32, MOST_EXPERTS = 1024;
-static const int64_t SMALL_ELEMENTS = 65536;       // logits of the one-launch kernel
+// Logits of the one-launch kernel.  Rows of 64 bf16, one launch against two, us on the device: 128 rows 7.5, 9.4; 1024 9.3, 9.6; 2048 11.7, 9.6.  The host
+// spends a launch less, too.
+static const int64_t SMALL_ELEMENTS = 65536;
 static const int SMALL_COUNTS = 2048;              // sequences times (experts + 2) that the one-launch kernel holds
 static const int KEPT_COUNTS = 16384;              // and that are counted in memory that every call leaves at 0
 

@@ -304,12 +304,12 @@ struct LogSum {
     }
 };
 
-// The first step's bound, by all threads: each warp finds the ceil(k / 8)-th largest of its 128 granules' largest entries, and k entries
-// reach the least of those eight keys.
+// The first step's bound, by all threads: each of eight warps finds the ceil(k / 8)-th largest of its 128 granules' largest entries, and k
+// entries reach the least of those keys.  Of fewer than 256 granules the first warps have 32 each, and only those are asked.
 template <typename T>
-__device__ __forceinline__ uint32_t first_bound(TopShared &sh, const typename Granule<T>::Most (&gm)[TU], int k)
+__device__ __forceinline__ uint32_t first_bound(TopShared &sh, const typename Granule<T>::Most (&gm)[TU], int k, int granules)
 {
-    const int want = (k + TW - 1) / TW;
+    const int asked = granules < 32 ? TW : min(TW, granules / 32), want = (k + asked - 1) / asked;
     uint32_t key = 0, gk[TU];
 #pragma unroll
     for (int u = 0; u < TU; u++) gk[u] = Order<T>::key(largest(gm[u]));
@@ -321,7 +321,7 @@ __device__ __forceinline__ uint32_t first_bound(TopShared &sh, const typename Gr
         if (n >= want) key = more;
         if (n == want) break;
     }
-    if ((threadIdx.x & 31) == 0) sh.least[threadIdx.x >> 5] = key;
+    if ((threadIdx.x & 31) == 0) sh.least[threadIdx.x >> 5] = (int)threadIdx.x >> 5 < asked ? key : 0xffffffffu;
     __syncthreads();
     key = sh.least[0];
 #pragma unroll
@@ -352,7 +352,7 @@ __device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, i
             gm[u] = g[u].most();
         }
         if (step == 0) {
-            base = first_bound<T>(sh, gm, k);
+            base = first_bound<T>(sh, gm, k, way.end - way.begin);
             if (threadIdx.x == 0) sh.base = *bound = base;
             __syncthreads();
         }
@@ -410,7 +410,7 @@ __device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, 
             gm[u] = g[u].most();
         }
         if (step == 0) {
-            const uint32_t key = first_bound<T>(sh, gm, k);
+            const uint32_t key = first_bound<T>(sh, gm, k, way.end - way.begin);
             bound = (u64)key << colbits;
             least_value = Order<T>::code(key);
         }
@@ -785,12 +785,15 @@ static int top_entries(int64_t nrows, int64_t ncols, const void *x, int64_t ldx,
         a.c = (float)(LOG2E_D / *temperature);
         a.inv = (float)(1.0 / *temperature);
     }
-    if (ncols > 512 || k > 32) return lse ? launch_long<T, true>(a) : launch_long<T, false>(a);
+    // By warps / by CTAs, 4096 rows, k = 8 and 32, us: 512 columns of bf16 5.7, 9.7 / 128, 131, 1024 of bf16 24, 34 / 137, 143 (the CTAs' bound was looser);
+    // 512 of f32 -, 24 / -, 124, 1024 of f32 93, 148 / 49, 58: a warp's two words an entry fill its registers.
+    if (ncols > (sizeof(T) == 2 ? 1024 : 512) || k > 32) return lse ? launch_long<T, true>(a) : launch_long<T, false>(a);
     if (ncols <= 32) launch_short<T, 1>(a);
     else if (ncols <= 64) launch_short<T, 2>(a);
     else if (ncols <= 128) launch_short<T, 4>(a);
     else if (ncols <= 256) launch_short<T, 8>(a);
-    else launch_short<T, 16>(a);
+    else if (ncols <= 512) launch_short<T, 16>(a);
+    else if constexpr (sizeof(T) == 2) launch_short<T, 32>(a);
     CB_LAUNCH_CHECK();
     return 0;
 }

@@ -340,7 +340,7 @@ def check_top(x, x64, k, tau=1.0, lse=True):
 
 
 TOP_SHAPES = [(1, 1, 1), (3, 5, 2), (40, 8, 2), (33, 64, 8), (70, 61, 61), (9, 100, 33), (65, 256, 8), (5, 511, 16), (4, 513, 40), (6, 1000, 1000), (2, 3000, 1024),
-              (3, 20011, 50), (1, 131072, 64), (2, 131072, 1024), (400, 9000, 12)]
+              (3, 20011, 50), (1, 131072, 64), (2, 131072, 1024), (400, 9000, 12), (37, 700, 20), (9, 1024, 32), (9, 1025, 32), (6, 1000, 33)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
