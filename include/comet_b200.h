@@ -641,8 +641,9 @@ COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f32_i64(
      loss    = scale * sum_t weight[t] * rows[t]                            (weight may be NULL: all 1)
      grad    = d loss / d x, in x's type; may be x itself (same ldx), or NULL: no gradient.
    A row that stores nothing, or nothing but -inf, or whose weight is 0, has a loss and a gradient of 0, and its logits are
-   not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf.  Columns of a row ascend; repeated ones are next to each other, and their p
-   add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
+   not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf; the q of what is not listed is 0 in f32 once
+   it lies more than 87 temperatures below the largest logit.  Columns of a row ascend; repeated ones are next to each other, and
+   their p add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
    bits). */
 COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_bf16_i64(
     int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *val, int32_t val_bytes, const
