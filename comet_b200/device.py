@@ -18,7 +18,10 @@ from .api import PLUS_PAIR, PLUS_TIMES, as_sparse  # noqa: F401
 
 
 class DeviceCSR:
-    """A CSR (or DCSR when ``row_ids`` is set) matrix in device memory, int64 / float64."""
+    """A CSR (or DCSR when ``row_ids`` is set) matrix in device memory, int64 indices.
+
+    The sparse operations take float64 values and refuse others; ``top_entries`` gives float32 values, which ``distill_loss`` takes.  Of
+    such a matrix S, ``DeviceCSR(S.nrows, S.ncols, S.pos, S.crd, S.val.double())`` is one for the sparse operations."""
 
     def __init__(self, nrows, ncols, pos, crd, val, row_ids=None):
         self.nrows, self.ncols = int(nrows), int(ncols)
@@ -62,6 +65,16 @@ def _check_cuda(*ts):
             raise ValueError("device entry points need contiguous CUDA tensors")
 
 
+def _check_f64(*ts):
+    """Values that the f64 entry points read or write by their address."""
+    for t in ts:
+        if t is not None:
+            if not (t.is_cuda and t.is_contiguous()):
+                raise ValueError("device entry points need contiguous CUDA tensors")
+            if t.dtype is not torch.float64:
+                raise ValueError("this operation takes float64 values, not %s; convert them with .double()" % t.dtype)
+
+
 _ready = None
 
 
@@ -78,7 +91,8 @@ def _call(name, *args):
 
 
 def spmv(A, x, y=None, semiring=PLUS_TIMES, accumulate=False):
-    _check_cuda(A.pos, A.crd, A.val, x, y)
+    _check_cuda(A.pos, A.crd)
+    _check_f64(A.val, x, y)
     if y is None:
         # rows the matrix does not store, and the values that are added to, start at zero; any other row is written
         new = torch.zeros if A.row_ids is not None or A.nstored < A.nrows or accumulate else torch.empty
@@ -90,9 +104,10 @@ def spmv(A, x, y=None, semiring=PLUS_TIMES, accumulate=False):
 
 def spmm(A, B, C=None, semiring=PLUS_TIMES, accumulate=False, variant=0):
     """B may be a column slice of a wider row-major array (unit column stride); its row stride is passed on."""
-    _check_cuda(A.pos, A.crd, A.val, C)
-    if not B.is_cuda or B.dim() != 2 or B.stride(1) != 1:
-        raise ValueError("B must be a CUDA matrix with unit column stride")
+    _check_cuda(A.pos, A.crd)
+    _check_f64(A.val, C)
+    if not B.is_cuda or B.dim() != 2 or B.stride(1) != 1 or B.dtype is not torch.float64:
+        raise ValueError("B must be a CUDA matrix of float64 values with unit column stride")
     k = B.shape[1]
     if C is None:
         C = torch.empty((A.nrows, k), dtype=torch.float64, device=B.device)
@@ -106,7 +121,8 @@ def spmm(A, B, C=None, semiring=PLUS_TIMES, accumulate=False, variant=0):
 
 def sddmm(S, X, Y, out=None):
     """Y is [ncols, K] row-major."""
-    _check_cuda(S.pos, S.crd, S.val, X, Y, out)
+    _check_cuda(S.pos, S.crd)
+    _check_f64(S.val, X, Y, out)
     if out is None:
         out = torch.empty(S.nnz, dtype=torch.float64, device=X.device)
     _call("comet_b200_dev_sddmm_f64_i64", S.nrows, S.nnz, X.shape[1], S.pos.data_ptr(), S.crd.data_ptr(),
@@ -122,7 +138,8 @@ class SpgemmResult:
 
 def spgemm_symbolic(A, B, M=None, semiring=PLUS_TIMES):
     """Returns (handle, cpos tensor, nnz)."""
-    _check_cuda(A.pos, A.crd, A.val, B.pos, B.crd, B.val)
+    _check_cuda(A.pos, A.crd, B.pos, B.crd)
+    _check_f64(A.val, B.val)
     cpos = torch.empty(A.nrows + 1, dtype=torch.int64, device=A.pos.device)
     out = (ctypes.c_int64 * 2)()
     at = ctypes.addressof(out)
@@ -137,6 +154,8 @@ def spgemm_numeric(handle, nnz, device, keep=False, crd=None, val=None):
     if crd is None:
         crd = torch.empty(max(nnz, 1), dtype=torch.int64, device=device)[:nnz]
         val = torch.empty(max(nnz, 1), dtype=torch.float64, device=device)[:nnz]
+    if val.dtype is not torch.float64:
+        raise ValueError("this operation writes float64 values, not %s" % val.dtype)
     _call("comet_b200_dev_spgemm_numeric_f64_i64", handle, crd.data_ptr(), val.data_ptr(), int(keep), _stream())
     return crd, val
 
