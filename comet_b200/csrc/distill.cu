@@ -34,10 +34,26 @@ struct DistillArgs {
     int64_t ldx;
     void *grad;
     int64_t ldg;
+    double inv;                  // 1 / temperature
     float c, by, scale;          // log2(e) / temperature, scale / temperature
     float *rows, *loss;
     unsigned *counter;           // null: another kernel adds the rows up
 };
+
+// log p and p of an entry.  With lse p is not normalised afterwards, and what it is off by is the rest's error too, so the difference
+// that the exponential is taken of is rounded twice, its residue a factor of p: f32 products of the size of lse would leave p 1e-6 of
+// itself off.  A row has tens of entries, whose f64 operations take no time that shows.
+struct Weight {
+    float log, p;
+};
+__device__ __forceinline__ Weight weight_of(double log)
+{
+    Weight w;
+    w.log = (float)log;
+    w.p = expf(w.log);
+    if (w.log > -104.0f && w.log < 89.0f) w.p = fmaf(w.p, (float)(log - w.log), w.p);              // neither 0 nor infinite
+    return w;
+}
 
 // what a CTA tells the others of its row: the maximum of its part, sums of 2^((x - maximum) c) of elements that are not
 // stored and of those that are, of p's weights and of p's weights times (x - maximum) c
@@ -223,16 +239,17 @@ distill_kernel(const DistillArgs a)
                 if (!REST || !(bits[i >> 5] >> (i & 31) & 1)) s2.x += exp2_fast(u.of(to_float(elem[i])));
         }
         s2.x = warp_sum(s2.x + s2.y);
-        // of the entries: p's weights, times their log2; in this part: weights, times (x - m) c, and stored columns' 2^((x - m) c)
+        // of the entries: p's weights, times their logarithm; in this part: weights, times (x - m) c, and stored columns' 2^((x - m) c)
         float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        const float zref = REST ? a.lse[t] * LOG2E : zm;
-        auto log_p = [&](int64_t e) { return REST ? fmaf((float)z[e], a.c, -zref) : ((float)z[e] - zref) * a.c; };
+        const float zref = REST ? a.lse[t] : zm;
+        auto weight = [&](int64_t e) { return weight_of(REST ? fma((double)z[e], a.inv, -(double)zref) : ((double)z[e] - (double)zref) * a.inv); };
         if (entries) {
             for (int64_t e = lo + tid; e < hi; e += DT) {
                 const int64_t col = a.crd[e], j = col - col0;
-                const float lp = log_p(e), p = exp2_fast(lp);
+                const Weight y = weight(e);
+                const float p = y.p;
                 s[0] += p;
-                if (!(p <= 0.0f)) s[1] += p * lp;
+                if (!(p <= 0.0f)) s[1] += p * y.log;
                 if (col < 0 || col >= a.ncols) {
                     s[1] = __int_as_float(0x7fffffff);
                 } else if (j >= 0 && j < (int64_t)n * N) {
@@ -339,16 +356,15 @@ distill_kernel(const DistillArgs a)
                 const int64_t col = a.crd[e], j = col - col0;
                 if (j < 0 || j >= (int64_t)n * N || col < 0 || col >= a.ncols || (e > lo && a.crd[e - 1] == col)) continue;
                 float pj = 0.0f;                   // repeated columns are next to each other: their sum
-                for (int64_t i = e; i < hi && a.crd[i] == col; i++) pj += exp2_fast(log_p(i));
+                for (int64_t i = e; i < hi && a.crd[i] == col; i++) pj += weight(i).p;
                 g[col] = from_float<T>(part_of * exp2_fast(top.of(to_float(elem[j]))) - by * (pj * inv));
             }
             if (rank != 0 || warp != 0) return;
         }
         const float l2 = total == 0.0f ? 0.0f : log2f(total), plogp = sum_of(sums[1]);
         if (lane == 0) {
-            const float loss = REST ? plogp - pu + p * l2 + (left > 0.0f ? left * (log2f(left) - log2f(others) + l2) : 0.0f)
-                                    : (plogp - pu) / p - log2f(p) + l2;
-            a.rows[t] = loss * LN2;
+            a.rows[t] = REST ? fmaf(p * l2 - pu + (left > 0.0f ? left * (log2f(left) - log2f(others) + l2) : 0.0f), LN2, plogp)
+                             : (plogp - pu * LN2) / p + (l2 - log2f(p)) * LN2;
         }
     }
     if (!a.counter) return;
@@ -403,7 +419,7 @@ static int distill_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
         CB_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
         return 0;
     }
-    DistillArgs a = {nrows, (int)ncols, 0, pos, crd, val, lse, weight, x, ldx, grad, ldg, (float)((double)LOG2E_D / temperature),
+    DistillArgs a = {nrows, (int)ncols, 0, pos, crd, val, lse, weight, x, ldx, grad, ldg, 1.0 / temperature, (float)((double)LOG2E_D / temperature),
                      (float)(scale / temperature), (float)scale, rows, loss, next_counter()};
     if (!a.counter) return 1;
     return val_bytes == 4 ? launch_distill<T, float>(a, st) : launch_distill<T, double>(a, st);
