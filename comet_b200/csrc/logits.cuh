@@ -50,6 +50,8 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return r;
 }
 
+__device__ __forceinline__ double max_nan(double a, double b) { return a != a || a > b ? a : b; }
+
 // two f32 operations in one instruction
 __device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
@@ -247,6 +249,12 @@ __device__ __forceinline__ float warp_max(float v)
     float r;
     asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
+}
+__device__ __forceinline__ double warp_max(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
 // N values per thread to their sums (or maxima) over the CTA, in every thread.  `room` holds N * WARPS floats and is free

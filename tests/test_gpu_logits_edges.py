@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_gpu_logits import TOL, csr, distill, log_sum_exp, logits, teacher
+from tests.test_gpu_logits import TOL, close_gradient, csr, distill, log_sum_exp, logits, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,27 @@ def test_distill_probabilities_beside_a_large_sum(near, tau):
     assert (np.abs(got - p) <= 2.0 ** -21 * p + 1e-20).all()
     wrows, _, _, _, roff = distill(pos, crd, val, x64, tau, lse)
     assert (np.abs(rows.double().cpu().numpy() - wrows) <= 2.0 ** -20 / TOL * roff).all()
+
+
+def test_distill_float64_teachers_keep_their_digits():
+    """Values whose differences are lost in f32, and values beyond it.  Gradients are scaled by the temperature: a q below 2^-126 is 0, and LEAST is
+    of that size."""
+    rng = np.random.default_rng(21)
+    x, x64 = logits(rng, 40, 3001, "f32")
+    S, pos, crd, val = teacher(rng, 40, 3001, 20, True, np.float64)
+    for shift, tau in ((1e8, 1.0), (-1e8, 0.5), (1e12, 0.01), (1e8, 1e-3)):
+        more = np.round((val + shift) * 2 ** 10) / 2 ** 10
+        S, pos = csr(40, 3001, np.diff(pos), crd, more, np.float64)
+        less = more - shift                                            # exact: the shift is no part of the probabilities
+        wrows, _, wgrad, off, roff = distill(pos, crd, less, x64, tau, scale=tau)
+        check_float64(S, x, tau, wrows, wgrad, off, roff)
+    S, pos = csr(2, 3001, [3, 2], [5, 6, 9, 0, 3000], [1e300, 1e300, 5e299, -1e300, -2e300], np.float64)
+    wrows, _, wgrad, off, roff = distill(pos, np.array([5, 6, 9, 0, 3000]), np.array([0.0, 0.0, -1e30, 0.0, -1e30]), x64[:2])
+    check_float64(S, x[:2], 1.0, wrows, wgrad, off, roff)
+
+
+def check_float64(S, x, tau, wrows, wgrad, off, roff):
+    from comet_b200 import device
+    _, rows, grad = device.distill_loss(S, x, temperature=tau, scale=tau)
+    assert (np.abs(rows.double().cpu().numpy() - wrows) <= roff).all()
+    close_gradient(grad, wgrad, off, "f32")
