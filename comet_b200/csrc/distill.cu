@@ -66,19 +66,20 @@ struct Told {
     float m, others, stored, p, pu;
 };
 
-// (x - m) c.  As x c - m c it is one operation, and the rounding of m c is a factor that all of a row's terms and their sum
-// have alike; m c may be beyond f32 where the difference is not.
+// (x - m) c.  Where m c is less than NEAR it is x c - m c, one operation, and the rounding of m c is a factor that all of a CTA's
+// terms and their sum have alike; `lacks` is what it is off by, which a CTA on the other side of NEAR has to know.
 struct Exponent {
-    float c, m, mc;
+    float c, m, mc, lacks;
     bool near;
     __device__ __forceinline__ Exponent(float most, float c_) : c(c_), m(most == MINUS_INF ? 0.0f : most)
     {
         mc = m * c;
-        near = fabsf(mc) < 1e30f;
+        near = fabsf(mc) < NEAR;
+        lacks = near ? fmaf(m, c, -mc) : 0.0f;
     }
     __device__ __forceinline__ float of(float x) const { return near ? fmaf(x, c, -mc) : (x - m) * c; }
     __device__ __forceinline__ float2 of(float2 x) const { return fma2(x, make_float2(c, c), make_float2(-mc, -mc)); }      // near
-    __device__ __forceinline__ float to(const Exponent &o) const { return near && o.near ? mc - o.mc : (m - o.m) * c; }
+    __device__ __forceinline__ float to(const Exponent &o) const { return near && o.near ? mc - o.mc : (m - o.m) * c - lacks + o.lacks; }
 };
 
 template <int N>

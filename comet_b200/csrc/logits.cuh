@@ -14,6 +14,8 @@ static const double LOG2E_D = 1.4426950408889634;
 #ifdef __CUDACC__
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float MINUS_INF = -__builtin_huge_valf();
+// (x - m) c as x c - (m c) is off by the rounding of m c, the same for all x: a factor of less than 2^(1/4) up to here, and beyond f32 from 2^31 on.
+constexpr float NEAR = 4194304.0f;
 
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

@@ -281,7 +281,7 @@ struct LogSum {
             m = nm;
             mc = m == MINUS_INF ? 0.0f : m * c;
         }
-        if (fabsf(mc) < 1e30f) {
+        if (fabsf(mc) < NEAR) {                    // what the rounding of mc does to s is below the rounding of the result, m c + log2(s)
 #pragma unroll
             for (int u = 0; u < TU; u++) {
                 float2 v[N / 2];
@@ -292,7 +292,7 @@ struct LogSum {
                     s = add2(s, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
                 }
             }
-        } else {                                   // m * c may be beyond f32 where x - m is not; and NaN, and infinity
+        } else {                                   // and NaN, and infinity
 #pragma unroll
             for (int u = 0; u < TU; u++) {
                 float v[N];

@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_gpu_logits import TOL, close_gradient, csr, distill, log_sum_exp, logits, teacher
+from tests.test_gpu_logits import TOL, TYPES, check_top, close_gradient, csr, distill, log_sum_exp, logits, teacher, torch_type
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,56 @@ def check_float64(S, x, tau, wrows, wgrad, off, roff):
     _, rows, grad = device.distill_loss(S, x, temperature=tau, scale=tau)
     assert (np.abs(rows.double().cpu().numpy() - wrows) <= roff).all()
     close_gradient(grad, wgrad, off, "f32")
+
+
+def large_quotients(kind, cols):
+    """Rows of one large value, of one above all, of two values, and of neighbours of 18.125: (CUDA tensor, the same values in f64)."""
+    import torch
+    rng = np.random.default_rng(cols)
+    most = {"bf16": 1e20, "f32": 1e20, "f16": 6e4}[kind]
+    rows = [np.full(cols, s * v) for v in (1e9, 1e10, 1e20) if v <= most for s in (1, -1)]
+    rows += [np.where(np.arange(cols) == cols // 2, b, 1.5 * b if b < 0 else 0.5 * b) for b in (-most / 2, most / 2)]
+    rows += [np.where(rng.random(cols) < 0.5, b, 1.5 * b if b < 0 else 0.5 * b) for b in (-most / 2, most / 2, 18.125, -18.125)]
+    unit = {"bf16": 2.0 ** -3, "f16": 2.0 ** -6, "f32": 2.0 ** -19}[kind]               # the spacing of the type at 18
+    rows += [18.125 + unit * rng.integers(0, 4, cols), -18.125 - unit * rng.integers(0, 4, cols),
+             18.125 + unit * (np.arange(cols) * 8 // cols)]                             # each CTA's part has a maximum of its own
+    x = torch.from_numpy(np.array(rows, np.float64)).float().to(torch_type(kind))
+    return x.cuda(), x.double().numpy()
+
+
+# 18.125 log2(e) over the temperature lies at 2^22 and on both sides of it
+BESIDE = [v * math.log2(math.e) / 2 ** 22 for v in (18.125, 18.126, 18.124)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [300, 9001, 131072])
+def test_distill_large_quotients(cols, kind):
+    x, x64 = large_quotients(kind, cols)
+    rng = np.random.default_rng(cols + 1)
+    S, pos, crd, val = teacher(rng, len(x64), cols, 12, False)
+    for tau in [1.0, 1e-7, 1e-9] + BESIDE:
+        check_quotients(S, pos, crd, val, x, x64, kind, tau)
+    for tau in [1.0] + BESIDE:                                         # a sum of 10^8 has no digits behind the point
+        check_quotients(S, pos, crd, val, x, x64, kind, tau, np.array([log_sum_exp(val[a:b] / tau) + 0.3 for a, b in zip(pos, pos[1:])], np.float32))
+
+
+def check_quotients(S, pos, crd, val, x, x64, kind, tau, lse=None):
+    """As check_distill.  Where what is not listed is below f32's range, a loss with a sum is infinite: more than 0.2 (87 - 1) it has to be."""
+    import torch
+    from comet_b200 import device
+    _, rows, grad = device.distill_loss(S, x, temperature=tau, lse=None if lse is None else torch.from_numpy(lse).cuda(), scale=tau)
+    wrows, _, wgrad, off, roff = distill(pos, crd, val, x64, tau, lse, None, tau)
+    got = rows.double().cpu().numpy()
+    assert not np.isnan(got).any() and not grad.isnan().any()
+    far = np.isposinf(got)
+    assert (wrows[far] > 17).all() and not (far.any() and lse is None)
+    assert (np.abs(got - wrows)[~far] <= roff[~far]).all()
+    close_gradient(grad[torch.from_numpy(~far).cuda()], wgrad[~far], off[~far], kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [300, 9001, 131072])
+def test_top_entries_sums_of_large_quotients(cols, kind):
+    x, x64 = large_quotients(kind, cols)
+    for tau in [1.0, 1e-7, 1e-9] + BESIDE:
+        check_top(x, x64, 5, tau)
