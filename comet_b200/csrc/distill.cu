@@ -60,6 +60,11 @@ __device__ __forceinline__ Weight weight_of(double log)
     return w;
 }
 
+// What 1 - sum p may be by rounding alone, where lse is a sum of the entries' own: lse comes with some roundings of the size of lse and of the
+// largest logit, 2^-22 of them together, exponentials and sums of up to 32 numbers a thread add 2^-19.  A rest within it counts as none where
+// no column is left for it, instead of making the loss infinite.
+__device__ __forceinline__ float rounding_of(float lse, float most) { return fminf(0x1p-20f * (2.0f + fabsf(lse) + fabsf(most)), 0.5f); }
+
 // what a CTA tells the others of its row: the maximum of its part, sums of 2^((x - maximum) c) of elements that are not
 // stored and of those that are, of p's weights and of p's weights times (x - maximum) c
 struct Told {
@@ -315,7 +320,8 @@ distill_kernel(const DistillArgs a)
             pu += __shfl_xor_sync(0xffffffffu, pu, i);
         }
         const float total = REST ? others + stored : others, p = sum_of(sums[0]);
-        const float left = REST ? fmaxf(0.0f, 1.0f - p) : 0.0f;
+        float left = REST ? fmaxf(0.0f, 1.0f - p) : 0.0f;
+        if (REST && others == 0.0f && left <= rounding_of((float)sum, (float)(zm * a.inv))) left = 0.0f;
         if (GRAD) {
             const float by = w * a.by, part_of = total == 0.0f ? 0.0f : __fdividef(by, total);      // total 0: every logit is -inf
             const float of = left > 0.0f && others > 0.0f ? part_of * (1.0f - left * (total / others)) : part_of;

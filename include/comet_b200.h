@@ -642,7 +642,8 @@ COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f32_i64(
      grad    = d loss / d x, in x's type; may be x itself (same ldx), or NULL: no gradient.
    A row that stores nothing, or nothing but -inf, or whose weight is 0, has a loss and a gradient of 0, and its logits are
    not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf; the q of what is not listed is 0 in f32 once
-   it lies more than 87 temperatures below the largest logit.  Columns of a row ascend; repeated ones are next to each other, and
+   it lies more than 87 temperatures below the largest logit.  A rest that is 0 but for rounding (left below 2^-20 (2 + |lse| +
+   |largest val / temperature|)) and has a q of 0, as where all columns are listed, adds nothing.  Columns of a row ascend; repeated ones are next to each other, and
    their p add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
    bits). */
 COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_bf16_i64(

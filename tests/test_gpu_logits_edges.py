@@ -113,3 +113,43 @@ def test_top_entries_sums_of_large_quotients(cols, kind):
     x, x64 = large_quotients(kind, cols)
     for tau in [1.0, 1e-7, 1e-9] + BESIDE:
         check_top(x, x64, 5, tau)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols,k,near", [(1, 1, 0.0), (64, 64, 0.0), (64, 64, 30.0), (700, 700, -20.0), (1024, 1024, 5.0), (5000, 40, 10.0)])
+@pytest.mark.parametrize("tau", [1.0, 0.7])
+def test_distill_complete_lists(cols, k, near, tau, kind):
+    """The teacher lists all that it gives any probability, and the student has none elsewhere: what the list's sum lacks of 1 is rounding.  The sum is
+    off by less than TOL, and so is each p beside the teacher's own: twice the tolerance of a list without a sum."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(cols + k)
+    n = 300
+    t, t64 = logits(rng, n, cols, "f32")
+    t += near
+    x, _ = logits(rng, n, cols, kind)
+    if k < cols:
+        hidden = torch.ones((n, cols), dtype=torch.bool)
+        hidden.scatter_(1, torch.from_numpy(np.argsort(rng.random((n, cols)), 1)[:, :k].copy()), False)
+        t[hidden.cuda()] = -math.inf
+        x[hidden.cuda()] = -math.inf
+    S, lse = device.top_entries(t, k, temperature=tau, lse=True)
+    loss, rows, grad = device.distill_loss(S, x, temperature=tau, lse=lse)
+    crd, val = S.crd.cpu().numpy(), S.val.double().cpu().numpy()
+    wrows, wloss, wgrad, off, roff = distill(np.arange(n + 1) * k, crd, val, x.double().cpu().numpy(), tau)
+    assert (np.abs(rows.double().cpu().numpy() - wrows) <= 2 * roff).all()
+    assert math.isfinite(float(loss))
+    close_gradient(grad, wgrad, 2 * off, kind)
+
+
+def test_distill_a_rest_that_the_student_cannot_have():
+    """A complete list whose sum lacks more than rounding: the rest has a probability, and the student gives it none."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(22)
+    x, x64 = logits(rng, 3, 40, "f32")
+    S, lse = device.top_entries(x + 1, 40, lse=True)
+    lse += torch.tensor([0.0, 0.001, 0.4], device="cuda")
+    loss, rows, grad = device.distill_loss(S, x, lse=lse)
+    assert abs(float(rows[0])) < TOL * 30 and rows[1] == math.inf and rows[2] == math.inf and loss == math.inf
+    assert not grad.isnan().any()
