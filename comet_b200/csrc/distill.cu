@@ -3,7 +3,8 @@
 //   p_j = exp(z_j / temperature) / sum over the row's entries                      (without lse)
 //   p_j = exp(z_j / temperature - lse), left = max(0, 1 - sum p)                   (with lse: the rest is one outcome)
 // a row's loss is sum p (log p - log q) [+ left (log left - log q_rest), q_rest = the sum of q where nothing is stored], and
-//   d loss / d x_j = (q_j - p_j) / temperature where an entry is stored, q_j (1 - left / q_rest) / temperature elsewhere.
+//   d loss / d x_j = (M q_j - p_j) / temperature where an entry is stored, q_j (M - left / q_rest) / temperature elsewhere,
+// with M = sum p + left: 1, unless the list's probabilities exceed 1 and nothing is left.
 // q_rest is a sum of its own, not 1 minus the rest: where the teacher lists nearly all, the difference would have no digits left.
 //
 // A cluster of CTAs takes a row: each has its part of the row copied into shared memory (16 bytes a copy, no registers), so
@@ -323,7 +324,8 @@ distill_kernel(const DistillArgs a)
         float left = REST ? fmaxf(0.0f, 1.0f - p) : 0.0f;
         if (REST && others == 0.0f && left <= rounding_of((float)sum, (float)(zm * a.inv))) left = 0.0f;
         if (GRAD) {
-            const float by = w * a.by, part_of = total == 0.0f ? 0.0f : __fdividef(by, total);      // total 0: every logit is -inf
+            const float by = w * a.by, sum_p = REST && left == 0.0f ? p : 1.0f;
+            const float part_of = total == 0.0f ? 0.0f : sum_p * __fdividef(by, total);             // total 0: every logit is -inf
             const float of = left > 0.0f && others > 0.0f ? part_of * (1.0f - left * (total / others)) : part_of;
             const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
             if (alike && top.near && col0 >= 0 && col0 + n * N <= a.ncols) {            // no granule that is not all the row's

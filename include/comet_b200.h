@@ -643,7 +643,8 @@ COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f32_i64(
    A row that stores nothing, or nothing but -inf, or whose weight is 0, has a loss and a gradient of 0, and its logits are
    not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf; the q of what is not listed is 0 in f32 once
    it lies more than 87 temperatures below the largest logit.  A rest that is 0 but for rounding (left below 2^-20 (2 + |lse| +
-   |largest val / temperature|)) and has a q of 0, as where all columns are listed, adds nothing.  Columns of a row ascend; repeated ones are next to each other, and
+   |largest val / temperature|)) and has a q of 0, as where all columns are listed, adds nothing.  Where the p exceed 1 together (an lse
+   below the list's own), left is 0 and the gradient that of the sum over the list, (sum p) q - p.  Columns of a row ascend; repeated ones are next to each other, and
    their p add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
    bits). */
 COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_bf16_i64(

@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_gpu_logits import TOL, TYPES, check_top, close_gradient, csr, distill, log_sum_exp, logits, teacher, torch_type
+from tests.test_gpu_logits import TOL, TYPES, check_top, close_gradient, csr, distill, log_softmax, log_sum_exp, logits, teacher, torch_type
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,51 @@ def test_distill_a_rest_that_the_student_cannot_have():
     loss, rows, grad = device.distill_loss(S, x, lse=lse)
     assert abs(float(rows[0])) < TOL * 30 and rows[1] == math.inf and rows[2] == math.inf and loss == math.inf
     assert not grad.isnan().any()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols,less", [(40, 0.3), (9001, 0.01), (131072, 2.0)])
+def test_distill_lists_above_their_sum(cols, less, kind):
+    """A list whose probabilities add up to more than 1: nothing is left, and the gradient is that of sum p (log p - log q), (sum p) q - p."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(cols)
+    x, x64 = logits(rng, 6, cols, kind)
+    S, pos, crd, val = teacher(rng, 6, cols, 9, False)
+    for tau in (1.0, 2.0):
+        lse = np.array([log_sum_exp(val[a:b] / tau) - less for a, b in zip(pos, pos[1:])], np.float32)
+        loss, rows, grad = device.distill_loss(S, x, temperature=tau, lse=torch.from_numpy(lse).cuda(), scale=64.0)
+        wrows, wgrad, off, roff = np.zeros(6), np.zeros_like(x64), np.zeros_like(x64), np.zeros(6)
+        for t in range(6):
+            at = slice(pos[t], pos[t + 1])
+            logq = log_softmax(x64[t] / tau)
+            logp = val[at] / tau - float(lse[t])
+            p = np.exp(logp)
+            wrows[t] = (p * (logp - logq[crd[at]])).sum()
+            roff[t] = TOL * p.sum() * (1 + np.abs(logp).max() + np.abs(logq[crd[at]]).max())
+            wgrad[t], off[t] = p.sum() * np.exp(logq), 2 * p.sum() * np.exp(logq)      # the sum is off by TOL too
+            wgrad[t, crd[at]] -= p
+            off[t, crd[at]] += p
+        assert (np.abs(rows.double().cpu().numpy() - wrows) <= roff).all()
+        close_gradient(grad, wgrad * 64 / tau, TOL * off * 64 / tau, kind)
+
+
+@pytest.mark.parametrize("listed", [7, 40])
+def test_distill_gradient_of_lists_above_their_sum_against_differences(listed):
+    """Central differences with h = 1/16: the third derivative of (sum p) log sum exp is below 0.1 e^0.4, so h^2 / 6 times it is below 1e-4; two losses below
+    12 within 1e-6 of themselves, over 2 h, add 2e-4."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(23)
+    x, _ = logits(rng, 1, 40, "f32", 1.0)
+    S, pos, crd, val = teacher(rng, 1, 40, listed, False)
+    lse = torch.tensor([log_sum_exp(val) - 0.4], dtype=torch.float32, device="cuda")
+    grad = device.distill_loss(S, x, lse=lse)[2]
+    h = 1 / 16
+    for j in list(crd[:4]) + [0, 39, 20]:
+        at = []
+        for d in (h, -h):
+            y = x.clone()
+            y[0, j] += d
+            at.append(float(device.distill_loss(S, y, lse=lse, grad=False)[0]))
+        assert abs((at[0] - at[1]) / (2 * h) - float(grad[0, j])) < 3e-4
