@@ -304,6 +304,9 @@ struct LogSum {
     }
 };
 
+// The log of a row's sum; with a maximum of +inf (no NaN then) s is of differences of infinities, and the sum is +inf.
+__device__ __forceinline__ float log_of_sum(float m, float s, float inv) { return fabsf(m) == -MINUS_INF ? m : fmaf(log2f(s), LN2, m * inv); }
+
 // The first step's bound, by all threads: each of eight warps finds the ceil(k / 8)-th largest of its 128 granules' largest entries, and k
 // entries reach the least of those keys.  Of fewer than 256 granules the first warps have 32 each, and only those are asked.
 template <typename T>
@@ -539,7 +542,7 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         cluster_wait();
         if (rank != 0) return;
     }
-    if (LSE && tid == 0) lse[t] = m == MINUS_INF ? m : fmaf(log2f(s), LN2, m * inv);
+    if (LSE && tid == 0) lse[t] = log_of_sum(m, s, inv);
     if (tid == 0) {
         pos[t] = t * k;
         if (t == nrows - 1) pos[nrows] = nrows * k;
@@ -720,7 +723,7 @@ top_short_kernel(int64_t nrows, int ncols, const T *__restrict__ xs, int64_t ldx
 #pragma unroll
         for (int r = 0; r < R; r++) s += exp2_fast((to_float(part.v[r]) - m) * c);
         s = warp_sum(s);
-        if (lane == 0) lse[t] = m == MINUS_INF ? m : fmaf(log2f(s), LN2, m * inv);
+        if (lane == 0) lse[t] = log_of_sum(m, s, inv);
     }
 }
 

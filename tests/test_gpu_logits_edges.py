@@ -201,3 +201,21 @@ def test_distill_gradient_of_lists_above_their_sum_against_differences(listed):
             y[0, j] += d
             at.append(float(device.distill_loss(S, y, lse=lse, grad=False)[0]))
         assert abs((at[0] - at[1]) / (2 * h) - float(grad[0, j])) < 3e-4
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols,k", [(5, 2), (64, 8), (300, 40), (900, 9), (9001, 20), (9001, 600), (131072, 8)])
+def test_top_entries_sum_of_infinity(cols, k, kind):
+    """The sum of a row with +inf is +inf, with NaN NaN."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(cols)
+    x, _ = logits(rng, 8, cols, kind)
+    for t, at in enumerate([(0,), (cols - 1,), (cols // 2, 1), (0, cols - 1), (3,)]):
+        x[t, list(at)] = math.inf
+    x[3, 1] = -math.inf
+    x[4, 4 % cols] = math.nan
+    x[5, :] = math.inf
+    x[6, :] = -math.inf
+    got = device.top_entries(x, k, lse=True)[1].cpu()
+    assert (got[[0, 1, 2, 3, 5]] == math.inf).all() and got[4].isnan() and got[6] == -math.inf and got[7].isfinite()
