@@ -428,7 +428,7 @@ static int distill_loss(int64_t nrows, int64_t ncols, const int64_t *pos, const 
     const double temperature = temperature_scale[0], scale = temperature_scale[1];
     if (nrows < 0 || ncols <= 0) return fail("distill_loss: %lld rows of %lld columns", (long long)nrows, (long long)ncols);
     if (ldx < ncols || (grad && ldg < ncols)) return fail("distill_loss: leading dimension smaller than the number of columns");
-    if (!(temperature > 0.0) || temperature > 1e30) return fail("distill_loss: temperature %g is not a positive number", temperature);
+    if (!temperature_fits(temperature)) return fail("distill_loss: temperature %g is not a number of 1e-38 to 1e30", temperature);
     if (val_bytes != 4 && val_bytes != 8) return fail("distill_loss: the teacher's values have 4 or 8 bytes");
     if (ncols > (int64_t)MOST_CLUSTER * MOST_SLICE / (int64_t)sizeof(T) - 64)
         return fail("distill_loss: rows of %lld columns do not fit the shared memory of eight SMs", (long long)ncols);

@@ -10,6 +10,8 @@ namespace cb200 {
 
 static const int MOST_CLUSTER = 8;                  // CTAs of a cluster that every device takes
 static const double LOG2E_D = 1.4426950408889634;
+// 1 / temperature and log2(e) / temperature are f32 numbers
+inline bool temperature_fits(double t) { return t >= 1e-38 && t <= 1e30; }
 
 #ifdef __CUDACC__
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;

@@ -777,7 +777,8 @@ static int top_entries(int64_t nrows, int64_t ncols, const void *x, int64_t ldx,
     if (ldx < ncols) return fail("top_entries: leading dimension smaller than the number of columns");
     if (k < 1 || k > ncols || k > MOST_K) return fail("top_entries: %lld entries a row; 1 to %d, and no more than a row has", (long long)k, MOST_K);
     if (nrows > 0x7fffffffLL) return fail("top_entries: more than 2^31 rows");
-    if (lse && !(*temperature > 0.0 && *temperature <= 1e30)) return fail("top_entries: temperature %g is not a positive number", *temperature);
+    if (lse && !temperature) return fail("top_entries: the sum needs a temperature");
+    if (temperature && !temperature_fits(*temperature)) return fail("top_entries: temperature %g is not a number of 1e-38 to 1e30", *temperature);
     if ((uintptr_t)x % sizeof(T)) return fail("top_entries: an address that is not a multiple of the element's size");
     if (nrows == 0) {
         CB_CUDA(cudaMemsetAsync(pos, 0, sizeof(int64_t), st));

@@ -616,12 +616,12 @@ COMET_B200_EXPORT int32_t comet_b200_dev_masked_spgemm_count_f64_i64(
 /* Dense operands are row-major with unit column stride, in bf16, f16 or f32 (the suffix); arithmetic is in f32 and a result  */
 /* is rounded once.  Any row stride and any address that is a multiple of the element's size will do.  The floating options */
 /* are read from host memory during the call.  Refused (non-zero status): no columns, a leading dimension below the number   */
-/* of columns, a temperature that is not positive, and what each entry point names.                                          */
+/* of columns, a temperature below 1e-38 or above 1e30, and what each entry point names.                                     */
 
 /* The k largest entries (1 <= k <= 1024, k <= ncols < 2^30) of each row of x as a CSR matrix: pos[nrows+1], crd and val
    [nrows*k], columns ascending.  Of equal entries the lower column is taken; NaN is above all numbers, -0 equals 0, and
    -inf is an entry like any other.  lse (may be NULL): lse[nrows] = log(sum_j exp(x_j / *temperature)) of the whole row,
-   -inf for a row of -inf, +inf for a row with +inf and without NaN. */
+   -inf for a row of -inf, +inf for a row with +inf and without NaN.  temperature may be NULL where lse is. */
 COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_bf16_i64(
     int64_t nrows, int64_t ncols, const void *x, int64_t ldx, int64_t k, const double *temperature, int64_t *pos,
     int64_t *crd, float *val, float *lse, void *stream);

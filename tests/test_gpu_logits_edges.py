@@ -219,3 +219,19 @@ def test_top_entries_sum_of_infinity(cols, k, kind):
     x[6, :] = -math.inf
     got = device.top_entries(x, k, lse=True)[1].cpu()
     assert (got[[0, 1, 2, 3, 5]] == math.inf).all() and got[4].isnan() and got[6] == -math.inf and got[7].isfinite()
+
+
+def test_temperatures_that_are_refused():
+    """1 / temperature has to be an f32 number; without a sum the entries' temperature is checked all the same."""
+    import torch
+    from comet_b200 import _lib, device
+    x = torch.zeros((4, 9), device="cuda")
+    S, _ = csr(4, 9, [1, 1, 1, 1], [0, 1, 2, 3], [1, 1, 1, 1])
+    for bad in (0.0, -1.0, math.nan, math.inf, 1e-39, 1e31):
+        for call in (lambda: device.distill_loss(S, x, temperature=bad), lambda: device.top_entries(x, 2, temperature=bad, lse=True),
+                     lambda: device.top_entries(x, 2, temperature=bad)):
+            with pytest.raises(_lib.CometB200Error, match="temperature"):
+                call()
+    for good in (1e-37, 1e30):
+        assert abs(float(device.distill_loss(S, x, temperature=good, scale=0.25)[0]) - math.log(9)) < TOL * 4
+        assert abs(float(device.top_entries(x, 2, temperature=good, lse=True)[1][0]) - math.log(9)) < TOL * 4
