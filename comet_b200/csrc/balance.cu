@@ -153,7 +153,7 @@ __device__ __forceinline__ double take_rows(const BalanceArgs &a, const Tally &t
 #pragma unroll
             for (int q = 0; q < Q; q++) {
                 if (WHOLE) {
-                    if (has(q, 0)) n.x[q] = __ldg((const uint4 *)r + q * G + l);
+                    if (has(q, 0)) n.x[q] = ((const uint4 *)r)[q * G + l];       // no read-only load: the gradient may be R
                 } else {
                     T *v = (T *)&n.x[q];
 #pragma unroll

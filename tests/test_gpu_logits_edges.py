@@ -7,7 +7,8 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_gpu_logits import TOL, TYPES, check_top, close_gradient, csr, distill, log_softmax, log_sum_exp, logits, teacher, torch_type
+from tests.test_gpu_logits import (TOL, TYPES, check_balance, check_top, choices, close_gradient, csr, distill, log_softmax, log_sum_exp, logits,
+                                   teacher, torch_type)
 
 pytestmark = pytest.mark.gpu
 
@@ -235,3 +236,21 @@ def test_temperatures_that_are_refused():
     for good in (1e-37, 1e30):
         assert abs(float(device.distill_loss(S, x, temperature=good, scale=0.25)[0]) - math.log(9)) < TOL * 4
         assert abs(float(device.top_entries(x, 2, temperature=good, lse=True)[1][0]) - math.log(9)) < TOL * 4
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,cols", [(9000, 8), (9000, 64), (3000, 256), (700, 1024), (9000, 9), (2000, 100)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_balance_in_place_beyond_one_cluster(rows, cols, scores, kind):
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows + cols)
+    x, x64 = logits(rng, rows, cols, kind)
+    S, pos, crd = choices(rng, rows, cols, min(cols, 4), True)
+    seq = torch.tensor([0, rows // 3, rows // 3, rows], device="cuda")
+    apart = device.balance_loss(S, x, seq=seq, scores=scores, scale=64.0)
+    check_balance(S, pos, crd, x.clone(), x64, kind, seq.tolist(), None, scores, 64.0)
+    loss, counts, grad = device.balance_loss(S, x, seq=seq, scores=scores, scale=64.0, grad=x)
+    assert grad is x
+    for a, b in zip(apart, (loss, counts, x)):
+        assert torch.equal(a, b)
