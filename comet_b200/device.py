@@ -179,7 +179,9 @@ def masked_pair_count(A, B, M, row_lo=0, row_hi=None, out=None):
 
 
 # Rows of logits beside a CSR matrix.  The logits are CUDA matrices with unit column stride, in bf16, f16 or f32; the
-# results are new tensors, and every call is asynchronous on the current stream.
+# results are new tensors without a graph (the gradients are for torch.autograd.backward), and every call is asynchronous on the
+# current stream.  A gradient written in place of the logits counts as an operation in place: a graph that has saved them refuses its
+# backward pass.
 _LOGITS = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
 _TOP, _DISTILL, _BALANCE = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _LOGITS.items()}
                             for op in ("top_entries", "distill_loss", "balance_loss"))
@@ -239,7 +241,9 @@ def _gradient(what, X, shape, grad):
         return None, 0, 0
     if grad.dtype is not X.dtype or grad.shape != shape:
         raise ValueError(what + ": the gradient must have the logits' shape, type and device")
-    return grad, grad.data_ptr(), _check_logits(what, grad)[2]
+    ld = _check_logits(what, grad)[2]
+    torch.autograd.graph.increment_version(grad)       # written by its address: a graph that has saved it has to know
+    return grad, grad.data_ptr(), ld
 
 
 def top_entries(X, k, temperature=1.0, lse=False):

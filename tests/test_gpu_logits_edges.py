@@ -254,3 +254,21 @@ def test_balance_in_place_beyond_one_cluster(rows, cols, scores, kind):
     assert grad is x
     for a, b in zip(apart, (loss, counts, x)):
         assert torch.equal(a, b)
+
+
+def test_gradients_in_place_are_seen_by_autograd():
+    """Logits that a graph has saved and that a call overwrites: the backward pass refuses them, as after any operation in place."""
+    import torch
+    from comet_b200 import device
+    S, _ = csr(4, 9, [1, 1, 1, 1], [0, 1, 2, 3], [1, 1, 1, 1])
+    for op in (device.distill_loss, device.balance_loss):
+        w = torch.randn((4, 9), device="cuda", requires_grad=True)
+        y = w * 2
+        z = (y * y).sum()
+        op(S, y.detach(), grad=y.detach())
+        with pytest.raises(RuntimeError, match="inplace"):
+            z.backward()
+        y = w * 2
+        z = (y * y).sum()
+        op(S, y.detach())                                              # a gradient of its own disturbs nothing
+        z.backward()
