@@ -434,7 +434,7 @@ static int launch_balance(BalanceArgs a, cudaStream_t st)
     if (words <= SMALL_COUNTS && a.nrows * a.ncols <= SMALL_ELEMENTS && a.nrows * 4 < SMALL_ELEMENTS) {
         int ranks = 1;
         while (ranks < MOST_CLUSTER && a.nrows * a.ncols > (int64_t)ranks * 4096) ranks *= 2;
-        return launch_cluster(balance_small_kernel<T, G, Q, SIGMOID, WHOLE>, (unsigned)ranks, ranks, BT, 0, st, a);
+        return launch_cluster(balance_small_kernel<T, G, Q, SIGMOID, WHOLE>, (unsigned)ranks, ranks, BT, 0, 0, st, a);
     }
     constexpr int AT_ONCE = BW * 32 / G;
     const int64_t most = (int64_t)sm_count() * 8;

@@ -402,11 +402,11 @@ static int launch_distill(DistillArgs a, cudaStream_t st)
     int ranks = 1;
     while (ranks < MOST_CLUSTER && (ceil_div(all, ranks) * 16 > SLICE + 64 || (a.nrows * ranks < sm_count() && all / ranks >= 2 * DT))) ranks *= 2;
     a.slice = ((int)ceil_div(all, ranks) + 1) & ~1;
-    const size_t smem = (size_t)a.slice * 16 + (REST ? ((size_t)a.slice * N + 127) / 128 * 16 : 0);
+    auto room = [](size_t granules) { return granules * 16 + (REST ? (granules * N + 127) / 128 * 16 : 0); };
     if (a.slice * 16 > MOST_SLICE) return fail("distill_loss: rows of %d columns do not fit the shared memory of eight SMs", a.ncols);
     const bool few = a.nrows <= 256;               // the last row's warp adds them up
     if (!few) a.counter = nullptr;
-    CB_TRY(launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, smem, st, a));
+    CB_TRY(launch_cluster(distill_kernel<T, TV, REST, GRAD>, (unsigned)(a.nrows * ranks), ranks, DT, room(a.slice), room(MOST_SLICE / 16), st, a));
     if (!few) CB_CUDA(launch_behind(distill_sum_kernel, dim3(1), 1024, 0, st, a));
     return 0;
 }

@@ -350,11 +350,12 @@ __device__ __forceinline__ bool last_of(unsigned *counter, unsigned ctas)
     return atomicInc(counter, ctas - 1) == ctas - 1;
 }
 
-// `ctas` CTAs in clusters of `ranks`
+// `ctas` CTAs in clusters of `ranks`.  `most`: the dynamic shared memory of the kernel's largest call.  It is the limit in every call, so that a
+// second host thread, on its way to another call, does not lower the limit between this one's setting and its launch.
 template <typename... P, typename... A>
-inline int launch_cluster(void (*kernel)(P...), unsigned ctas, int ranks, int threads, size_t smem, cudaStream_t st, A... args)
+inline int launch_cluster(void (*kernel)(P...), unsigned ctas, int ranks, int threads, size_t smem, size_t most, cudaStream_t st, A... args)
 {
-    if (smem > 16 * 1024) CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 16 * 1024) CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = ranks;

@@ -763,7 +763,7 @@ static int launch_long(const TopCall &a)
     if (a.nrows * ranks > 0x7fffffffLL) return fail("top_entries: more than 2^31 rows");
     // beyond 256 entries the candidates of a row without barriers would not fit their room
     auto kernel = a.k <= 256 ? top_kernel<T, LSE, true> : top_kernel<T, LSE, false>;
-    return launch_cluster(kernel, (unsigned)(a.nrows * ranks), ranks, TT, smem, a.st, a.nrows, a.ncols, (int)ceil_div(all, ranks),
+    return launch_cluster(kernel, (unsigned)(a.nrows * ranks), ranks, TT, smem, smem, a.st, a.nrows, a.ncols, (int)ceil_div(all, ranks),
                           (const T *)a.x, a.ldx, a.k, colbits, a.c, a.inv, a.pos, a.crd, a.val, a.lse);
 }
 

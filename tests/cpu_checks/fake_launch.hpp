@@ -27,6 +27,7 @@ static std::map<const void *, std::string> &names()
 }
 static std::vector<Launch> launches;
 static std::function<void(const std::string &, void **)> on_launch;
+static std::function<void(const std::string &, int)> on_shared_limit;              // a kernel's largest dynamic shared memory is set
 static size_t pool_room = ~(size_t)0;               // what one cudaMallocAsync may ask for
 
 static int launched(const char *name)
@@ -83,7 +84,11 @@ cudaError_t __cudaPopCallConfiguration(dim3 *grid, dim3 *block, size_t *smem, vo
 }
 cudaError_t cudaLaunchKernel(const void *f, dim3 grid, dim3 block, void **args, size_t, cudaStream_t) { return fake::launch(f, grid, block, args); }
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *c, const void *f, void **args) { return fake::launch(f, c->gridDim, c->blockDim, args); }
-cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
+cudaError_t cudaFuncSetAttribute(const void *f, cudaFuncAttribute what, int v)
+{
+    if (fake::on_shared_limit && what == cudaFuncAttributeMaxDynamicSharedMemorySize) fake::on_shared_limit(fake::names()[f], v);
+    return cudaSuccess;
+}
 cudaError_t cudaGetDevice(int *d) { *d = 0; return cudaSuccess; }
 cudaError_t cudaGetLastError() { return cudaSuccess; }
 const char *cudaGetErrorString(cudaError_t) { return "made to fail"; }

@@ -74,3 +74,12 @@ def test_scratch_that_a_call_can_do_without(tmp_path):
                            os.path.join(ROOT, "comet_b200", "csrc", "runtime.cu"), "-no-pie",
                            "-Wl,--unresolved-symbols=ignore-in-object-files", "-o", exe])
     assert output(exe) == "ok"
+
+
+def test_a_kernel_of_rows_of_logits_has_one_limit(tmp_path_factory):
+    """Two host threads set a kernel's limit at once: had each call its own, the smaller one could come between the larger one and its launch."""
+    lines = output(link(tmp_path_factory, "distill_limit_check.cpp", "distill.o"), 9000, 50021, 131072, 380000).splitlines()
+    assert len(lines) == 8
+    for line in lines:
+        low, high = map(int, line.split())
+        assert low == high <= 226 * 1024                               # 227 KB with what is not dynamic
