@@ -21,8 +21,8 @@
 namespace cb200 {
 
 static const int BT = 256, BW = BT / 32, MOST_EXPERTS = 1024;
-// Logits of the one-launch kernel.  Rows of 64 bf16, one launch against two, us on the device: 128 rows 7.5, 9.4; 1024 9.3, 9.6; 2048 11.7, 9.6.  The host
-// spends a launch less, too.
+// Logits of the one-launch kernel.  bf16, one launch against two, us on the device (calls in a graph): 128 rows of 64 6.3, 8.1; 1000 of 64 7.9, 8.1; 250 of 256 8.2,
+// 8.6; 63 of 1024 9.6, 11.3; 4096 of 8 7.4, 8.0, but 8000 of 8 10.8, 8.1.  2048 rows of 64 would take 2 us more than with two.  The host spends a launch less, too.
 static const int64_t SMALL_ELEMENTS = 65536;
 static const int SMALL_COUNTS = 2048;              // sequences times (experts + 2) that the one-launch kernel holds
 static const int KEPT_COUNTS = 16384;              // and that are counted in memory that every call leaves at 0

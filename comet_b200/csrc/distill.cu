@@ -11,9 +11,9 @@
 // X is read from HBM once, and the maximum, the sums and the gradient are three passes over shared memory.  What the CTAs of
 // a row have to tell each other are five floats, written into each other's shared memory.
 //
-// Bound: HBM, the bytes of X and of the gradient, but the clock first: 4096 x 131072 bf16 with gradient take 482 us (4.46 TB/s) where the bytes take
+// Bound: HBM, the bytes of X and of the gradient, but the clock first: 4096 x 131072 bf16 with gradient take 487 us (4.42 TB/s) where the bytes take
 // 328: 20 warps on an SM issue an instruction every second clock (dependences, the exponential unit 53 % of the time, the barriers of a
-// row), and under this load the SM clock falls to about 1.5 GHz.  65536 columns of f16 without a gradient: 125 us, 72 by the bytes.
+// row), and under this load the SM clock falls to about 1.5 GHz.  65536 columns of f16 without a gradient: 124 us, 72 by the bytes.
 // Slices of 32 KB by 128 threads leave room for six CTAs on an SM, which fill each other's waits: 506 us at the time, with 64 KB and 256
 // threads 514, with 32 KB and 256 threads 543.  A cluster that stays and goes from row to row, with the next one on its way: 495 to 640.
 #include "logits.cuh"

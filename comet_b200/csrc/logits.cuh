@@ -343,7 +343,7 @@ __device__ __forceinline__ unsigned long long peer_load(const unsigned long long
 }
 
 // One of the counters by which the last CTA of a launch finds out that it is the last.  Each goes back to 0 by itself
-// (atomicInc), a call takes the next one of 1024, so calls on two streams do not meet.
+// (atomicInc); a call takes the next one of 1024.
 __device__ __forceinline__ bool last_of(unsigned *counter, unsigned ctas)
 {
     __threadfence();

@@ -7,9 +7,10 @@
 // that k entries reach, so few entries of the rest pass it; they are candidates, in shared memory.  A histogram of their keys
 // raises the bound (stream_free), or, when they become many, the k largest are kept and the k-th is the new bound (stream_stepwise).
 //
-// Bound: 4096 x 131072 bf16, k = 64, with the log of the sum: 279 us, 3.85 TB/s, 164 by the bytes: instructions, 45 k a row of which 16 k are the
-// exponentials' sums.  777 x 50021 f16, k = 200, without: 53 us, 12 by the bytes: the choice among the candidates (five waves of CTAs end
-// with it).  One row of 131072 f32 in a cluster of eight: 18 us.  A step with a barrier each, bounds by selection: 362 us for the first.
+// Bound: 4096 x 131072 bf16, k = 64, with the log of the sum: 282 us, 3.81 TB/s, 164 by the bytes: instructions, 52 k a row of which 16 k are the
+// exponentials' sums.  777 x 50021 f16, k = 200, without: 53 us, 12 by the bytes: the choice among the candidates, with which each of 1.75
+// waves of CTAs ends (three on an SM).  One row of 131072 f32 in a cluster of eight: 18 us.  A step with a barrier each, bounds by selection: 362 us
+// for the first.
 #include <atomic>
 
 #include "logits.cuh"

@@ -248,7 +248,8 @@ def _gradient(what, X, shape, grad):
 
 def top_entries(X, k, temperature=1.0, lse=False):
     """The k largest entries of each row of X (1 <= k <= 1024) as a DeviceCSR with float32 values, columns ascending; of equal entries the lower
-    column, NaN above all numbers.  Returns (matrix, the log of the sum of each row's exp(X / temperature), or None)."""
+    column, NaN above all numbers.  Returns (matrix, the log of the sum of each row's exp(X / temperature), or None); the sparse operations take the
+    matrix with its values converted to float64."""
     n, m, ld = _check_logits("top_entries", X)
     k = int(k)
     if not 1 <= k <= min(1024, m):
@@ -265,10 +266,12 @@ def distill_loss(S, X, temperature=1.0, lse=None, weight=None, scale=1.0, grad=T
     """Distillation from a teacher's top logits: S holds them (DeviceCSR of X's shape, float32 or float64 values, columns of a row ascending), X the
     student's.  With q = softmax(X / temperature) and p = exp(S / temperature) over the sum of the row's entries, a row's loss is
     sum p (log p - log q) over the entries.  lse: the log of the sum of exp(teacher / temperature) over the teacher's whole rows, as top_entries gives
-    it; p is then a part of the whole row, and all that is not stored counts as one outcome.  Rows that store nothing, or whose weight is 0, are
+    it; p is then a part of the whole row, and all that is not stored counts as one outcome (none, where the list's p are 1 but for rounding and the
+    student gives nothing to the rest).  Rows that store nothing, or whose weight is 0, are
     left out.  One entry in each row: the cross entropy with that column.
 
-    Returns (scale * sum of weight * rows, rows, its gradient).  grad: True (a new tensor), False (none), or a tensor to write it to, such as X."""
+    Returns (scale * sum of weight * rows, rows, the gradient of the first with respect to X).  grad: True (a new tensor), False (none), or a tensor to write
+    it to, such as X."""
     n, m, ld = shape = _check_logits("distill_loss", X)
     pos, crd = _check_beside("distill_loss", S, n, m)
     width = 4 if S.val.dtype is torch.float32 else 8
@@ -288,7 +291,8 @@ def balance_loss(S, R, seq=None, mask=None, scores="softmax", scale=1.0, grad=Tr
     nothing do not).  The loss is scale * the mean over sequences with such rows of E * sum_e f_e P_e, f_e the share of the sequence's entries in column e and
     P_e the mean over its rows of p_e, with p = softmax(R) or, for scores="sigmoid", sigmoid(R) over the row's sum.
 
-    Returns (loss, counts[sequences, E] as int64, gradient with respect to R).  grad: True (a new tensor), False (none), or a tensor to write it to."""
+    Returns (loss, counts[sequences, E] as int64, gradient with respect to R).  grad: True (a new tensor), False (none), or a tensor to write it to, such
+    as R.  Calls on one device share the memory that counts, and must not overlap."""
     n, m, ld = shape = _check_logits("balance_loss", R)
     pos, crd = _check_beside("balance_loss", S, n, m)
     if scores not in ("softmax", "sigmoid"):

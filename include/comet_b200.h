@@ -644,7 +644,8 @@ COMET_B200_EXPORT int32_t comet_b200_dev_top_entries_f32_i64(
    not read.  A p of 0 adds nothing.  A q of 0 under a p that is not gives +inf; the q of what is not listed is 0 in f32 once
    it lies more than 87 temperatures below the largest logit.  A rest that is 0 but for rounding (left below 2^-20 (2 + |lse| +
    |largest val / temperature|)) and has a q of 0, as where all columns are listed, adds nothing.  Where the p exceed 1 together (an lse
-   below the list's own), left is 0 and the gradient that of the sum over the list, (sum p) q - p.  Columns of a row ascend; repeated ones are next to each other, and
+   below the list's own), left is 0 and the gradient that of the sum over the list, (sum p) q - p.  log p is a difference in f64 with
+   lse, and in val's type without; val beyond f32 may be double.  Columns of a row ascend; repeated ones are next to each other, and
    their p add up.  A column outside the matrix makes the row's loss NaN.  A row may have up to 1.5 MB (786,368 columns of 16
    bits). */
 COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_bf16_i64(
@@ -666,7 +667,8 @@ COMET_B200_EXPORT int32_t comet_b200_dev_distill_loss_f32_i64(
      counts[s][e] = entries of active rows in column e,   p = softmax(r), or sigmoid(r) / sum sigmoid(r) if sigmoid != 0
      loss = *scale * mean over sequences with active rows of  ncols * sum_e (counts[s][e] / K_s) * (mean over active rows of p_e)
      grad = d loss / d r (the counts have no gradient), in r's type, 0 in rows that are not active; may be r itself, or NULL.
-   A row whose logits are all -inf counts, and has p = 0.  A column outside the matrix makes the loss NaN. */
+   A row whose logits are all -inf counts, and has p = 0.  A column outside the matrix makes the loss NaN.  The counting uses device memory that all
+   calls on a device share: calls that overlap mix their counts. */
 COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_bf16_i64(
     int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, int64_t nseq, const int64_t *seq, const
     uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
