@@ -238,6 +238,21 @@ def test_temperatures_that_are_refused():
         assert abs(float(device.top_entries(x, 2, temperature=good, lse=True)[1][0]) - math.log(9)) < TOL * 4
 
 
+def test_entry_points_without_a_temperature():
+    """The C entry of top_entries takes no temperature where it gives no sum, and refuses its absence where it does."""
+    import torch
+    from comet_b200 import _lib, device
+    x = torch.randn((3, 40), device="cuda")
+    pos, crd = torch.empty(4, dtype=torch.int64, device="cuda"), torch.empty(6, dtype=torch.int64, device="cuda")
+    val, lse = torch.empty(6, device="cuda"), torch.empty(3, device="cuda")
+    call = lambda sums: device._call("comet_b200_dev_top_entries_f32_i64", 3, 40, x.data_ptr(), 40, 2, 0, pos.data_ptr(), crd.data_ptr(),  # noqa: E731
+                                     val.data_ptr(), sums, device._stream())
+    call(0)
+    assert torch.equal(val.view(3, 2).sort(1).values, x.topk(2, 1).values.sort(1).values)
+    with pytest.raises(_lib.CometB200Error, match="temperature"):
+        call(lse.data_ptr())
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("rows,cols", [(9000, 8), (9000, 64), (3000, 256), (700, 1024), (9000, 9), (2000, 100)])
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
