@@ -1,0 +1,683 @@
+// The feed-forward block of a router's experts.  A CSR matrix says which rows of x (tokens) go to which experts; its entries e = (t, j) have a row each
+// in h.  With w = [gate; up] of expert j (2 inner x width) and v (width x inner):
+//   gated     h_e = act(gate x_t) * (up x_t)                 dz_e = [dh_e * up x_t * act'(gate x_t), dh_e * act(gate x_t)]
+//                                                            dx_t = sum_e w' dz_e,  dw_j = sum_e dz_e x_t'
+//   combine   y_t = sum_e val_e v h_e                        dval_e = h_e (v' dy_t),  dh_e = val_e v' dy_t,  dv_j = sum_e val_e dy_t h_e'
+// act(g) = g s(u) with the logistic function s, u = g for silu and 2 sqrt(2 / pi) (g + 0.044715 g^3) for gelu (its tanh form).
+//
+// All of these are one kernel: tiles of 128 x 256 sums in tensor memory, 64 terms a step, with the operands' tiles in a ring of four in shared
+// memory.  A warp fetches (rows of x, h, dz and dy by their number, four a copy, so nothing is sorted or copied first; padding is a number outside, and
+// reads as zeros), a thread issues the products, four warps take the sums of the tile before out of tensor memory.  Three forms:
+//   ROWS   rows of a tile's tokens, times a weight whose rows are outputs                (forward passes, dz)
+//   BACK   the same, times a weight whose rows are the sum's index                       (dx, v' dy)
+//   OUTER  sums over an expert's tokens of two rows                                      (dw, dv)
+// Sums of a token's experts go through f32 rows, one for each entry, and are added in the entries' order: the same bits in every call.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <string.h>
+
+#include "groups.cuh"
+#include "logits.cuh"
+#include "stream.cuh"
+#include "tensor.cuh"
+
+namespace cb200 {
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static int make_map(const char *what, const void *base, bool bf16, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                    CUtensorMap *map)
+{
+    static EncodeTiled encode = nullptr;
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn || q != cudaDriverEntryPointSuccess)
+            return fail("%s: cuTensorMapEncodeTiled is not available from this driver", what);
+        encode = (EncodeTiled)fn;
+    }
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, (void *)base, dims, strides, box, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : fail("%s: cuTensorMapEncodeTiled refused a map (error %d)", what, (int)r);
+}
+
+int make_gather_map(const char *what, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, CUtensorMap *map)
+{
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, 1};
+    return make_map(what, base, bf16, 2, dims, strides, box, map);
+}
+
+int make_box_map(const char *what, const void *base, bool bf16, int64_t depth, int64_t rows, int64_t cols, int box_rows, CUtensorMap *map)
+{
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth}, strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(cols * rows) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    return make_map(what, base, bf16, 3, dims, strides, box, map);
+}
+
+enum Form { ROWS, BACK, OUTER };
+enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
+
+static const int TM = 128, TN = 256, TK = 64, RING = 4;
+static const int A_BYTES = TM * TK * 2, B_BYTES = TN * TK * 2, STEP_BYTES = A_BYTES + B_BYTES;
+static const int PRODUCT_THREADS = 192, PRODUCT_SMEM = RING * STEP_BYTES + 1024;
+
+struct ProductArgs {
+    Groups g;
+    const int *rows_a, *rows_b;      // the numbers of each slot's row of a, of b (OUTER)
+    int none_a, none_b;              // a number outside
+    int terms;                       // of the sums (not OUTER)
+    int tiles_m, tiles_n;            // tiles of a weight's rows (OUTER), tiles of columns
+    int rows, cols;                  // of an expert's result (OUTER), of a result row
+    int64_t nnz;
+    bool gelu;
+    const void *other;               // dh, h
+    const float *val;
+    void *out, *scaled;              // 16-bit results; val * h
+    float *sums;                     // rows of f32, or sums of products per tile of columns
+};
+
+__device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + exp2_fast(-LOG2E * u)); }
+// what s() takes, and its slope
+__device__ __forceinline__ float2 gate_of(float g, bool gelu)
+{
+    constexpr float A = 1.5957691216057308f, B = 0.044715f;                          // 2 sqrt(2 / pi)
+    return gelu ? make_float2(A * fmaf(B * g * g, g, g), A * fmaf(3.0f * B * g, g, 1.0f)) : make_float2(g, 1.0f);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *to, const float *v)
+{
+    Granule<T> out;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = v[i];
+    out.pack(f);
+    *(uint4 *)to = out.w;
+}
+template <typename T>
+__device__ __forceinline__ void load8(float *v, const T *from)
+{
+    Granule<T> in;
+    in.w = *(const uint4 *)from;
+    float f[8];
+    in.unpack(f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = f[i];
+}
+
+// A tile's sums, 32 columns at a time, by the thread that has the row; at: tensor memory of the warp's rows.  entry < 0: nothing to store.
+template <typename T, int SUMS>
+__device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, bool none, int tile_m, int tile_n, int group, int row, int64_t entry)
+{
+    if constexpr (SUMS == GATED || SUMS == GATED_GRAD) {
+        const int f0 = tile_n * (TN / 2), inner = a.cols;
+#pragma unroll 1
+        for (int c = 0; c < TN / 2; c += 32) {
+            __syncwarp();
+            if (f0 + c >= inner) break;            // the same for all
+            float gate[32], up[32];
+            tmem_load(at + c, gate);
+            tmem_load(at + TN / 2 + c, up);
+            if (entry < 0) continue;
+            if (SUMS == GATED) {
+                T *h = (T *)a.out + entry * inner + f0 + c;
+#pragma unroll
+                for (int i = 0; i < 32; i++) gate[i] = gate[i] * logistic(gate_of(gate[i], a.gelu).x) * up[i];
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    if (f0 + c + i < inner) store8<T>(h + i, gate + i);
+            } else {
+                T *dz = (T *)a.out + entry * 2 * inner + f0 + c;
+                const T *dh = (const T *)a.other + entry * inner + f0 + c;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (f0 + c + i >= inner) break;
+                    float d[8];
+                    load8<T>(d, dh + i);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float g = gate[i + j];
+                        const float2 u = gate_of(g, a.gelu);
+                        const float s = logistic(u.x);
+                        gate[i + j] = d[j] * up[i + j] * fmaf(g * s * (1.0f - s), u.y, s);
+                        up[i + j] = d[j] * g * s;
+                    }
+                    store8<T>(dz + i, gate + i);
+                    store8<T>(dz + inner + i, up + i);
+                }
+            }
+        }
+    } else if constexpr (SUMS == ENTRY_ROWS) {
+        const int c0 = tile_n * TN;
+        const float by = entry >= 0 && a.val ? a.val[entry] : 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < TN; c += 32) {
+            __syncwarp();
+            if (c0 + c >= a.cols) break;
+            float v[32];
+            tmem_load(at + c, v);
+            if (entry < 0) continue;
+            float4 *to = (float4 *)(a.sums + entry * a.cols + c0 + c);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                if (c0 + c + i < a.cols) to[i / 4] = make_float4(by * v[i], by * v[i + 1], by * v[i + 2], by * v[i + 3]);
+        }
+    } else if constexpr (SUMS == COMBINE_GRAD) {
+        const int c0 = tile_n * TN;
+        const float by = entry >= 0 ? a.val[entry] : 0.0f;
+        float sum = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < TN; c += 32) {
+            __syncwarp();
+            if (c0 + c >= a.cols) break;
+            float v[32];
+            tmem_load(at + c, v);
+            if (entry < 0) continue;
+            const int64_t first = entry * a.cols + c0 + c;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                if (c0 + c + i >= a.cols) break;
+                float h[8];
+                load8<T>(h, (const T *)a.other + first + i);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    sum = fmaf(v[i + j], h[j], sum);
+                    v[i + j] *= by;
+                    h[j] *= by;
+                }
+                store8<T>((T *)a.out + first + i, v + i);
+                store8<T>((T *)a.scaled + first + i, h);
+            }
+        }
+        if (entry >= 0) a.sums[tile_n * a.nnz + entry] = sum;
+    } else {
+        const int c0 = tile_n * TN, r = tile_m * TM + row;
+        T *out = (T *)a.out + ((int64_t)group * a.rows + r) * a.cols + c0;
+#pragma unroll 1
+        for (int c = 0; c < TN; c += 32) {
+            __syncwarp();
+            if (c0 + c >= a.cols) break;
+            float v[32];
+            if (none) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = 0.0f;
+            } else {
+                tmem_load(at + c, v);
+            }
+            if (r >= a.rows) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+                if (c0 + c + i < a.cols) store8<T>(out + c + i, v + i);
+        }
+    }
+}
+
+// An entry whose column is no expert's: NaN.  By four warps.
+template <typename T, int SUMS>
+__device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
+{
+    const int bad = SUMS == WEIGHT ? 0 : a.g.head[1];
+    const float nan = __int_as_float(0x7fffffff);
+    for (int i = blockIdx.x; i < bad; i += gridDim.x) {
+        const int64_t entry = a.g.order[a.g.slots - 1 - i];
+        const int cols = SUMS == GATED_GRAD ? 2 * a.cols : a.cols;
+        for (int c = thread; c < cols; c += 128) {
+            if (SUMS == ENTRY_ROWS) a.sums[entry * cols + c] = nan;
+            else ((T *)a.out)[entry * cols + c] = from_float<T>(nan);
+            if (SUMS == COMBINE_GRAD && c % TN == 0) a.sums[c / TN * a.nnz + entry] = nan;
+        }
+    }
+}
+
+template <typename T, int FORM, int SUMS>
+__global__ void __launch_bounds__(PRODUCT_THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
+{
+    constexpr bool BF16 = sizeof(T) == 2 && Granule<T>::N == 8 && !__is_same(T, __half);
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * RING + 4 + 1];
+    __shared__ uint32_t tmem_room;
+    __shared__ int broken_word;
+    volatile int *broken = &broken_word;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
+                   last = taken + 16;
+    if (warp == 1) tmem_alloc(smem_at(&tmem_room), 2 * TN);
+    if (tid == 0) {
+        for (int i = 0; i < RING; i++) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            bar_init(done + 8 * i, 1);
+            bar_init(taken + 8 * i, 4);
+        }
+        bar_init(last, 1);
+        broken_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_room;
+    wait_for_previous();
+
+    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
+    struct Tile {
+        int m, n, group, steps, slot;
+    };
+    auto tile_of = [&](int id) {
+        Tile t;
+        if (FORM == OUTER) {
+            t.group = id / (a.tiles_m * a.tiles_n);
+            const int rest = id % (a.tiles_m * a.tiles_n);
+            t.m = rest / a.tiles_n;
+            t.n = rest % a.tiles_n;
+            t.steps = (a.g.counts[t.group] + TK - 1) / TK;
+            t.slot = a.g.first[t.group] * GROUP_TILE;
+        } else {
+            t.m = id / a.tiles_n;
+            t.n = id % a.tiles_n;
+            t.group = a.g.column[t.m];
+            t.steps = (a.terms + TK - 1) / TK;
+            t.slot = t.m * GROUP_TILE;
+        }
+        return t;
+    };
+    auto numbers = [&](const int *list, int slot, int none) {
+        int4 r = *(const int4 *)(list + slot);
+        r.x = r.x < 0 ? none : r.x;
+        r.y = r.y < 0 ? none : r.y;
+        r.z = r.z < 0 ? none : r.z;
+        r.w = r.w < 0 ? none : r.w;
+        return r;
+    };
+
+    unsigned step = 0;                             // steps so far; stage = step % RING
+    if (warp == 0) {                               // fetches
+        for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
+            const Tile t = tile_of(id);
+            int4 ra, rb;
+            if (FORM != OUTER) ra = numbers(a.rows_a, t.slot + 4 * lane, a.none_a);
+            bool on = true;
+            for (int k = 0; k < t.steps; k++, step++) {
+                const unsigned s = step % RING;
+                const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
+                if (FORM == OUTER) {
+                    ra = numbers(a.rows_a, t.slot + k * TK + 4 * (lane & 15), a.none_a);
+                    rb = numbers(a.rows_b, t.slot + k * TK + 4 * (lane & 15), a.none_b);
+                }
+                on = bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken);
+                on = __all_sync(0xffffffffu, on);
+                if (!on) break;
+                if (lane == 0) bar_expect(bar, STEP_BYTES);
+                __syncwarp();
+                if (FORM == OUTER) {
+                    // blocks of 64 columns: two of a, four of b, 16 copies each
+                    for (int b = lane >> 4; b < 6; b += 2) {
+                        if (b < 2) load_rows(to + b * 8192 + (lane & 15) * 512, &map_a, t.m * TM + b * 64, ra, bar);
+                        else load_rows(to + b * 8192 + (lane & 15) * 512, &map_b, t.n * TN + (b - 2) * 64, rb, bar);
+                    }
+                } else {
+                    load_rows(to + lane * 512, &map_a, k * TK, ra, bar);
+                    if (FORM == ROWS) {
+                        if (lane < 2) {
+                            if (SUMS == GATED || SUMS == GATED_GRAD)
+                                load_box(to + A_BYTES + lane * (B_BYTES / 2), &map_b, k * TK, t.n * (TN / 2), 2 * t.group + lane, bar);
+                            else
+                                load_box(to + A_BYTES + lane * (B_BYTES / 2), &map_b, k * TK, t.n * TN + lane * (TN / 2), t.group, bar);
+                        }
+                    } else if (lane < 4) {
+                        load_box(to + A_BYTES + lane * 8192, &map_b, t.n * TN + lane * 64, k * TK, t.group, bar);
+                    }
+                }
+            }
+            if (!on) break;
+        }
+        // what is under way lands before the CTA ends
+        if (*broken) {
+            volatile int late = 0;
+            for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
+        }
+    } else if (warp == 1) {                        // issues the products
+        if (lane == 0) {
+            constexpr uint32_t kind = product_descriptor(BF16, TM, TN, FORM == OUTER, FORM != ROWS);
+            unsigned tile = 0;
+            bool on = true;
+            for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
+                const int steps = tile_of(id).steps;
+                if (steps == 0) continue;
+                const unsigned b = tile & 1;
+                on = bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken);
+                tmem_fence_after();
+                for (int k = 0; on && k < steps; k++, step++) {
+                    const unsigned s = step % RING;
+                    on = bar_wait(full + 8 * s, step / RING & 1, broken);
+                    if (!on) break;
+                    tmem_fence_after();
+                    const uint32_t at = ring + s * STEP_BYTES;
+                    const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
+                    // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
+                    constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
+#pragma unroll
+                    for (int i = 0; i < TK / 16; i++) product(tmem + b * TN, da + i * next_a, db + i * next_b, kind, k + i > 0);
+                    products_to(empty + 8 * s);
+                }
+                if (on) products_to(done + 8 * b);
+                tile++;
+            }
+            if (*broken) {                         // products under way end before tensor memory is given back
+                volatile int late = 0;
+                products_to(last);
+                bar_wait(last, 0, &late);
+            }
+        }
+        __syncwarp();
+    } else {                                       // takes the sums
+        spoil<T, SUMS>(a, tid - 64);
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        unsigned tile = 0;
+        for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
+            const Tile t = tile_of(id);
+            const unsigned b = tile & 1;
+            const int64_t entry = FORM == OUTER ? -1 : a.g.order[t.slot + row];
+            if (t.steps > 0) {
+                bool on = bar_wait(done + 8 * b, tile / 2 & 1, broken);
+                on = __all_sync(0xffffffffu, on);
+                if (!on) break;
+                tmem_fence_after();
+            }
+            take_sums<T, SUMS>(a, tmem + b * TN + ((uint32_t)quarter << 21), t.steps == 0, t.m, t.n, t.group, row, entry);
+            if (t.steps > 0) {
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(taken + 8 * b);
+                tile++;
+            }
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 1) tmem_free(tmem, 2 * TN);
+    if (tid == 0 && *broken) a.g.head[2] = 1;
+}
+
+// A token's f32 rows, added in order: 4 columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256)
+add_rows_kernel(int64_t nrows, int cols, const int64_t *__restrict__ pos, const float *__restrict__ sums, T *__restrict__ out)
+{
+    wait_for_previous();
+    const int64_t parts = cols / 8, all = nrows * parts, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= all) return;
+    const int64_t t = i / parts, c = i % parts * 8, lo = pos[t], hi = pos[t + 1];
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const float4 *from = (const float4 *)(sums + lo * cols + c);
+#pragma unroll 4
+    for (int64_t e = lo; e < hi; e++, from += cols / 4) {
+        const float4 x = __ldcs(from), y = __ldcs(from + 1);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    store8<T>(out + t * cols + c, v);
+}
+
+__global__ void __launch_bounds__(256)
+add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__restrict__ out)
+{
+    wait_for_previous();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float v = 0.0f;
+    for (int p = 0; p < parts; p++) v += sums[p * n + i];
+    out[i] = v;
+}
+
+template <typename T, int FORM, int SUMS>
+static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, const ProductArgs &a, cudaStream_t st)
+{
+    auto kernel = product_kernel<T, FORM, SUMS>;
+    CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
+    const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
+    if (tiles > 0x7fffffffLL) return fail("experts: more than 2^31 tiles");
+    const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+    CB_CUDA(launch_behind(kernel, dim3(grid), PRODUCT_THREADS, PRODUCT_SMEM, st, map_a, map_b, a));
+    return 0;
+}
+
+struct Sizes {
+    int64_t nrows, nexperts, nnz, width, inner;
+};
+static int check(const char *what, const Sizes &s)
+{
+    if (s.nrows < 0 || s.nnz < 0 || s.nexperts < 1 || s.nexperts > MOST_GROUPS)
+        return fail("%s: %lld entries in %lld rows of %lld experts (1 to %d)", what, (long long)s.nnz, (long long)s.nrows, (long long)s.nexperts, MOST_GROUPS);
+    if (s.nrows > 0x7ffffff0LL || s.nnz > 0x70000000LL) return fail("%s: more than 2^31 rows, or 1.8e9 entries", what);
+    if (s.width < 8 || s.inner < 8 || s.width % 8 || s.inner % 8 || s.width > 1 << 20 || s.inner > 1 << 20)
+        return fail("%s: width %lld and inner %lld; multiples of 8 up to 2^20", what, (long long)s.width, (long long)s.inner);
+    return 0;
+}
+static int check_at(const char *what, const void *p)
+{
+    return (uintptr_t)p % 16 ? fail("%s: an address that is not a multiple of 16 bytes", what) : 0;
+}
+static int check_rows(const char *what, const void *p, int64_t ld, int64_t cols)
+{
+    if (ld < cols || ld % 8) return fail("%s: a row stride of %lld elements; a multiple of 8, and no less than the row's %lld", what, (long long)ld, (long long)cols);
+    return check_at(what, p);
+}
+
+template <typename T>
+static ProductArgs arguments(const Sizes &s, int32_t *plan)
+{
+    ProductArgs a;
+    memset(&a, 0, sizeof(a));
+    a.g = groups_in(plan, s.nnz, s.nexperts);
+    a.nnz = s.nnz;
+    return a;
+}
+template <typename T>
+static constexpr bool is_bf16() { return !__is_same(T, __half); }
+
+template <typename T>
+static int add_rows(const Sizes &s, const int64_t *pos, const float *sums, void *out, cudaStream_t st)
+{
+    if (s.nrows == 0) return 0;
+    CB_CUDA(launch_behind(add_rows_kernel<T>, dim3((unsigned)ceil_div(s.nrows * (s.width / 8), 256)), 256, 0, st, s.nrows, (int)s.width, pos, sums, (T *)out));
+    return 0;
+}
+
+template <typename T>
+static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void *x, int64_t ldx, const void *w, void *h, cudaStream_t st)
+{
+    const char *what = "gated_experts";
+    clear_error();
+    CB_TRY(check(what, s));
+    CB_TRY(check_rows(what, x, ldx, s.width));
+    CB_TRY(check_at(what, w));
+    CB_TRY(check_at(what, h));
+    if (s.nnz == 0 || s.nrows == 0) return 0;
+    alignas(64) CUtensorMap ma, mb;
+    CB_TRY(make_gather_map(what, x, is_bf16<T>(), s.nrows, s.width, ldx, &ma));
+    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
+    ProductArgs a = arguments<T>(s, plan);
+    a.rows_a = a.g.token;
+    a.none_a = (int)s.nrows;
+    a.terms = (int)s.width;
+    a.tiles_n = (int)ceil_div(s.inner, TN / 2);
+    a.cols = (int)s.inner;
+    a.gelu = gelu != 0;
+    a.out = h;
+    return launch_product<T, ROWS, GATED>(ma, mb, a, st);
+}
+
+// dz: room for nnz x 2 inner; sums: for nnz x width floats (null with dx)
+template <typename T>
+static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, int32_t *plan, const void *x, int64_t ldx, const void *w, const void *dh,
+                              void *dz, float *sums, void *dx, void *dw, cudaStream_t st)
+{
+    const char *what = "gated_experts_grad";
+    clear_error();
+    CB_TRY(check(what, s));
+    CB_TRY(check_rows(what, x, ldx, s.width));
+    for (const void *p : {w, dh, (const void *)dz, (const void *)sums, (const void *)dx, (const void *)dw}) CB_TRY(check_at(what, p));
+    if (s.nnz == 0 || s.nrows == 0) {
+        if (dx) CB_CUDA(cudaMemsetAsync(dx, 0, s.nrows * s.width * sizeof(T), st));
+        if (dw) CB_CUDA(cudaMemsetAsync(dw, 0, 2 * s.nexperts * s.inner * s.width * sizeof(T), st));
+        return 0;
+    }
+    alignas(64) CUtensorMap ma, mb;
+    CB_TRY(make_gather_map(what, x, is_bf16<T>(), s.nrows, s.width, ldx, &ma));
+    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
+    ProductArgs a = arguments<T>(s, plan);
+    a.rows_a = a.g.token;
+    a.none_a = (int)s.nrows;
+    a.terms = (int)s.width;
+    a.tiles_n = (int)ceil_div(s.inner, TN / 2);
+    a.cols = (int)s.inner;
+    a.gelu = gelu != 0;
+    a.other = dh;
+    a.out = dz;
+    CB_TRY((launch_product<T, ROWS, GATED_GRAD>(ma, mb, a, st)));
+    alignas(64) CUtensorMap mz;
+    CB_TRY(make_gather_map(what, dz, is_bf16<T>(), s.nnz, 2 * s.inner, 2 * s.inner, &mz));
+    if (dx) {
+        a = arguments<T>(s, plan);
+        CB_TRY(make_box_map(what, w, is_bf16<T>(), s.nexperts, 2 * s.inner, s.width, TK, &mb));
+        a.rows_a = a.g.order;
+        a.none_a = (int)s.nnz;
+        a.terms = 2 * (int)s.inner;
+        a.tiles_n = (int)ceil_div(s.width, TN);
+        a.cols = (int)s.width;
+        a.sums = sums;
+        CB_TRY((launch_product<T, BACK, ENTRY_ROWS>(mz, mb, a, st)));
+        CB_TRY(add_rows<T>(s, pos, sums, dx, st));
+    }
+    if (dw) {
+        a = arguments<T>(s, plan);
+        a.rows_a = a.g.order;
+        a.none_a = (int)s.nnz;
+        a.rows_b = a.g.token;
+        a.none_b = (int)s.nrows;
+        a.rows = 2 * (int)s.inner;
+        a.cols = (int)s.width;
+        a.tiles_m = (int)ceil_div(2 * s.inner, TM);
+        a.tiles_n = (int)ceil_div(s.width, TN);
+        a.out = dw;
+        CB_TRY((launch_product<T, OUTER, WEIGHT>(mz, ma, a, st)));
+    }
+    return 0;
+}
+
+// sums: room for nnz x width floats
+template <typename T>
+static int combine_experts(const Sizes &s, const int64_t *pos, int32_t *plan, const void *h, const float *val, const void *v, float *sums, void *y,
+                           cudaStream_t st)
+{
+    const char *what = "combine_experts";
+    clear_error();
+    CB_TRY(check(what, s));
+    for (const void *p : {h, v, (const void *)sums, (const void *)y}) CB_TRY(check_at(what, p));
+    if (s.nnz == 0 || s.nrows == 0) {
+        CB_CUDA(cudaMemsetAsync(y, 0, s.nrows * s.width * sizeof(T), st));
+        return 0;
+    }
+    alignas(64) CUtensorMap ma, mb;
+    CB_TRY(make_gather_map(what, h, is_bf16<T>(), s.nnz, s.inner, s.inner, &ma));
+    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TN / 2, &mb));
+    ProductArgs a = arguments<T>(s, plan);
+    a.rows_a = a.g.order;
+    a.none_a = (int)s.nnz;
+    a.terms = (int)s.inner;
+    a.tiles_n = (int)ceil_div(s.width, TN);
+    a.cols = (int)s.width;
+    a.val = val;
+    a.sums = sums;
+    CB_TRY((launch_product<T, ROWS, ENTRY_ROWS>(ma, mb, a, st)));
+    return add_rows<T>(s, pos, sums, y, st);
+}
+
+// scaled: room for nnz x inner; sums: for nnz x ceil(inner / 256) floats
+template <typename T>
+static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, const float *val, const void *v, const void *dy, int64_t lddy, void *scaled,
+                                float *sums, void *dh, void *dv, float *dval, cudaStream_t st)
+{
+    const char *what = "combine_experts_grad";
+    clear_error();
+    CB_TRY(check(what, s));
+    CB_TRY(check_rows(what, dy, lddy, s.width));
+    for (const void *p : {h, v, (const void *)scaled, (const void *)dh, (const void *)dv}) CB_TRY(check_at(what, p));
+    if (s.nnz == 0 || s.nrows == 0) {
+        if (dv) CB_CUDA(cudaMemsetAsync(dv, 0, s.nexperts * s.inner * s.width * sizeof(T), st));
+        return 0;
+    }
+    alignas(64) CUtensorMap my, mb;
+    CB_TRY(make_gather_map(what, dy, is_bf16<T>(), s.nrows, s.width, lddy, &my));
+    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TK, &mb));
+    ProductArgs a = arguments<T>(s, plan);
+    a.rows_a = a.g.token;
+    a.none_a = (int)s.nrows;
+    a.terms = (int)s.width;
+    a.tiles_n = (int)ceil_div(s.inner, TN);
+    a.cols = (int)s.inner;
+    a.other = h;
+    a.val = val;
+    a.out = dh;
+    a.scaled = scaled;
+    a.sums = sums;
+    CB_TRY((launch_product<T, BACK, COMBINE_GRAD>(my, mb, a, st)));
+    CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, a.tiles_n, sums, dval));
+    if (dv) {
+        alignas(64) CUtensorMap mh;
+        CB_TRY(make_gather_map(what, scaled, is_bf16<T>(), s.nnz, s.inner, s.inner, &mh));
+        a = arguments<T>(s, plan);
+        a.rows_a = a.g.token;
+        a.none_a = (int)s.nrows;
+        a.rows_b = a.g.order;
+        a.none_b = (int)s.nnz;
+        a.rows = (int)s.width;
+        a.cols = (int)s.inner;
+        a.tiles_m = (int)ceil_div(s.width, TM);
+        a.tiles_n = (int)ceil_div(s.inner, TN);
+        a.out = dv;
+        CB_TRY((launch_product<T, OUTER, WEIGHT>(my, mh, a, st)));
+    }
+    return 0;
+}
+
+}  // namespace cb200
+
+#define EXPERTS(suffix, T)                                                                                                                             \
+    extern "C" int32_t comet_b200_dev_gated_experts_##suffix##_i64(int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner,         \
+                                                                   int32_t gelu, int32_t *plan, const void *x, int64_t ldx, const void *w, void *h,     \
+                                                                   void *stream)                                                                       \
+    {                                                                                                                                                  \
+        return cb200::gated_experts<T>({nrows, nexperts, nnz, width, inner}, gelu, plan, x, ldx, w, h, (cudaStream_t)stream);                          \
+    }                                                                                                                                                  \
+    extern "C" int32_t comet_b200_dev_gated_experts_grad_##suffix##_i64(                                                                               \
+        int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t gelu, const int64_t *pos, int32_t *plan, const void *x,     \
+        int64_t ldx, const void *w, const void *dh, void *dz, float *sums, void *dx, void *dw, void *stream)                                           \
+    {                                                                                                                                                  \
+        return cb200::gated_experts_grad<T>({nrows, nexperts, nnz, width, inner}, gelu, pos, plan, x, ldx, w, dh, dz, sums, dx, dw,                    \
+                                            (cudaStream_t)stream);                                                                                     \
+    }                                                                                                                                                  \
+    extern "C" int32_t comet_b200_dev_combine_experts_##suffix##_i64(int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner,       \
+                                                                     const int64_t *pos, int32_t *plan, const void *h, const float *val,               \
+                                                                     const void *v, float *sums, void *y, void *stream)                                \
+    {                                                                                                                                                  \
+        return cb200::combine_experts<T>({nrows, nexperts, nnz, width, inner}, pos, plan, h, val, v, sums, y, (cudaStream_t)stream);                   \
+    }                                                                                                                                                  \
+    extern "C" int32_t comet_b200_dev_combine_experts_grad_##suffix##_i64(                                                                             \
+        int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t *plan, const void *h, const float *val, const void *v,      \
+        const void *dy, int64_t lddy, void *scaled, float *sums, void *dh, void *dv, float *dval, void *stream)                                        \
+    {                                                                                                                                                  \
+        return cb200::combine_experts_grad<T>({nrows, nexperts, nnz, width, inner}, plan, h, val, v, dy, lddy, scaled, sums, dh, dv, dval,             \
+                                              (cudaStream_t)stream);                                                                                   \
+    }
+EXPERTS(bf16, __nv_bfloat16)
+EXPERTS(f16, __half)

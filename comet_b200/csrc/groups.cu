@@ -1,0 +1,134 @@
+// Entries of a CSR matrix grouped by column: a stable counting sort in one launch, by a cluster of up to eight CTAs.
+//
+// A warp has a stretch of rows, a lane a row of 32 of them at a time; it counts its entries by column (lanes with the same column find each
+// other, so there are no atomics and the order is always the same), the counts are summed over the warps and, through the
+// cluster's shared memory, over the CTAs, and a second walk over the rows puts each entry where the sums say.
+//
+// Bound: the chains of loads of the two walks.
+#include "groups.cuh"
+#include "logits.cuh"
+
+namespace cb200 {
+
+static const int GT = 1024, GW = GT / 32;
+
+__global__ void __launch_bounds__(GT)
+group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
+{
+    extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
+    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], sums[GW];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    int *own = warps + (size_t)warp * n;
+    for (int i = tid; i < GW * n; i += GT) warps[i] = 0;
+    if (rank == 0 && tid < GROUP_HEAD) g.head[tid] = 0;
+    __syncthreads();
+    const int64_t each = (nrows + (int64_t)ranks * GW - 1) / ((int64_t)ranks * GW), from = min((rank * GW + warp) * each, nrows);
+    const int64_t to = min(from + each, nrows);
+    // each lane's entries of a row, one after the other; what(entry, its row, its column, the lanes that have the same one)
+    auto walk = [&](auto what) {
+        for (int64_t r = from; r < to; r += 32) {
+            int64_t lo = 0, hi = 0;
+            if (r + lane < to) {
+                lo = min(max(pos[r + lane], (int64_t)0), nnz);
+                hi = min(max(pos[r + lane + 1], lo), nnz);
+            }
+            int64_t next = lo < hi ? crd[lo] : 0;
+            while (__any_sync(0xffffffffu, lo < hi)) {
+                const bool on = lo < hi;
+                const int64_t col = next, e = lo++;
+                if (lo < hi) next = crd[lo];
+                const bool good = on && col >= 0 && col < n;
+                const unsigned alike = __match_any_sync(0xffffffffu, good ? (int)col : -1);
+                if (on) what(e, r + lane, good ? (int)col : -1, alike);
+                __syncwarp();
+            }
+        }
+    };
+    walk([&](int64_t, int64_t, int col, unsigned alike) {
+        if (col >= 0 && lane == __ffs(alike) - 1) own[col] += __popc(alike);
+    });
+    __syncthreads();
+    int total = 0, before = 0;
+    if (tid < n) {
+        int sum = 0;
+        for (int w = 0; w < GW; w++) {
+            const int v = warps[w * n + tid];
+            warps[w * n + tid] = sum;
+            sum += v;
+        }
+        mine[tid] = sum;
+    }
+    __syncthreads();
+    if (ranks > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (tid < n)
+        for (unsigned r = 0; r < ranks; r++) {
+            const int v = ranks > 1 ? peer_load(&mine[tid], r) : mine[tid];
+            if (r < rank) before += v;
+            total += v;
+        }
+    const int tiles = (total + GROUP_TILE - 1) / GROUP_TILE;
+    int upto = tiles;                              // inclusive sums over the columns
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) upto += sums[w];
+    if (tid < n) {
+        start[tid] = (upto - tiles) * GROUP_TILE + before;
+        if (rank == 0) {
+            g.counts[tid] = total;
+            g.first[tid] = upto - tiles;
+            for (int i = 0; i < tiles; i++) g.column[upto - tiles + i] = tid;
+            if (tid == n - 1) g.first[n] = g.head[0] = upto;
+        }
+        if (tid % ranks == rank)
+            for (int i = total; i < tiles * GROUP_TILE; i++) g.order[(int64_t)(upto - tiles) * GROUP_TILE + i] = g.token[(int64_t)(upto - tiles) * GROUP_TILE + i] = -1;
+    }
+    __syncthreads();
+    for (int i = tid; i < GW * n; i += GT) warps[i] += start[i % n];
+    __syncthreads();
+    if (ranks > 1) cluster_arrive();               // this CTA has read the others' counts
+    walk([&](int64_t e, int64_t row, int col, unsigned alike) {
+        if (col < 0) {
+            g.order[g.slots - 1 - atomicAdd(&g.head[1], 1)] = (int)e;
+            return;
+        }
+        const int at = own[col] + __popc(alike & ((1u << lane) - 1));
+        __syncwarp(alike);
+        if (lane == 31 - __clz(alike)) own[col] = at + 1;
+        g.order[at] = (int)e;
+        g.token[at] = (int)row;
+    });
+    __syncwarp();
+    if (ranks > 1) cluster_wait();                 // its own stay until they have been read
+}
+
+static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_t *pos, const int64_t *crd, int32_t *plan, cudaStream_t st)
+{
+    clear_error();
+    if (nrows < 0 || nnz < 0 || ncols < 1 || ncols > MOST_GROUPS)
+        return fail("group_entries: %lld entries in %lld rows of %lld columns (1 to %d)", (long long)nnz, (long long)nrows, (long long)ncols, MOST_GROUPS);
+    if (nrows > 0x7fffffffLL || nnz > 0x70000000LL) return fail("group_entries: more than 2^31 rows, or 1.8e9 entries");
+    const size_t row = (size_t)ncols * GW * sizeof(int);
+    int ranks = 1;                                 // a CTA has 1024 rows under way at a time
+    while (ranks < MOST_CLUSTER && nrows > (int64_t)ranks * GT) ranks *= 2;
+    return launch_cluster(group_kernel, (unsigned)ranks, ranks, GT, row, (size_t)MOST_GROUPS * GW * sizeof(int), st, nrows, nnz, pos, crd,
+                          groups_in(plan, nnz, ncols));
+}
+
+}  // namespace cb200
+
+extern "C" int64_t comet_b200_dev_group_entries_size(int64_t nnz, int64_t ncols) { return cb200::group_size(nnz, ncols); }
+
+extern "C" int32_t comet_b200_dev_group_entries_i64(int64_t nrows, int64_t ncols, int64_t nnz, const int64_t *pos, const int64_t *crd, int32_t *plan,
+                                                    void *stream)
+{
+    return cb200::group_entries(nrows, ncols, nnz, pos, crd, plan, (cudaStream_t)stream);
+}

@@ -312,3 +312,140 @@ def balance_loss(S, R, seq=None, mask=None, scores="softmax", scale=1.0, grad=Tr
     _call(_BALANCE[R.dtype], n, m, pos, crd, nseq, bounds, on, int(scores == "sigmoid"), R.data_ptr(), ld, to, ldg, options[0], counts.data_ptr(),
           loss.data_ptr(), _stream())
     return loss, counts, out
+
+
+# A router's experts: products of the rows that a CSR matrix (rows tokens, columns experts) sends to each of them.  The operands are contiguous CUDA
+# tensors in bf16 or f16, but for rows of tokens, whose stride may be any multiple of 8 elements; sums are in f32 and results rounded once.
+_EXPERTS = {torch.bfloat16: "bf16", torch.float16: "f16"}
+_GATED, _GATED_GRAD, _COMBINE, _COMBINE_GRAD = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _EXPERTS.items()}
+                                                for op in ("gated_experts", "gated_experts_grad", "combine_experts", "combine_experts_grad"))
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+class EntryGroups:
+    """The entries of a CSR matrix by column, as group_entries gives them.  `S` is the matrix, whose pos and crd must stay as they were."""
+
+    def __init__(self, S, plan):
+        self.S, self.plan = S, plan
+
+    def check(self):
+        """Raises if a kernel that worked with these groups gave up waiting for its own copies or products (its results are incomplete then).  Waits
+        for the device."""
+        if int(self.plan[2]):
+            raise _lib.CometB200Error("experts: a wait inside a kernel ran out; results of these groups are incomplete")
+
+
+def group_entries(S):
+    """The entries of S (DeviceCSR, at most 1024 columns; rows tokens, columns experts) grouped by column, for gated_experts and combine_experts and their
+    gradients: once for a router's choices, whatever is computed with them.  An entry whose column lies outside makes its results NaN."""
+    if S.row_ids is not None:
+        raise ValueError("group_entries: the matrix must be CSR (a row that stores nothing is empty there)")
+    if not 1 <= S.ncols <= 1024:
+        raise ValueError("group_entries: 1 to 1024 columns")
+    if not S.pos.is_cuda or S.nnz > 0x70000000 or S.nrows > 0x7ffffff0:
+        raise ValueError("group_entries: a matrix on a CUDA device, with fewer than 2^31 rows and at most 1.8e9 entries")
+    pos, crd = _check_beside("group_entries", S, S.nrows, S.ncols)
+    nnz, n = S.nnz, S.ncols
+    tiles = nnz // 128 + min(nnz, n) + 1                       # as csrc/groups.cuh counts
+    plan = S.pos.new_empty(16 + (n + 3) // 4 * 4 + (n + 4) // 4 * 4 + (tiles + 3) // 4 * 4 + 256 * tiles, dtype=torch.int32)
+    _call("comet_b200_dev_group_entries_i64", S.nrows, n, nnz, pos, crd, plan.data_ptr(), _stream())
+    return EntryGroups(S, plan)
+
+
+def _check_experts(what, G, name, M, entries, cols=None):
+    """(columns, row stride) of a matrix with a row for each entry (contiguous) or each token."""
+    if not (isinstance(M, torch.Tensor) and M.dtype in _EXPERTS and M.dim() == 2) or M.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("%s: %s must be a matrix of bfloat16 or float16 on the current CUDA device" % (what, name))
+    n, m = M.shape
+    ld, step = M.stride()
+    if n <= 1:
+        ld, step = m, step if n else 1
+    if n != (G.S.nnz if entries else G.S.nrows) or (cols is not None and m != cols):
+        raise ValueError("%s: %s must have a row for each %s%s" % (what, name, "entry" if entries else "row of the matrix of entries",
+                                                                    "" if cols is None else ", and %d columns" % cols))
+    if (step != 1 and m != 1) or ld < m or ld % 8 or (entries and ld != m) or M.data_ptr() % 16:
+        raise ValueError("%s: rows of %s must be contiguous%s and begin at multiples of 16 bytes" % (what, name, " and without gaps" if entries else ""))
+    return m, ld
+
+
+def _check_weights(what, G, name, W, dtype, rows, cols):
+    """Of one matrix per expert: the sizes that are None."""
+    if not isinstance(W, torch.Tensor) or W.dim() != 3 or W.dtype is not dtype or W.get_device() != torch._C._cuda_getDevice() or not W.is_contiguous() \
+            or W.data_ptr() % 16:
+        raise ValueError("%s: %s must be a contiguous tensor of three dimensions, of the other operands' type and device, at a multiple of 16 bytes" % (what, name))
+    e, r, c = W.shape
+    if e != G.S.ncols or (rows is not None and r != rows) or (cols is not None and c != cols) or c % 8 or c < 8:
+        raise ValueError("%s: %s must be [%d, %s, %s], its last size a multiple of 8" % (what, name, G.S.ncols, "any" if rows is None else rows,
+                                                                                       "any" if cols is None else cols))
+    return r, c
+
+
+def _check_gated(what, G, X, W, activation):
+    width, ld = _check_experts(what, G, "X", X, False)
+    rows, _ = _check_weights(what, G, "W", W, X.dtype, None, width)
+    if rows % 16 or rows < 16:
+        raise ValueError(what + ": W must have twice as many rows an expert as H has columns, which is a multiple of 8")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(what + ": activation must be 'silu' or 'gelu'")
+    return (G.S.nrows, G.S.ncols, G.S.nnz, width, rows // 2, _ACTIVATIONS[activation]), ld
+
+
+def gated_experts(G, X, W, activation="silu"):
+    """The first half of experts' feed-forward blocks.  G: group_entries of S; X [rows of S, width]; W [experts, 2 inner, width], an expert's gate first, then
+    its up projection.  Returns H [entries of S, inner]: for the entry (t, j), act(gate_j x_t) * (up_j x_t), in the order of the entries.
+    activation: "silu", or "gelu" (the tanh form).  width and inner are multiples of 8."""
+    sizes, ld = _check_gated("gated_experts", G, X, W, activation)
+    H = X.new_empty((G.S.nnz, sizes[4]))
+    _call(_GATED[X.dtype], *sizes, G.plan.data_ptr(), X.data_ptr(), ld, W.data_ptr(), H.data_ptr(), _stream())
+    return H
+
+
+def gated_experts_grad(G, X, W, d_H, activation="silu", grad_x=True, grad_w=True):
+    """The gradients of gated_experts with respect to X and W, from d_H, the one with respect to H (None where grad_x or grad_w is False).  The products of the
+    forward pass are computed again; their gradients are rounded to X's type before they are multiplied with W and X."""
+    sizes, ld = _check_gated("gated_experts_grad", G, X, W, activation)
+    if d_H.dtype is not X.dtype:
+        raise ValueError("gated_experts_grad: d_H must have X's type")
+    _check_experts("gated_experts_grad", G, "d_H", d_H, True, sizes[4])
+    nnz, width, inner = sizes[2:5]
+    new = X.new_empty
+    dz, sums = new((nnz, 2 * inner)), new((nnz, width), dtype=torch.float32) if grad_x else None
+    d_X, d_W = new((G.S.nrows, width)) if grad_x else None, new(W.shape) if grad_w else None
+    _call(_GATED_GRAD[X.dtype], *sizes, G.S.pos.data_ptr(), G.plan.data_ptr(), X.data_ptr(), ld, W.data_ptr(), d_H.data_ptr(), dz.data_ptr(), _p(sums),
+          _p(d_X), _p(d_W), _stream())
+    return d_X, d_W
+
+
+def _check_combine(what, G, H, V):
+    inner, _ = _check_experts(what, G, "H", H, True)
+    width, _ = _check_weights(what, G, "V", V, H.dtype, None, inner)
+    if width % 8:
+        raise ValueError(what + ": V must have a multiple of 8 rows an expert")
+    if G.S.val is None:
+        raise ValueError(what + ": the matrix of entries needs values, the weights of the experts' outputs")
+    return (G.S.nrows, G.S.ncols, G.S.nnz, width, inner), _check_vector(what, G.S.val, torch.float32, G.S.nnz)
+
+
+def combine_experts(G, H, V):
+    """The second half: Y [rows of S, width], for each row the sum over its entries (t, j) of S's value (float32) times V_j h, h the entry's row of H
+    [entries, inner]; V [experts, width, inner].  A row that stores nothing gives zeros."""
+    sizes, val = _check_combine("combine_experts", G, H, V)
+    Y, sums = H.new_empty((sizes[0], sizes[3])), H.new_empty((sizes[2], sizes[3]), dtype=torch.float32)
+    _call(_COMBINE[H.dtype], *sizes, G.S.pos.data_ptr(), G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), sums.data_ptr(), Y.data_ptr(), _stream())
+    return Y
+
+
+def combine_experts_grad(G, H, V, d_Y, grad_v=True):
+    """The gradients of combine_experts with respect to H, V (None where grad_v is False) and S's values (float32), from d_Y, the one with respect to Y.  For V's,
+    the products of values and rows of H are rounded to H's type first."""
+    sizes, val = _check_combine("combine_experts_grad", G, H, V)
+    if d_Y.dtype is not H.dtype:
+        raise ValueError("combine_experts_grad: d_Y must have H's type")
+    _, ld = _check_experts("combine_experts_grad", G, "d_Y", d_Y, False, sizes[3])
+    nnz, inner = sizes[2], sizes[4]
+    new = H.new_empty
+    scaled, sums = new((nnz, inner)), new(nnz * ((inner + 255) // 256), dtype=torch.float32)
+    d_H, d_V, d_values = new((nnz, inner)), new(V.shape) if grad_v else None, new(nnz, dtype=torch.float32)
+    _call(_COMBINE_GRAD[H.dtype], *sizes, G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), d_Y.data_ptr(), ld, scaled.data_ptr(), sums.data_ptr(),
+          d_H.data_ptr(), _p(d_V), d_values.data_ptr(), _stream())
+    return d_H, d_V, d_values

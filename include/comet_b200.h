@@ -682,6 +682,55 @@ COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_f32_i64(
     uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
     int64_t *counts, float *loss, void *stream);
 
+/* ---- a router's experts --------------------------------------------------------------------------------------------------- */
+/* pos/crd: a CSR matrix of which experts (columns) take which tokens (rows), nnz entries, columns of a row in any order.  The  */
+/* operands are bf16 or f16 (the suffix), row-major, at multiples of 16 bytes; width and inner are multiples of 8.  Arithmetic   */
+/* is in f32, results are rounded once; the same call gives the same bits.                                                       */
+
+/* The entries grouped by column, for the calls below: `plan` is int32 memory of comet_b200_dev_group_entries_size(nnz, ncols)
+   elements at a multiple of 16 bytes, which they read.  1 <= ncols <= 1024.  Element 2 becomes 1 if a later call that works with the plan gave up
+   waiting inside a kernel (its results are incomplete then).  An entry whose column is outside makes its results NaN. */
+COMET_B200_EXPORT int64_t comet_b200_dev_group_entries_size(int64_t nnz, int64_t ncols);
+COMET_B200_EXPORT int32_t comet_b200_dev_group_entries_i64(
+    int64_t nrows, int64_t ncols, int64_t nnz, const int64_t *pos, const int64_t *crd, int32_t *plan, void *stream);
+
+/* h[nnz x inner]: for the entry (t, j) act(gate_j x_t) * (up_j x_t), with w[nexperts x 2 inner x width] holding gate_j above up_j and
+   act(g) = g / (1 + exp(-g)), or, with gelu != 0, g / (1 + exp(-2 sqrt(2 / pi) (g + 0.044715 g^3))).  x: nrows x width with a row stride of
+   ldx, a multiple of 8. */
+COMET_B200_EXPORT int32_t comet_b200_dev_gated_experts_bf16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t gelu, int32_t *plan, const void *x,
+    int64_t ldx, const void *w, void *h, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_gated_experts_f16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t gelu, int32_t *plan, const void *x,
+    int64_t ldx, const void *w, void *h, void *stream);
+
+/* Its gradients dx[nrows x width] and dw (w's shape; either may be NULL) from dh (h's shape).  dz: room for nnz x 2 inner elements (the gradients of
+   the products, rounded to the operands' type); sums: for nnz x width floats (may be NULL where dx is). */
+COMET_B200_EXPORT int32_t comet_b200_dev_gated_experts_grad_bf16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t gelu, const int64_t *pos, int32_t *plan,
+    const void *x, int64_t ldx, const void *w, const void *dh, void *dz, float *sums, void *dx, void *dw, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_gated_experts_grad_f16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t gelu, const int64_t *pos, int32_t *plan,
+    const void *x, int64_t ldx, const void *w, const void *dh, void *dz, float *sums, void *dx, void *dw, void *stream);
+
+/* y[nrows x width] = for each row the sum over its entries (t, j) of val * v_j h, h the entry's row of h[nnz x inner], v[nexperts x width x
+   inner]; 0 for a row that stores nothing.  sums: room for nnz x width floats. */
+COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_bf16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, int32_t *plan, const void *h,
+    const float *val, const void *v, float *sums, void *y, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_f16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, int32_t *plan, const void *h,
+    const float *val, const void *v, float *sums, void *y, void *stream);
+
+/* Its gradients dh (h's shape), dv (v's shape; may be NULL) and dval[nnz] from dy (nrows x width, row stride lddy, a multiple of 8).  scaled: room
+   for nnz x inner elements (val * h, rounded to the operands' type, which dv is computed with); sums: for nnz x ceil(inner / 256) floats. */
+COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_grad_bf16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t *plan, const void *h, const float *val,
+    const void *v, const void *dy, int64_t lddy, void *scaled, float *sums, void *dh, void *dv, float *dval, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_grad_f16_i64(
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t *plan, const void *h, const float *val,
+    const void *v, const void *dy, int64_t lddy, void *scaled, float *sums, void *dh, void *dv, float *dval, void *stream);
+
 /* Measurement aid (no counterpart in the reference): the bare gather SpMM / SDDMM are built around.  For
    each of the nnz column indices the k-double row b[crd[p], :] is read and folded into a sum; out
    (device, at least 8 * ctas_per_sm * SM-count doubles) receives one partial sum per warp.  fold_rows > 0
