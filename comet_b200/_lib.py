@@ -110,6 +110,8 @@ for _t in ("bf16", "f16", "f32"):
                                                     [c_int64, c_void_p, c_int64] + [c_void_p] * 4),
         "comet_b200_dev_balance_loss_%s_i64" % _t: (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32,
                                                     c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 4),
+        "comet_b200_dev_log_probs_%s_i64" % _t: (c_int32, [c_int64] * 2 + [c_void_p] * 3 + [c_int64] + [c_void_p] * 4 + [c_int64] + [c_void_p] * 4),
+        "comet_b200_dev_log_probs_grad_%s_i64" % _t: (c_int32, [c_int64] * 2 + [c_void_p] * 3 + [c_int64] + [c_void_p] * 6 + [c_int64, c_void_p]),
     })
 # a router's experts, per type of their operands
 SIGNATURES["comet_b200_dev_group_entries_size"] = (c_int64, [c_int64, c_int64])

@@ -1,0 +1,387 @@
+// Log probabilities of given columns of rows of logits, the rows' entropies, and the gradient of both.  With u = x / temperature, m a row's largest logit,
+// s = sum exp(u - m / temperature) and the pattern's entries (t, j):
+//   value = (x_j - m) / temperature - log s,     entropy H = log s - sum exp(u - m / temperature) (u - m / temperature) / s
+// and, with q = exp(value) of every column, d and h the gradients of the values and of the entropy that come in,
+//   dx_j = (sum of d at j - q_j sum of d - h q_j (log q_j + H)) / temperature.
+// What is kept from one to the other is m and log s, two f32 numbers: log s is small whatever the logits and the temperature are, so q is as good
+// as the difference x - m.
+//
+// Forward: one pass; each thread has a maximum and sums of its own (rows.cuh), joined over the CTA and, where there are few rows, over a cluster that
+// has cut the row.  Backward: one pass over pieces of rows, which no other CTA reads, so the gradient may take the place of the logits.
+#include "rows.cuh"
+
+namespace cb200 {
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(TT, 4)
+prob_kernel(int ncols, int slice, const T *__restrict__ xs, int64_t ldx, float c, float inv, const ProbCall a)
+{
+    extern __shared__ uint4 ring[];
+    __shared__ float room[3 * TW], told[3 * MOST_CLUSTER];
+    const int tid = threadIdx.x;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    const int64_t t = blockIdx.x / ranks;
+    const T *x = xs + t * ldx;
+    Way<T> way;
+    way.ring = ring;
+    way.from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15);
+    way.off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+    way.ncols = ncols;
+    way.all = (way.off + ncols + Way<T>::N - 1) / Way<T>::N;
+    way.begin = min((int)rank * slice, way.all);
+    way.end = min(way.begin + slice, way.all);
+    if (ranks > 1) cluster_arrive_relaxed();       // only to say that it is there
+    ProbSum<ENTROPY> sum;
+    sum.start();
+    way.start();
+    const int steps = way.steps();
+    for (int step = 0; step < steps; step++) {
+        const Granule<T> *mine = way.stage(step);
+        Granule<T> g[TU];
+#pragma unroll
+        for (int u = 0; u < TU; u++) g[u] = mine[u * TT];
+        sum.add(g, most_of(most_of(g[0].most(), g[1].most()), most_of(g[2].most(), g[3].most())), c);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float q[2], r[1] = {sum.m};
+    sum.total(q[0], q[1]);
+    cta_reduce<1, TW, true>(r, room);
+    shift_to(r[0], sum.m, c, q[0], q[1]);
+    cta_reduce<2, TW, false>(q, room + TW);
+    float m = r[0], s = q[0], ent = q[1];
+    if (ranks > 1) {
+        cluster_wait();
+        if (tid < (int)ranks) {
+            store_peer(&told[3 * rank], tid, m);
+            store_peer(&told[3 * rank + 1], tid, s);
+            store_peer(&told[3 * rank + 2], tid, ent);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (rank != 0) return;
+        m = told[0];
+        for (unsigned i = 1; i < ranks; i++) m = max_nan(m, told[3 * i]);
+        s = ent = 0.0f;
+        for (unsigned i = 0; i < ranks; i++) {
+            float os = told[3 * i + 1], oe = told[3 * i + 2];
+            shift_to(m, told[3 * i], c, os, oe);
+            s += os;
+            ent += oe;
+        }
+    }
+    give_probs(a, t, x, ncols, RowProb(m, s, ent), inv, tid, TT);
+}
+
+// A row's granules to registers, lane by lane; -inf where there is no row.
+template <typename T, int G>
+__device__ __forceinline__ void load_row(Granule<T> (&g)[G], const T *x, int ncols, int lane)
+{
+    constexpr int N = Granule<T>::N;
+    const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15);
+    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T), all = (off + ncols + N - 1) / N;
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+        const int at = i * 32 + lane;
+        g[i] = Granule<T>::least();
+        if (at < all) {
+            g[i].w = from[at];
+            if (at == 0 || at == all - 1) {
+                T *v = (T *)&g[i];
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    if (at * N + k < off || at * N + k >= off + ncols) v[k] = from_float<T>(MINUS_INF);
+            }
+        }
+    }
+}
+
+// Short rows: a warp each.
+template <typename T, int G, bool ENTROPY>
+__global__ void __launch_bounds__(128)
+prob_short_kernel(int64_t nrows, int ncols, const T *__restrict__ xs, int64_t ldx, float c, float inv, const ProbCall a)
+{
+    const int lane = threadIdx.x & 31;
+    const int64_t t = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
+    if (t >= nrows) return;
+    const T *x = xs + t * ldx;
+    Granule<T> g[G];
+    load_row<T, G>(g, x, ncols, lane);
+    typename Granule<T>::Most most = g[0].most();
+#pragma unroll
+    for (int i = 1; i < G; i++) most = most_of(most, g[i].most());
+    ProbSum<ENTROPY> sum;
+    sum.start();
+    sum.add(g, most, c);
+    float s, ent;
+    sum.total(s, ent);
+    const float m = warp_max(sum.m);
+    shift_to(m, sum.m, c, s, ent);
+    s = warp_sum(s);
+    if (ENTROPY) ent = warp_sum(ent);
+    give_probs(a, t, x, ncols, RowProb(m, s, ent), inv, lane, 32);
+}
+
+struct ProbGrad {
+    int64_t nrows;
+    int ncols;
+    const int64_t *pos, *crd;
+    const float *sums, *values, *entropy, *by_entropy;           // values: their gradients; by_entropy: the entropies' (null: none)
+    int64_t ldx, ldg;
+    float c, inv;
+};
+
+// A row's terms: dx = q (a + b log2 q) where no entry is, and exponents.
+template <bool ENTROPY>
+struct GradRow {
+    float c, m, mc, less, a, b;
+    bool near, none, zero;
+    __device__ __forceinline__ GradRow(const ProbGrad &p, int64_t t, float sum)
+    {
+        const float2 row = ((const float2 *)p.sums)[t];
+        c = p.c;
+        m = row.x;
+        none = m == MINUS_INF;
+        mc = none ? 0.0f : m * c;
+        near = fabsf(mc) < NEAR;
+        less = row.y * LOG2E + (near && !none ? fmaf(m, c, -mc) : 0.0f);             // what the exponent is beyond log2 q
+        const float h = ENTROPY ? p.by_entropy[t] : 0.0f;
+        a = -p.inv * (sum + (ENTROPY && h != 0.0f ? h * p.entropy[t] : 0.0f));
+        b = ENTROPY ? -p.inv * LN2 * h : 0.0f;
+        zero = none || (sum == 0.0f && h == 0.0f);
+    }
+    __device__ __forceinline__ float2 of(float2 x) const
+    {
+        float2 d = near ? fma2(x, make_float2(c, c), make_float2(-mc, -mc)) : make_float2((x.x - m) * c, (x.y - m) * c);
+        d = add2(d, make_float2(-less, -less));
+        const float2 q = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        if (!ENTROPY) return mul2(q, make_float2(a, a));
+        // a q of 0 gives 0, whatever its logarithm: that may be -inf
+        return mul2(q, fma2(make_float2(fmaxf(d.x, -16384.0f), fmaxf(d.y, -16384.0f)), make_float2(b, b), make_float2(a, a)));
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void put_granule(T *g, int col, int ncols, bool alike, const float2 (&v)[Granule<T>::N / 2])
+{
+    constexpr int N = Granule<T>::N;
+    Granule<T> out;
+    out.pack(v);
+    if (alike && col >= 0 && col + N <= ncols) {
+        *(uint4 *)(g + col) = out.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (col + k >= 0 && col + k < ncols) g[col + k] = ((const T *)&out)[k];
+    }
+}
+
+// A piece of a row a CTA: GG granules a thread.  The entries in it leave their gradients in shared memory, with a bit each that says so.
+static const int GT = 256, GG = 4;
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(GT)
+prob_grad_kernel(const ProbGrad p, int pieces, const T *xs, T *grad)
+{
+    constexpr int N = Granule<T>::N, COLS = GT * GG * N;
+    __shared__ uint32_t bits[COLS / 32];
+    __shared__ float came[COLS];
+    const int tid = threadIdx.x, piece = blockIdx.x % pieces;
+    const int64_t t = blockIdx.x / pieces, lo = p.pos[t], hi = p.pos[t + 1];
+    const T *x = xs + t * p.ldx;
+    T *g = grad + t * p.ldg;
+    const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15) + piece * GT * GG;
+    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T), all = (off + p.ncols + N - 1) / N, col0 = piece * COLS - off;
+    const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+    Granule<T> in[GG];
+#pragma unroll
+    for (int i = 0; i < GG; i++)
+        if (piece * GT * GG + i * GT + tid < all) in[i].w = from[i * GT + tid];
+    bool mine = false;
+    if (lo < hi) {
+        for (int i = tid; i < COLS / 32; i += GT) bits[i] = 0;
+        __syncthreads();
+        for (int64_t e = lo + tid; e < hi; e += GT) {
+            const int64_t col = p.crd[e], j = col - col0;
+            if (j < 0 || j >= COLS || col < 0 || col >= p.ncols || (e > lo && p.crd[e - 1] == col)) continue;
+            float d = 0.0f;                        // repeated columns are next to each other
+            for (int64_t i = e; i < hi && p.crd[i] == col; i++) d += p.values[i];
+            came[j] = d * p.inv;
+            atomicOr(&bits[j >> 5], 1u << (j & 31));
+            mine = true;
+        }
+        mine = __syncthreads_or(mine);
+    }
+    float sum = 0.0f;
+    for (int64_t e = lo; e < hi; e++) sum += p.values[e];
+    const GradRow<ENTROPY> row(p, t, sum);
+#pragma unroll
+    for (int i = 0; i < GG; i++) {
+        const int at = i * GT + tid, col = col0 + at * N;
+        if (piece * GT * GG + at >= all) continue;
+        float2 v[N / 2];
+        in[i].unpack(v);
+#pragma unroll
+        for (int k = 0; k < N / 2; k++) v[k] = row.zero ? make_float2(0.0f, 0.0f) : row.of(v[k]);
+        if (mine) {
+            const unsigned on = N == 8 ? ((const uint8_t *)bits)[at] : ((const uint8_t *)bits)[at >> 1] >> ((at & 1) * 4) & 15;
+            if (on)
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    if (on >> k & 1) ((float *)v)[k] = row.none ? 0.0f : ((const float *)v)[k] + came[at * N + k];
+        }
+        put_granule<T>(g, col, p.ncols, alike, v);
+    }
+}
+
+// Short rows: a warp each, which has the whole row in registers.
+template <typename T, int G, bool ENTROPY>
+__global__ void __launch_bounds__(128)
+prob_grad_short_kernel(const ProbGrad p, const T *xs, T *grad)
+{
+    constexpr int N = Granule<T>::N;
+    const int lane = threadIdx.x & 31;
+    const int64_t t = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
+    if (t >= p.nrows) return;
+    const T *x = xs + t * p.ldx;
+    T *g = grad + t * p.ldg;
+    Granule<T> in[G];
+    load_row<T, G>(in, x, p.ncols, lane);
+    const int64_t lo = p.pos[t], hi = p.pos[t + 1];
+    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+    const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+    float sum = 0.0f;
+    for (int64_t e = lo; e < hi; e++) sum += p.values[e];
+    const GradRow<ENTROPY> row(p, t, sum);
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+        const int at = i * 32 + lane, col = at * N - off;
+        if (col >= p.ncols) continue;
+        float2 v[N / 2];
+        in[i].unpack(v);
+#pragma unroll
+        for (int k = 0; k < N / 2; k++) v[k] = row.zero ? make_float2(0.0f, 0.0f) : row.of(v[k]);
+        if (!row.none)
+            for (int64_t e = lo; e < hi; e++) {
+                const int64_t j = p.crd[e] - col;
+                if (j >= 0 && j < N && p.crd[e] >= 0 && p.crd[e] < p.ncols) {
+                    const float d = p.values[e] * p.inv;
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        if (j == k) ((float *)v)[k] += d;
+                }
+            }
+        put_granule<T>(g, col, p.ncols, alike, v);
+    }
+}
+
+template <typename T>
+static int check_logits(const char *what, int64_t nrows, int64_t ncols, const void *x, int64_t ldx, const double *temperature)
+{
+    if (nrows < 0 || ncols <= 0 || ncols >= 1LL << 30) return fail("%s: %lld rows of %lld columns", what, (long long)nrows, (long long)ncols);
+    if (ldx < ncols) return fail("%s: leading dimension smaller than the number of columns", what);
+    if (nrows > 0x7fffffffLL / MOST_CLUSTER) return fail("%s: more than 2^28 rows", what);
+    if (!temperature_fits(*temperature)) return fail("%s: temperature %g is not a number of 1e-38 to 1e30", what, *temperature);
+    if ((uintptr_t)x % sizeof(T)) return fail("%s: an address that is not a multiple of the element's size", what);
+    return 0;
+}
+
+// granules a lane that take any row of ncols columns; 0: the row is not short
+template <typename T>
+static int lane_granules(int64_t ncols)
+{
+    const int64_t all = (ncols + 2 * Granule<T>::N - 2) / Granule<T>::N;
+    return all <= 32 ? 1 : all <= 64 ? 2 : all <= 128 ? 4 : all <= 256 ? 8 : 0;
+}
+
+template <typename T, bool ENTROPY>
+static int launch_probs(int64_t nrows, int ncols, const T *x, int64_t ldx, float c, float inv, const ProbCall &a, cudaStream_t st)
+{
+    const unsigned grid = (unsigned)ceil_div(nrows, 4);
+    switch (lane_granules<T>(ncols)) {
+    case 1: prob_short_kernel<T, 1, ENTROPY><<<grid, 128, 0, st>>>(nrows, ncols, x, ldx, c, inv, a); break;
+    case 2: prob_short_kernel<T, 2, ENTROPY><<<grid, 128, 0, st>>>(nrows, ncols, x, ldx, c, inv, a); break;
+    case 4: prob_short_kernel<T, 4, ENTROPY><<<grid, 128, 0, st>>>(nrows, ncols, x, ldx, c, inv, a); break;
+    case 8: prob_short_kernel<T, 8, ENTROPY><<<grid, 128, 0, st>>>(nrows, ncols, x, ldx, c, inv, a); break;
+    default: {
+        const int all = (ncols + 2 * Granule<T>::N - 2) / Granule<T>::N;
+        int ranks = 1;
+        while (ranks < MOST_CLUSTER && nrows * ranks <= sm_count() && all / ranks >= 2 * TT) ranks *= 2;
+        const size_t smem = (size_t)STAGES * TU * TT * 16;
+        return launch_cluster(prob_kernel<T, ENTROPY>, (unsigned)(nrows * ranks), ranks, TT, smem, smem, st, ncols, (int)ceil_div(all, ranks), x, ldx, c, inv, a);
+    }
+    }
+    CB_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T>
+static int log_probs(int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature, float *values,
+                     float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, cudaStream_t st)
+{
+    clear_error();
+    CB_TRY(check_logits<T>("log_probs", nrows, ncols, x, ldx, temperature));
+    if (k < 0 || k > ncols || k > 1024) return fail("log_probs: %lld alternatives a row; 0 to 1024, and no more than a row has columns", (long long)k);
+    if (nrows == 0) {
+        if (k) CB_CUDA(cudaMemsetAsync(best_pos, 0, sizeof(int64_t), st));
+        return 0;
+    }
+    const ProbCall a = {pos, crd, values, sums, entropy};
+    const float c = (float)(LOG2E_D / *temperature), inv = (float)(1.0 / *temperature);
+    if (k) return top_log_probs<T>(nrows, (int)ncols, (const T *)x, ldx, (int)k, c, inv, best_pos, best_crd, best_val, a, st);
+    return entropy ? launch_probs<T, true>(nrows, (int)ncols, (const T *)x, ldx, c, inv, a, st)
+                   : launch_probs<T, false>(nrows, (int)ncols, (const T *)x, ldx, c, inv, a, st);
+}
+
+template <typename T, bool ENTROPY>
+static int launch_grad(const ProbGrad &p, const T *x, T *grad, cudaStream_t st)
+{
+    const unsigned grid = (unsigned)ceil_div(p.nrows, 4);
+    switch (lane_granules<T>(p.ncols)) {
+    case 1: prob_grad_short_kernel<T, 1, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
+    case 2: prob_grad_short_kernel<T, 2, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
+    case 4: prob_grad_short_kernel<T, 4, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
+    case 8: prob_grad_short_kernel<T, 8, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
+    default: {
+        const int64_t pieces = ceil_div((p.ncols + 2 * Granule<T>::N - 2) / Granule<T>::N, GT * GG);
+        if (pieces * p.nrows > 0x7fffffffLL) return fail("log_probs_grad: more than 2^31 pieces of rows");
+        prob_grad_kernel<T, ENTROPY><<<(unsigned)(pieces * p.nrows), GT, 0, st>>>(p, (int)pieces, x, grad);
+    }
+    }
+    CB_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T>
+static int log_probs_grad(int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+                          const float *sums, const float *values, const float *entropy, const float *by_entropy, void *grad, int64_t ldg, cudaStream_t st)
+{
+    clear_error();
+    CB_TRY(check_logits<T>("log_probs_grad", nrows, ncols, x, ldx, temperature));
+    if (ldg < ncols) return fail("log_probs_grad: leading dimension smaller than the number of columns");
+    if ((uintptr_t)grad % sizeof(T)) return fail("log_probs_grad: an address that is not a multiple of the element's size");
+    if (by_entropy && !entropy) return fail("log_probs_grad: the entropies' gradients need the entropies");
+    if (nrows == 0) return 0;
+    const ProbGrad p = {nrows, (int)ncols, pos, crd, sums, values, entropy, by_entropy, ldx, ldg, (float)(LOG2E_D / *temperature), (float)(1.0 / *temperature)};
+    return by_entropy ? launch_grad<T, true>(p, (const T *)x, (T *)grad, st) : launch_grad<T, false>(p, (const T *)x, (T *)grad, st);
+}
+
+}  // namespace cb200
+
+#define LOG_PROBS(suffix, T)                                                                                                                           \
+    extern "C" int32_t comet_b200_dev_log_probs_##suffix##_i64(int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x,    \
+                                                               int64_t ldx, const double *temperature, float *values, float *sums, float *entropy,     \
+                                                               int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, void *stream)         \
+    {                                                                                                                                                  \
+        return cb200::log_probs<T>(nrows, ncols, pos, crd, x, ldx, temperature, values, sums, entropy, k, best_pos, best_crd, best_val,                \
+                                   (cudaStream_t)stream);                                                                                              \
+    }                                                                                                                                                  \
+    extern "C" int32_t comet_b200_dev_log_probs_grad_##suffix##_i64(                                                                                   \
+        int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,                    \
+        const float *sums, const float *d_values, const float *entropy, const float *d_entropy, void *grad, int64_t ldg, void *stream)                 \
+    {                                                                                                                                                  \
+        return cb200::log_probs_grad<T>(nrows, ncols, pos, crd, x, ldx, temperature, sums, d_values, entropy, d_entropy, grad, ldg,                    \
+                                        (cudaStream_t)stream);                                                                                         \
+    }
+LOG_PROBS(bf16, __nv_bfloat16)
+LOG_PROBS(f16, __half)
+LOG_PROBS(f32, float)

@@ -14,6 +14,7 @@
 #include <atomic>
 
 #include "logits.cuh"
+#include "rows.cuh"
 
 namespace cb200 {
 
@@ -40,7 +41,7 @@ unsigned *next_counter()
     return p + turn++ % 1024;
 }
 
-static const int TT = 256, TW = TT / 32, TU = 4, STAGES = 3, MOST_K = 1024, ROOM = 2048;
+static const int MOST_K = 1024, ROOM = 2048;
 
 typedef unsigned long long u64;
 
@@ -101,7 +102,7 @@ struct TopShared {
     int digit, left, exact;
     int count;
     uint32_t base, bound;          // keys that k entries reach: the first, and the best so far
-    float room[2 * TW], m, s;
+    float room[3 * TW], m, s, e;
     u64 ends[2 * TW];
     uint32_t least[TW];
 };
@@ -211,102 +212,20 @@ __device__ u64 keep_largest(TopShared &sh, int n, int k)
     return least;
 }
 
-// A thread's way through a row, or a CTA's part of one: a ring of stages in shared memory, of which it copies and reads the same 16
-// bytes each time, so the ring needs no barriers.
-template <typename T>
-struct Way {
-    static constexpr int N = Granule<T>::N;
-    uint4 *ring;                                   // STAGES * TU * TT
-    const uint4 *from;                             // the row's granule 0
-    int begin, end, all, off, ncols;               // the part, the row's granules, elements before the row, its columns
-    const uint4 *next;
-    int left, put, at;
-
-    __device__ __forceinline__ int steps() const { return (end - begin + TU * TT - 1) / (TU * TT); }
-    __device__ __forceinline__ void fetch()
-    {
-#pragma unroll
-        for (int u = 0; u < TU; u++)
-            if (u * TT < left) copy_granule(ring + (put * TU + u) * TT + threadIdx.x, next + u * TT);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        next += TU * TT;
-        left -= TU * TT;
-        put = put == STAGES - 1 ? 0 : put + 1;
-    }
-    __device__ __forceinline__ void start()
-    {
-        next = from + begin + threadIdx.x;
-        left = end - begin - (int)threadIdx.x;
-        put = at = 0;
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; i++) fetch();
-    }
-    // the thread's granules of a step, TT apart; -inf where there is no row
-    __device__ __forceinline__ Granule<T> *stage(int step)
-    {
-        fetch();
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        Granule<T> *mine = (Granule<T> *)(ring + at * TU * TT + threadIdx.x);
-        at = at == STAGES - 1 ? 0 : at + 1;
-        const int first = begin + step * TU * TT;
-        if (first == 0 || first + TU * TT > min(end, all - 1)) {
-#pragma unroll
-            for (int u = 0; u < TU; u++) {
-                const int i = first + threadIdx.x + u * TT;
-                if (i == 0 || i >= all - 1 || i >= end) {
-                    T *v = (T *)&mine[u * TT];
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (i >= end || i * N + e < off || i * N + e >= off + ncols) v[e] = from_float<T>(MINUS_INF);
-                }
-            }
-        }
-        return mine;
-    }
-    __device__ __forceinline__ int column(int step, int u, int e) const { return (begin + (step * TU + u) * TT + (int)threadIdx.x) * N + e - off; }
+// What is summed beside the choice: nothing, exp(x / temperature) (LSE), or all that log probabilities take.
+enum { NOTHING, LSE_ONLY, PROBS, PROBS_ENTROPY };
+template <int SUM>
+struct SumOf {
+    typedef ProbSum<SUM == PROBS_ENTROPY> Type;
 };
-
-// A thread's sum of exp(x / temperature): its maximum, that times c, and two sums of 2^(x c - mc).
-struct LogSum {
-    float m, mc;
-    float2 s;
-    template <typename T>
-    __device__ __forceinline__ void add(const Granule<T> (&g)[TU], typename Granule<T>::Most most, float c)
-    {
-        constexpr int N = Granule<T>::N;
-        const float nm = max_nan(m, to_float(largest(most)));
-        if (nm != m) {
-            const float f = exp2_fast((m - nm) * c);
-            s.x *= f;
-            s.y *= f;
-            m = nm;
-            mc = m == MINUS_INF ? 0.0f : m * c;
-        }
-        if (fabsf(mc) < NEAR) {                    // what the rounding of mc does to s is below the rounding of the result, m c + log2(s)
-#pragma unroll
-            for (int u = 0; u < TU; u++) {
-                float2 v[N / 2];
-                g[u].unpack(v);
-#pragma unroll
-                for (int e = 0; e < N / 2; e++) {
-                    const float2 d = fma2(v[e], make_float2(c, c), make_float2(-mc, -mc));
-                    s = add2(s, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
-                }
-            }
-        } else {                                   // and NaN, and infinity
-#pragma unroll
-            for (int u = 0; u < TU; u++) {
-                float v[N];
-                g[u].unpack(v);
-#pragma unroll
-                for (int e = 0; e < N; e++) s.x += exp2_fast((v[e] - m) * c);
-            }
-        }
-    }
+template <>
+struct SumOf<NOTHING> {
+    typedef LogSum Type;
 };
-
-// The log of a row's sum; with a maximum of +inf (no NaN then) s is of differences of infinities, and the sum is +inf.
-__device__ __forceinline__ float log_of_sum(float m, float s, float inv) { return fabsf(m) == -MINUS_INF ? m : fmaf(log2f(s), LN2, m * inv); }
+template <>
+struct SumOf<LSE_ONLY> {
+    typedef LogSum Type;
+};
 
 // The first step's bound, by all threads: each of eight warps finds the ceil(k / 8)-th largest of its 128 granules' largest entries, and k
 // entries reach the least of those keys.  Of fewer than 256 granules the first warps have 32 each, and only those are asked.
@@ -336,8 +255,8 @@ __device__ __forceinline__ uint32_t first_bound(TopShared &sh, const typename Gr
 // Candidates without barriers.  Each one is counted in a histogram of keys above the first bound, and every 64th makes its warp
 // look for the highest digit that k entries reach: the other warps' bound from their next step on.  It only rises, and holds
 // whenever it is read.  count > ROOM afterwards: the row is one (in order, or of few values) that has to be taken step by step.
-template <typename T, bool LSE>
-__device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, int colbits, float c, LogSum &sum)
+template <typename T, int SUM>
+__device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, int colbits, float c, typename SumOf<SUM>::Type &sum)
 {
     constexpr int N = Granule<T>::N, DIGIT = Order<T>::DIGIT;
     const u64 low = (1ull << colbits) - 1;
@@ -360,7 +279,7 @@ __device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, i
             if (threadIdx.x == 0) sh.base = *bound = base;
             __syncthreads();
         }
-        if (LSE) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
+        if (SUM) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
         if (over) continue;
         const T least = Order<T>::code(*bound);
         unsigned pending = 0;
@@ -385,7 +304,7 @@ __device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, i
             if (highest_digit(sh.hist, k, digit, above, own)) atomicMax((unsigned *)bound, base + ((uint32_t)digit << DIGIT));
             __syncwarp();
             over = __any_sync(0xffffffffu, *(volatile int *)&sh.count > ROOM);         // the same in every lane
-            if (!LSE && over) break;
+            if (!SUM && over) break;
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -394,8 +313,8 @@ __device__ __forceinline__ void stream_free(TopShared &sh, Way<T> &way, int k, i
 
 // Candidates step by step: when they become many, the k largest are kept and the k-th of them is the new bound.  Holds for
 // every row and k.  Leaves the k largest.
-template <typename T, bool LSE>
-__device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, int colbits, float c, LogSum &sum)
+template <typename T, int SUM>
+__device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, int colbits, float c, typename SumOf<SUM>::Type &sum)
 {
     constexpr int N = Granule<T>::N;
     const u64 low = (1ull << colbits) - 1;
@@ -418,7 +337,7 @@ __device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, 
             bound = (u64)key << colbits;
             least_value = Order<T>::code(key);
         }
-        if (LSE) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
+        if (SUM) sum.add(g, most_of(most_of(gm[0], gm[1]), most_of(gm[2], gm[3])), c);
         unsigned pending = 0;
 #pragma unroll
         for (int u = 0; u < TU; u++) pending |= g[u].at_least(least_value) << (u * N);
@@ -451,11 +370,12 @@ __device__ __noinline__ void stream_stepwise(TopShared &sh, Way<T> &way, int k, 
 }
 
 // Long rows, or many entries of them: a CTA, or a cluster of them, per row.
-template <typename T, bool LSE, bool FREE>
+template <typename T, int SUM, bool FREE>
 __global__ void __launch_bounds__(TT, 3)
 top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_t ldx, int k, int colbits, float c, float inv, int64_t *__restrict__ pos,
-           int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse)
+           int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse, const ProbCall probs)
 {
+    constexpr bool PROB = SUM >= PROBS;
     extern __shared__ uint4 ring[];
     __shared__ TopShared sh;
     const int tid = threadIdx.x;
@@ -470,7 +390,9 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
     way.all = (way.off + ncols + Way<T>::N - 1) / Way<T>::N;
     way.begin = min((int)rank * slice, way.all);
     way.end = min(way.begin + slice, way.all);
-    LogSum sum = {MINUS_INF, 0.0f, make_float2(0.0f, 0.0f)};
+    typename SumOf<SUM>::Type sum;
+    if constexpr (PROB) sum.start();
+    else sum = {MINUS_INF, 0.0f, make_float2(0.0f, 0.0f)};
     const u64 low = (1ull << colbits) - 1;
     if (FREE) {
         sh.hist[tid] = 0;
@@ -479,11 +401,12 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
             sh.base = sh.bound = 0;
         }
         __syncthreads();
-        stream_free<T, LSE>(sh, way, k, colbits, c, sum);
+        stream_free<T, SUM>(sh, way, k, colbits, c, sum);
         const int n = sh.count;
         __syncthreads();                           // all have read it
         if (n > ROOM) {
-            stream_stepwise<T, false>(sh, way, k, colbits, c, sum);
+            LogSum none;
+            stream_stepwise<T, NOTHING>(sh, way, k, colbits, c, none);
         } else if (n > k) {                        // those that do not reach the last bound go
             if (tid < 32) {
                 int digit, above, own;
@@ -503,10 +426,27 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
             if (sh.count > ROOM / MOST_CLUSTER) keep_largest(sh, sh.count, k);
         }
     } else {
-        stream_stepwise<T, LSE>(sh, way, k, colbits, c, sum);
+        stream_stepwise<T, SUM>(sh, way, k, colbits, c, sum);
     }
-    float m = sum.m, s = sum.s.x + sum.s.y;
-    if (LSE) {
+    float m = sum.m, s = 0.0f, ent = 0.0f;
+    if constexpr (PROB) sum.total(s, ent);
+    else s = sum.s.x + sum.s.y;
+    if (PROB) {
+        float r[1] = {m}, q[2];
+        cta_reduce<1, TW, true>(r, sh.room);
+        shift_to(r[0], m, c, s, ent);
+        q[0] = s;
+        q[1] = ent;
+        cta_reduce<2, TW, false>(q, sh.room + TW);
+        m = r[0];
+        s = q[0];
+        ent = q[1];
+        if (tid == 0) {
+            sh.m = m;
+            sh.s = s;
+            sh.e = ent;
+        }
+    } else if (SUM) {
         float r[1] = {m}, q[1];
         cta_reduce<1, TW, true>(r, sh.room);
         q[0] = m == MINUS_INF ? 0.0f : s * exp2_fast((m - r[0]) * c);
@@ -531,7 +471,15 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
                 if (tid == 0) sh.count = have + n;
                 __syncthreads();
                 if (sh.count > ROOM - most) keep_largest(sh, sh.count, k);
-                if (LSE) {
+                if (PROB) {
+                    const float om = peer_load(&sh.m, r), nm = max_nan(m, om);
+                    float os = peer_load(&sh.s, r), oe = peer_load(&sh.e, r);
+                    shift_to(nm, m, c, s, ent);
+                    shift_to(nm, om, c, os, oe);
+                    m = nm;
+                    s += os;
+                    ent += oe;
+                } else if (SUM) {
                     const float om = peer_load(&sh.m, r), os = peer_load(&sh.s, r), nm = max_nan(m, om);
                     s = (m == MINUS_INF ? 0.0f : s * exp2_fast((m - nm) * c)) + (om == MINUS_INF ? 0.0f : os * exp2_fast((om - nm) * c));
                     m = nm;
@@ -543,7 +491,10 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         cluster_wait();
         if (rank != 0) return;
     }
-    if (LSE && tid == 0) lse[t] = log_of_sum(m, s, inv);
+    if (SUM == LSE_ONLY && tid == 0) lse[t] = log_of_sum(m, s, inv);
+    const RowProb p(m, s, ent);
+    if (PROB) give_probs(probs, t, x, ncols, p, inv, tid, TT);
+    auto value = [&](uint32_t key) { return PROB ? p.of(Order<T>::value(key), inv) : Order<T>::value(key); };
     if (tid == 0) {
         pos[t] = t * k;
         if (t == nrows - 1) pos[nrows] = nrows * k;
@@ -568,21 +519,21 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
             int at = 0;
             for (int i = 0; i < n; i++) at += (sh.cand[i] & low) > (it & low);
             crd[t * k + at] = (int64_t)(low - (it & low));
-            val[t * k + at] = Order<T>::value((uint32_t)(it >> colbits));
+            val[t * k + at] = value((uint32_t)(it >> colbits));
         }
         return;
     }
-    int p = 1;
-    while (p < k) p *= 2;
+    int room = 1;
+    while (room < k) room *= 2;
     u64 *v = sh.cand + MOST_K;
-    for (int i = tid; i < p; i += TT) {
+    for (int i = tid; i < room; i += TT) {
         const u64 it = i < k ? sh.cand[i] : 0;
         v[i] = i < k ? (low - (it & low)) << 32 | it >> colbits : ~0ull;
     }
     __syncthreads();
-    for (int size = 2; size <= p; size *= 2)
+    for (int size = 2; size <= room; size *= 2)
         for (int step = size / 2; step > 0; step /= 2) {
-            for (int i = tid; i < p / 2; i += TT) {
+            for (int i = tid; i < room / 2; i += TT) {
                 const int lo = i / step * step * 2 + i % step, hi = lo + step;
                 const u64 a = v[lo], b = v[hi];
                 if ((a > b) == ((lo & size) == 0)) {
@@ -594,7 +545,7 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         }
     for (int i = tid; i < k; i += TT) {
         crd[t * k + i] = (int64_t)(v[i] >> 32);
-        val[t * k + i] = Order<T>::value((uint32_t)v[i]);
+        val[t * k + i] = value((uint32_t)v[i]);
     }
 }
 
@@ -641,10 +592,10 @@ struct Short<float> {
 //
 // Bound: instructions; 65536 rows of 256 and k = 8 in bf16 take 27 us, 6 by the bytes; 65 when the lane that gives an entry looked for its next
 // one.  16384 rows of 64 in f32: 10 us on the device.
-template <typename T, int R, bool LSE>
+template <typename T, int R, int SUM>
 __global__ void __launch_bounds__(128)
 top_short_kernel(int64_t nrows, int ncols, const T *__restrict__ xs, int64_t ldx, bool whole, int k, float c, float inv, int64_t *__restrict__ pos,
-                 int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse)
+                 int64_t *__restrict__ crd, float *__restrict__ val, float *__restrict__ lse, const ProbCall probs)
 {
     constexpr bool ONE = Order<T>::BITS == 16;
     const int lane = threadIdx.x & 31;
@@ -706,25 +657,39 @@ top_short_kernel(int64_t nrows, int ncols, const T *__restrict__ xs, int64_t ldx
             own[R - 1].none();
         }
     }
+    RowProb p(MINUS_INF, 0.0f, 0.0f);
+    if (SUM) {
+        float m = MINUS_INF, s = 0.0f, ent = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; r++) m = max_nan(m, to_float(part.v[r]));
+        m = warp_max(m);
+        if (SUM == LSE_ONLY) {
+#pragma unroll
+            for (int r = 0; r < R; r++) s += exp2_fast((to_float(part.v[r]) - m) * c);
+            s = warp_sum(s);
+            if (lane == 0) lse[t] = log_of_sum(m, s, inv);
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float d = (to_float(part.v[r]) - m) * c, q = exp2_fast(d);
+                s += q;
+                if (SUM == PROBS_ENTROPY) ent = fmaf(q, fmaxf(d, -16384.0f), ent);
+            }
+            s = warp_sum(s);
+            if (SUM == PROBS_ENTROPY) ent = warp_sum(ent);
+            p = RowProb(m, s, ent);
+            give_probs(probs, t, x, ncols, p, inv, lane, 32);
+        }
+    }
     int place = 0;
     for (int i = 0; i < k; i++) place += __shfl_sync(0xffffffffu, col, i) < col;
     if (lane < k) {
         crd[t * k + place] = col;
-        val[t * k + place] = Order<T>::value(got);
+        val[t * k + place] = SUM >= PROBS ? p.of(Order<T>::value(got), inv) : Order<T>::value(got);
     }
     if (lane == 0) {
         pos[t] = t * k;
         if (t == nrows - 1) pos[nrows] = nrows * k;
-    }
-    if (LSE) {
-        float m = MINUS_INF, s = 0.0f;
-#pragma unroll
-        for (int r = 0; r < R; r++) m = max_nan(m, to_float(part.v[r]));
-        m = warp_max(m);
-#pragma unroll
-        for (int r = 0; r < R; r++) s += exp2_fast((to_float(part.v[r]) - m) * c);
-        s = warp_sum(s);
-        if (lane == 0) lse[t] = log_of_sum(m, s, inv);
     }
 }
 
@@ -738,6 +703,8 @@ struct TopCall {
     int64_t *pos, *crd;
     float *val, *lse;
     cudaStream_t st;
+    int sum;
+    ProbCall probs;
 };
 
 template <typename T, int R>
@@ -746,13 +713,12 @@ static void launch_short(const TopCall &a)
     const size_t piece = sizeof(T) * R < 16 ? sizeof(T) * R : 16;
     const bool whole = (uintptr_t)a.x % piece == 0 && a.ldx * (int64_t)sizeof(T) % (int64_t)piece == 0;
     const unsigned grid = (unsigned)ceil_div(a.nrows, 4);
-    if (a.lse)
-        top_short_kernel<T, R, true><<<grid, 128, 0, a.st>>>(a.nrows, a.ncols, (const T *)a.x, a.ldx, whole, a.k, a.c, a.inv, a.pos, a.crd, a.val, a.lse);
-    else
-        top_short_kernel<T, R, false><<<grid, 128, 0, a.st>>>(a.nrows, a.ncols, (const T *)a.x, a.ldx, whole, a.k, a.c, a.inv, a.pos, a.crd, a.val, a.lse);
+    auto kernel = a.sum == NOTHING ? top_short_kernel<T, R, NOTHING> : a.sum == LSE_ONLY ? top_short_kernel<T, R, LSE_ONLY> : a.sum == PROBS ? top_short_kernel<T, R, PROBS>
+                                                                                                                              : top_short_kernel<T, R, PROBS_ENTROPY>;
+    kernel<<<grid, 128, 0, a.st>>>(a.nrows, a.ncols, (const T *)a.x, a.ldx, whole, a.k, a.c, a.inv, a.pos, a.crd, a.val, a.lse, a.probs);
 }
 
-template <typename T, bool LSE>
+template <typename T, int SUM>
 static int launch_long(const TopCall &a)
 {
     constexpr int N = Granule<T>::N;
@@ -763,10 +729,39 @@ static int launch_long(const TopCall &a)
     const size_t smem = (size_t)STAGES * TU * TT * 16;
     if (a.nrows * ranks > 0x7fffffffLL) return fail("top_entries: more than 2^31 rows");
     // beyond 256 entries the candidates of a row without barriers would not fit their room
-    auto kernel = a.k <= 256 ? top_kernel<T, LSE, true> : top_kernel<T, LSE, false>;
+    auto kernel = a.k <= 256 ? top_kernel<T, SUM, true> : top_kernel<T, SUM, false>;
     return launch_cluster(kernel, (unsigned)(a.nrows * ranks), ranks, TT, smem, smem, a.st, a.nrows, a.ncols, (int)ceil_div(all, ranks),
-                          (const T *)a.x, a.ldx, a.k, colbits, a.c, a.inv, a.pos, a.crd, a.val, a.lse);
+                          (const T *)a.x, a.ldx, a.k, colbits, a.c, a.inv, a.pos, a.crd, a.val, a.lse, a.probs);
 }
+
+template <typename T>
+static int launch_top(const TopCall &a)
+{
+    // By warps / by CTAs, 4096 rows, k = 8 and 32, us: 512 columns of bf16 5.7, 9.7 / 128, 131, 1024 of bf16 24, 34 / 137, 143 (the CTAs' bound was looser);
+    // 512 of f32 -, 24 / -, 124, 1024 of f32 93, 148 / 49, 58: a warp's two words an entry fill its registers.
+    if (a.ncols > (sizeof(T) == 2 ? 1024 : 512) || a.k > 32)
+        return a.sum == NOTHING ? launch_long<T, NOTHING>(a) : a.sum == LSE_ONLY ? launch_long<T, LSE_ONLY>(a) : a.sum == PROBS ? launch_long<T, PROBS>(a)
+                                                                                                              : launch_long<T, PROBS_ENTROPY>(a);
+    if (a.ncols <= 32) launch_short<T, 1>(a);
+    else if (a.ncols <= 64) launch_short<T, 2>(a);
+    else if (a.ncols <= 128) launch_short<T, 4>(a);
+    else if (a.ncols <= 256) launch_short<T, 8>(a);
+    else if (a.ncols <= 512) launch_short<T, 16>(a);
+    else if constexpr (sizeof(T) == 2) launch_short<T, 32>(a);
+    CB_LAUNCH_CHECK();
+    return 0;
+}
+
+// log_probs with alternatives: the choice and the sums in one pass
+template <typename T>
+int top_log_probs(int64_t nrows, int ncols, const T *x, int64_t ldx, int k, float c, float inv, int64_t *pos, int64_t *crd, float *val, const ProbCall &probs,
+                  cudaStream_t st)
+{
+    return launch_top<T>({nrows, ncols, x, ldx, k, c, inv, pos, crd, val, nullptr, st, probs.entropy ? PROBS_ENTROPY : PROBS, probs});
+}
+template int top_log_probs(int64_t, int, const __nv_bfloat16 *, int64_t, int, float, float, int64_t *, int64_t *, float *, const ProbCall &, cudaStream_t);
+template int top_log_probs(int64_t, int, const __half *, int64_t, int, float, float, int64_t *, int64_t *, float *, const ProbCall &, cudaStream_t);
+template int top_log_probs(int64_t, int, const float *, int64_t, int, float, float, int64_t *, int64_t *, float *, const ProbCall &, cudaStream_t);
 
 template <typename T>
 static int top_entries(int64_t nrows, int64_t ncols, const void *x, int64_t ldx, int64_t k, const double *temperature, int64_t *pos, int64_t *crd,
@@ -785,22 +780,12 @@ static int top_entries(int64_t nrows, int64_t ncols, const void *x, int64_t ldx,
         CB_CUDA(cudaMemsetAsync(pos, 0, sizeof(int64_t), st));
         return 0;
     }
-    TopCall a = {nrows, (int)ncols, x, ldx, (int)k, 0.0f, 0.0f, pos, crd, val, lse, st};
+    TopCall a = {nrows, (int)ncols, x, ldx, (int)k, 0.0f, 0.0f, pos, crd, val, lse, st, lse ? LSE_ONLY : NOTHING, {}};
     if (lse) {
         a.c = (float)(LOG2E_D / *temperature);
         a.inv = (float)(1.0 / *temperature);
     }
-    // By warps / by CTAs, 4096 rows, k = 8 and 32, us: 512 columns of bf16 5.7, 9.7 / 128, 131, 1024 of bf16 24, 34 / 137, 143 (the CTAs' bound was looser);
-    // 512 of f32 -, 24 / -, 124, 1024 of f32 93, 148 / 49, 58: a warp's two words an entry fill its registers.
-    if (ncols > (sizeof(T) == 2 ? 1024 : 512) || k > 32) return lse ? launch_long<T, true>(a) : launch_long<T, false>(a);
-    if (ncols <= 32) launch_short<T, 1>(a);
-    else if (ncols <= 64) launch_short<T, 2>(a);
-    else if (ncols <= 128) launch_short<T, 4>(a);
-    else if (ncols <= 256) launch_short<T, 8>(a);
-    else if (ncols <= 512) launch_short<T, 16>(a);
-    else if constexpr (sizeof(T) == 2) launch_short<T, 32>(a);
-    CB_LAUNCH_CHECK();
-    return 0;
+    return launch_top<T>(a);
 }
 
 }  // namespace cb200

@@ -183,8 +183,8 @@ def masked_pair_count(A, B, M, row_lo=0, row_hi=None, out=None):
 # current stream.  A gradient written in place of the logits counts as an operation in place: a graph that has saved them refuses its
 # backward pass.
 _LOGITS = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
-_TOP, _DISTILL, _BALANCE = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _LOGITS.items()}
-                            for op in ("top_entries", "distill_loss", "balance_loss"))
+_TOP, _DISTILL, _BALANCE, _PROBS, _PROBS_GRAD = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _LOGITS.items()}
+                                                 for op in ("top_entries", "distill_loss", "balance_loss", "log_probs", "log_probs_grad"))
 _numbers = {}
 
 
@@ -312,6 +312,51 @@ def balance_loss(S, R, seq=None, mask=None, scores="softmax", scale=1.0, grad=Tr
     _call(_BALANCE[R.dtype], n, m, pos, crd, nseq, bounds, on, int(scores == "sigmoid"), R.data_ptr(), ld, to, ldg, options[0], counts.data_ptr(),
           loss.data_ptr(), _stream())
     return loss, counts, out
+
+
+def log_probs(S, X, temperature=1.0, entropy=False, top=0):
+    """Log probabilities, under softmax(X / temperature), of the columns that S stores (DeviceCSR of X's shape; its values are not looked at: a row's given
+    tokens, in any order, or none).  top: the alternatives, each row's `top` most likely columns (0 to 1024).
+
+    Returns (values of S's entries, sums, entropies or None, a DeviceCSR of the alternatives' log probabilities, columns ascending, or None), all float32.
+    sums [rows, 2] is what log_probs_grad takes: the row's largest logit m, and log s = the log of the sum of exp((X - m) / temperature);
+    m / temperature + log s is the lse of top_entries.  A row of -inf has log probabilities of -inf and an entropy of 0."""
+    n, m, ld = _check_logits("log_probs", X)
+    pos, crd = _check_beside("log_probs", S, n, m)
+    top = int(top)
+    if not 0 <= top <= min(1024, m):
+        raise ValueError("log_probs: top must be between 0 and 1024, and at most the number of columns")
+    new, f32 = X.new_empty, torch.float32
+    values, sums, ent = new(S.nnz, dtype=f32), new((n, 2), dtype=f32), new(n, dtype=f32) if entropy else None
+    best, at = None, (0, 0, 0)
+    if top:
+        best = DeviceCSR(n, m, new(n + 1, dtype=torch.int64), new(n * top, dtype=torch.int64), new(n * top, dtype=f32))
+        at = best.pos.data_ptr(), best.crd.data_ptr(), best.val.data_ptr()
+    _call(_PROBS[X.dtype], n, m, pos, crd, X.data_ptr(), ld, _floats(float(temperature))[0], values.data_ptr(), sums.data_ptr(), _p(ent), top, *at, _stream())
+    return values, sums, ent, best
+
+
+def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperature=1.0, grad=True):
+    """The gradient with respect to X of what log_probs gives, from d_values (float32, one for each of S's entries; columns of a row ascending) and, with the
+    entropies, d_entropy (float32, one for each row).  sums and entropy: of log_probs at the same temperature.  grad: True (a new tensor), or a tensor to write
+    it to, such as X.  The alternatives have no gradient here: as S of a second call they have."""
+    n, m, ld = shape = _check_logits("log_probs_grad", X)
+    pos, crd = _check_beside("log_probs_grad", S, n, m)
+    d_val = _check_vector("log_probs_grad", d_values, torch.float32, S.nnz)
+    if sums.shape != (n, 2):
+        raise ValueError("log_probs_grad: sums must be what log_probs gives, [%d, 2]" % n)
+    kept = _check_vector("log_probs_grad", sums.view(-1), torch.float32, 2 * n)
+    ent = d_ent = 0
+    if d_entropy is not None:
+        if entropy is None:
+            raise ValueError("log_probs_grad: d_entropy needs the entropies")
+        d_ent = _check_vector("log_probs_grad", d_entropy, torch.float32, n)
+        ent = _check_vector("log_probs_grad", entropy, torch.float32, n)
+    if grad is None or grad is False:
+        raise ValueError("log_probs_grad: grad is True, or a tensor to write to")
+    out, to, ldg = _gradient("log_probs_grad", X, shape[:2], grad)
+    _call(_PROBS_GRAD[X.dtype], n, m, pos, crd, X.data_ptr(), ld, _floats(float(temperature))[0], kept, d_val, ent, d_ent, to, ldg, _stream())
+    return out
 
 
 # A router's experts: products of the rows that a CSR matrix (rows tokens, columns experts) sends to each of them.  The operands are contiguous CUDA

@@ -682,6 +682,36 @@ COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_f32_i64(
     uint8_t *mask, int32_t sigmoid, const void *r, int64_t ldr, void *grad, int64_t ldg, const double *scale,
     int64_t *counts, float *loss, void *stream);
 
+/* Log probabilities of given columns.  pos/crd: a CSR matrix of x's shape (ncols < 2^30) whose columns are asked for; in any order, repeated or not.
+     values[nnz]   = (x_j - m) / *temperature - log s   with m the row's largest logit, s = sum_j exp((x_j - m) / *temperature)
+     sums[2 nrows] = m, log s of each row (m / *temperature + log s is what top_entries gives as lse)
+     entropy[nrows] = -sum_j q_j log q_j (may be NULL)
+     best_pos/best_crd/best_val: with k > 0 the row's k largest entries as top_entries gives them, with their log probabilities.
+   A row of -inf has log probabilities of -inf, sums of -inf and 0 and an entropy of 0; a row with NaN or +inf has NaN.  A logit of -inf adds
+   nothing to the entropy.  A column outside the matrix gives NaN. */
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_bf16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    float *values, float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_f16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    float *values, float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_f32_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    float *values, float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, void *stream);
+
+/* Their gradient: grad = d loss / d x in x's type, from d_values[nnz] and (with the entropies; both may be NULL) d_entropy[nrows], and the sums of the forward
+   call at the same temperature.  May be x itself (same ldx).  Columns of a row ascend, repeated ones are next to each other and add up; one outside
+   the matrix only adds to the row's sum.  A row whose d_values add up to 0, with a d_entropy of 0, is 0 but at its entries, and so is all of a row of -inf. */
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_bf16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    const float *sums, const float *d_values, const float *entropy, const float *d_entropy, void *grad, int64_t ldg, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_f16_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    const float *sums, const float *d_values, const float *entropy, const float *d_entropy, void *grad, int64_t ldg, void *stream);
+COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_f32_i64(
+    int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
+    const float *sums, const float *d_values, const float *entropy, const float *d_entropy, void *grad, int64_t ldg, void *stream);
+
 /* ---- a router's experts --------------------------------------------------------------------------------------------------- */
 /* pos/crd: a CSR matrix of which experts (columns) take which tokens (rows), nnz entries, columns of a row in any order.  The  */
 /* operands are bf16 or f16 (the suffix), row-major, at multiples of 16 bytes; width and inner are multiples of 8.  Arithmetic   */
