@@ -6,8 +6,10 @@
 // act(g) = g s(u) with the logistic function s, u = g for silu and 2 sqrt(2 / pi) (g + 0.044715 g^3) for gelu (its tanh form).
 //
 // All of these are one kernel: tiles of 128 x 256 sums in tensor memory, 64 terms a step, with the operands' tiles in a ring of four in shared
-// memory.  A warp fetches (rows of x, h, dz and dy by their number, four a copy, so nothing is sorted or copied first; padding is a number outside, and
-// reads as zeros), a thread issues the products, four warps take the sums of the tile before out of tensor memory.  Three forms:
+// memory.  Four warps fetch, a thread issues the products, four warps take the sums of the tile before out of tensor memory.  Weights, and what a kernel
+// before has left in the order of the slots (dz, val h), come by tensor copies; rows of x, h and dy by their number, 16 bytes a copy, so that nothing is
+// sorted first (a tensor copy of four numbered rows takes about 70 clocks whatever their width: gated_batch, 65536 entries, 1200 us with them).
+// Three forms:
 //   ROWS   rows of a tile's tokens, times a weight whose rows are outputs                (forward passes, dz)
 //   BACK   the same, times a weight whose rows are the sum's index                       (dx, v' dy)
 //   OUTER  sums over an expert's tokens of two rows                                      (dw, dv)
@@ -44,13 +46,6 @@ static int make_map(const char *what, const void *base, bool bf16, int rank, con
     return r == CUDA_SUCCESS ? 0 : fail("%s: cuTensorMapEncodeTiled refused a map (error %d)", what, (int)r);
 }
 
-int make_gather_map(const char *what, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, CUtensorMap *map)
-{
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, 1};
-    return make_map(what, base, bf16, 2, dims, strides, box, map);
-}
-
 int make_box_map(const char *what, const void *base, bool bf16, int64_t depth, int64_t rows, int64_t cols, int box_rows, CUtensorMap *map)
 {
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth}, strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(cols * rows) * 2};
@@ -63,12 +58,14 @@ enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 
 static const int TM = 128, TN = 256, TK = 64, RING = 4;
 static const int A_BYTES = TM * TK * 2, B_BYTES = TN * TK * 2, STEP_BYTES = A_BYTES + B_BYTES;
-static const int PRODUCT_THREADS = 192, PRODUCT_SMEM = RING * STEP_BYTES + 1024;
+static const int FETCHERS = 128, PRODUCT_THREADS = 128 + FETCHERS + 32, PRODUCT_SMEM = RING * STEP_BYTES + 1024;
 
 struct ProductArgs {
     Groups g;
-    const int *rows_a, *rows_b;      // the numbers of each slot's row of a, of b (OUTER)
-    int none_a, none_b;              // a number outside
+    const int *numbers;              // of each slot's row of the operand that is fetched by rows
+    const void *numbered;            // that operand: its rows, their stride, and their columns
+    int64_t ld;
+    int numbered_cols;
     int terms;                       // of the sums (not OUTER)
     int tiles_m, tiles_n;            // tiles of a weight's rows (OUTER), tiles of columns
     int rows, cols;                  // of an expert's result (OUTER), of a result row
@@ -78,6 +75,18 @@ struct ProductArgs {
     const float *val;
     void *out, *scaled;              // 16-bit results; val * h
     float *sums;                     // rows of f32, or sums of products per tile of columns
+
+    void number(const int *list, const void *rows, int64_t stride, int64_t n)
+    {
+        numbers = list;
+        numbered = rows;
+        ld = stride;
+        numbered_cols = (int)n;
+    }
+};
+
+struct Tile {
+    int m, n, group, steps, slot;    // slot: the first one
 };
 
 __device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + exp2_fast(-LOG2E * u)); }
@@ -111,10 +120,10 @@ __device__ __forceinline__ void load8(float *v, const T *from)
 
 // A tile's sums, 32 columns at a time, by the thread that has the row; at: tensor memory of the warp's rows.  entry < 0: nothing to store.
 template <typename T, int SUMS>
-__device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, bool none, int tile_m, int tile_n, int group, int row, int64_t entry)
+__device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, bool none, const Tile &t, int row, int64_t entry)
 {
     if constexpr (SUMS == GATED || SUMS == GATED_GRAD) {
-        const int f0 = tile_n * (TN / 2), inner = a.cols;
+        const int f0 = t.n * (TN / 2), inner = a.cols;
 #pragma unroll 1
         for (int c = 0; c < TN / 2; c += 32) {
             __syncwarp();
@@ -122,8 +131,8 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, boo
             float gate[32], up[32];
             tmem_load(at + c, gate);
             tmem_load(at + TN / 2 + c, up);
-            if (entry < 0) continue;
             if (SUMS == GATED) {
+                if (entry < 0) continue;
                 T *h = (T *)a.out + entry * inner + f0 + c;
 #pragma unroll
                 for (int i = 0; i < 32; i++) gate[i] = gate[i] * logistic(gate_of(gate[i], a.gelu).x) * up[i];
@@ -131,20 +140,25 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, boo
                 for (int i = 0; i < 32; i += 8)
                     if (f0 + c + i < inner) store8<T>(h + i, gate + i);
             } else {
-                T *dz = (T *)a.out + entry * 2 * inner + f0 + c;
+                T *dz = (T *)a.out + (int64_t)(t.slot + row) * 2 * inner + f0 + c;
                 const T *dh = (const T *)a.other + entry * inner + f0 + c;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     if (f0 + c + i >= inner) break;
-                    float d[8];
-                    load8<T>(d, dh + i);
+                    if (entry >= 0) {
+                        float d[8];
+                        load8<T>(d, dh + i);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float g = gate[i + j];
-                        const float2 u = gate_of(g, a.gelu);
-                        const float s = logistic(u.x);
-                        gate[i + j] = d[j] * up[i + j] * fmaf(g * s * (1.0f - s), u.y, s);
-                        up[i + j] = d[j] * g * s;
+                        for (int j = 0; j < 8; j++) {
+                            const float g = gate[i + j];
+                            const float2 u = gate_of(g, a.gelu);
+                            const float s = logistic(u.x);
+                            gate[i + j] = d[j] * up[i + j] * fmaf(g * s * (1.0f - s), u.y, s);
+                            up[i + j] = d[j] * g * s;
+                        }
+                    } else {                       // a row of the sums over an expert's tokens that adds nothing
+#pragma unroll
+                        for (int j = 0; j < 8; j++) gate[i + j] = up[i + j] = 0.0f;
                     }
                     store8<T>(dz + i, gate + i);
                     store8<T>(dz + inner + i, up + i);
@@ -152,7 +166,7 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, boo
             }
         }
     } else if constexpr (SUMS == ENTRY_ROWS) {
-        const int c0 = tile_n * TN;
+        const int c0 = t.n * TN;
         const float by = entry >= 0 && a.val ? a.val[entry] : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < TN; c += 32) {
@@ -167,36 +181,37 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, boo
                 if (c0 + c + i < a.cols) to[i / 4] = make_float4(by * v[i], by * v[i + 1], by * v[i + 2], by * v[i + 3]);
         }
     } else if constexpr (SUMS == COMBINE_GRAD) {
-        const int c0 = tile_n * TN;
+        const int c0 = t.n * TN;
         const float by = entry >= 0 ? a.val[entry] : 0.0f;
-        float sum = 0.0f;
+        float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
         for (int c = 0; c < TN; c += 32) {
             __syncwarp();
             if (c0 + c >= a.cols) break;
             float v[32];
             tmem_load(at + c, v);
-            if (entry < 0) continue;
             const int64_t first = entry * a.cols + c0 + c;
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
                 if (c0 + c + i >= a.cols) break;
-                float h[8];
-                load8<T>(h, (const T *)a.other + first + i);
+                float h[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                if (entry >= 0) {
+                    load8<T>(h, (const T *)a.other + first + i);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    sum = fmaf(v[i + j], h[j], sum);
-                    v[i + j] *= by;
-                    h[j] *= by;
+                    for (int j = 0; j < 8; j++) {
+                        sum[j] = fmaf(v[i + j], h[j], sum[j]);
+                        v[i + j] *= by;
+                        h[j] *= by;
+                    }
+                    store8<T>((T *)a.out + first + i, v + i);
                 }
-                store8<T>((T *)a.out + first + i, v + i);
-                store8<T>((T *)a.scaled + first + i, h);
+                store8<T>((T *)a.scaled + (int64_t)(t.slot + row) * a.cols + c0 + c + i, h);
             }
         }
-        if (entry >= 0) a.sums[tile_n * a.nnz + entry] = sum;
+        if (entry >= 0) a.sums[t.n * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     } else {
-        const int c0 = tile_n * TN, r = tile_m * TM + row;
-        T *out = (T *)a.out + ((int64_t)group * a.rows + r) * a.cols + c0;
+        const int c0 = t.n * TN, r = t.m * TM + row;
+        T *out = (T *)a.out + ((int64_t)t.group * a.rows + r) * a.cols + c0;
 #pragma unroll 1
         for (int c = 0; c < TN; c += 32) {
             __syncwarp();
@@ -220,11 +235,11 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, boo
 template <typename T, int SUMS>
 __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 {
-    const int bad = SUMS == WEIGHT ? 0 : a.g.head[1];
+    const int bad = SUMS == WEIGHT || SUMS == GATED_GRAD ? 0 : a.g.head[1];
     const float nan = __int_as_float(0x7fffffff);
     for (int i = blockIdx.x; i < bad; i += gridDim.x) {
         const int64_t entry = a.g.order[a.g.slots - 1 - i];
-        const int cols = SUMS == GATED_GRAD ? 2 * a.cols : a.cols;
+        const int cols = a.cols;
         for (int c = thread; c < cols; c += 128) {
             if (SUMS == ENTRY_ROWS) a.sums[entry * cols + c] = nan;
             else ((T *)a.out)[entry * cols + c] = from_float<T>(nan);
@@ -233,11 +248,15 @@ __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
     }
 }
 
-template <typename T, int FORM, int SUMS>
+// NUMBERED: the operand whose rows come by their number: A (the tile's rows), B (its columns, OUTER), or none
+enum Numbered { NUMBERED_A, NUMBERED_B, NUMBERED_NONE };
+
+template <typename T, int FORM, int NUMBERED, int SUMS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
 {
-    constexpr bool BF16 = sizeof(T) == 2 && Granule<T>::N == 8 && !__is_same(T, __half);
+    constexpr bool BF16 = !__is_same(T, __half);
+    constexpr unsigned TENSOR_BYTES = (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + (NUMBERED == NUMBERED_B ? 0 : B_BYTES);
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * RING + 4 + 1];
     __shared__ uint32_t tmem_room;
@@ -246,10 +265,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
                    last = taken + 16;
-    if (warp == 1) tmem_alloc(smem_at(&tmem_room), 2 * TN);
+    if (warp == 8) tmem_alloc(smem_at(&tmem_room), 2 * TN);
     if (tid == 0) {
         for (int i = 0; i < RING; i++) {
-            bar_init(full + 8 * i, 1);
+            bar_init(full + 8 * i, NUMBERED == NUMBERED_NONE ? 1 : 1 + FETCHERS);
             bar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -267,9 +286,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     wait_for_previous();
 
     const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
-    struct Tile {
-        int m, n, group, steps, slot;
-    };
     auto tile_of = [&](int id) {
         Tile t;
         if (FORM == OUTER) {
@@ -288,65 +304,88 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         return t;
     };
-    auto numbers = [&](const int *list, int slot, int none) {
-        int4 r = *(const int4 *)(list + slot);
-        r.x = r.x < 0 ? none : r.x;
-        r.y = r.y < 0 ? none : r.y;
-        r.z = r.z < 0 ? none : r.z;
-        r.w = r.w < 0 ? none : r.w;
-        return r;
-    };
 
-    unsigned step = 0;                             // steps so far; stage = step % RING
-    if (warp == 0) {                               // fetches
-        for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
+    if (warp >= 4 && warp < 8) {                   // fetches
+        unsigned step = 0;                         // steps so far; stage = step % RING
+        bool on = true;
+        const int me = tid - 128, chunk = me & 7, row = me >> 3;
+        // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
+        const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
+        const char *base = (const char *)a.numbered + chunk * 16;
+        const int64_t stride = a.ld * 2;
+        for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
             const Tile t = tile_of(id);
-            int4 ra, rb;
-            if (FORM != OUTER) ra = numbers(a.rows_a, t.slot + 4 * lane, a.none_a);
-            bool on = true;
+            const char *from[8];
+            unsigned there = 0;
+            if (NUMBERED == NUMBERED_A && FORM != OUTER) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int n = a.numbers[t.slot + row + 16 * i];
+                    from[i] = base + max(n, 0) * stride;
+                    there |= (n >= 0 ? 1u : 0u) << i;
+                }
+            }
+            int next[4];
+            if (NUMBERED != NUMBERED_NONE && FORM == OUTER && t.steps)
+#pragma unroll
+                for (int i = 0; i < 4; i++) next[i] = a.numbers[t.slot + row + 16 * i];
             for (int k = 0; k < t.steps; k++, step++) {
                 const unsigned s = step % RING;
                 const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
-                if (FORM == OUTER) {
-                    ra = numbers(a.rows_a, t.slot + k * TK + 4 * (lane & 15), a.none_a);
-                    rb = numbers(a.rows_b, t.slot + k * TK + 4 * (lane & 15), a.none_b);
-                }
                 on = bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken);
                 on = __all_sync(0xffffffffu, on);
                 if (!on) break;
-                if (lane == 0) bar_expect(bar, STEP_BYTES);
-                __syncwarp();
-                if (FORM == OUTER) {
-                    // blocks of 64 columns: two of a, four of b, 16 copies each
-                    for (int b = lane >> 4; b < 6; b += 2) {
-                        if (b < 2) load_rows(to + b * 8192 + (lane & 15) * 512, &map_a, t.m * TM + b * 64, ra, bar);
-                        else load_rows(to + b * 8192 + (lane & 15) * 512, &map_b, t.n * TN + (b - 2) * 64, rb, bar);
-                    }
-                } else {
-                    load_rows(to + lane * 512, &map_a, k * TK, ra, bar);
+                if (me == 0) {
+                    bar_expect(bar, TENSOR_BYTES);
                     if (FORM == ROWS) {
-                        if (lane < 2) {
-                            if (SUMS == GATED || SUMS == GATED_GRAD)
-                                load_box(to + A_BYTES + lane * (B_BYTES / 2), &map_b, k * TK, t.n * (TN / 2), 2 * t.group + lane, bar);
-                            else
-                                load_box(to + A_BYTES + lane * (B_BYTES / 2), &map_b, k * TK, t.n * TN + lane * (TN / 2), t.group, bar);
-                        }
-                    } else if (lane < 4) {
-                        load_box(to + A_BYTES + lane * 8192, &map_b, t.n * TN + lane * 64, k * TK, t.group, bar);
+                        const int n = t.n * (SUMS == ENTRY_ROWS ? TN : TN / 2), second = SUMS == ENTRY_ROWS ? TN / 2 : 0;
+                        const int z = SUMS == ENTRY_ROWS ? t.group : 2 * t.group;
+                        load_box(to + A_BYTES, &map_b, k * TK, n, z, bar);
+                        load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, n + second, SUMS == ENTRY_ROWS ? z : z + 1, bar);
+                    } else if (FORM == BACK) {
+                        if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * TN + i * 64, k * TK, t.group, bar);
+                    } else if (NUMBERED == NUMBERED_A) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * TN + i * 64, t.slot + k * TK, 0, bar);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
                     }
                 }
+                if (NUMBERED == NUMBERED_A && FORM != OUTER) {
+                    const bool in = k * TK + chunk * 8 < a.numbered_cols;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
+                } else if (NUMBERED != NUMBERED_NONE) {
+                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : 4;
+                    const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
+                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * TN;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const char *src = base + max(next[i], 0) * stride;
+#pragma unroll
+                        for (int b = 0; b < BLOCKS; b++) {
+                            const bool in = col0 + b * 64 + chunk * 8 < a.numbered_cols;
+                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && next[i] >= 0);
+                        }
+                        if (k + 1 < t.steps) next[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
+                    }
+                }
+                if (NUMBERED != NUMBERED_NONE) copies_to(bar);
             }
-            if (!on) break;
         }
         // what is under way lands before the CTA ends
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (*broken) {
             volatile int late = 0;
             for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
         }
-    } else if (warp == 1) {                        // issues the products
+    } else if (warp == 8) {                        // issues the products
         if (lane == 0) {
             constexpr uint32_t kind = product_descriptor(BF16, TM, TN, FORM == OUTER, FORM != ROWS);
-            unsigned tile = 0;
+            unsigned tile = 0, step = 0;
             bool on = true;
             for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
                 const int steps = tile_of(id).steps;
@@ -358,6 +397,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const unsigned s = step % RING;
                     on = bar_wait(full + 8 * s, step / RING & 1, broken);
                     if (!on) break;
+                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
                     tmem_fence_after();
                     const uint32_t at = ring + s * STEP_BYTES;
                     const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
@@ -378,8 +418,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         __syncwarp();
     } else {                                       // takes the sums
-        spoil<T, SUMS>(a, tid - 64);
-        const int quarter = warp & 3, row = quarter * 32 + lane;
+        spoil<T, SUMS>(a, tid);
+        const int row = warp * 32 + lane;
         unsigned tile = 0;
         for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
             const Tile t = tile_of(id);
@@ -391,7 +431,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (!on) break;
                 tmem_fence_after();
             }
-            take_sums<T, SUMS>(a, tmem + b * TN + ((uint32_t)quarter << 21), t.steps == 0, t.m, t.n, t.group, row, entry);
+            take_sums<T, SUMS>(a, tmem + b * TN + ((uint32_t)warp << 21), t.steps == 0, t, row, entry);
             if (t.steps > 0) {
                 tmem_fence_before();
                 __syncwarp();
@@ -403,7 +443,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    if (warp == 1) tmem_free(tmem, 2 * TN);
+    if (warp == 8) tmem_free(tmem, 2 * TN);
     if (tid == 0 && *broken) a.g.head[2] = 1;
 }
 
@@ -438,10 +478,10 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
     out[i] = v;
 }
 
-template <typename T, int FORM, int SUMS>
+template <typename T, int FORM, int NUMBERED, int SUMS>
 static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, const ProductArgs &a, cudaStream_t st)
 {
-    auto kernel = product_kernel<T, FORM, SUMS>;
+    auto kernel = product_kernel<T, FORM, NUMBERED, SUMS>;
     CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
     const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
     if (tiles > 0x7fffffffLL) return fail("experts: more than 2^31 tiles");
@@ -502,21 +542,19 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
     CB_TRY(check_at(what, w));
     CB_TRY(check_at(what, h));
     if (s.nnz == 0 || s.nrows == 0) return 0;
-    alignas(64) CUtensorMap ma, mb;
-    CB_TRY(make_gather_map(what, x, is_bf16<T>(), s.nrows, s.width, ldx, &ma));
+    alignas(64) CUtensorMap mb;
     CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
-    a.rows_a = a.g.token;
-    a.none_a = (int)s.nrows;
+    a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
     a.tiles_n = (int)ceil_div(s.inner, TN / 2);
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.out = h;
-    return launch_product<T, ROWS, GATED>(ma, mb, a, st);
+    return launch_product<T, ROWS, NUMBERED_A, GATED>(mb, mb, a, st);
 }
 
-// dz: room for nnz x 2 inner; sums: for nnz x width floats (null with dx)
+// dz: room for slots x 2 inner; sums: for nnz x width floats (null with dx)
 template <typename T>
 static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, int32_t *plan, const void *x, int64_t ldx, const void *w, const void *dh,
                               void *dz, float *sums, void *dx, void *dw, cudaStream_t st)
@@ -531,45 +569,39 @@ static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, 
         if (dw) CB_CUDA(cudaMemsetAsync(dw, 0, 2 * s.nexperts * s.inner * s.width * sizeof(T), st));
         return 0;
     }
-    alignas(64) CUtensorMap ma, mb;
-    CB_TRY(make_gather_map(what, x, is_bf16<T>(), s.nrows, s.width, ldx, &ma));
+    alignas(64) CUtensorMap mb;
     CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
-    a.rows_a = a.g.token;
-    a.none_a = (int)s.nrows;
+    a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
     a.tiles_n = (int)ceil_div(s.inner, TN / 2);
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.other = dh;
     a.out = dz;
-    CB_TRY((launch_product<T, ROWS, GATED_GRAD>(ma, mb, a, st)));
+    CB_TRY((launch_product<T, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, st)));
     alignas(64) CUtensorMap mz;
-    CB_TRY(make_gather_map(what, dz, is_bf16<T>(), s.nnz, 2 * s.inner, 2 * s.inner, &mz));
     if (dx) {
         a = arguments<T>(s, plan);
         CB_TRY(make_box_map(what, w, is_bf16<T>(), s.nexperts, 2 * s.inner, s.width, TK, &mb));
-        a.rows_a = a.g.order;
-        a.none_a = (int)s.nnz;
+        CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TM, &mz));
         a.terms = 2 * (int)s.inner;
         a.tiles_n = (int)ceil_div(s.width, TN);
         a.cols = (int)s.width;
         a.sums = sums;
-        CB_TRY((launch_product<T, BACK, ENTRY_ROWS>(mz, mb, a, st)));
+        CB_TRY((launch_product<T, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, st)));
         CB_TRY(add_rows<T>(s, pos, sums, dx, st));
     }
     if (dw) {
         a = arguments<T>(s, plan);
-        a.rows_a = a.g.order;
-        a.none_a = (int)s.nnz;
-        a.rows_b = a.g.token;
-        a.none_b = (int)s.nrows;
+        CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TK, &mz));
+        a.number(a.g.token, x, ldx, s.width);
         a.rows = 2 * (int)s.inner;
         a.cols = (int)s.width;
         a.tiles_m = (int)ceil_div(2 * s.inner, TM);
         a.tiles_n = (int)ceil_div(s.width, TN);
         a.out = dw;
-        CB_TRY((launch_product<T, OUTER, WEIGHT>(mz, ma, a, st)));
+        CB_TRY((launch_product<T, OUTER, NUMBERED_B, WEIGHT>(mz, mz, a, st)));
     }
     return 0;
 }
@@ -587,22 +619,20 @@ static int combine_experts(const Sizes &s, const int64_t *pos, int32_t *plan, co
         CB_CUDA(cudaMemsetAsync(y, 0, s.nrows * s.width * sizeof(T), st));
         return 0;
     }
-    alignas(64) CUtensorMap ma, mb;
-    CB_TRY(make_gather_map(what, h, is_bf16<T>(), s.nnz, s.inner, s.inner, &ma));
+    alignas(64) CUtensorMap mb;
     CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
-    a.rows_a = a.g.order;
-    a.none_a = (int)s.nnz;
+    a.number(a.g.order, h, s.inner, s.inner);
     a.terms = (int)s.inner;
     a.tiles_n = (int)ceil_div(s.width, TN);
     a.cols = (int)s.width;
     a.val = val;
     a.sums = sums;
-    CB_TRY((launch_product<T, ROWS, ENTRY_ROWS>(ma, mb, a, st)));
+    CB_TRY((launch_product<T, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, st)));
     return add_rows<T>(s, pos, sums, y, st);
 }
 
-// scaled: room for nnz x inner; sums: for nnz x ceil(inner / 256) floats
+// scaled: room for slots x inner; sums: for nnz x ceil(inner / 256) floats
 template <typename T>
 static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, const float *val, const void *v, const void *dy, int64_t lddy, void *scaled,
                                 float *sums, void *dh, void *dv, float *dval, cudaStream_t st)
@@ -616,12 +646,10 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
         if (dv) CB_CUDA(cudaMemsetAsync(dv, 0, s.nexperts * s.inner * s.width * sizeof(T), st));
         return 0;
     }
-    alignas(64) CUtensorMap my, mb;
-    CB_TRY(make_gather_map(what, dy, is_bf16<T>(), s.nrows, s.width, lddy, &my));
+    alignas(64) CUtensorMap mb;
     CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TK, &mb));
     ProductArgs a = arguments<T>(s, plan);
-    a.rows_a = a.g.token;
-    a.none_a = (int)s.nrows;
+    a.number(a.g.token, dy, lddy, s.width);
     a.terms = (int)s.width;
     a.tiles_n = (int)ceil_div(s.inner, TN);
     a.cols = (int)s.inner;
@@ -630,22 +658,19 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
     a.out = dh;
     a.scaled = scaled;
     a.sums = sums;
-    CB_TRY((launch_product<T, BACK, COMBINE_GRAD>(my, mb, a, st)));
+    CB_TRY((launch_product<T, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, st)));
     CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, a.tiles_n, sums, dval));
     if (dv) {
         alignas(64) CUtensorMap mh;
-        CB_TRY(make_gather_map(what, scaled, is_bf16<T>(), s.nnz, s.inner, s.inner, &mh));
         a = arguments<T>(s, plan);
-        a.rows_a = a.g.token;
-        a.none_a = (int)s.nrows;
-        a.rows_b = a.g.order;
-        a.none_b = (int)s.nnz;
+        CB_TRY(make_box_map(what, scaled, is_bf16<T>(), 1, a.g.slots, s.inner, TK, &mh));
+        a.number(a.g.token, dy, lddy, s.width);
         a.rows = (int)s.width;
         a.cols = (int)s.inner;
         a.tiles_m = (int)ceil_div(s.width, TM);
         a.tiles_n = (int)ceil_div(s.inner, TN);
         a.out = dv;
-        CB_TRY((launch_product<T, OUTER, WEIGHT>(my, mh, a, st)));
+        CB_TRY((launch_product<T, OUTER, NUMBERED_A, WEIGHT>(mh, mh, a, st)));
     }
     return 0;
 }

@@ -7,10 +7,8 @@
 
 namespace cb200 {
 
-// Tensor maps of 16-bit elements with 128-byte rows in shared memory, swizzled (experts.cu).  rows x cols with a row stride of ld elements, boxes of
-// one row of 64 columns (for copies of four rows by number):
-int make_gather_map(const char *what, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, CUtensorMap *map);
-// depth x rows x cols, contiguous, boxes of box_rows rows of 64 columns:
+// A tensor map of 16-bit elements, depth x rows x cols, contiguous, with boxes of box_rows rows of 64 columns, which are 128-byte rows in shared memory,
+// swizzled (experts.cu).
 int make_box_map(const char *what, const void *base, bool bf16, int64_t depth, int64_t rows, int64_t cols, int box_rows, CUtensorMap *map);
 
 #ifdef __CUDACC__
@@ -57,12 +55,18 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, i
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(c), "r"(r), "r"(z), "r"(bar) : "memory");
 }
-// four rows by number; one outside the map reads as zeros
-__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int c, int4 r, uint32_t bar)
+// 16 bytes, or zeros where `on` is not
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void *src, bool on)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                 ::"r"(dst), "l"(map), "r"(c), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+// the thread arrives at the barrier when its copies so far have landed
+__device__ __forceinline__ void copies_to(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// what threads have written to shared memory, and this thread knows of, is seen by products issued from here on
+__device__ __forceinline__ void shared_to_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_alloc(uint32_t at, unsigned columns)
 {

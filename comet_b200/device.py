@@ -370,8 +370,8 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 class EntryGroups:
     """The entries of a CSR matrix by column, as group_entries gives them.  `S` is the matrix, whose pos and crd must stay as they were."""
 
-    def __init__(self, S, plan):
-        self.S, self.plan = S, plan
+    def __init__(self, S, plan, slots):
+        self.S, self.plan, self.slots = S, plan, slots
 
     def check(self):
         """Raises if a kernel that worked with these groups gave up waiting for its own copies or products (its results are incomplete then).  Waits
@@ -394,7 +394,7 @@ def group_entries(S):
     tiles = nnz // 128 + min(nnz, n) + 1                       # as csrc/groups.cuh counts
     plan = S.pos.new_empty(16 + (n + 3) // 4 * 4 + (n + 4) // 4 * 4 + (tiles + 3) // 4 * 4 + 256 * tiles, dtype=torch.int32)
     _call("comet_b200_dev_group_entries_i64", S.nrows, n, nnz, pos, crd, plan.data_ptr(), _stream())
-    return EntryGroups(S, plan)
+    return EntryGroups(S, plan, 128 * tiles)
 
 
 def _check_experts(what, G, name, M, entries, cols=None):
@@ -454,7 +454,7 @@ def gated_experts_grad(G, X, W, d_H, activation="silu", grad_x=True, grad_w=True
     _check_experts("gated_experts_grad", G, "d_H", d_H, True, sizes[4])
     nnz, width, inner = sizes[2:5]
     new = X.new_empty
-    dz, sums = new((nnz, 2 * inner)), new((nnz, width), dtype=torch.float32) if grad_x else None
+    dz, sums = new((G.slots, 2 * inner)), new((nnz, width), dtype=torch.float32) if grad_x else None
     d_X, d_W = new((G.S.nrows, width)) if grad_x else None, new(W.shape) if grad_w else None
     _call(_GATED_GRAD[X.dtype], *sizes, G.S.pos.data_ptr(), G.plan.data_ptr(), X.data_ptr(), ld, W.data_ptr(), d_H.data_ptr(), dz.data_ptr(), _p(sums),
           _p(d_X), _p(d_W), _stream())
@@ -489,7 +489,7 @@ def combine_experts_grad(G, H, V, d_Y, grad_v=True):
     _, ld = _check_experts("combine_experts_grad", G, "d_Y", d_Y, False, sizes[3])
     nnz, inner = sizes[2], sizes[4]
     new = H.new_empty
-    scaled, sums = new((nnz, inner)), new(nnz * ((inner + 255) // 256), dtype=torch.float32)
+    scaled, sums = new((G.slots, inner)), new(nnz * ((inner + 255) // 256), dtype=torch.float32)
     d_H, d_V, d_values = new((nnz, inner)), new(V.shape) if grad_v else None, new(nnz, dtype=torch.float32)
     _call(_COMBINE_GRAD[H.dtype], *sizes, G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), d_Y.data_ptr(), ld, scaled.data_ptr(), sums.data_ptr(),
           d_H.data_ptr(), _p(d_V), d_values.data_ptr(), _stream())
