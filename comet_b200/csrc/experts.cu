@@ -56,9 +56,17 @@ int make_box_map(const char *what, const void *base, bool bf16, int64_t depth, i
 enum Form { ROWS, BACK, OUTER };
 enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 
-static const int TM = 128, TN = 256, TK = 64, RING = 4;
-static const int A_BYTES = TM * TK * 2, B_BYTES = TN * TK * 2, STEP_BYTES = A_BYTES + B_BYTES;
-static const int FETCHERS = 128, PRODUCT_THREADS = 128 + FETCHERS + 32, PRODUCT_SMEM = RING * STEP_BYTES + 1024;
+// A tile has 128 rows and W columns.  W = 256 where there are tiles enough for the chip; else 64, two CTAs on an SM: the weights of few tokens' experts
+// are read by all SMs then (one token, 8 experts of 1024 x 2048 gates and ups: @GATED_ONE@ us against 21).
+static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64, RING = 4;
+static const int A_BYTES = TM * TK * 2;
+static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 32;
+template <int W>
+struct Shape {
+    static constexpr int B_BYTES = W * TK * 2, STEP = A_BYTES + B_BYTES;
+    static constexpr int TAKEN = W == WIDE ? 128 : 32;         // bytes of a row that a warp takes out at a time
+    static constexpr int SMEM = RING * STEP + TAKERS * TAKEN + 1024;
+};
 
 struct ProductArgs {
     Groups g;
@@ -118,144 +126,212 @@ __device__ __forceinline__ void load8(float *v, const T *from)
     for (int i = 0; i < 8; i++) v[i] = f[i];
 }
 
-// A tile's sums, 32 columns at a time, by the thread that has the row; at: tensor memory of the warp's rows.  entry < 0: nothing to store.
-template <typename T, int SUMS>
-__device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t at, bool none, const Tile &t, int row, int64_t entry)
+// A warp's 32 rows of BYTES bytes in shared memory, on their way to or from global memory: a thread has a row, but reads and writes of global memory are
+// of whole rows, BYTES / 16 neighbouring lanes each.  (Stores by the threads of the rows touch 32 lines an instruction: the sums of combine_batch
+// were taken out in twice the time of the products.)
+template <typename E, int BYTES>
+struct Stage {
+    static constexpr int LANES = BYTES / 16, N = 16 / sizeof(E), COLS = BYTES / sizeof(E);
+    unsigned char *room;
+    int lane;
+    __device__ __forceinline__ uint4 &at(int row, int chunk) const { return *(uint4 *)(room + row * BYTES + ((chunk ^ (row & (LANES - 1))) << 4)); }
+    __device__ __forceinline__ void put(int chunk, const float *v) const
+    {
+        Granule<E> out;
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) f[i] = v[i];
+        out.pack(f);
+        at(lane, chunk) = out.w;
+    }
+    __device__ __forceinline__ void get(int chunk, float *v) const
+    {
+        Granule<E> in;
+        in.w = at(lane, chunk);
+        float f[N];
+        in.unpack(f);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = f[i];
+    }
+    // rows from base + first (each thread's own; negative: none), `cols` of them there
+    __device__ __forceinline__ void out(E *base, int64_t first, int cols) const
+    {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < LANES; i++) {
+            const int row = i * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+            const int64_t to = __shfl_sync(0xffffffffu, first, row);
+            if (to >= 0 && chunk * N < cols) *(uint4 *)(base + to + chunk * N) = at(row, chunk);
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void in(const E *base, int64_t first, int cols) const
+    {
+#pragma unroll
+        for (int i = 0; i < LANES; i++) {
+            const int row = i * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+            const int64_t from = __shfl_sync(0xffffffffu, first, row);
+            at(row, chunk) = from >= 0 && chunk * N < cols ? *(const uint4 *)(base + from + chunk * N) : make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+    }
+};
+
+// A tile's sums, by two warps for each 32 rows, a half of the columns each; tmem: tensor memory of the rows.  entry: that of the thread's row,
+// negative if there is none.
+template <typename T, int W, int SUMS>
+__device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, bool none, const Tile &t, int half, int row, int64_t entry, unsigned char *room)
 {
+    constexpr int BYTES = Shape<W>::TAKEN;
+    const Stage<T, BYTES> st = {room, (int)threadIdx.x & 31};
     if constexpr (SUMS == GATED || SUMS == GATED_GRAD) {
-        const int f0 = t.n * (TN / 2), inner = a.cols;
+        constexpr int MINE = W / 4, PART = MINE < 32 ? MINE : 32;                    // columns of the warp, at a time
+        static_assert(MINE == st.COLS, "one row of the stage");
+        const int inner = a.cols, f0 = t.n * (W / 2) + half * MINE, left = inner - f0;
+        if (left <= 0) return;
+        const uint32_t at = tmem + half * MINE;
+        if (SUMS == GATED) {
+#pragma unroll
+            for (int c = 0; c < MINE; c += PART) {
+                float gate[PART], up[PART];
+                tmem_load(at + c, gate);
+                tmem_load(at + W / 2 + c, up);
+#pragma unroll
+                for (int i = 0; i < PART; i++) gate[i] = gate[i] * logistic(gate_of(gate[i], a.gelu).x) * up[i];
+#pragma unroll
+                for (int i = 0; i < PART; i += 8) st.put((c + i) / 8, gate + i);
+            }
+            st.out((T *)a.out, entry < 0 ? -1 : entry * inner + f0, left);
+        } else {
+            // PART columns at a time: with all 64 there are not registers enough
+            const Stage<T, PART * 2> part = {room, (int)threadIdx.x & 31};
 #pragma unroll 1
-        for (int c = 0; c < TN / 2; c += 32) {
-            __syncwarp();
-            if (f0 + c >= inner) break;            // the same for all
-            float gate[32], up[32];
-            tmem_load(at + c, gate);
-            tmem_load(at + TN / 2 + c, up);
-            if (SUMS == GATED) {
-                if (entry < 0) continue;
-                T *h = (T *)a.out + entry * inner + f0 + c;
+            for (int c = 0; c < MINE; c += PART) {
+                float d[PART], gate[PART], up[PART];
+                part.in((const T *)a.other, entry < 0 ? -1 : entry * inner + f0 + c, left - c);          // a row of zeros where there is none
 #pragma unroll
-                for (int i = 0; i < 32; i++) gate[i] = gate[i] * logistic(gate_of(gate[i], a.gelu).x) * up[i];
+                for (int i = 0; i < PART; i += 8) part.get(i / 8, d + i);
+                tmem_load(at + c, gate);
+                tmem_load(at + W / 2 + c, up);
 #pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    if (f0 + c + i < inner) store8<T>(h + i, gate + i);
-            } else {
-                T *dz = (T *)a.out + (int64_t)(t.slot + row) * 2 * inner + f0 + c;
-                const T *dh = (const T *)a.other + entry * inner + f0 + c;
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (f0 + c + i >= inner) break;
-                    if (entry >= 0) {
-                        float d[8];
-                        load8<T>(d, dh + i);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const float g = gate[i + j];
-                            const float2 u = gate_of(g, a.gelu);
-                            const float s = logistic(u.x);
-                            gate[i + j] = d[j] * up[i + j] * fmaf(g * s * (1.0f - s), u.y, s);
-                            up[i + j] = d[j] * g * s;
-                        }
-                    } else {                       // a row of the sums over an expert's tokens that adds nothing
-#pragma unroll
-                        for (int j = 0; j < 8; j++) gate[i + j] = up[i + j] = 0.0f;
-                    }
-                    store8<T>(dz + i, gate + i);
-                    store8<T>(dz + inner + i, up + i);
+                for (int i = 0; i < PART; i++) {
+                    const float g = gate[i];
+                    const float2 u = gate_of(g, a.gelu);
+                    const float s = logistic(u.x);
+                    gate[i] = d[i] * up[i] * fmaf(g * s * (1.0f - s), u.y, s);
+                    up[i] = d[i] * g * s;
                 }
+                const int64_t to = (int64_t)(t.slot + row) * 2 * inner + f0 + c;
+#pragma unroll
+                for (int i = 0; i < PART; i += 8) part.put(i / 8, gate + i);
+                part.out((T *)a.out, to, left - c);
+#pragma unroll
+                for (int i = 0; i < PART; i += 8) part.put(i / 8, up + i);
+                part.out((T *)a.out, to + inner, left - c);
             }
         }
     } else if constexpr (SUMS == ENTRY_ROWS) {
-        const int c0 = t.n * TN;
+        constexpr int MINE = W / 2, PART = BYTES / 4;
+        const Stage<float, BYTES> rows = {room, (int)threadIdx.x & 31};
+        const int c0 = t.n * W + half * MINE;
         const float by = entry >= 0 && a.val ? a.val[entry] : 1.0f;
 #pragma unroll 1
-        for (int c = 0; c < TN; c += 32) {
-            __syncwarp();
+        for (int c = 0; c < MINE; c += W == WIDE ? 32 : 16) {
             if (c0 + c >= a.cols) break;
-            float v[32];
-            tmem_load(at + c, v);
-            if (entry < 0) continue;
-            float4 *to = (float4 *)(a.sums + entry * a.cols + c0 + c);
+            float v[W == WIDE ? 32 : 16];
+            __syncwarp();
+            tmem_load(tmem + half * MINE + c, v);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                if (c0 + c + i < a.cols) to[i / 4] = make_float4(by * v[i], by * v[i + 1], by * v[i + 2], by * v[i + 3]);
+            for (int p = 0; p < (W == WIDE ? 32 : 16); p += PART) {
+#pragma unroll
+                for (int i = 0; i < PART; i++) v[p + i] *= by;
+#pragma unroll
+                for (int i = 0; i < PART; i += 4) rows.put(i / 4, v + p + i);
+                rows.out(a.sums, entry < 0 ? -1 : entry * a.cols + c0 + c + p, a.cols - c0 - c - p);
+            }
         }
     } else if constexpr (SUMS == COMBINE_GRAD) {
-        const int c0 = t.n * TN;
+        constexpr int MINE = W / 2, PART = st.COLS < 32 ? st.COLS : 32;
+        const Stage<T, PART * 2> part = {room, (int)threadIdx.x & 31};
+        const int c0 = t.n * W + half * MINE;
         const float by = entry >= 0 ? a.val[entry] : 0.0f;
         float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-        for (int c = 0; c < TN; c += 32) {
-            __syncwarp();
-            if (c0 + c >= a.cols) break;
-            float v[32];
-            tmem_load(at + c, v);
-            const int64_t first = entry * a.cols + c0 + c;
+        for (int c = 0; c < MINE; c += PART) {
+            const int left = a.cols - c0 - c;
+            if (left <= 0) break;
+            const int64_t first = entry < 0 ? -1 : entry * a.cols + c0 + c;
+            float h[PART], v[PART];
+            part.in((const T *)a.other, first, left);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-                if (c0 + c + i >= a.cols) break;
-                float h[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                if (entry >= 0) {
-                    load8<T>(h, (const T *)a.other + first + i);
+            for (int i = 0; i < PART; i += 8) part.get(i / 8, h + i);
+            tmem_load(tmem + half * MINE + c, v);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        sum[j] = fmaf(v[i + j], h[j], sum[j]);
-                        v[i + j] *= by;
-                        h[j] *= by;
-                    }
-                    store8<T>((T *)a.out + first + i, v + i);
-                }
-                store8<T>((T *)a.scaled + (int64_t)(t.slot + row) * a.cols + c0 + c + i, h);
+            for (int i = 0; i < PART; i++) {
+                if (entry >= 0) sum[i % 8] = fmaf(v[i], h[i], sum[i % 8]);
+                v[i] *= by;
+                h[i] *= by;
             }
+#pragma unroll
+            for (int i = 0; i < PART; i += 8) part.put(i / 8, v + i);
+            part.out((T *)a.out, first, left);
+            // a row of zeros adds nothing to the sums over an expert's tokens
+#pragma unroll
+            for (int i = 0; i < PART; i += 8) part.put(i / 8, h + i);
+            part.out((T *)a.scaled, (int64_t)(t.slot + row) * a.cols + c0 + c, left);
         }
-        if (entry >= 0) a.sums[t.n * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+        if (entry >= 0) a.sums[(t.n * 2 + half) * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     } else {
-        const int c0 = t.n * TN, r = t.m * TM + row;
-        T *out = (T *)a.out + ((int64_t)t.group * a.rows + r) * a.cols + c0;
+        constexpr int MINE = W / 2, PART = st.COLS < 32 ? st.COLS : 32;
+        const int c0 = t.n * W + half * MINE, r = t.m * TM + row;
+        const int64_t first = r < a.rows ? ((int64_t)t.group * a.rows + r) * a.cols + c0 : -1;
 #pragma unroll 1
-        for (int c = 0; c < TN; c += 32) {
-            __syncwarp();
+        for (int c = 0; c < MINE; c += st.COLS) {
             if (c0 + c >= a.cols) break;
-            float v[32];
-            if (none) {
+            __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = 0.0f;
-            } else {
-                tmem_load(at + c, v);
+            for (int p = 0; p < st.COLS; p += PART) {
+                float v[PART];
+                if (none) {                        // an expert without tokens
+#pragma unroll
+                    for (int i = 0; i < PART; i++) v[i] = 0.0f;
+                } else {
+                    tmem_load(tmem + half * MINE + c + p, v);
+                }
+#pragma unroll
+                for (int i = 0; i < PART; i += 8) st.put((p + i) / 8, v + i);
             }
-            if (r >= a.rows) continue;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-                if (c0 + c + i < a.cols) store8<T>(out + c + i, v + i);
+            st.out((T *)a.out, first < 0 ? -1 : first + c, a.cols - c0 - c);
         }
     }
 }
 
-// An entry whose column is no expert's: NaN.  By four warps.
-template <typename T, int SUMS>
+// An entry whose column is no expert's: NaN.
+template <typename T, int W, int SUMS>
 __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 {
     const int bad = SUMS == WEIGHT || SUMS == GATED_GRAD ? 0 : a.g.head[1];
     const float nan = __int_as_float(0x7fffffff);
     for (int i = blockIdx.x; i < bad; i += gridDim.x) {
         const int64_t entry = a.g.order[a.g.slots - 1 - i];
-        const int cols = a.cols;
-        for (int c = thread; c < cols; c += 128) {
-            if (SUMS == ENTRY_ROWS) a.sums[entry * cols + c] = nan;
-            else ((T *)a.out)[entry * cols + c] = from_float<T>(nan);
-            if (SUMS == COMBINE_GRAD && c % TN == 0) a.sums[c / TN * a.nnz + entry] = nan;
+        for (int c = thread; c < a.cols; c += TAKERS) {
+            if (SUMS == ENTRY_ROWS) a.sums[entry * a.cols + c] = nan;
+            else ((T *)a.out)[entry * a.cols + c] = from_float<T>(nan);
         }
+        if (SUMS == COMBINE_GRAD)
+            for (int p = thread; p < 2 * a.tiles_n; p += TAKERS) a.sums[p * a.nnz + entry] = nan;
     }
 }
 
 // NUMBERED: the operand whose rows come by their number: A (the tile's rows), B (its columns, OUTER), or none
 enum Numbered { NUMBERED_A, NUMBERED_B, NUMBERED_NONE };
 
-template <typename T, int FORM, int NUMBERED, int SUMS>
-__global__ void __launch_bounds__(PRODUCT_THREADS, 1)
+template <typename T, int W, int FORM, int NUMBERED, int SUMS>
+__global__ void __launch_bounds__(PRODUCT_THREADS, W == WIDE ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
 {
     constexpr bool BF16 = !__is_same(T, __half);
+    constexpr int B_BYTES = Shape<W>::B_BYTES, STEP_BYTES = Shape<W>::STEP;
     constexpr unsigned TENSOR_BYTES = (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + (NUMBERED == NUMBERED_B ? 0 : B_BYTES);
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * RING + 4 + 1];
@@ -263,9 +339,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     __shared__ int broken_word;
     volatile int *broken = &broken_word;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int ISSUER = (TAKERS + FETCHERS) / 32;
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
                    last = taken + 16;
-    if (warp == 8) tmem_alloc(smem_at(&tmem_room), 2 * TN);
+    if (warp == ISSUER) tmem_alloc(smem_at(&tmem_room), 2 * W);
     if (tid == 0) {
         for (int i = 0; i < RING; i++) {
             bar_init(full + 8 * i, NUMBERED == NUMBERED_NONE ? 1 : 1 + FETCHERS);
@@ -273,7 +350,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         for (int i = 0; i < 2; i++) {
             bar_init(done + 8 * i, 1);
-            bar_init(taken + 8 * i, 4);
+            bar_init(taken + 8 * i, TAKERS / 32);
         }
         bar_init(last, 1);
         broken_word = 0;
@@ -305,10 +382,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         return t;
     };
 
-    if (warp >= 4 && warp < 8) {                   // fetches
+    if (warp >= TAKERS / 32 && warp < ISSUER) {    // fetches
         unsigned step = 0;                         // steps so far; stage = step % RING
         bool on = true;
-        const int me = tid - 128, chunk = me & 7, row = me >> 3;
+        const int me = tid - TAKERS, chunk = me & 7, row = me >> 3;
         // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
         const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
         const char *base = (const char *)a.numbered + chunk * 16;
@@ -338,17 +415,17 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (me == 0) {
                     bar_expect(bar, TENSOR_BYTES);
                     if (FORM == ROWS) {
-                        const int n = t.n * (SUMS == ENTRY_ROWS ? TN : TN / 2), second = SUMS == ENTRY_ROWS ? TN / 2 : 0;
+                        const int n = t.n * (SUMS == ENTRY_ROWS ? W : W / 2), second = SUMS == ENTRY_ROWS ? W / 2 : 0;
                         const int z = SUMS == ENTRY_ROWS ? t.group : 2 * t.group;
                         load_box(to + A_BYTES, &map_b, k * TK, n, z, bar);
                         load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, n + second, SUMS == ENTRY_ROWS ? z : z + 1, bar);
                     } else if (FORM == BACK) {
                         if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * TN + i * 64, k * TK, t.group, bar);
+                        for (int i = 0; i < W / 64; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * W + i * 64, k * TK, t.group, bar);
                     } else if (NUMBERED == NUMBERED_A) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * TN + i * 64, t.slot + k * TK, 0, bar);
+                        for (int i = 0; i < W / 64; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * W + i * 64, t.slot + k * TK, 0, bar);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
@@ -359,9 +436,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
                 } else if (NUMBERED != NUMBERED_NONE) {
-                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : 4;
+                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : W / 64;
                     const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
-                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * TN;
+                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const char *src = base + max(next[i], 0) * stride;
@@ -382,9 +459,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             volatile int late = 0;
             for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
         }
-    } else if (warp == 8) {                        // issues the products
+    } else if (warp == ISSUER) {                   // issues the products
         if (lane == 0) {
-            constexpr uint32_t kind = product_descriptor(BF16, TM, TN, FORM == OUTER, FORM != ROWS);
+            constexpr uint32_t kind = product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
             unsigned tile = 0, step = 0;
             bool on = true;
             for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
@@ -404,7 +481,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
                     constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
 #pragma unroll
-                    for (int i = 0; i < TK / 16; i++) product(tmem + b * TN, da + i * next_a, db + i * next_b, kind, k + i > 0);
+                    for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
                     products_to(empty + 8 * s);
                 }
                 if (on) products_to(done + 8 * b);
@@ -418,8 +495,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         __syncwarp();
     } else {                                       // takes the sums
-        spoil<T, SUMS>(a, tid);
-        const int row = warp * 32 + lane;
+        spoil<T, W, SUMS>(a, tid);
+        const int row = (warp & 3) * 32 + lane;
+        unsigned char *room = raw + (ring - smem_at(raw)) + RING * STEP_BYTES + warp * 32 * Shape<W>::TAKEN;
         unsigned tile = 0;
         for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
             const Tile t = tile_of(id);
@@ -431,7 +509,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (!on) break;
                 tmem_fence_after();
             }
-            take_sums<T, SUMS>(a, tmem + b * TN + ((uint32_t)warp << 21), t.steps == 0, t, row, entry);
+            take_sums<T, W, SUMS>(a, tmem + b * W + ((uint32_t)(warp & 3) << 21), t.steps == 0, t, warp >> 2, row, entry, room);
             if (t.steps > 0) {
                 tmem_fence_before();
                 __syncwarp();
@@ -443,7 +521,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    if (warp == 8) tmem_free(tmem, 2 * TN);
+    if (warp == ISSUER) tmem_free(tmem, 2 * W);
     if (tid == 0 && *broken) a.g.head[2] = 1;
 }
 
@@ -478,15 +556,19 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
     out[i] = v;
 }
 
-template <typename T, int FORM, int NUMBERED, int SUMS>
-static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, const ProductArgs &a, cudaStream_t st)
+// wide or narrow tiles for products of tokens' rows
+static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) < sm_count(); }
+
+template <typename T, int W, int FORM, int NUMBERED, int SUMS>
+static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, ProductArgs a, int64_t columns, cudaStream_t st)
 {
-    auto kernel = product_kernel<T, FORM, NUMBERED, SUMS>;
-    CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
+    auto kernel = product_kernel<T, W, FORM, NUMBERED, SUMS>;
+    CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<W>::SMEM));
+    a.tiles_n = (int)ceil_div(columns, W);
     const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
+    const int64_t most = sm_count() * (W == WIDE ? 1 : 2);
     if (tiles > 0x7fffffffLL) return fail("experts: more than 2^31 tiles");
-    const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
-    CB_CUDA(launch_behind(kernel, dim3(grid), PRODUCT_THREADS, PRODUCT_SMEM, st, map_a, map_b, a));
+    CB_CUDA(launch_behind(kernel, dim3((unsigned)(tiles < most ? tiles : most)), PRODUCT_THREADS, Shape<W>::SMEM, st, map_a, map_b, a));
     return 0;
 }
 
@@ -543,15 +625,16 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
     CB_TRY(check_at(what, h));
     if (s.nnz == 0 || s.nrows == 0) return 0;
     alignas(64) CUtensorMap mb;
-    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
+    const bool few = narrow(a.g, s.nnz, 2 * s.inner);
+    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
-    a.tiles_n = (int)ceil_div(s.inner, TN / 2);
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.out = h;
-    return launch_product<T, ROWS, NUMBERED_A, GATED>(mb, mb, a, st);
+    return few ? launch_product<T, NARROW, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st)
+               : launch_product<T, WIDE, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st);
 }
 
 // dz: room for slots x 2 inner; sums: for nnz x width floats (null with dx)
@@ -570,26 +653,27 @@ static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, 
         return 0;
     }
     alignas(64) CUtensorMap mb;
-    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
+    const bool few = narrow(a.g, s.nnz, 2 * s.inner);
+    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
-    a.tiles_n = (int)ceil_div(s.inner, TN / 2);
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.other = dh;
     a.out = dz;
-    CB_TRY((launch_product<T, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, st)));
+    CB_TRY(few ? (launch_product<T, NARROW, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, 2 * s.inner, st))
+               : (launch_product<T, WIDE, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, 2 * s.inner, st)));
     alignas(64) CUtensorMap mz;
     if (dx) {
         a = arguments<T>(s, plan);
         CB_TRY(make_box_map(what, w, is_bf16<T>(), s.nexperts, 2 * s.inner, s.width, TK, &mb));
         CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TM, &mz));
         a.terms = 2 * (int)s.inner;
-        a.tiles_n = (int)ceil_div(s.width, TN);
-        a.cols = (int)s.width;
+            a.cols = (int)s.width;
         a.sums = sums;
-        CB_TRY((launch_product<T, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, st)));
+        CB_TRY(narrow(a.g, s.nnz, s.width) ? (launch_product<T, NARROW, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, s.width, st))
+                                           : (launch_product<T, WIDE, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, s.width, st)));
         CB_TRY(add_rows<T>(s, pos, sums, dx, st));
     }
     if (dw) {
@@ -599,9 +683,8 @@ static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, 
         a.rows = 2 * (int)s.inner;
         a.cols = (int)s.width;
         a.tiles_m = (int)ceil_div(2 * s.inner, TM);
-        a.tiles_n = (int)ceil_div(s.width, TN);
-        a.out = dw;
-        CB_TRY((launch_product<T, OUTER, NUMBERED_B, WEIGHT>(mz, mz, a, st)));
+            a.out = dw;
+        CB_TRY((launch_product<T, WIDE, OUTER, NUMBERED_B, WEIGHT>(mz, mz, a, s.width, st)));
     }
     return 0;
 }
@@ -620,19 +703,20 @@ static int combine_experts(const Sizes &s, const int64_t *pos, int32_t *plan, co
         return 0;
     }
     alignas(64) CUtensorMap mb;
-    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TN / 2, &mb));
     ProductArgs a = arguments<T>(s, plan);
+    const bool few = narrow(a.g, s.nnz, s.width);
+    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.order, h, s.inner, s.inner);
     a.terms = (int)s.inner;
-    a.tiles_n = (int)ceil_div(s.width, TN);
     a.cols = (int)s.width;
     a.val = val;
     a.sums = sums;
-    CB_TRY((launch_product<T, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, st)));
+    CB_TRY(few ? (launch_product<T, NARROW, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, s.width, st))
+               : (launch_product<T, WIDE, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, s.width, st)));
     return add_rows<T>(s, pos, sums, y, st);
 }
 
-// scaled: room for slots x inner; sums: for nnz x ceil(inner / 256) floats
+// scaled: room for slots x inner; sums: for nnz x 2 ceil(inner / 64) floats
 template <typename T>
 static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, const float *val, const void *v, const void *dy, int64_t lddy, void *scaled,
                                 float *sums, void *dh, void *dv, float *dval, cudaStream_t st)
@@ -651,15 +735,16 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
     ProductArgs a = arguments<T>(s, plan);
     a.number(a.g.token, dy, lddy, s.width);
     a.terms = (int)s.width;
-    a.tiles_n = (int)ceil_div(s.inner, TN);
     a.cols = (int)s.inner;
     a.other = h;
     a.val = val;
     a.out = dh;
     a.scaled = scaled;
     a.sums = sums;
-    CB_TRY((launch_product<T, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, st)));
-    CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, a.tiles_n, sums, dval));
+    const bool few = narrow(a.g, s.nnz, s.inner);
+    CB_TRY(few ? (launch_product<T, NARROW, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, s.inner, st))
+               : (launch_product<T, WIDE, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, s.inner, st)));
+    CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, 2 * (int)ceil_div(s.inner, few ? NARROW : WIDE), sums, dval));
     if (dv) {
         alignas(64) CUtensorMap mh;
         a = arguments<T>(s, plan);
@@ -668,9 +753,8 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
         a.rows = (int)s.width;
         a.cols = (int)s.inner;
         a.tiles_m = (int)ceil_div(s.width, TM);
-        a.tiles_n = (int)ceil_div(s.inner, TN);
-        a.out = dv;
-        CB_TRY((launch_product<T, OUTER, NUMBERED_A, WEIGHT>(mh, mh, a, st)));
+            a.out = dv;
+        CB_TRY((launch_product<T, WIDE, OUTER, NUMBERED_A, WEIGHT>(mh, mh, a, s.inner, st)));
     }
     return 0;
 }

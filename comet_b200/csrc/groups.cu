@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(GT)
 group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
 {
     extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
-    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], sums[GW];
+    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], sums[GW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     int *own = warps + (size_t)warp * n;
@@ -25,7 +25,7 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     __syncthreads();
     const int64_t each = (nrows + (int64_t)ranks * GW - 1) / ((int64_t)ranks * GW), from = min((rank * GW + warp) * each, nrows);
     const int64_t to = min(from + each, nrows);
-    // each lane's entries of a row, one after the other; what(entry, its row, its column, the lanes that have the same one)
+    // each lane's entries of a row, one after the other, eight on their way at a time; what(entry, its row, its column, the lanes that have the same one)
     auto walk = [&](auto what) {
         for (int64_t r = from; r < to; r += 32) {
             int64_t lo = 0, hi = 0;
@@ -33,15 +33,19 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
                 lo = min(max(pos[r + lane], (int64_t)0), nnz);
                 hi = min(max(pos[r + lane + 1], lo), nnz);
             }
-            int64_t next = lo < hi ? crd[lo] : 0;
-            while (__any_sync(0xffffffffu, lo < hi)) {
-                const bool on = lo < hi;
-                const int64_t col = next, e = lo++;
-                if (lo < hi) next = crd[lo];
-                const bool good = on && col >= 0 && col < n;
-                const unsigned alike = __match_any_sync(0xffffffffu, good ? (int)col : -1);
-                if (on) what(e, r + lane, good ? (int)col : -1, alike);
-                __syncwarp();
+            for (; __any_sync(0xffffffffu, lo < hi); lo += 8) {
+                int64_t col[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) col[i] = lo + i < hi ? crd[lo + i] : -1;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const bool on = lo + i < hi;
+                    if (!__any_sync(0xffffffffu, on)) break;
+                    const int c = col[i] >= 0 && col[i] < n ? (int)col[i] : -1;
+                    const unsigned alike = __match_any_sync(0xffffffffu, c);
+                    if (on) what(lo + i, r + lane, c, alike);
+                    __syncwarp();
+                }
             }
         }
     };
@@ -82,16 +86,20 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     for (int w = 0; w < warp; w++) upto += sums[w];
     if (tid < n) {
         start[tid] = (upto - tiles) * GROUP_TILE + before;
+        whole[tid] = total;
+        ends[tid] = upto;
         if (rank == 0) {
             g.counts[tid] = total;
             g.first[tid] = upto - tiles;
-            for (int i = 0; i < tiles; i++) g.column[upto - tiles + i] = tid;
             if (tid == n - 1) g.first[n] = g.head[0] = upto;
         }
-        if (tid % ranks == rank)
-            for (int i = total; i < tiles * GROUP_TILE; i++) g.order[(int64_t)(upto - tiles) * GROUP_TILE + i] = g.token[(int64_t)(upto - tiles) * GROUP_TILE + i] = -1;
     }
     __syncthreads();
+    for (int c = rank * GW + warp; c < n; c += ranks * GW) {                         // a warp has a column's tiles and the rest of its last one
+        const int sum = whole[c], first = ends[c] - (sum + GROUP_TILE - 1) / GROUP_TILE;
+        for (int i = first + lane; i < ends[c]; i += 32) g.column[i] = c;
+        for (int64_t i = (int64_t)first * GROUP_TILE + sum + lane; i < (int64_t)ends[c] * GROUP_TILE; i += 32) g.order[i] = g.token[i] = -1;
+    }
     for (int i = tid; i < GW * n; i += GT) warps[i] += start[i % n];
     __syncthreads();
     if (ranks > 1) cluster_arrive();               // this CTA has read the others' counts

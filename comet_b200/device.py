@@ -489,7 +489,7 @@ def combine_experts_grad(G, H, V, d_Y, grad_v=True):
     _, ld = _check_experts("combine_experts_grad", G, "d_Y", d_Y, False, sizes[3])
     nnz, inner = sizes[2], sizes[4]
     new = H.new_empty
-    scaled, sums = new((G.slots, inner)), new(nnz * ((inner + 255) // 256), dtype=torch.float32)
+    scaled, sums = new((G.slots, inner)), new(nnz * ((inner + 63) // 64 * 2), dtype=torch.float32)
     d_H, d_V, d_values = new((nnz, inner)), new(V.shape) if grad_v else None, new(nnz, dtype=torch.float32)
     _call(_COMBINE_GRAD[H.dtype], *sizes, G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), d_Y.data_ptr(), ld, scaled.data_ptr(), sums.data_ptr(),
           d_H.data_ptr(), _p(d_V), d_values.data_ptr(), _stream())

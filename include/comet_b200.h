@@ -753,7 +753,7 @@ COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_f16_i64(
     const float *val, const void *v, float *sums, void *y, void *stream);
 
 /* Its gradients dh (h's shape), dv (v's shape; may be NULL) and dval[nnz] from dy (nrows x width, row stride lddy, a multiple of 8).  scaled: room
-   for slots x inner elements (slots as above) (val * h, rounded to the operands' type, which dv is computed with); sums: for nnz x ceil(inner / 256) floats. */
+   for slots x inner elements (slots as above) (val * h, rounded to the operands' type, which dv is computed with); sums: for nnz x 2 ceil(inner / 64) floats. */
 COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_grad_bf16_i64(
     int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t *plan, const void *h, const float *val,
     const void *v, const void *dy, int64_t lddy, void *scaled, float *sums, void *dh, void *dv, float *dval, void *stream);
