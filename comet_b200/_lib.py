@@ -120,7 +120,7 @@ for _t in ("bf16", "f16"):
     SIGNATURES.update({
         "comet_b200_dev_gated_experts_%s_i64" % _t: (c_int32, [c_int64] * 5 + [c_int32] + [c_void_p] * 2 + [c_int64] + [c_void_p] * 3),
         "comet_b200_dev_gated_experts_grad_%s_i64" % _t: (c_int32, [c_int64] * 5 + [c_int32] + [c_void_p] * 3 + [c_int64] + [c_void_p] * 7),
-        "comet_b200_dev_combine_experts_%s_i64" % _t: (c_int32, [c_int64] * 5 + [c_void_p] * 8),
+        "comet_b200_dev_combine_experts_%s_i64" % _t: (c_int32, [c_int64] * 5 + [c_void_p] * 9),
         "comet_b200_dev_combine_experts_grad_%s_i64" % _t: (c_int32, [c_int64] * 5 + [c_void_p] * 5 + [c_int64] + [c_void_p] * 6),
     })
 SIGNATURES["comet_b200_ciface_free"] = (None, [c_void_p])

@@ -18,6 +18,8 @@
 #include <cuda_fp16.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "groups.cuh"
 #include "logits.cuh"
 #include "stream.cuh"
@@ -556,6 +558,210 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
     out[i] = v;
 }
 
+// Few tokens: products of a weight's rows with a handful of vectors, by the ordinary cores.  Neighbouring rows of an expert's weight are one piece of
+// memory, so a CTA's share comes in copies of up to 32 KB.  Six teams of four warps have a stage each: while one of them works on its stage, the others'
+// copies are under way, what an SM has to have in flight for the memory's full rate.  The vectors come through the L1 cache.
+static const int FEW_ROWS = 8, FEW_SUMS = 4;       // rows of x, of y up to which this is taken
+static const int FEW_STAGES = 6, FEW_BYTES = 32 * 1024, FEW_SMEM = FEW_STAGES * FEW_BYTES, FEW_ENTRIES = 8, TEAM = 128, FEW_THREADS = FEW_STAGES * TEAM;
+
+// Of R rows in shared memory, `next` bytes apart, and B vectors: a lane's part of their products.  A vector is loaded once for all the rows.
+template <typename T, int R, int B>
+__device__ __forceinline__ void dots(const unsigned char *row, unsigned next, const uint4 *const (&x)[B], int parts, int lane, float2 (&sum)[R][B])
+{
+    constexpr int N = Granule<T>::N;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < B; i++) sum[r][i] = make_float2(0.0f, 0.0f);
+    constexpr int U = B == 1 ? 8 : 4;
+    for (int c = lane; c < parts; c += 32 * U) {
+        uint4 v[U][B];
+#pragma unroll
+        for (int j = 0; j < U; j++)
+#pragma unroll
+            for (int i = 0; i < B; i++) v[j][i] = c + 32 * j < parts ? __ldg(x[i] + c + 32 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (c + 32 * j < parts)
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    float2 w[N / 2];
+                    Granule<T>{((const uint4 *)(row + r * next))[c + 32 * j]}.unpack(w);
+#pragma unroll
+                    for (int i = 0; i < B; i++) {
+                        float2 y[N / 2];
+                        Granule<T>{v[j][i]}.unpack(y);
+#pragma unroll
+                        for (int k = 0; k < N / 2; k++) sum[r][i] = fma2(w[k], y[k], sum[r][i]);
+                    }
+                }
+    }
+}
+
+__device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory"); }
+
+// What both kernels do: steps, which the teams take in turn.  issue(step, stage's address, barrier) copies a step's rows, by one thread; take(step, stage) works
+// on them.
+template <typename Issue, typename Take>
+__device__ __forceinline__ void few_steps(int steps, unsigned char *ring, int *head, Issue issue, Take take)
+{
+    __shared__ __align__(8) uint64_t bars[FEW_STAGES];
+    __shared__ int broken_word;
+    volatile int *broken = &broken_word;
+    const int team = threadIdx.x / TEAM;
+    const bool first = threadIdx.x % TEAM == 0;
+    unsigned char *stage = ring + team * FEW_BYTES;
+    const uint32_t bar = smem_at(bars + team);
+    if (threadIdx.x == 0) broken_word = 0;
+    if (first) {
+        bar_init(bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (team < steps) issue(team, smem_at(stage), bar);
+    }
+    __syncthreads();
+    unsigned parity = 0;
+    for (int step = team; step < steps; step += FEW_STAGES, parity ^= 1) {
+        if (!bar_wait(bar, parity, broken)) break;
+        take(step, stage);
+        team_sync(team);
+        if (first && step + FEW_STAGES < steps) issue(step + FEW_STAGES, smem_at(stage), bar);
+    }
+    if (*broken && first) {                        // gave up: what is under way lands first
+        volatile int late = 0;
+        bar_wait(bar, parity, &late);
+        head[2] = 1;
+    }
+}
+
+// Steps of `each` columns of h, gate and up rows of a tile's expert.
+template <typename T>
+__global__ void __launch_bounds__(FEW_THREADS)
+gated_few_kernel(const ProductArgs a, const T *__restrict__ w, int each)
+{
+    extern __shared__ __align__(128) unsigned char ring[];
+    wait_for_previous();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x % TEAM >> 5, inner = a.cols, width = a.terms, pieces = (inner + each - 1) / each;
+    if (a.g.head[1] && threadIdx.x < TAKERS) spoil<T, WIDE, GATED>(a, threadIdx.x);
+    const int64_t units = (int64_t)a.g.head[0] * pieces;
+    const int steps = units > blockIdx.x ? (int)((units - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+    auto unit = [&](int step) { return blockIdx.x + (int64_t)step * gridDim.x; };
+    const unsigned second = (unsigned)each * width * sizeof(T);
+    few_steps(
+        steps, ring, a.g.head,
+        [&](int step, uint32_t to, uint32_t bar) {
+            const int m = (int)(unit(step) / pieces), f = (int)(unit(step) % pieces) * each;
+            const unsigned bytes = (unsigned)min(each, inner - f) * width * sizeof(T);
+            const T *gate = w + ((int64_t)a.g.column[m] * 2 * inner + f) * width;
+            bar_expect(bar, 2 * bytes);
+            load_bytes(to, gate, bytes, bar);
+            load_bytes(to + second, gate + (int64_t)inner * width, bytes, bar);
+        },
+        [&](int step, const unsigned char *stage) {
+            const int m = (int)(unit(step) / pieces), f = (int)(unit(step) % pieces) * each, group = a.g.column[m], slot = m * GROUP_TILE;
+            const int count = min(GROUP_TILE, a.g.counts[group] - (m - a.g.first[group]) * GROUP_TILE), rows = min(each, inner - f), parts = width / 8;
+            for (int r = warp; r < rows; r += TEAM / 32) {
+                auto give = [&](auto batch, int e0) {
+                    constexpr int B = decltype(batch)::value;
+                    const uint4 *x[B];
+#pragma unroll
+                    for (int i = 0; i < B; i++) x[i] = (const uint4 *)((const T *)a.numbered + a.numbers[slot + e0 + i] * a.ld);
+                    float2 sum[2][B];
+                    dots<T, 2, B>(stage + (size_t)r * width * sizeof(T), second, x, parts, lane, sum);
+#pragma unroll
+                    for (int i = 0; i < B; i++) {
+                        const float g = warp_sum(sum[0][i].x + sum[0][i].y), u = warp_sum(sum[1][i].x + sum[1][i].y);
+                        if (lane == 0)
+                            ((T *)a.out)[(int64_t)a.g.order[slot + e0 + i] * inner + f + r] = from_float<T>(g * logistic(gate_of(g, a.gelu).x) * u);
+                    }
+                };
+                int e = 0;
+                for (; e + 2 <= count; e += 2) give(std::integral_constant<int, 2>(), e);
+                if (e < count) give(std::integral_constant<int, 1>(), e);
+            }
+        });
+}
+
+// Steps of `each` elements of a row of y: all its entries, eight at a time, two of them a warp; a team stays with its elements until they are summed.
+template <typename T>
+__global__ void __launch_bounds__(FEW_THREADS)
+combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const T *__restrict__ v, int each)
+{
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ float sums[FEW_STAGES][TEAM / 32][FEW_BYTES / FEW_ENTRIES / 16];      // a row has 16 bytes or more
+    __shared__ int64_t first[FEW_SUMS + 1];
+    wait_for_previous();
+    const int tid = threadIdx.x, lane = tid & 31, team = tid / TEAM, warp = tid % TEAM >> 5, width = a.rows, inner = a.terms, nrows = a.tiles_m;
+    const int pieces = (width + each - 1) / each;
+    if (tid <= nrows) first[tid] = pos[tid];
+    __syncthreads();
+    // the CTA's elements: units blockIdx.x, + gridDim.x, ... of rows x pieces; the team's: every FEW_STAGES-th of those, in batches of eight entries
+    const int units = nrows * pieces, mine = units > (int)blockIdx.x ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    struct Step {
+        int unit, batch, row, d;
+        int64_t lo, hi;
+    };
+    auto begin = [&](int unit, int batch) {
+        const int u = (int)blockIdx.x + unit * (int)gridDim.x;
+        Step s = {unit, batch, u / pieces, u % pieces * each, 0, 0};
+        s.lo = first[s.row] + (int64_t)batch * FEW_ENTRIES;
+        s.hi = min(s.lo + FEW_ENTRIES, first[s.row + 1]);
+        return s;
+    };
+    const unsigned room = FEW_BYTES / FEW_ENTRIES;
+    // a step's number says no more than how many there were: a team's next step is the next batch of its unit, or its next unit
+    Step now = begin(team < mine ? team : 0, 0);
+    auto after = [&](const Step &s) { return s.hi < first[s.row + 1] ? begin(s.unit, s.batch + 1) : begin(s.unit + FEW_STAGES < mine ? s.unit + FEW_STAGES : s.unit, 0); };
+    int count = 0;                                 // the team's steps
+    for (int u = team; u < mine; u += FEW_STAGES) {
+        const int row = ((int)blockIdx.x + u * (int)gridDim.x) / pieces;
+        count += max(1, (int)((first[row + 1] - first[row] + FEW_ENTRIES - 1) / FEW_ENTRIES));
+    }
+    few_steps(
+        count ? team + (count - 1) * FEW_STAGES + 1 : 0, ring, a.g.head,
+        [&](int step, uint32_t to, uint32_t bar) {
+            const Step s = step < FEW_STAGES ? now : after(now);
+            const unsigned bytes = (unsigned)min(each, width - s.d) * inner * sizeof(T);
+            bar_expect(bar, (unsigned)(s.hi - s.lo) * bytes);
+            for (int64_t e = s.lo; e < s.hi; e++) {
+                const int64_t col = crd[e];
+                load_bytes(to + (unsigned)(e - s.lo) * room, v + ((col >= 0 && col < a.g.ngroups ? col : 0) * width + s.d) * inner, bytes, bar);
+            }
+        },
+        [&](int step, const unsigned char *stage) {
+            if (step >= FEW_STAGES) now = after(now);
+            const int rows = min(each, width - now.d);
+            const unsigned next = (unsigned)inner * sizeof(T);
+            auto give = [&](auto batch, int r) {
+                constexpr int R = decltype(batch)::value;
+                float sum[R] = {};
+#pragma unroll
+                for (int i = 0; i < FEW_ENTRIES; i += TEAM / 32) {
+                    const int64_t e = now.lo + i + warp;
+                    if (e >= now.hi) break;
+                    const int64_t col = crd[e];
+                    const float by = col >= 0 && col < a.g.ngroups ? a.val[e] : __int_as_float(0x7fffffff);
+                    const uint4 *const x[1] = {(const uint4 *)((const T *)a.numbered + e * inner)};
+                    float2 d[R][1];
+                    dots<T, R, 1>(stage + (i + warp) * room + r * next, next, x, inner / 8, lane, d);
+#pragma unroll
+                    for (int j = 0; j < R; j++) sum[j] = fmaf(by, d[j][0].x + d[j][0].y, sum[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < R; j++) {
+                    const float s = warp_sum(sum[j]);
+                    if (lane == 0) sums[team][warp][r + j] = now.batch == 0 ? s : sums[team][warp][r + j] + s;
+                }
+            };
+            int r = 0;
+            for (; r + 2 <= rows; r += 2) give(std::integral_constant<int, 2>(), r);
+            if (r < rows) give(std::integral_constant<int, 1>(), r);
+            if (now.hi < first[now.row + 1]) return;
+            team_sync(team);
+            for (int r = tid % TEAM; r < rows; r += TEAM)
+                ((T *)a.out)[(int64_t)now.row * width + now.d + r] = from_float<T>((sums[team][0][r] + sums[team][1][r]) + (sums[team][2][r] + sums[team][3][r]));
+        });
+}
+
 // wide or narrow tiles for products of tokens' rows
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) < sm_count(); }
 
@@ -627,12 +833,21 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
     alignas(64) CUtensorMap mb;
     ProductArgs a = arguments<T>(s, plan);
     const bool few = narrow(a.g, s.nnz, 2 * s.inner);
-    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.out = h;
+    if (s.nrows <= FEW_ROWS && s.width * 2 * (int64_t)sizeof(T) <= FEW_BYTES) {
+        // no fewer steps than SMs, if there are rows enough
+        const int64_t fit = FEW_BYTES / (s.width * 2 * (int64_t)sizeof(T)), most = group_tiles(s.nnz, s.nexperts) - 1, share = ceil_div(most * s.inner, sm_count());
+        const int each = (int)(fit < share ? fit : share);
+        const int64_t units = most * ceil_div(s.inner, each);
+        CB_CUDA(cudaFuncSetAttribute(gated_few_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
+        CB_CUDA(launch_behind(gated_few_kernel<T>, dim3((unsigned)(units < sm_count() ? units : sm_count())), FEW_THREADS, FEW_SMEM, st, a, (const T *)w, each));
+        return 0;
+    }
+    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
     return few ? launch_product<T, NARROW, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st)
                : launch_product<T, WIDE, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st);
 }
@@ -691,7 +906,7 @@ static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, 
 
 // sums: room for nnz x width floats
 template <typename T>
-static int combine_experts(const Sizes &s, const int64_t *pos, int32_t *plan, const void *h, const float *val, const void *v, float *sums, void *y,
+static int combine_experts(const Sizes &s, const int64_t *pos, const int64_t *crd, int32_t *plan, const void *h, const float *val, const void *v, float *sums, void *y,
                            cudaStream_t st)
 {
     const char *what = "combine_experts";
@@ -700,6 +915,21 @@ static int combine_experts(const Sizes &s, const int64_t *pos, int32_t *plan, co
     for (const void *p : {h, v, (const void *)sums, (const void *)y}) CB_TRY(check_at(what, p));
     if (s.nnz == 0 || s.nrows == 0) {
         CB_CUDA(cudaMemsetAsync(y, 0, s.nrows * s.width * sizeof(T), st));
+        return 0;
+    }
+    if (s.nrows <= FEW_SUMS && s.inner * (int64_t)sizeof(T) <= FEW_BYTES / FEW_ENTRIES) {
+        const int64_t fit = FEW_BYTES / FEW_ENTRIES / (s.inner * (int64_t)sizeof(T)), share = ceil_div(s.nrows * s.width, sm_count());
+        const int each = (int)(fit < share ? fit : share);
+        const int64_t units = s.nrows * ceil_div(s.width, each);
+        ProductArgs a = arguments<T>(s, plan);
+        a.numbered = h;
+        a.val = val;
+        a.out = y;
+        a.terms = (int)s.inner;
+        a.rows = (int)s.width;
+        a.tiles_m = (int)s.nrows;
+        CB_CUDA(cudaFuncSetAttribute(combine_few_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
+        CB_CUDA(launch_behind(combine_few_kernel<T>, dim3((unsigned)(units < sm_count() ? units : sm_count())), FEW_THREADS, FEW_SMEM, st, a, pos, crd, (const T *)v, each));
         return 0;
     }
     alignas(64) CUtensorMap mb;
@@ -776,10 +1006,10 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
                                             (cudaStream_t)stream);                                                                                     \
     }                                                                                                                                                  \
     extern "C" int32_t comet_b200_dev_combine_experts_##suffix##_i64(int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner,       \
-                                                                     const int64_t *pos, int32_t *plan, const void *h, const float *val,               \
+                                                                     const int64_t *pos, const int64_t *crd, int32_t *plan, const void *h, const float *val, \
                                                                      const void *v, float *sums, void *y, void *stream)                                \
     {                                                                                                                                                  \
-        return cb200::combine_experts<T>({nrows, nexperts, nnz, width, inner}, pos, plan, h, val, v, sums, y, (cudaStream_t)stream);                   \
+        return cb200::combine_experts<T>({nrows, nexperts, nnz, width, inner}, pos, crd, plan, h, val, v, sums, y, (cudaStream_t)stream);                   \
     }                                                                                                                                                  \
     extern "C" int32_t comet_b200_dev_combine_experts_grad_##suffix##_i64(                                                                             \
         int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, int32_t *plan, const void *h, const float *val, const void *v,      \

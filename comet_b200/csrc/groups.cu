@@ -7,19 +7,24 @@
 // Bound: the chains of loads of the two walks.
 #include "groups.cuh"
 #include "logits.cuh"
+#include "stream.cuh"
 
 namespace cb200 {
 
 static const int GT = 1024, GW = GT / 32;
+// entries of a CTA that its shared memory has room for beside the counts
+__host__ __device__ inline int most_sorted(int ngroups) { return ngroups <= 512 ? 8192 : 4096; }
+static size_t room_for(int64_t ngroups) { return (size_t)ngroups * GW * sizeof(int) + most_sorted((int)ngroups) * (sizeof(int2) + sizeof(short)); }
 
 __global__ void __launch_bounds__(GT)
 group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
 {
     extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
-    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], sums[GW];
+    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], sums[GW + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     int *own = warps + (size_t)warp * n;
+    let_next_start();                              // it waits for this one's end before it reads
     for (int i = tid; i < GW * n; i += GT) warps[i] = 0;
     if (rank == 0 && tid < GROUP_HEAD) g.head[tid] = 0;
     __syncthreads();
@@ -74,6 +79,21 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
             if (r < rank) before += v;
             total += v;
         }
+    // the CTA's own, one column after the other
+    {
+        int v = tid < n ? mine[tid] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        if (lane == 31) sums[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) v += sums[w];
+        if (tid < n) local[tid] = v - mine[tid];
+        __syncthreads();
+        if (tid == GT - 1) sums[GW] = v;
+    }
     const int tiles = (total + GROUP_TILE - 1) / GROUP_TILE;
     int upto = tiles;                              // inclusive sums over the columns
 #pragma unroll
@@ -100,9 +120,17 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
         for (int i = first + lane; i < ends[c]; i += 32) g.column[i] = c;
         for (int64_t i = (int64_t)first * GROUP_TILE + sum + lane; i < (int64_t)ends[c] * GROUP_TILE; i += 32) g.order[i] = g.token[i] = -1;
     }
-    for (int i = tid; i < GW * n; i += GT) warps[i] += start[i % n];
+    // where a warp's entries go: to their slots, or to their places among the CTA's own
+    const int here = sums[GW], sortable = most_sorted(n);
+    for (int i = tid; i < GW * n; i += GT) warps[i] += here <= sortable ? local[i % n] : start[i % n];
     __syncthreads();
+    if (here <= sortable)
+        for (int c = tid; c < n; c += GT) start[c] -= local[c];
     if (ranks > 1) cluster_arrive();               // this CTA has read the others' counts
+    // Few enough for shared memory: the CTA's entries are put in order there, and leave in runs (a column's are next to each other).
+    int2 *sorted = (int2 *)(warps + (size_t)GW * n);
+    unsigned short *of = (unsigned short *)(sorted + sortable);
+    const bool staged = here <= sortable;
     walk([&](int64_t e, int64_t row, int col, unsigned alike) {
         if (col < 0) {
             g.order[g.slots - 1 - atomicAdd(&g.head[1], 1)] = (int)e;
@@ -111,11 +139,87 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
         const int at = own[col] + __popc(alike & ((1u << lane) - 1));
         __syncwarp(alike);
         if (lane == 31 - __clz(alike)) own[col] = at + 1;
-        g.order[at] = (int)e;
-        g.token[at] = (int)row;
+        if (staged) {
+            sorted[at] = make_int2((int)e, (int)row);
+            of[at] = (unsigned short)col;
+        } else {
+            g.order[at] = (int)e;
+            g.token[at] = (int)row;
+        }
     });
+    if (staged) {
+        __syncthreads();
+        for (int i = tid; i < here; i += GT) {
+            const int2 v = sorted[i];
+            const int at = start[of[i]] + i;
+            g.order[at] = v.x;
+            g.token[at] = v.y;
+        }
+    }
     __syncwarp();
     if (ranks > 1) cluster_wait();                 // its own stay until they have been read
+}
+
+// The same for few entries of few rows: a thread has an entry, and counts those of its column before it.
+static const int FEW = 256, FEW_ROWS = 1024;
+__global__ void __launch_bounds__(FEW)
+group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
+{
+    __shared__ int rows[FEW_ROWS + 1], cols[FEW], count[MOST_GROUPS], first[MOST_GROUPS], sums[FEW / 32], bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
+    let_next_start();
+    const int64_t mine = tid < nnz ? crd[tid] : -1;
+    for (int i = tid; i <= nrows; i += FEW) rows[i] = (int)min(max(pos[i], (int64_t)0), (int64_t)nnz);
+    const int col = mine >= 0 && mine < n ? (int)mine : -1;
+    cols[tid] = col;
+    for (int i = tid; i < n; i += FEW) count[i] = 0;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    int before = 0, row = 0;
+    if (tid < nnz) {
+        if (col >= 0) atomicAdd(&count[col], 1);
+        for (int i = 0; i < tid; i++) before += cols[i] == col;
+        for (int step = FEW_ROWS / 2; step > 0; step /= 2)                           // the last row that begins at or before the entry
+            if (row + step < nrows && rows[row + step] <= tid) row += step;
+    }
+    __syncthreads();
+    // each thread: four columns
+    int tiles = 0, upto;
+    for (int i = 4 * tid; i < min(4 * tid + 4, n); i++) tiles += (count[i] + GROUP_TILE - 1) / GROUP_TILE;
+    upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) upto += sums[w];
+    int at = upto - tiles;
+    for (int i = 4 * tid; i < min(4 * tid + 4, n); i++) {
+        first[i] = at;
+        g.first[i] = at;
+        g.counts[i] = count[i];
+        for (int e = 0; e < count[i]; e += GROUP_TILE) g.column[at++] = i;
+    }
+    if (tid == FEW - 1) g.first[n] = upto;
+    if (tid > 0 && tid < GROUP_HEAD && tid != 1) g.head[tid] = 0;
+    if (tid == FEW - 1) g.head[0] = upto;
+    __syncthreads();
+    for (int c = warp; c < n; c += FEW / 32) {
+        const int sum = count[c], end = (sum + GROUP_TILE - 1) / GROUP_TILE * GROUP_TILE;
+        for (int i = sum + lane; i < end; i += 32) g.order[first[c] * GROUP_TILE + i] = g.token[first[c] * GROUP_TILE + i] = -1;
+    }
+    if (tid < nnz) {
+        if (col >= 0) {
+            g.order[first[col] * GROUP_TILE + before] = tid;
+            g.token[first[col] * GROUP_TILE + before] = row;
+        } else {
+            g.order[g.slots - 1 - atomicAdd(&bad, 1)] = tid;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) g.head[1] = bad;
 }
 
 static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_t *pos, const int64_t *crd, int32_t *plan, cudaStream_t st)
@@ -124,10 +228,14 @@ static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_
     if (nrows < 0 || nnz < 0 || ncols < 1 || ncols > MOST_GROUPS)
         return fail("group_entries: %lld entries in %lld rows of %lld columns (1 to %d)", (long long)nnz, (long long)nrows, (long long)ncols, MOST_GROUPS);
     if (nrows > 0x7fffffffLL || nnz > 0x70000000LL) return fail("group_entries: more than 2^31 rows, or 1.8e9 entries");
-    const size_t row = (size_t)ncols * GW * sizeof(int);
+    if (nnz <= FEW && nrows <= FEW_ROWS) {         // one token's 8 entries: @FEW@ us, 7.1 by the cluster's kernel
+        group_few_kernel<<<1, FEW, 0, st>>>((int)nrows, (int)nnz, pos, crd, groups_in(plan, nnz, ncols));
+        CB_LAUNCH_CHECK();
+        return 0;
+    }
     int ranks = 1;                                 // a CTA has 1024 rows under way at a time
     while (ranks < MOST_CLUSTER && nrows > (int64_t)ranks * GT) ranks *= 2;
-    return launch_cluster(group_kernel, (unsigned)ranks, ranks, GT, row, (size_t)MOST_GROUPS * GW * sizeof(int), st, nrows, nnz, pos, crd,
+    return launch_cluster(group_kernel, (unsigned)ranks, ranks, GT, room_for(ncols), room_for(MOST_GROUPS), st, nrows, nnz, pos, crd,
                           groups_in(plan, nnz, ncols));
 }
 

@@ -136,28 +136,45 @@ template <bool ENTROPY>
 struct GradRow {
     float c, m, mc, less, a, b;
     bool near, none, zero;
-    __device__ __forceinline__ GradRow(const ProbGrad &p, int64_t t, float sum)
+    __device__ __forceinline__ GradRow(const ProbGrad &p, float2 row, float h, float entropy, float sum)
     {
-        const float2 row = ((const float2 *)p.sums)[t];
         c = p.c;
         m = row.x;
         none = m == MINUS_INF;
         mc = none ? 0.0f : m * c;
         near = fabsf(mc) < NEAR;
         less = row.y * LOG2E + (near && !none ? fmaf(m, c, -mc) : 0.0f);             // what the exponent is beyond log2 q
-        const float h = ENTROPY ? p.by_entropy[t] : 0.0f;
-        a = -p.inv * (sum + (ENTROPY && h != 0.0f ? h * p.entropy[t] : 0.0f));
+        a = -p.inv * (sum + (ENTROPY && h != 0.0f ? h * entropy : 0.0f));
         b = ENTROPY ? -p.inv * LN2 * h : 0.0f;
         zero = none || (sum == 0.0f && h == 0.0f);
     }
-    __device__ __forceinline__ float2 of(float2 x) const
+    __device__ __forceinline__ float2 from_exponent(float2 d) const
     {
-        float2 d = near ? fma2(x, make_float2(c, c), make_float2(-mc, -mc)) : make_float2((x.x - m) * c, (x.y - m) * c);
         d = add2(d, make_float2(-less, -less));
         const float2 q = make_float2(exp2_fast(d.x), exp2_fast(d.y));
         if (!ENTROPY) return mul2(q, make_float2(a, a));
         // a q of 0 gives 0, whatever its logarithm: that may be -inf
         return mul2(q, fma2(make_float2(fmaxf(d.x, -16384.0f), fmaxf(d.y, -16384.0f)), make_float2(b, b), make_float2(a, a)));
+    }
+    template <int G, int H>
+    __device__ __forceinline__ void all(float2 (&v)[G][H]) const
+    {
+        if (zero) {
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int k = 0; k < H; k++) v[i][k] = make_float2(0.0f, 0.0f);
+        } else if (near) {
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int k = 0; k < H; k++) v[i][k] = from_exponent(fma2(v[i][k], make_float2(c, c), make_float2(-mc, -mc)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int k = 0; k < H; k++) v[i][k] = from_exponent(make_float2((v[i][k].x - m) * c, (v[i][k].y - m) * c));
+        }
     }
 };
 
@@ -176,61 +193,80 @@ __device__ __forceinline__ void put_granule(T *g, int col, int ncols, bool alike
     }
 }
 
-// A piece of a row a CTA: GG granules a thread.  The entries in it leave their gradients in shared memory, with a bit each that says so.
-static const int GT = 256, GG = 4;
+// A lane's share of a row's entries, 32 at a time: their sum, by every warp.
+__device__ __forceinline__ float sum_entries(const float *values, int64_t lo, int64_t hi, int lane)
+{
+    float sum = 0.0f;
+    for (int64_t e = lo + lane; e < hi; e += 32) sum += values[e];
+    return warp_sum(sum);
+}
+// Adds the entries' gradients to the granules of the warp: granule i of a lane begins at column col0 + i * stride * N + first * N, first the lane's place.
+template <int G, int N>
+__device__ __forceinline__ void add_entries(const ProbGrad &p, int64_t lo, int64_t hi, int col0, int stride, int warp_first, int lane, float2 (&v)[G][N / 2])
+{
+    for (int64_t e0 = lo; e0 < hi; e0 += 32) {
+        int granule = 0, at = 0;
+        float d = 0.0f;
+        bool mine = false;
+        if (e0 + lane < hi) {
+            const int64_t col = p.crd[e0 + lane], j = col - col0;
+            if (col >= 0 && col < p.ncols && j >= 0 && j < (int64_t)G * stride * N) {
+                granule = (int)j / N;
+                at = (int)j % N;
+                mine = (granule % stride & ~31) == warp_first;
+                if (mine) d = p.values[e0 + lane] * p.inv;
+            }
+        }
+        for (unsigned on = __ballot_sync(0xffffffffu, mine); on; on &= on - 1) {
+            const int who = __ffs(on) - 1, g = __shfl_sync(0xffffffffu, granule, who), k = __shfl_sync(0xffffffffu, at, who);
+            const float x = __shfl_sync(0xffffffffu, d, who);
+            const int to = g % stride - warp_first == lane ? g / stride * N + k : -1;
+            // no branch: the granules stay in registers
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int n = 0; n < N / 2; n++) {
+                    v[i][n].x += to == i * N + 2 * n ? x : 0.0f;
+                    v[i][n].y += to == i * N + 2 * n + 1 ? x : 0.0f;
+                }
+        }
+    }
+}
+
+// A piece of a row a CTA, G granules a thread: 128 bytes of f32, 64 of 16 bits.  No barrier: a warp finds its granules' entries itself.
+static const int GT = 256;
+template <typename T>
+constexpr int grad_granules() { return sizeof(T) == 4 ? 8 : 4; }
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(GT)
 prob_grad_kernel(const ProbGrad p, int pieces, const T *xs, T *grad)
 {
-    constexpr int N = Granule<T>::N, COLS = GT * GG * N;
-    __shared__ uint32_t bits[COLS / 32];
-    __shared__ float came[COLS];
-    const int tid = threadIdx.x, piece = blockIdx.x % pieces;
-    const int64_t t = blockIdx.x / pieces, lo = p.pos[t], hi = p.pos[t + 1];
+    constexpr int N = Granule<T>::N, G = grad_granules<T>();
+    const int tid = threadIdx.x, lane = tid & 31, piece = blockIdx.x % pieces;
+    const int64_t t = blockIdx.x / pieces;
     const T *x = xs + t * p.ldx;
     T *g = grad + t * p.ldg;
-    const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15) + piece * GT * GG;
-    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T), all = (off + p.ncols + N - 1) / N, col0 = piece * COLS - off;
+    const uint4 *from = (const uint4 *)((uintptr_t)x & ~(uintptr_t)15) + piece * GT * G;
+    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T), left = (off + p.ncols + N - 1) / N - piece * GT * G, col0 = piece * GT * G * N - off;
     const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
-    Granule<T> in[GG];
+    Granule<T> in[G];
 #pragma unroll
-    for (int i = 0; i < GG; i++)
-        if (piece * GT * GG + i * GT + tid < all) in[i].w = from[i * GT + tid];
-    bool mine = false;
-    if (lo < hi) {
-        for (int i = tid; i < COLS / 32; i += GT) bits[i] = 0;
-        __syncthreads();
-        for (int64_t e = lo + tid; e < hi; e += GT) {
-            const int64_t col = p.crd[e], j = col - col0;
-            if (j < 0 || j >= COLS || col < 0 || col >= p.ncols || (e > lo && p.crd[e - 1] == col)) continue;
-            float d = 0.0f;                        // repeated columns are next to each other
-            for (int64_t i = e; i < hi && p.crd[i] == col; i++) d += p.values[i];
-            came[j] = d * p.inv;
-            atomicOr(&bits[j >> 5], 1u << (j & 31));
-            mine = true;
-        }
-        mine = __syncthreads_or(mine);
+    for (int i = 0; i < G; i++) {
+        in[i].w = make_uint4(0, 0, 0, 0);
+        if (i * GT + tid < left) in[i].w = from[i * GT + tid];
     }
-    float sum = 0.0f;
-    for (int64_t e = lo; e < hi; e++) sum += p.values[e];
-    const GradRow<ENTROPY> row(p, t, sum);
+    const int64_t lo = p.pos[t], hi = p.pos[t + 1];
+    const float2 kept = ((const float2 *)p.sums)[t];
+    const float h = ENTROPY ? p.by_entropy[t] : 0.0f, ent = ENTROPY ? p.entropy[t] : 0.0f;
+    const GradRow<ENTROPY> row(p, kept, h, ent, sum_entries(p.values, lo, hi, lane));
+    float2 v[G][N / 2];
 #pragma unroll
-    for (int i = 0; i < GG; i++) {
-        const int at = i * GT + tid, col = col0 + at * N;
-        if (piece * GT * GG + at >= all) continue;
-        float2 v[N / 2];
-        in[i].unpack(v);
+    for (int i = 0; i < G; i++) in[i].unpack(v[i]);
+    row.all(v);
+    if (!row.none) add_entries<G, N>(p, lo, hi, col0, GT, tid & ~31, lane, v);
 #pragma unroll
-        for (int k = 0; k < N / 2; k++) v[k] = row.zero ? make_float2(0.0f, 0.0f) : row.of(v[k]);
-        if (mine) {
-            const unsigned on = N == 8 ? ((const uint8_t *)bits)[at] : ((const uint8_t *)bits)[at >> 1] >> ((at & 1) * 4) & 15;
-            if (on)
-#pragma unroll
-                for (int k = 0; k < N; k++)
-                    if (on >> k & 1) ((float *)v)[k] = row.none ? 0.0f : ((const float *)v)[k] + came[at * N + k];
-        }
-        put_granule<T>(g, col, p.ncols, alike, v);
-    }
+    for (int i = 0; i < G; i++)
+        if (i * GT + tid < left) put_granule<T>(g, col0 + (i * GT + tid) * N, p.ncols, alike, v[i]);
 }
 
 // Short rows: a warp each, which has the whole row in registers.
@@ -249,29 +285,15 @@ prob_grad_short_kernel(const ProbGrad p, const T *xs, T *grad)
     const int64_t lo = p.pos[t], hi = p.pos[t + 1];
     const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
     const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
-    float sum = 0.0f;
-    for (int64_t e = lo; e < hi; e++) sum += p.values[e];
-    const GradRow<ENTROPY> row(p, t, sum);
+    const float h = ENTROPY ? p.by_entropy[t] : 0.0f, ent = ENTROPY ? p.entropy[t] : 0.0f;
+    const GradRow<ENTROPY> row(p, ((const float2 *)p.sums)[t], h, ent, sum_entries(p.values, lo, hi, lane));
+    float2 v[G][N / 2];
 #pragma unroll
-    for (int i = 0; i < G; i++) {
-        const int at = i * 32 + lane, col = at * N - off;
-        if (col >= p.ncols) continue;
-        float2 v[N / 2];
-        in[i].unpack(v);
+    for (int i = 0; i < G; i++) in[i].unpack(v[i]);
+    row.all(v);
+    if (!row.none) add_entries<G, N>(p, lo, hi, -off, 32, 0, lane, v);
 #pragma unroll
-        for (int k = 0; k < N / 2; k++) v[k] = row.zero ? make_float2(0.0f, 0.0f) : row.of(v[k]);
-        if (!row.none)
-            for (int64_t e = lo; e < hi; e++) {
-                const int64_t j = p.crd[e] - col;
-                if (j >= 0 && j < N && p.crd[e] >= 0 && p.crd[e] < p.ncols) {
-                    const float d = p.values[e] * p.inv;
-#pragma unroll
-                    for (int k = 0; k < N; k++)
-                        if (j == k) ((float *)v)[k] += d;
-                }
-            }
-        put_granule<T>(g, col, p.ncols, alike, v);
-    }
+    for (int i = 0; i < G; i++) put_granule<T>(g, (i * 32 + lane) * N - off, p.ncols, alike, v[i]);
 }
 
 template <typename T>
@@ -342,7 +364,7 @@ static int launch_grad(const ProbGrad &p, const T *x, T *grad, cudaStream_t st)
     case 4: prob_grad_short_kernel<T, 4, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
     case 8: prob_grad_short_kernel<T, 8, ENTROPY><<<grid, 128, 0, st>>>(p, x, grad); break;
     default: {
-        const int64_t pieces = ceil_div((p.ncols + 2 * Granule<T>::N - 2) / Granule<T>::N, GT * GG);
+        const int64_t pieces = ceil_div((p.ncols + 2 * Granule<T>::N - 2) / Granule<T>::N, GT * grad_granules<T>());
         if (pieces * p.nrows > 0x7fffffffLL) return fail("log_probs_grad: more than 2^31 pieces of rows");
         prob_grad_kernel<T, ENTROPY><<<(unsigned)(pieces * p.nrows), GT, 0, st>>>(p, (int)pieces, x, grad);
     }

@@ -55,6 +55,11 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, i
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(c), "r"(r), "r"(z), "r"(bar) : "memory");
 }
+// contiguous bytes, a multiple of 16
+__device__ __forceinline__ void load_bytes(uint32_t dst, const void *src, unsigned bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // 16 bytes, or zeros where `on` is not
 __device__ __forceinline__ void copy_or_zero(uint32_t dst, const void *src, bool on)
 {

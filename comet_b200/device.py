@@ -476,7 +476,7 @@ def combine_experts(G, H, V):
     [entries, inner]; V [experts, width, inner].  A row that stores nothing gives zeros."""
     sizes, val = _check_combine("combine_experts", G, H, V)
     Y, sums = H.new_empty((sizes[0], sizes[3])), H.new_empty((sizes[2], sizes[3]), dtype=torch.float32)
-    _call(_COMBINE[H.dtype], *sizes, G.S.pos.data_ptr(), G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), sums.data_ptr(), Y.data_ptr(), _stream())
+    _call(_COMBINE[H.dtype], *sizes, G.S.pos.data_ptr(), G.S.crd.data_ptr(), G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), sums.data_ptr(), Y.data_ptr(), _stream())
     return Y
 
 

@@ -746,11 +746,11 @@ COMET_B200_EXPORT int32_t comet_b200_dev_gated_experts_grad_f16_i64(
 /* y[nrows x width] = for each row the sum over its entries (t, j) of val * v_j h, h the entry's row of h[nnz x inner], v[nexperts x width x
    inner]; 0 for a row that stores nothing.  sums: room for nnz x width floats. */
 COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_bf16_i64(
-    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, int32_t *plan, const void *h,
-    const float *val, const void *v, float *sums, void *y, void *stream);
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, const int64_t *crd, int32_t *plan,
+    const void *h, const float *val, const void *v, float *sums, void *y, void *stream);
 COMET_B200_EXPORT int32_t comet_b200_dev_combine_experts_f16_i64(
-    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, int32_t *plan, const void *h,
-    const float *val, const void *v, float *sums, void *y, void *stream);
+    int64_t nrows, int64_t nexperts, int64_t nnz, int64_t width, int64_t inner, const int64_t *pos, const int64_t *crd, int32_t *plan,
+    const void *h, const float *val, const void *v, float *sums, void *y, void *stream);
 
 /* Its gradients dh (h's shape), dv (v's shape; may be NULL) and dval[nnz] from dy (nrows x width, row stride lddy, a multiple of 8).  scaled: room
    for slots x inner elements (slots as above) (val * h, rounded to the operands' type, which dv is computed with); sums: for nnz x 2 ceil(inner / 64) floats. */
