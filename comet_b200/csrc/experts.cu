@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 #include <string.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "groups.cuh"
@@ -60,12 +61,15 @@ enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 
 // A tile has 128 rows and W columns.  W = 256 where there are tiles enough for the chip; else 64, two CTAs on an SM: the weights of few tokens' experts
 // are read by all SMs then (one token, 8 experts of 1024 x 2048 gates and ups: @GATED_ONE@ us against 21).
-static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64, RING = 4;
+static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64;
 static const int A_BYTES = TM * TK * 2;
+static const int PAIR_ENTRIES = 320;               // entries an expert from which on products of tokens' rows go by pairs
 static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 32;
-template <int W>
+// PAIR: two CTAs of a cluster share a product of 256 x 256, with 128 rows of either operand each: two thirds of the bytes that two tiles of their own
+// take from the L2, which is what bounds these products (@PAIR@).
+template <int W, bool PAIR>
 struct Shape {
-    static constexpr int B_BYTES = W * TK * 2, STEP = A_BYTES + B_BYTES;
+    static constexpr int B_ROWS = PAIR ? W / 2 : W, B_BYTES = B_ROWS * TK * 2, STEP = A_BYTES + B_BYTES, RING = PAIR ? 6 : 4;
     static constexpr int TAKEN = W == WIDE ? 128 : 32;         // bytes of a row that a warp takes out at a time
     static constexpr int SMEM = RING * STEP + TAKERS * TAKEN + 1024;
 };
@@ -97,6 +101,7 @@ struct ProductArgs {
 
 struct Tile {
     int m, n, group, steps, slot;    // slot: the first one
+    bool there;                      // not the second of a pair that has none
 };
 
 __device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + exp2_fast(-LOG2E * u)); }
@@ -184,7 +189,7 @@ struct Stage {
 template <typename T, int W, int SUMS>
 __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, bool none, const Tile &t, int half, int row, int64_t entry, unsigned char *room)
 {
-    constexpr int BYTES = Shape<W>::TAKEN;
+    constexpr int BYTES = Shape<W, false>::TAKEN;
     const Stage<T, BYTES> st = {room, (int)threadIdx.x & 31};
     if constexpr (SUMS == GATED || SUMS == GATED_GRAD) {
         constexpr int MINE = W / 4, PART = MINE < 32 ? MINE : 32;                    // columns of the warp, at a time
@@ -223,13 +228,13 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
                     gate[i] = d[i] * up[i] * fmaf(g * s * (1.0f - s), u.y, s);
                     up[i] = d[i] * g * s;
                 }
-                const int64_t to = (int64_t)(t.slot + row) * 2 * inner + f0 + c;
+                const int64_t to = t.there ? (int64_t)(t.slot + row) * 2 * inner + f0 + c : -1;
 #pragma unroll
                 for (int i = 0; i < PART; i += 8) part.put(i / 8, gate + i);
                 part.out((T *)a.out, to, left - c);
 #pragma unroll
                 for (int i = 0; i < PART; i += 8) part.put(i / 8, up + i);
-                part.out((T *)a.out, to + inner, left - c);
+                part.out((T *)a.out, to < 0 ? to : to + inner, left - c);
             }
         }
     } else if constexpr (SUMS == ENTRY_ROWS) {
@@ -280,7 +285,7 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
             // a row of zeros adds nothing to the sums over an expert's tokens
 #pragma unroll
             for (int i = 0; i < PART; i += 8) part.put(i / 8, h + i);
-            part.out((T *)a.scaled, (int64_t)(t.slot + row) * a.cols + c0 + c, left);
+            part.out((T *)a.scaled, t.there ? (int64_t)(t.slot + row) * a.cols + c0 + c : -1, left);
         }
         if (entry >= 0) a.sums[(t.n * 2 + half) * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     } else {
@@ -309,7 +314,7 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
 }
 
 // An entry whose column is no expert's: NaN.
-template <typename T, int W, int SUMS>
+template <typename T, int SUMS>
 __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 {
     const int bad = SUMS == WEIGHT || SUMS == GATED_GRAD ? 0 : a.g.head[1];
@@ -328,31 +333,34 @@ __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 // NUMBERED: the operand whose rows come by their number: A (the tile's rows), B (its columns, OUTER), or none
 enum Numbered { NUMBERED_A, NUMBERED_B, NUMBERED_NONE };
 
-template <typename T, int W, int FORM, int NUMBERED, int SUMS>
+template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, W == WIDE ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
 {
     constexpr bool BF16 = !__is_same(T, __half);
-    constexpr int B_BYTES = Shape<W>::B_BYTES, STEP_BYTES = Shape<W>::STEP;
+    typedef Shape<W, PAIR> S;
+    constexpr int B_BYTES = S::B_BYTES, STEP_BYTES = S::STEP, RING = S::RING, CTAS = PAIR ? 2 : 1;
     constexpr unsigned TENSOR_BYTES = (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + (NUMBERED == NUMBERED_B ? 0 : B_BYTES);
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * RING + 4 + 1];
+    __shared__ __align__(8) uint64_t bars[3 * RING + 4 + 1];
     __shared__ uint32_t tmem_room;
     __shared__ int broken_word;
     volatile int *broken = &broken_word;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int ISSUER = (TAKERS + FETCHERS) / 32;
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
-                   last = taken + 16;
-    if (warp == ISSUER) tmem_alloc(smem_at(&tmem_room), 2 * W);
+                   last = taken + 16, ready = last + 8;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    if (warp == ISSUER) tmem_alloc<PAIR>(smem_at(&tmem_room), 2 * W);
     if (tid == 0) {
         for (int i = 0; i < RING; i++) {
             bar_init(full + 8 * i, NUMBERED == NUMBERED_NONE ? 1 : 1 + FETCHERS);
             bar_init(empty + 8 * i, 1);
+            bar_init(ready + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
             bar_init(done + 8 * i, 1);
-            bar_init(taken + 8 * i, TAKERS / 32);
+            bar_init(taken + 8 * i, CTAS * TAKERS / 32);
         }
         bar_init(last, 1);
         broken_word = 0;
@@ -360,24 +368,32 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     tmem_fence_before();
     __syncthreads();
+    if (PAIR) {                                    // the other one's barriers are there
+        cluster_arrive();
+        cluster_wait();
+    }
     tmem_fence_after();
     const uint32_t tmem = tmem_room;
     wait_for_previous();
 
-    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
+    const int mine = blockIdx.x / CTAS, all = gridDim.x / CTAS;
+    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[PAIR ? 3 : 0] * a.tiles_n;
     auto tile_of = [&](int id) {
         Tile t;
+        t.there = true;
         if (FORM == OUTER) {
             t.group = id / (a.tiles_m * a.tiles_n);
             const int rest = id % (a.tiles_m * a.tiles_n);
-            t.m = rest / a.tiles_n;
+            t.m = rest / a.tiles_n * CTAS + rank;
             t.n = rest % a.tiles_n;
             t.steps = (a.g.counts[t.group] + TK - 1) / TK;
             t.slot = a.g.first[t.group] * GROUP_TILE;
         } else {
-            t.m = id / a.tiles_n;
+            const int first = PAIR ? a.g.pairs[id / a.tiles_n] : id / a.tiles_n;
+            t.m = first + rank;
             t.n = id % a.tiles_n;
-            t.group = a.g.column[t.m];
+            t.group = a.g.column[first];
+            if (PAIR) t.there = t.m < a.g.first[t.group + 1];
             t.steps = (a.terms + TK - 1) / TK;
             t.slot = t.m * GROUP_TILE;
         }
@@ -392,22 +408,35 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
         const char *base = (const char *)a.numbered + chunk * 16;
         const int64_t stride = a.ld * 2;
-        for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
-            const Tile t = tile_of(id);
+        // what a tile's copies begin with is loaded while the tile before is fetched
+        constexpr int NUMBERS = FORM == OUTER ? 4 : 8;
+        Tile t = {}, after = {};
+        int number[NUMBERS], number_after[NUMBERS];
+        auto ahead = [&](int id) {
+            if (id < tiles) after = tile_of(id);
+        };
+        auto numbers = [&]() {
+            if (NUMBERED != NUMBERED_NONE)
+#pragma unroll
+                for (int i = 0; i < NUMBERS; i++) number_after[i] = after.there ? a.numbers[after.slot + row + 16 * i] : -1;
+        };
+        ahead(mine);
+        if (mine < tiles && after.steps) numbers();
+        for (int id = mine; on && id < tiles; id += all) {
+            t = after;
+#pragma unroll
+            for (int i = 0; i < NUMBERS; i++) number[i] = number_after[i];
+            ahead(id + all);
             const char *from[8];
             unsigned there = 0;
             if (NUMBERED == NUMBERED_A && FORM != OUTER) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int n = a.numbers[t.slot + row + 16 * i];
-                    from[i] = base + max(n, 0) * stride;
-                    there |= (n >= 0 ? 1u : 0u) << i;
+                for (int i = 0; i < NUMBERS; i++) {
+                    from[i] = base + max(number[i], 0) * stride;
+                    there |= (number[i] >= 0 ? 1u : 0u) << i;
                 }
             }
-            int next[4];
-            if (NUMBERED != NUMBERED_NONE && FORM == OUTER && t.steps)
-#pragma unroll
-                for (int i = 0; i < 4; i++) next[i] = a.numbers[t.slot + row + 16 * i];
+            if (t.steps <= 1 && id + all < tiles && after.steps) numbers();
             for (int k = 0; k < t.steps; k++, step++) {
                 const unsigned s = step % RING;
                 const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
@@ -416,18 +445,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (!on) break;
                 if (me == 0) {
                     bar_expect(bar, TENSOR_BYTES);
+                    constexpr int BLOCKS = S::B_ROWS / 64;
+                    const int n0 = t.n * W + (PAIR ? rank * (W / 2) : 0);            // of the operand's rows, this CTA's first
                     if (FORM == ROWS) {
-                        const int n = t.n * (SUMS == ENTRY_ROWS ? W : W / 2), second = SUMS == ENTRY_ROWS ? W / 2 : 0;
-                        const int z = SUMS == ENTRY_ROWS ? t.group : 2 * t.group;
-                        load_box(to + A_BYTES, &map_b, k * TK, n, z, bar);
-                        load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, n + second, SUMS == ENTRY_ROWS ? z : z + 1, bar);
+                        // an expert's gate rows, and as many up rows; or rows of the one weight
+                        constexpr bool GATES = SUMS != ENTRY_ROWS;
+                        if (PAIR) {
+                            load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group + rank : t.group, bar);
+                        } else {
+                            load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
+                            load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, GATES ? t.n * (W / 2) : n0 + W / 2, GATES ? 2 * t.group + 1 : t.group, bar);
+                        }
                     } else if (FORM == BACK) {
                         if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
 #pragma unroll
-                        for (int i = 0; i < W / 64; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * W + i * 64, k * TK, t.group, bar);
+                        for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, k * TK, t.group, bar);
                     } else if (NUMBERED == NUMBERED_A) {
 #pragma unroll
-                        for (int i = 0; i < W / 64; i++) load_box(to + A_BYTES + i * 8192, &map_b, t.n * W + i * 64, t.slot + k * TK, 0, bar);
+                        for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, t.slot + k * TK, 0, bar);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
@@ -438,21 +473,22 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
                 } else if (NUMBERED != NUMBERED_NONE) {
-                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : W / 64;
+                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : S::B_ROWS / 64;
                     const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
-                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W;
+                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W + (PAIR ? rank * (W / 2) : 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const char *src = base + max(next[i], 0) * stride;
+                        const char *src = base + max(number[i], 0) * stride;
 #pragma unroll
                         for (int b = 0; b < BLOCKS; b++) {
                             const bool in = col0 + b * 64 + chunk * 8 < a.numbered_cols;
-                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && next[i] >= 0);
+                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && number[i] >= 0);
                         }
-                        if (k + 1 < t.steps) next[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
+                        if (k + 1 < t.steps) number[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
                     }
                 }
                 if (NUMBERED != NUMBERED_NONE) copies_to(bar);
+                if (k + 2 == t.steps && id + all < tiles && after.steps) numbers();
             }
         }
         // what is under way lands before the CTA ends
@@ -462,19 +498,35 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
         }
     } else if (warp == ISSUER) {                   // issues the products
-        if (lane == 0) {
-            constexpr uint32_t kind = product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
+        if (lane == 0 && rank == 1) {              // tells the first CTA what has landed here
+            unsigned step = 0;
+            bool on = true;
+            for (int id = mine; on && id < tiles; id += all) {
+                const int steps = tile_of(id).steps;
+                for (int k = 0; k < steps; k++, step++) {
+                    const unsigned s = step % RING;
+                    on = bar_wait(full + 8 * s, step / RING & 1, broken);
+                    if (!on) break;
+                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
+                    bar_arrive_first(ready + 8 * s);
+                }
+            }
+        } else if (lane == 0) {
+            constexpr uint32_t kind = product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
             unsigned tile = 0, step = 0;
             bool on = true;
-            for (int id = blockIdx.x; on && id < tiles; id += gridDim.x) {
-                const int steps = tile_of(id).steps;
+            int after = mine < tiles ? tile_of(mine).steps : 0;
+            for (int id = mine; on && id < tiles; id += all) {
+                const int steps = after;
+                if (id + all < tiles) after = tile_of(id + all).steps;
                 if (steps == 0) continue;
                 const unsigned b = tile & 1;
-                on = bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken);
+                on = bar_wait<PAIR>(taken + 8 * b, (tile / 2 & 1) ^ 1, broken);
                 tmem_fence_after();
                 for (int k = 0; on && k < steps; k++, step++) {
                     const unsigned s = step % RING;
                     on = bar_wait(full + 8 * s, step / RING & 1, broken);
+                    if (PAIR && on) on = bar_wait<true>(ready + 8 * s, step / RING & 1, broken);
                     if (!on) break;
                     if (NUMBERED != NUMBERED_NONE) shared_to_products();
                     tmem_fence_after();
@@ -483,28 +535,28 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
                     constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
 #pragma unroll
-                    for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
-                    products_to(empty + 8 * s);
+                    for (int i = 0; i < TK / 16; i++) product<PAIR>(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
+                    products_to<PAIR>(empty + 8 * s);
                 }
-                if (on) products_to(done + 8 * b);
+                if (on) products_to<PAIR>(done + 8 * b);
                 tile++;
             }
             if (*broken) {                         // products under way end before tensor memory is given back
                 volatile int late = 0;
-                products_to(last);
+                products_to<PAIR>(last);
                 bar_wait(last, 0, &late);
             }
         }
         __syncwarp();
     } else {                                       // takes the sums
-        spoil<T, W, SUMS>(a, tid);
+        spoil<T, SUMS>(a, tid);
         const int row = (warp & 3) * 32 + lane;
-        unsigned char *room = raw + (ring - smem_at(raw)) + RING * STEP_BYTES + warp * 32 * Shape<W>::TAKEN;
+        unsigned char *room = raw + (ring - smem_at(raw)) + RING * STEP_BYTES + warp * 32 * S::TAKEN;
         unsigned tile = 0;
-        for (int id = blockIdx.x; id < tiles; id += gridDim.x) {
+        for (int id = mine; id < tiles; id += all) {
             const Tile t = tile_of(id);
             const unsigned b = tile & 1;
-            const int64_t entry = FORM == OUTER ? -1 : a.g.order[t.slot + row];
+            const int64_t entry = FORM == OUTER || !t.there ? -1 : a.g.order[t.slot + row];
             if (t.steps > 0) {
                 bool on = bar_wait(done + 8 * b, tile / 2 & 1, broken);
                 on = __all_sync(0xffffffffu, on);
@@ -515,15 +567,22 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (t.steps > 0) {
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(taken + 8 * b);
+                if (lane == 0) {
+                    if (PAIR) bar_arrive_first(taken + 8 * b);
+                    else bar_arrive(taken + 8 * b);
+                }
                 tile++;
             }
         }
     }
     tmem_fence_before();
     __syncthreads();
+    if (PAIR) {                                    // nothing of this CTA is used by the other one any more
+        cluster_arrive();
+        cluster_wait();
+    }
     tmem_fence_after();
-    if (warp == ISSUER) tmem_free(tmem, 2 * W);
+    if (warp == ISSUER) tmem_free<PAIR>(tmem, 2 * W);
     if (tid == 0 && *broken) a.g.head[2] = 1;
 }
 
@@ -641,7 +700,7 @@ gated_few_kernel(const ProductArgs a, const T *__restrict__ w, int each)
     extern __shared__ __align__(128) unsigned char ring[];
     wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x % TEAM >> 5, inner = a.cols, width = a.terms, pieces = (inner + each - 1) / each;
-    if (a.g.head[1] && threadIdx.x < TAKERS) spoil<T, WIDE, GATED>(a, threadIdx.x);
+    if (a.g.head[1] && threadIdx.x < TAKERS) spoil<T, GATED>(a, threadIdx.x);
     const int64_t units = (int64_t)a.g.head[0] * pieces;
     const int steps = units > blockIdx.x ? (int)((units - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
     auto unit = [&](int step) { return blockIdx.x + (int64_t)step * gridDim.x; };
@@ -765,16 +824,66 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
 // wide or narrow tiles for products of tokens' rows
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) < sm_count(); }
 
-template <typename T, int W, int FORM, int NUMBERED, int SUMS>
+template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
 static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, ProductArgs a, int64_t columns, cudaStream_t st)
 {
-    auto kernel = product_kernel<T, W, FORM, NUMBERED, SUMS>;
-    CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<W>::SMEM));
+    typedef Shape<W, PAIR> S;
+    auto kernel = product_kernel<T, W, PAIR, FORM, NUMBERED, SUMS>;
+    CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     a.tiles_n = (int)ceil_div(columns, W);
+    if (FORM == OUTER) a.tiles_m = (int)ceil_div(a.rows, PAIR ? 2 * TM : TM);
     const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
-    const int64_t most = sm_count() * (W == WIDE ? 1 : 2);
-    if (tiles > 0x7fffffffLL) return fail("experts: more than 2^31 tiles");
-    CB_CUDA(launch_behind(kernel, dim3((unsigned)(tiles < most ? tiles : most)), PRODUCT_THREADS, Shape<W>::SMEM, st, map_a, map_b, a));
+    if (tiles > 0x3fffffffLL) return fail("experts: more than 2^30 tiles");
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(PRODUCT_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 2 : 1;
+    int64_t most = sm_count() * (W == WIDE ? 1 : 2);           // CTAs that run at the same time: each goes from tile to tile
+    if (PAIR) {
+        static std::atomic<int> fit{0};
+        int n = fit.load();
+        if (!n) {
+            cfg.gridDim = dim3((unsigned)(most / 2 * 2));
+            CB_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+            if (n < 1) return fail("experts: no room for a pair of CTAs");
+            fit.store(n);
+        }
+        most = 2 * (n < most / 2 ? n : most / 2);
+    }
+    const int64_t ctas = PAIR ? 2 * tiles : tiles;
+    cfg.gridDim = dim3((unsigned)(ctas < most ? ctas : most));
+    CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, a));
+    return 0;
+}
+
+// The shape that a product of `columns` columns takes: pairs where experts have tiles enough to make pairs of, on average; narrow tiles where wide ones
+// are fewer than SMs.
+template <typename T, int FORM, int NUMBERED, int SUMS, typename Maps>
+static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, Maps maps)
+{
+    alignas(64) CUtensorMap ma, mb;
+    memset(&ma, 0, sizeof(ma));
+    memset(&mb, 0, sizeof(mb));
+    if (FORM == OUTER || a.nnz >= a.g.ngroups * (int64_t)PAIR_ENTRIES) {
+        CB_TRY(maps(ma, mb, WIDE));
+        return launch_product<T, WIDE, true, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+    }
+    if constexpr (FORM != OUTER) {
+        if (narrow(a.g, a.nnz, columns)) {
+            CB_TRY(maps(ma, mb, NARROW));
+            return launch_product<T, NARROW, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+        }
+        CB_TRY(maps(ma, mb, WIDE));
+        return launch_product<T, WIDE, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+    }
     return 0;
 }
 
@@ -830,9 +939,7 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
     CB_TRY(check_at(what, w));
     CB_TRY(check_at(what, h));
     if (s.nnz == 0 || s.nrows == 0) return 0;
-    alignas(64) CUtensorMap mb;
     ProductArgs a = arguments<T>(s, plan);
-    const bool few = narrow(a.g, s.nnz, 2 * s.inner);
     a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
     a.cols = (int)s.inner;
@@ -847,9 +954,9 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
         CB_CUDA(launch_behind(gated_few_kernel<T>, dim3((unsigned)(units < sm_count() ? units : sm_count())), FEW_THREADS, FEW_SMEM, st, a, (const T *)w, each));
         return 0;
     }
-    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
-    return few ? launch_product<T, NARROW, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st)
-               : launch_product<T, WIDE, ROWS, NUMBERED_A, GATED>(mb, mb, a, 2 * s.inner, st);
+    return launch_shape<T, ROWS, NUMBERED_A, GATED>(a, 2 * s.inner, st, [&](CUtensorMap &, CUtensorMap &mb, int wide) {
+        return make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, wide / 2, &mb);
+    });
 }
 
 // dz: room for slots x 2 inner; sums: for nnz x width floats (null with dx)
@@ -867,39 +974,36 @@ static int gated_experts_grad(const Sizes &s, int32_t gelu, const int64_t *pos, 
         if (dw) CB_CUDA(cudaMemsetAsync(dw, 0, 2 * s.nexperts * s.inner * s.width * sizeof(T), st));
         return 0;
     }
-    alignas(64) CUtensorMap mb;
     ProductArgs a = arguments<T>(s, plan);
-    const bool few = narrow(a.g, s.nnz, 2 * s.inner);
-    CB_TRY(make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.token, x, ldx, s.width);
     a.terms = (int)s.width;
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.other = dh;
     a.out = dz;
-    CB_TRY(few ? (launch_product<T, NARROW, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, 2 * s.inner, st))
-               : (launch_product<T, WIDE, ROWS, NUMBERED_A, GATED_GRAD>(mb, mb, a, 2 * s.inner, st)));
-    alignas(64) CUtensorMap mz;
+    CB_TRY((launch_shape<T, ROWS, NUMBERED_A, GATED_GRAD>(a, 2 * s.inner, st, [&](CUtensorMap &, CUtensorMap &mb, int wide) {
+        return make_box_map(what, w, is_bf16<T>(), 2 * s.nexperts, s.inner, s.width, wide / 2, &mb);
+    })));
     if (dx) {
         a = arguments<T>(s, plan);
-        CB_TRY(make_box_map(what, w, is_bf16<T>(), s.nexperts, 2 * s.inner, s.width, TK, &mb));
-        CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TM, &mz));
         a.terms = 2 * (int)s.inner;
-            a.cols = (int)s.width;
+        a.cols = (int)s.width;
         a.sums = sums;
-        CB_TRY(narrow(a.g, s.nnz, s.width) ? (launch_product<T, NARROW, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, s.width, st))
-                                           : (launch_product<T, WIDE, BACK, NUMBERED_NONE, ENTRY_ROWS>(mz, mb, a, s.width, st)));
+        CB_TRY((launch_shape<T, BACK, NUMBERED_NONE, ENTRY_ROWS>(a, s.width, st, [&](CUtensorMap &mz, CUtensorMap &mb, int) {
+            CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TM, &mz));
+            return make_box_map(what, w, is_bf16<T>(), s.nexperts, 2 * s.inner, s.width, TK, &mb);
+        })));
         CB_TRY(add_rows<T>(s, pos, sums, dx, st));
     }
     if (dw) {
         a = arguments<T>(s, plan);
-        CB_TRY(make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TK, &mz));
         a.number(a.g.token, x, ldx, s.width);
         a.rows = 2 * (int)s.inner;
         a.cols = (int)s.width;
-        a.tiles_m = (int)ceil_div(2 * s.inner, TM);
-            a.out = dw;
-        CB_TRY((launch_product<T, WIDE, OUTER, NUMBERED_B, WEIGHT>(mz, mz, a, s.width, st)));
+        a.out = dw;
+        CB_TRY((launch_shape<T, OUTER, NUMBERED_B, WEIGHT>(a, s.width, st, [&](CUtensorMap &mz, CUtensorMap &, int) {
+            return make_box_map(what, dz, is_bf16<T>(), 1, a.g.slots, 2 * s.inner, TK, &mz);
+        })));
     }
     return 0;
 }
@@ -932,17 +1036,15 @@ static int combine_experts(const Sizes &s, const int64_t *pos, const int64_t *cr
         CB_CUDA(launch_behind(combine_few_kernel<T>, dim3((unsigned)(units < sm_count() ? units : sm_count())), FEW_THREADS, FEW_SMEM, st, a, pos, crd, (const T *)v, each));
         return 0;
     }
-    alignas(64) CUtensorMap mb;
     ProductArgs a = arguments<T>(s, plan);
-    const bool few = narrow(a.g, s.nnz, s.width);
-    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, (few ? NARROW : WIDE) / 2, &mb));
     a.number(a.g.order, h, s.inner, s.inner);
     a.terms = (int)s.inner;
     a.cols = (int)s.width;
     a.val = val;
     a.sums = sums;
-    CB_TRY(few ? (launch_product<T, NARROW, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, s.width, st))
-               : (launch_product<T, WIDE, ROWS, NUMBERED_A, ENTRY_ROWS>(mb, mb, a, s.width, st)));
+    CB_TRY((launch_shape<T, ROWS, NUMBERED_A, ENTRY_ROWS>(a, s.width, st, [&](CUtensorMap &, CUtensorMap &mb, int wide) {
+        return make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, wide / 2, &mb);
+    })));
     return add_rows<T>(s, pos, sums, y, st);
 }
 
@@ -960,8 +1062,6 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
         if (dv) CB_CUDA(cudaMemsetAsync(dv, 0, s.nexperts * s.inner * s.width * sizeof(T), st));
         return 0;
     }
-    alignas(64) CUtensorMap mb;
-    CB_TRY(make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TK, &mb));
     ProductArgs a = arguments<T>(s, plan);
     a.number(a.g.token, dy, lddy, s.width);
     a.terms = (int)s.width;
@@ -971,20 +1071,21 @@ static int combine_experts_grad(const Sizes &s, int32_t *plan, const void *h, co
     a.out = dh;
     a.scaled = scaled;
     a.sums = sums;
-    const bool few = narrow(a.g, s.nnz, s.inner);
-    CB_TRY(few ? (launch_product<T, NARROW, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, s.inner, st))
-               : (launch_product<T, WIDE, BACK, NUMBERED_A, COMBINE_GRAD>(mb, mb, a, s.inner, st)));
-    CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, 2 * (int)ceil_div(s.inner, few ? NARROW : WIDE), sums, dval));
+    int parts = 0;
+    CB_TRY((launch_shape<T, BACK, NUMBERED_A, COMBINE_GRAD>(a, s.inner, st, [&](CUtensorMap &, CUtensorMap &mb, int wide) {
+        parts = 2 * (int)ceil_div(s.inner, wide);
+        return make_box_map(what, v, is_bf16<T>(), s.nexperts, s.width, s.inner, TK, &mb);
+    })));
+    CB_CUDA(launch_behind(add_parts_kernel, dim3((unsigned)ceil_div(s.nnz, 256)), 256, 0, st, s.nnz, parts, sums, dval));
     if (dv) {
-        alignas(64) CUtensorMap mh;
         a = arguments<T>(s, plan);
-        CB_TRY(make_box_map(what, scaled, is_bf16<T>(), 1, a.g.slots, s.inner, TK, &mh));
         a.number(a.g.token, dy, lddy, s.width);
         a.rows = (int)s.width;
         a.cols = (int)s.inner;
-        a.tiles_m = (int)ceil_div(s.width, TM);
-            a.out = dv;
-        CB_TRY((launch_product<T, WIDE, OUTER, NUMBERED_A, WEIGHT>(mh, mh, a, s.inner, st)));
+        a.out = dv;
+        CB_TRY((launch_shape<T, OUTER, NUMBERED_A, WEIGHT>(a, s.inner, st, [&](CUtensorMap &, CUtensorMap &mh, int) {
+            return make_box_map(what, scaled, is_bf16<T>(), 1, a.g.slots, s.inner, TK, &mh);
+        })));
     }
     return 0;
 }

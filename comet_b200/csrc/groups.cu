@@ -1,7 +1,7 @@
 // Entries of a CSR matrix grouped by column: a stable counting sort in one launch, by a cluster of up to eight CTAs.
 //
 // A warp has a stretch of rows, a lane a row of 32 of them at a time; it counts its entries by column (lanes with the same column find each
-// other, so there are no atomics and the order is always the same), the counts are summed over the warps and, through the
+// other by votes on its bits, so there are no atomics and the order is always the same), the counts are summed over the warps and, through the
 // cluster's shared memory, over the CTAs, and a second walk over the rows puts each entry where the sums say.
 //
 // Bound: the chains of loads of the two walks.
@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(GT)
 group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
 {
     extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
-    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], sums[GW + 1];
+    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], pairs[MOST_GROUPS], sums[GW + 1], twos[GW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     int *own = warps + (size_t)warp * n;
@@ -30,6 +30,7 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     __syncthreads();
     const int64_t each = (nrows + (int64_t)ranks * GW - 1) / ((int64_t)ranks * GW), from = min((rank * GW + warp) * each, nrows);
     const int64_t to = min(from + each, nrows);
+    const int bits = 32 - __clz(n - 1);            // of a column (a vote a bit: match.any takes some 200 clocks, 6 votes 40)
     // each lane's entries of a row, one after the other, eight on their way at a time; what(entry, its row, its column, the lanes that have the same one)
     auto walk = [&](auto what) {
         for (int64_t r = from; r < to; r += 32) {
@@ -47,7 +48,11 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
                     const bool on = lo + i < hi;
                     if (!__any_sync(0xffffffffu, on)) break;
                     const int c = col[i] >= 0 && col[i] < n ? (int)col[i] : -1;
-                    const unsigned alike = __match_any_sync(0xffffffffu, c);
+                    unsigned alike = __ballot_sync(0xffffffffu, c >= 0);
+                    for (int b = 0; b < bits; b++) {
+                        const unsigned set = __ballot_sync(0xffffffffu, c >> b & 1);
+                        alike &= c >> b & 1 ? set : ~set;
+                    }
                     if (on) what(lo + i, r + lane, c, alike);
                     __syncwarp();
                 }
@@ -95,29 +100,45 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
         if (tid == GT - 1) sums[GW] = v;
     }
     const int tiles = (total + GROUP_TILE - 1) / GROUP_TILE;
-    int upto = tiles;                              // inclusive sums over the columns
+    int upto = tiles, two = (tiles + 1) / 2;       // inclusive sums over the columns
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        const int v = __shfl_up_sync(0xffffffffu, upto, o), w = __shfl_up_sync(0xffffffffu, two, o);
+        if (lane >= o) {
+            upto += v;
+            two += w;
+        }
     }
-    if (lane == 31) sums[warp] = upto;
+    if (lane == 31) {
+        sums[warp] = upto;
+        twos[warp] = two;
+    }
     __syncthreads();
-    for (int w = 0; w < warp; w++) upto += sums[w];
+    for (int w = 0; w < warp; w++) {
+        upto += sums[w];
+        two += twos[w];
+    }
     if (tid < n) {
         start[tid] = (upto - tiles) * GROUP_TILE + before;
         whole[tid] = total;
         ends[tid] = upto;
+        pairs[tid] = two - (tiles + 1) / 2;
         if (rank == 0) {
             g.counts[tid] = total;
             g.first[tid] = upto - tiles;
-            if (tid == n - 1) g.first[n] = g.head[0] = upto;
+            if (tid == n - 1) {
+                g.first[n] = g.head[0] = upto;
+                g.head[3] = two;
+            }
         }
     }
     __syncthreads();
     for (int c = rank * GW + warp; c < n; c += ranks * GW) {                         // a warp has a column's tiles and the rest of its last one
         const int sum = whole[c], first = ends[c] - (sum + GROUP_TILE - 1) / GROUP_TILE;
-        for (int i = first + lane; i < ends[c]; i += 32) g.column[i] = c;
+        for (int i = first + lane; i < ends[c]; i += 32) {
+            g.column[i] = c;
+            if ((i - first) % 2 == 0) g.pairs[pairs[c] + (i - first) / 2] = i;
+        }
         for (int64_t i = (int64_t)first * GROUP_TILE + sum + lane; i < (int64_t)ends[c] * GROUP_TILE; i += 32) g.order[i] = g.token[i] = -1;
     }
     // where a warp's entries go: to their slots, or to their places among the CTA's own
@@ -160,7 +181,8 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     if (ranks > 1) cluster_wait();                 // its own stay until they have been read
 }
 
-// The same for few entries of few rows: a thread has an entry, and counts those of its column before it.
+// The same for few entries of few rows: a thread has an entry, and counts those of its column before it.  No pairs of tiles: with so few entries nothing
+// takes tiles by pairs.
 static const int FEW = 256, FEW_ROWS = 1024;
 __global__ void __launch_bounds__(FEW)
 group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)

@@ -156,24 +156,18 @@ struct GradRow {
         // a q of 0 gives 0, whatever its logarithm: that may be -inf
         return mul2(q, fma2(make_float2(fmaxf(d.x, -16384.0f), fmaxf(d.y, -16384.0f)), make_float2(b, b), make_float2(a, a)));
     }
-    template <int G, int H>
-    __device__ __forceinline__ void all(float2 (&v)[G][H]) const
+    template <int H>
+    __device__ __forceinline__ void all(float2 (&v)[H]) const
     {
         if (zero) {
 #pragma unroll
-            for (int i = 0; i < G; i++)
-#pragma unroll
-                for (int k = 0; k < H; k++) v[i][k] = make_float2(0.0f, 0.0f);
+            for (int k = 0; k < H; k++) v[k] = make_float2(0.0f, 0.0f);
         } else if (near) {
 #pragma unroll
-            for (int i = 0; i < G; i++)
-#pragma unroll
-                for (int k = 0; k < H; k++) v[i][k] = from_exponent(fma2(v[i][k], make_float2(c, c), make_float2(-mc, -mc)));
+            for (int k = 0; k < H; k++) v[k] = from_exponent(fma2(v[k], make_float2(c, c), make_float2(-mc, -mc)));
         } else {
 #pragma unroll
-            for (int i = 0; i < G; i++)
-#pragma unroll
-                for (int k = 0; k < H; k++) v[i][k] = from_exponent(make_float2((v[i][k].x - m) * c, (v[i][k].y - m) * c));
+            for (int k = 0; k < H; k++) v[k] = from_exponent(make_float2((v[k].x - m) * c, (v[k].y - m) * c));
         }
     }
 };
@@ -200,36 +194,66 @@ __device__ __forceinline__ float sum_entries(const float *values, int64_t lo, in
     for (int64_t e = lo + lane; e < hi; e += 32) sum += values[e];
     return warp_sum(sum);
 }
-// Adds the entries' gradients to the granules of the warp: granule i of a lane begins at column col0 + i * stride * N + first * N, first the lane's place.
-template <int G, int N>
-__device__ __forceinline__ void add_entries(const ProbGrad &p, int64_t lo, int64_t hi, int col0, int stride, int warp_first, int lane, float2 (&v)[G][N / 2])
-{
-    for (int64_t e0 = lo; e0 < hi; e0 += 32) {
-        int granule = 0, at = 0;
-        float d = 0.0f;
-        bool mine = false;
-        if (e0 + lane < hi) {
-            const int64_t col = p.crd[e0 + lane], j = col - col0;
+// The entries among a warp's granules, 32 at a time, a lane each.  Granule i of a lane begins at column col0 + (i * stride + first + lane) * N.
+struct Hits {
+    int granule, at;                 // negative: not one of the warp's
+    float d;
+    template <int G, int N>
+    __device__ __forceinline__ void load(const ProbGrad &p, int64_t e, int64_t hi, int col0, int stride, int first)
+    {
+        granule = -1;
+        if (e < hi) {
+            const int64_t col = p.crd[e], j = col - col0;
             if (col >= 0 && col < p.ncols && j >= 0 && j < (int64_t)G * stride * N) {
-                granule = (int)j / N;
-                at = (int)j % N;
-                mine = (granule % stride & ~31) == warp_first;
-                if (mine) d = p.values[e0 + lane] * p.inv;
+                const int g = (int)j / N;
+                if ((g % stride & ~31) == first) {
+                    granule = g;
+                    at = (int)j % N;
+                    d = p.values[e] * p.inv;
+                }
             }
         }
-        for (unsigned on = __ballot_sync(0xffffffffu, mine); on; on &= on - 1) {
+    }
+    // those of granules `i`
+    template <int N>
+    __device__ __forceinline__ void add(int i, int stride, int first, int lane, float2 (&v)[N / 2]) const
+    {
+        for (unsigned on = __ballot_sync(0xffffffffu, granule >= 0 && granule / stride == i); on; on &= on - 1) {
             const int who = __ffs(on) - 1, g = __shfl_sync(0xffffffffu, granule, who), k = __shfl_sync(0xffffffffu, at, who);
             const float x = __shfl_sync(0xffffffffu, d, who);
-            const int to = g % stride - warp_first == lane ? g / stride * N + k : -1;
-            // no branch: the granules stay in registers
+            const int to = g % stride - first == lane ? k : -1;
+            // no branch: the granule stays in registers
 #pragma unroll
-            for (int i = 0; i < G; i++)
-#pragma unroll
-                for (int n = 0; n < N / 2; n++) {
-                    v[i][n].x += to == i * N + 2 * n ? x : 0.0f;
-                    v[i][n].y += to == i * N + 2 * n + 1 ? x : 0.0f;
-                }
+            for (int n = 0; n < N / 2; n++) {
+                v[n].x += to == 2 * n ? x : 0.0f;
+                v[n].y += to == 2 * n + 1 ? x : 0.0f;
+            }
         }
+    }
+};
+// Computes and stores a thread's granules: `left` of them, stride apart, are the row's.
+template <typename T, int G, bool ENTROPY>
+__device__ __forceinline__ void give_gradients(const ProbGrad &p, const GradRow<ENTROPY> &row, const Granule<T> (&in)[G], T *g, bool alike, int64_t lo, int64_t hi, int col0,
+                                               int stride, int place, int left)
+{
+    constexpr int N = Granule<T>::N;
+    const int lane = threadIdx.x & 31, first = place & ~31;
+    Hits hits;
+    hits.load<G, N>(p, lo + lane, hi, col0, stride, first);
+    const bool some = !row.none && __any_sync(0xffffffffu, hits.granule >= 0), more = !row.none && hi - lo > 32;
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+        float2 v[N / 2];
+        in[i].unpack(v);
+        row.all(v);
+        if (some) hits.add<N>(i, stride, first, lane, v);
+        if (more)
+            for (int64_t e = lo + 32; e < hi; e += 32) {
+                Hits h;
+                h.load<G, N>(p, e + lane, hi, col0, stride, first);
+                h.add<N>(i, stride, first, lane, v);
+            }
+        if (i * stride + place < left) put_granule<T>(g, col0 + (i * stride + place) * N, p.ncols, alike, v);
     }
 }
 
@@ -259,14 +283,7 @@ prob_grad_kernel(const ProbGrad p, int pieces, const T *xs, T *grad)
     const float2 kept = ((const float2 *)p.sums)[t];
     const float h = ENTROPY ? p.by_entropy[t] : 0.0f, ent = ENTROPY ? p.entropy[t] : 0.0f;
     const GradRow<ENTROPY> row(p, kept, h, ent, sum_entries(p.values, lo, hi, lane));
-    float2 v[G][N / 2];
-#pragma unroll
-    for (int i = 0; i < G; i++) in[i].unpack(v[i]);
-    row.all(v);
-    if (!row.none) add_entries<G, N>(p, lo, hi, col0, GT, tid & ~31, lane, v);
-#pragma unroll
-    for (int i = 0; i < G; i++)
-        if (i * GT + tid < left) put_granule<T>(g, col0 + (i * GT + tid) * N, p.ncols, alike, v[i]);
+    give_gradients<T, G, ENTROPY>(p, row, in, g, alike, lo, hi, col0, GT, tid, left);
 }
 
 // Short rows: a warp each, which has the whole row in registers.
@@ -287,13 +304,7 @@ prob_grad_short_kernel(const ProbGrad p, const T *xs, T *grad)
     const bool alike = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
     const float h = ENTROPY ? p.by_entropy[t] : 0.0f, ent = ENTROPY ? p.entropy[t] : 0.0f;
     const GradRow<ENTROPY> row(p, ((const float2 *)p.sums)[t], h, ent, sum_entries(p.values, lo, hi, lane));
-    float2 v[G][N / 2];
-#pragma unroll
-    for (int i = 0; i < G; i++) in[i].unpack(v[i]);
-    row.all(v);
-    if (!row.none) add_entries<G, N>(p, lo, hi, -off, 32, 0, lane, v);
-#pragma unroll
-    for (int i = 0; i < G; i++) put_granule<T>(g, (i * 32 + lane) * N - off, p.ncols, alike, v[i]);
+    give_gradients<T, G, ENTROPY>(p, row, in, g, alike, lo, hi, -off, 32, lane, 32 * G);
 }
 
 template <typename T>

@@ -135,22 +135,10 @@ def close(got, want, off, kind):
     assert float(over.max() if over.numel() else 0) <= 0, "off by %g more than %g at most" % (float(over.max()), float(off.max()))
 
 
-SHAPES = [
-    # rows, experts, chosen, width, inner
-    (1, 1, 1, 8, 8), (1, 8, 2, 64, 64), (1, 64, 8, 256, 128), (2, 3, 3, 72, 40), (5, 4, 1, 136, 264), (128, 1, 1, 64, 128), (129, 2, 1, 200, 136),
-    (300, 5, 2, 256, 512), (777, 10, 3, 1000, 712), (1500, 64, 6, 128, 96), (4099, 7, 2, 64, 72), (64, 1000, 5, 72, 24),
-]
-
-
-@pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("rows,experts,chosen,width,inner", SHAPES)
-@pytest.mark.parametrize("ragged", [False, True])
-def test_block(rows, experts, chosen, width, inner, ragged, kind):
+def run_block(rng, rows, experts, counts, width, inner, act, kind, columns=None):
+    """All operators in a row, each against the oracle."""
     from comet_b200 import device
-    rng = np.random.default_rng(rows * 31 + experts * 7 + width + ragged)
-    counts = rng.integers(0, chosen + 1, rows) if ragged else np.full(rows, chosen)
-    S, pos, crd, row = routes(rng, rows, experts, counts)
-    act = "gelu" if ragged else "silu"
+    S, pos, crd, row = routes(rng, rows, experts, counts, columns)
     O = Oracle(S, pos, crd, row, kind, act)
     X, W = matrix(rng, kind, rows, width), matrix(rng, kind, experts, 2 * inner, width, scale=width ** -0.5)
     V, dY = matrix(rng, kind, experts, width, inner, scale=inner ** -0.5), matrix(rng, kind, rows, width)
@@ -169,3 +157,29 @@ def test_block(rows, experts, chosen, width, inner, ragged, kind):
     close(dV, dv, ov, kind)
     close(dval, dvalue, oval + 1e-7 * dvalue.abs(), kind)
     G.check()
+
+
+SHAPES = [
+    # rows, experts, chosen, width, inner
+    (1, 1, 1, 8, 8), (1, 8, 2, 64, 64), (1, 64, 8, 256, 128), (2, 3, 3, 72, 40), (5, 4, 1, 136, 264), (128, 1, 1, 64, 128), (129, 2, 1, 200, 136),
+    (300, 5, 2, 256, 512), (777, 10, 3, 1000, 712), (1500, 64, 6, 128, 96), (4099, 7, 2, 64, 72), (64, 1000, 5, 72, 24),
+]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,experts,chosen,width,inner", SHAPES)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_block(rows, experts, chosen, width, inner, ragged, kind):
+    rng = np.random.default_rng(rows * 31 + experts * 7 + width + ragged)
+    counts = rng.integers(0, chosen + 1, rows) if ragged else np.full(rows, chosen)
+    run_block(rng, rows, experts, counts, width, inner, "gelu" if ragged else "silu", kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,experts,chosen,width,inner", [(700, 1, 1, 264, 200), (2000, 3, 2, 320, 384), (5000, 4, 1, 72, 1032)])
+def test_many_entries_an_expert(rows, experts, chosen, width, inner, kind):
+    """Tiles by pairs: even and odd numbers of them, an expert without any and one with few."""
+    rng = np.random.default_rng(rows)
+    weight = np.linspace(3, 0.2, experts) if experts < 4 else np.array([5, 0, 0.02, 2])
+    columns = [np.sort(rng.choice(experts, chosen, replace=False, p=weight / weight.sum())) for _ in range(rows)]
+    run_block(rng, rows, experts, np.full(rows, chosen), width, inner, "silu", kind, columns)
