@@ -63,10 +63,10 @@ enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 // are read by all SMs then (one token, 8 experts of 1024 x 2048 gates and ups: @GATED_ONE@ us against 21).
 static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64;
 static const int A_BYTES = TM * TK * 2;
-static const int PAIR_ENTRIES = 320;               // entries an expert from which on products of tokens' rows go by pairs
-static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 32;
+static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 64;
 // PAIR: two CTAs of a cluster share a product of 256 x 256, with 128 rows of either operand each: two thirds of the bytes that two tiles of their own
-// take from the L2, which is what bounds these products (@PAIR@).
+// take from the L2.  The sums over an expert's tokens go that way (dw of gated_grad_step 129 us, 139 by single CTAs; dv of combine_grad_step 76, 78).  Products
+// of tokens' rows do not: where an expert has an odd number of tiles one of a pair is empty (dz 145 against 135, dx 116, 114; gated_batch 483, 470).
 template <int W, bool PAIR>
 struct Shape {
     static constexpr int B_ROWS = PAIR ? W / 2 : W, B_BYTES = B_ROWS * TK * 2, STEP = A_BYTES + B_BYTES, RING = PAIR ? 6 : 4;
@@ -101,7 +101,6 @@ struct ProductArgs {
 
 struct Tile {
     int m, n, group, steps, slot;    // slot: the first one
-    bool there;                      // not the second of a pair that has none
 };
 
 __device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + exp2_fast(-LOG2E * u)); }
@@ -228,13 +227,13 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
                     gate[i] = d[i] * up[i] * fmaf(g * s * (1.0f - s), u.y, s);
                     up[i] = d[i] * g * s;
                 }
-                const int64_t to = t.there ? (int64_t)(t.slot + row) * 2 * inner + f0 + c : -1;
+                const int64_t to = (int64_t)(t.slot + row) * 2 * inner + f0 + c;
 #pragma unroll
                 for (int i = 0; i < PART; i += 8) part.put(i / 8, gate + i);
                 part.out((T *)a.out, to, left - c);
 #pragma unroll
                 for (int i = 0; i < PART; i += 8) part.put(i / 8, up + i);
-                part.out((T *)a.out, to < 0 ? to : to + inner, left - c);
+                part.out((T *)a.out, to + inner, left - c);
             }
         }
     } else if constexpr (SUMS == ENTRY_ROWS) {
@@ -285,7 +284,7 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
             // a row of zeros adds nothing to the sums over an expert's tokens
 #pragma unroll
             for (int i = 0; i < PART; i += 8) part.put(i / 8, h + i);
-            part.out((T *)a.scaled, t.there ? (int64_t)(t.slot + row) * a.cols + c0 + c : -1, left);
+            part.out((T *)a.scaled, (int64_t)(t.slot + row) * a.cols + c0 + c, left);
         }
         if (entry >= 0) a.sums[(t.n * 2 + half) * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     } else {
@@ -341,13 +340,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     typedef Shape<W, PAIR> S;
     constexpr int B_BYTES = S::B_BYTES, STEP_BYTES = S::STEP, RING = S::RING, CTAS = PAIR ? 2 : 1;
     constexpr unsigned TENSOR_BYTES = (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + (NUMBERED == NUMBERED_B ? 0 : B_BYTES);
+    static_assert(!PAIR || FORM == OUTER, "tiles of tokens have no pairs");
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[3 * RING + 4 + 1];
     __shared__ uint32_t tmem_room;
     __shared__ int broken_word;
     volatile int *broken = &broken_word;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int ISSUER = (TAKERS + FETCHERS) / 32;
+    constexpr int ISSUER = (TAKERS + FETCHERS) / 32, BOXES = ISSUER + 1;
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
                    last = taken + 16, ready = last + 8;
     const int rank = PAIR ? (int)cluster_rank() : 0;
@@ -377,10 +377,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     wait_for_previous();
 
     const int mine = blockIdx.x / CTAS, all = gridDim.x / CTAS;
-    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[PAIR ? 3 : 0] * a.tiles_n;
+    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
     auto tile_of = [&](int id) {
         Tile t;
-        t.there = true;
         if (FORM == OUTER) {
             t.group = id / (a.tiles_m * a.tiles_n);
             const int rest = id % (a.tiles_m * a.tiles_n);
@@ -389,73 +388,39 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             t.steps = (a.g.counts[t.group] + TK - 1) / TK;
             t.slot = a.g.first[t.group] * GROUP_TILE;
         } else {
-            const int first = PAIR ? a.g.pairs[id / a.tiles_n] : id / a.tiles_n;
-            t.m = first + rank;
+            t.m = id / a.tiles_n;
             t.n = id % a.tiles_n;
-            t.group = a.g.column[first];
-            if (PAIR) t.there = t.m < a.g.first[t.group + 1];
+            t.group = a.g.column[t.m];
             t.steps = (a.terms + TK - 1) / TK;
             t.slot = t.m * GROUP_TILE;
         }
         return t;
     };
 
-    if (warp >= TAKERS / 32 && warp < ISSUER) {    // fetches
+    // what is under way lands before the CTA ends
+    auto land = [&](unsigned step) {
+        volatile int late = 0;
+        for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
+    };
+    if (warp == BOXES) {                           // fetches by tensor copies
         unsigned step = 0;                         // steps so far; stage = step % RING
         bool on = true;
-        const int me = tid - TAKERS, chunk = me & 7, row = me >> 3;
-        // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
-        const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
-        const char *base = (const char *)a.numbered + chunk * 16;
-        const int64_t stride = a.ld * 2;
-        // what a tile's copies begin with is loaded while the tile before is fetched
-        constexpr int NUMBERS = FORM == OUTER ? 4 : 8;
-        Tile t = {}, after = {};
-        int number[NUMBERS], number_after[NUMBERS];
-        auto ahead = [&](int id) {
-            if (id < tiles) after = tile_of(id);
-        };
-        auto numbers = [&]() {
-            if (NUMBERED != NUMBERED_NONE)
-#pragma unroll
-                for (int i = 0; i < NUMBERS; i++) number_after[i] = after.there ? a.numbers[after.slot + row + 16 * i] : -1;
-        };
-        ahead(mine);
-        if (mine < tiles && after.steps) numbers();
         for (int id = mine; on && id < tiles; id += all) {
-            t = after;
-#pragma unroll
-            for (int i = 0; i < NUMBERS; i++) number[i] = number_after[i];
-            ahead(id + all);
-            const char *from[8];
-            unsigned there = 0;
-            if (NUMBERED == NUMBERED_A && FORM != OUTER) {
-#pragma unroll
-                for (int i = 0; i < NUMBERS; i++) {
-                    from[i] = base + max(number[i], 0) * stride;
-                    there |= (number[i] >= 0 ? 1u : 0u) << i;
-                }
-            }
-            if (t.steps <= 1 && id + all < tiles && after.steps) numbers();
+            const Tile t = tile_of(id);
+            constexpr int BLOCKS = S::B_ROWS / 64;
+            const int n0 = t.n * W + (PAIR ? rank * (W / 2) : 0);                    // of the operand's rows, this CTA's first
             for (int k = 0; k < t.steps; k++, step++) {
                 const unsigned s = step % RING;
                 const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
-                on = bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken);
-                on = __all_sync(0xffffffffu, on);
+                on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
                 if (!on) break;
-                if (me == 0) {
+                if (elect()) {
                     bar_expect(bar, TENSOR_BYTES);
-                    constexpr int BLOCKS = S::B_ROWS / 64;
-                    const int n0 = t.n * W + (PAIR ? rank * (W / 2) : 0);            // of the operand's rows, this CTA's first
                     if (FORM == ROWS) {
                         // an expert's gate rows, and as many up rows; or rows of the one weight
                         constexpr bool GATES = SUMS != ENTRY_ROWS;
-                        if (PAIR) {
-                            load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group + rank : t.group, bar);
-                        } else {
-                            load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
-                            load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, GATES ? t.n * (W / 2) : n0 + W / 2, GATES ? 2 * t.group + 1 : t.group, bar);
-                        }
+                        load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
+                        load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, GATES ? t.n * (W / 2) : n0 + W / 2, GATES ? 2 * t.group + 1 : t.group, bar);
                     } else if (FORM == BACK) {
                         if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
 #pragma unroll
@@ -468,84 +433,109 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
                     }
                 }
-                if (NUMBERED == NUMBERED_A && FORM != OUTER) {
+                __syncwarp();
+            }
+        }
+        if (*broken) land(step);
+    } else if (warp >= TAKERS / 32 && warp < ISSUER) {         // fetches rows by their number
+        unsigned step = 0;
+        bool on = NUMBERED != NUMBERED_NONE;
+        const int me = tid - TAKERS, chunk = me & 7, row = me >> 3;
+        // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
+        const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
+        const char *base = (const char *)a.numbered + chunk * 16;
+        const int64_t stride = a.ld * 2;
+        for (int id = mine; on && id < tiles; id += all) {
+            const Tile t = tile_of(id);
+            const char *from[8];
+            unsigned there = 0;
+            if (NUMBERED == NUMBERED_A && FORM != OUTER) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int n = a.numbers[t.slot + row + 16 * i];
+                    from[i] = base + max(n, 0) * stride;
+                    there |= (n >= 0 ? 1u : 0u) << i;
+                }
+            }
+            int next[4];
+            if (FORM == OUTER && t.steps)
+#pragma unroll
+                for (int i = 0; i < 4; i++) next[i] = a.numbers[t.slot + row + 16 * i];
+            for (int k = 0; k < t.steps; k++, step++) {
+                const unsigned s = step % RING;
+                const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
+                on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
+                if (!on) break;
+                if (FORM != OUTER) {
                     const bool in = k * TK + chunk * 8 < a.numbered_cols;
 #pragma unroll
                     for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
-                } else if (NUMBERED != NUMBERED_NONE) {
+                } else {
                     constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : S::B_ROWS / 64;
                     const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
                     const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W + (PAIR ? rank * (W / 2) : 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const char *src = base + max(number[i], 0) * stride;
+                        const char *src = base + max(next[i], 0) * stride;
 #pragma unroll
                         for (int b = 0; b < BLOCKS; b++) {
                             const bool in = col0 + b * 64 + chunk * 8 < a.numbered_cols;
-                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && number[i] >= 0);
+                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && next[i] >= 0);
                         }
-                        if (k + 1 < t.steps) number[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
+                        if (k + 1 < t.steps) next[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
                     }
                 }
-                if (NUMBERED != NUMBERED_NONE) copies_to(bar);
-                if (k + 2 == t.steps && id + all < tiles && after.steps) numbers();
+                copies_to(bar);
             }
         }
-        // what is under way lands before the CTA ends
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if (*broken) {
-            volatile int late = 0;
-            for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
-        }
     } else if (warp == ISSUER) {                   // issues the products
-        if (lane == 0 && rank == 1) {              // tells the first CTA what has landed here
-            unsigned step = 0;
-            bool on = true;
-            for (int id = mine; on && id < tiles; id += all) {
-                const int steps = tile_of(id).steps;
-                for (int k = 0; k < steps; k++, step++) {
-                    const unsigned s = step % RING;
-                    on = bar_wait(full + 8 * s, step / RING & 1, broken);
-                    if (!on) break;
-                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
-                    bar_arrive_first(ready + 8 * s);
-                }
-            }
-        } else if (lane == 0) {
-            constexpr uint32_t kind = product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
-            unsigned tile = 0, step = 0;
-            bool on = true;
-            int after = mine < tiles ? tile_of(mine).steps : 0;
-            for (int id = mine; on && id < tiles; id += all) {
-                const int steps = after;
-                if (id + all < tiles) after = tile_of(id + all).steps;
-                if (steps == 0) continue;
-                const unsigned b = tile & 1;
-                on = bar_wait<PAIR>(taken + 8 * b, (tile / 2 & 1) ^ 1, broken);
+        // the whole warp goes along, and one thread of it issues: operands are the warp's then, not a thread's
+        unsigned tile = 0, step = 0;
+        bool on = true;
+        int after = mine < tiles ? tile_of(mine).steps : 0;
+        for (int id = mine; on && id < tiles; id += all) {
+            const int steps = (int)__reduce_max_sync(0xffffffffu, (unsigned)after);  // the same in all, which the compiler does not know
+            if (id + all < tiles) after = tile_of(id + all).steps;
+            if (steps == 0) continue;
+            const unsigned b = tile & 1;
+            if (rank == 0) {
+                on = __all_sync(0xffffffffu, bar_wait<PAIR>(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
                 tmem_fence_after();
-                for (int k = 0; on && k < steps; k++, step++) {
-                    const unsigned s = step % RING;
-                    on = bar_wait(full + 8 * s, step / RING & 1, broken);
-                    if (PAIR && on) on = bar_wait<true>(ready + 8 * s, step / RING & 1, broken);
+            }
+            for (int k = 0; on && k < steps; k++, step++) {
+                const unsigned s = step % RING;
+                on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
+                if (!on) break;
+                if (NUMBERED != NUMBERED_NONE) shared_to_products();
+                if (PAIR && rank == 1) {           // tells the first CTA what has landed here
+                    if (elect()) bar_arrive_first(ready + 8 * s);
+                    continue;
+                }
+                if (PAIR) {
+                    on = __all_sync(0xffffffffu, bar_wait<true>(ready + 8 * s, step / RING & 1, broken));
                     if (!on) break;
-                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
-                    tmem_fence_after();
-                    const uint32_t at = ring + s * STEP_BYTES;
-                    const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
-                    // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
-                    constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
+                }
+                tmem_fence_after();
+                const uint32_t at = ring + s * STEP_BYTES;
+                const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
+                // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
+                constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
+                constexpr uint32_t kind = product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
+                if (elect()) {
 #pragma unroll
                     for (int i = 0; i < TK / 16; i++) product<PAIR>(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
                     products_to<PAIR>(empty + 8 * s);
+                    if (k + 1 == steps) products_to<PAIR>(done + 8 * b);
                 }
-                if (on) products_to<PAIR>(done + 8 * b);
-                tile++;
+                __syncwarp();
             }
-            if (*broken) {                         // products under way end before tensor memory is given back
-                volatile int late = 0;
-                products_to<PAIR>(last);
-                bar_wait(last, 0, &late);
-            }
+            tile++;
+        }
+        if (*broken && rank == 0) {                // products under way end before tensor memory is given back
+            volatile int late = 0;
+            if (elect()) products_to<PAIR>(last);
+            bar_wait(last, 0, &late);
         }
         __syncwarp();
     } else {                                       // takes the sums
@@ -556,11 +546,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (int id = mine; id < tiles; id += all) {
             const Tile t = tile_of(id);
             const unsigned b = tile & 1;
-            const int64_t entry = FORM == OUTER || !t.there ? -1 : a.g.order[t.slot + row];
+            const int64_t entry = FORM == OUTER ? -1 : a.g.order[t.slot + row];
             if (t.steps > 0) {
-                bool on = bar_wait(done + 8 * b, tile / 2 & 1, broken);
-                on = __all_sync(0xffffffffu, on);
-                if (!on) break;
+                if (!__all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken))) break;
                 tmem_fence_after();
             }
             take_sums<T, W, SUMS>(a, tmem + b * W + ((uint32_t)(warp & 3) << 21), t.steps == 0, t, warp >> 2, row, entry, room);
@@ -864,19 +852,17 @@ static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, Pr
     return 0;
 }
 
-// The shape that a product of `columns` columns takes: pairs where experts have tiles enough to make pairs of, on average; narrow tiles where wide ones
-// are fewer than SMs.
+// The shape that a product of `columns` columns takes: pairs for sums over an expert's tokens; narrow tiles where wide ones are fewer than SMs.
 template <typename T, int FORM, int NUMBERED, int SUMS, typename Maps>
 static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, Maps maps)
 {
     alignas(64) CUtensorMap ma, mb;
     memset(&ma, 0, sizeof(ma));
     memset(&mb, 0, sizeof(mb));
-    if (FORM == OUTER || a.nnz >= a.g.ngroups * (int64_t)PAIR_ENTRIES) {
+    if constexpr (FORM == OUTER) {
         CB_TRY(maps(ma, mb, WIDE));
         return launch_product<T, WIDE, true, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
-    }
-    if constexpr (FORM != OUTER) {
+    } else {
         if (narrow(a.g, a.nnz, columns)) {
             CB_TRY(maps(ma, mb, NARROW));
             return launch_product<T, NARROW, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
@@ -884,7 +870,6 @@ static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, 
         CB_TRY(maps(ma, mb, WIDE));
         return launch_product<T, WIDE, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
     }
-    return 0;
 }
 
 struct Sizes {

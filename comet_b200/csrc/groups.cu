@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(GT)
 group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
 {
     extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
-    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], pairs[MOST_GROUPS], sums[GW + 1], twos[GW];
+    __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], sums[GW + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     int *own = warps + (size_t)warp * n;
@@ -100,45 +100,29 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
         if (tid == GT - 1) sums[GW] = v;
     }
     const int tiles = (total + GROUP_TILE - 1) / GROUP_TILE;
-    int upto = tiles, two = (tiles + 1) / 2;       // inclusive sums over the columns
+    int upto = tiles;                              // inclusive sums over the columns
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o), w = __shfl_up_sync(0xffffffffu, two, o);
-        if (lane >= o) {
-            upto += v;
-            two += w;
-        }
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
     }
-    if (lane == 31) {
-        sums[warp] = upto;
-        twos[warp] = two;
-    }
+    if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    for (int w = 0; w < warp; w++) {
-        upto += sums[w];
-        two += twos[w];
-    }
+    for (int w = 0; w < warp; w++) upto += sums[w];
     if (tid < n) {
         start[tid] = (upto - tiles) * GROUP_TILE + before;
         whole[tid] = total;
         ends[tid] = upto;
-        pairs[tid] = two - (tiles + 1) / 2;
         if (rank == 0) {
             g.counts[tid] = total;
             g.first[tid] = upto - tiles;
-            if (tid == n - 1) {
-                g.first[n] = g.head[0] = upto;
-                g.head[3] = two;
-            }
+            if (tid == n - 1) g.first[n] = g.head[0] = upto;
         }
     }
     __syncthreads();
     for (int c = rank * GW + warp; c < n; c += ranks * GW) {                         // a warp has a column's tiles and the rest of its last one
         const int sum = whole[c], first = ends[c] - (sum + GROUP_TILE - 1) / GROUP_TILE;
-        for (int i = first + lane; i < ends[c]; i += 32) {
-            g.column[i] = c;
-            if ((i - first) % 2 == 0) g.pairs[pairs[c] + (i - first) / 2] = i;
-        }
+        for (int i = first + lane; i < ends[c]; i += 32) g.column[i] = c;
         for (int64_t i = (int64_t)first * GROUP_TILE + sum + lane; i < (int64_t)ends[c] * GROUP_TILE; i += 32) g.order[i] = g.token[i] = -1;
     }
     // where a warp's entries go: to their slots, or to their places among the CTA's own
@@ -181,8 +165,7 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     if (ranks > 1) cluster_wait();                 // its own stay until they have been read
 }
 
-// The same for few entries of few rows: a thread has an entry, and counts those of its column before it.  No pairs of tiles: with so few entries nothing
-// takes tiles by pairs.
+// The same for few entries of few rows: a thread has an entry, and counts those of its column before it.
 static const int FEW = 256, FEW_ROWS = 1024;
 __global__ void __launch_bounds__(FEW)
 group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
@@ -250,7 +233,8 @@ static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_
     if (nrows < 0 || nnz < 0 || ncols < 1 || ncols > MOST_GROUPS)
         return fail("group_entries: %lld entries in %lld rows of %lld columns (1 to %d)", (long long)nnz, (long long)nrows, (long long)ncols, MOST_GROUPS);
     if (nrows > 0x7fffffffLL || nnz > 0x70000000LL) return fail("group_entries: more than 2^31 rows, or 1.8e9 entries");
-    if (nnz <= FEW && nrows <= FEW_ROWS) {         // one token's 8 entries: @FEW@ us, 7.1 by the cluster's kernel
+    // one token's 8 entries: 4.9 us, 7.1 by the cluster's kernel
+    if (nnz <= FEW && nrows <= FEW_ROWS) {
         group_few_kernel<<<1, FEW, 0, st>>>((int)nrows, (int)nnz, pos, crd, groups_in(plan, nnz, ncols));
         CB_LAUNCH_CHECK();
         return 0;

@@ -10,10 +10,9 @@ static const int GROUP_TILE = 128, MOST_GROUPS = 1024;
 // Where things are in the caller's int32 array.  `bad` entries (their column lies outside) are no tile's; the last `bad` elements of order are
 // their numbers.
 struct Groups {
-    int *head;                   // tiles, bad, status (not 0: a wait ran out), pairs of tiles
+    int *head;                   // tiles, bad, status (not 0: a wait ran out)
     int *counts, *first;         // of each column: entries, first tile (and one more: the number of tiles)
     int *column;                 // of each tile
-    int *pairs;                  // the first tile of each pair of neighbouring tiles of a column (the last one of a column may be alone)
     int *order, *token;          // of each slot: the entry, its row
     int64_t slots;
     int ngroups;
@@ -24,7 +23,7 @@ inline int64_t group_tiles(int64_t nnz, int64_t ngroups) { return nnz / GROUP_TI
 inline int64_t group_size(int64_t nnz, int64_t ngroups)
 {
     const int64_t tiles = group_tiles(nnz, ngroups);
-    return GROUP_HEAD + (ngroups + 3) / 4 * 4 + (ngroups + 4) / 4 * 4 + 2 * ((tiles + 3) / 4 * 4) + 2 * tiles * GROUP_TILE;
+    return GROUP_HEAD + (ngroups + 3) / 4 * 4 + (ngroups + 4) / 4 * 4 + (tiles + 3) / 4 * 4 + 2 * tiles * GROUP_TILE;
 }
 inline Groups groups_in(int *plan, int64_t nnz, int64_t ngroups)
 {
@@ -34,8 +33,7 @@ inline Groups groups_in(int *plan, int64_t nnz, int64_t ngroups)
     g.counts = plan + GROUP_HEAD;
     g.first = g.counts + (ngroups + 3) / 4 * 4;
     g.column = g.first + (ngroups + 4) / 4 * 4;
-    g.pairs = g.column + (tiles + 3) / 4 * 4;
-    g.order = g.pairs + (tiles + 3) / 4 * 4;
+    g.order = g.column + (tiles + 3) / 4 * 4;
     g.slots = tiles * GROUP_TILE;
     g.token = g.order + g.slots;
     g.ngroups = (int)ngroups;

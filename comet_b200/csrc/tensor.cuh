@@ -39,19 +39,19 @@ __device__ __forceinline__ bool bar_try_cluster(uint32_t bar, unsigned parity)
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// arrives at the same barrier of the cluster's first CTA
+// Arrives at the same barrier of the cluster's first CTA.  What it tells is that copies into this CTA's shared memory have landed, which the thread has seen; a
+// release for the whole cluster waits for every access under way, 1000 clocks a step.
 __device__ __forceinline__ void bar_arrive_first(uint32_t bar)
 {
-    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar) : "memory");
 }
 // Waits for a phase; false after two seconds, or once another wait of the CTA has run out (*broken).
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int *broken)
 {
-    for (int i = 0; i < 64; i++)
-        if (CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity)) return true;
     unsigned long long began = 0;
     for (;;) {
+        // unrolled by the compiler: a loop of one look at a time let the products of gated_batch wait 2 % longer
         for (int i = 0; i < 64; i++)
             if (CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity)) return true;
         if (*broken) return false;
@@ -63,6 +63,13 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile
             return false;
         }
     }
+}
+// one thread of a warp that is together
+__device__ __forceinline__ bool elect()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : : "memory");
+    return r != 0;
 }
 
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int c, int r, int z, uint32_t bar)

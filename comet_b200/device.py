@@ -392,7 +392,7 @@ def group_entries(S):
     pos, crd = _check_beside("group_entries", S, S.nrows, S.ncols)
     nnz, n = S.nnz, S.ncols
     tiles = nnz // 128 + min(nnz, n) + 1                       # as csrc/groups.cuh counts
-    plan = S.pos.new_empty(16 + (n + 3) // 4 * 4 + (n + 4) // 4 * 4 + (tiles + 3) // 4 * 8 + 256 * tiles, dtype=torch.int32)
+    plan = S.pos.new_empty(16 + (n + 3) // 4 * 4 + (n + 4) // 4 * 4 + (tiles + 3) // 4 * 4 + 256 * tiles, dtype=torch.int32)
     _call("comet_b200_dev_group_entries_i64", S.nrows, n, nnz, pos, crd, plan.data_ptr(), _stream())
     return EntryGroups(S, plan, 128 * tiles)
 
