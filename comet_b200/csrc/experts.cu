@@ -605,10 +605,10 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
     out[i] = v;
 }
 
-// Few tokens: products of a weight's rows with a handful of vectors, by the ordinary cores.  Neighbouring rows of an expert's weight are one piece of
+// A single token: products of a weight's rows with its vectors, by the ordinary cores.  Neighbouring rows of an expert's weight are one piece of
 // memory, so a CTA's share comes in copies of up to 32 KB.  Six teams of four warps have a stage each: while one of them works on its stage, the others'
 // copies are under way, what an SM has to have in flight for the memory's full rate.  The vectors come through the L1 cache.
-static const int FEW_ROWS = 8, FEW_SUMS = 4;       // rows of x, of y up to which this is taken
+// 8 experts of 64, in L2, us: 14.1 and 11.8 (gated, combine); by the tensor cores 17.5 and 13.3, and with two tokens 25 and 14 where this takes 32 and 18.
 static const int FEW_STAGES = 6, FEW_BYTES = 32 * 1024, FEW_SMEM = FEW_STAGES * FEW_BYTES, FEW_ENTRIES = 8, TEAM = 128, FEW_THREADS = FEW_STAGES * TEAM;
 
 // Of R rows in shared memory, `next` bytes apart, and B vectors: a lane's part of their products.  A vector is loaded once for all the rows.
@@ -735,38 +735,28 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
 {
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ float sums[FEW_STAGES][TEAM / 32][FEW_BYTES / FEW_ENTRIES / 16];      // a row has 16 bytes or more
-    __shared__ int64_t first[FEW_SUMS + 1];
     wait_for_previous();
-    const int tid = threadIdx.x, lane = tid & 31, team = tid / TEAM, warp = tid % TEAM >> 5, width = a.rows, inner = a.terms, nrows = a.tiles_m;
-    const int pieces = (width + each - 1) / each;
-    if (tid <= nrows) first[tid] = pos[tid];
-    __syncthreads();
-    // the CTA's elements: units blockIdx.x, + gridDim.x, ... of rows x pieces; the team's: every FEW_STAGES-th of those, in batches of eight entries
-    const int units = nrows * pieces, mine = units > (int)blockIdx.x ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int tid = threadIdx.x, lane = tid & 31, team = tid / TEAM, warp = tid % TEAM >> 5, width = a.rows, inner = a.terms;
+    const int64_t first = pos[0], last = pos[1];
+    // the CTA's pieces of y: blockIdx.x, + gridDim.x, ...; the team's: every FEW_STAGES-th of those, each in batches of eight entries
+    const int pieces = (width + each - 1) / each, mine = pieces > (int)blockIdx.x ? (pieces - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int batches = max(1, (int)((last - first + FEW_ENTRIES - 1) / FEW_ENTRIES)), count = mine > team ? (mine - 1 - team) / FEW_STAGES * batches + batches : 0;
     struct Step {
-        int unit, batch, row, d;
+        int batch, d;
         int64_t lo, hi;
     };
-    auto begin = [&](int unit, int batch) {
-        const int u = (int)blockIdx.x + unit * (int)gridDim.x;
-        Step s = {unit, batch, u / pieces, u % pieces * each, 0, 0};
-        s.lo = first[s.row] + (int64_t)batch * FEW_ENTRIES;
-        s.hi = min(s.lo + FEW_ENTRIES, first[s.row + 1]);
+    auto at = [&](int step) {
+        const int n = step / FEW_STAGES, piece = (int)blockIdx.x + (team + n / batches * FEW_STAGES) * (int)gridDim.x;
+        Step s = {n % batches, piece * each, 0, 0};
+        s.lo = first + (int64_t)s.batch * FEW_ENTRIES;
+        s.hi = min(s.lo + FEW_ENTRIES, last);
         return s;
     };
     const unsigned room = FEW_BYTES / FEW_ENTRIES;
-    // a step's number says no more than how many there were: a team's next step is the next batch of its unit, or its next unit
-    Step now = begin(team < mine ? team : 0, 0);
-    auto after = [&](const Step &s) { return s.hi < first[s.row + 1] ? begin(s.unit, s.batch + 1) : begin(s.unit + FEW_STAGES < mine ? s.unit + FEW_STAGES : s.unit, 0); };
-    int count = 0;                                 // the team's steps
-    for (int u = team; u < mine; u += FEW_STAGES) {
-        const int row = ((int)blockIdx.x + u * (int)gridDim.x) / pieces;
-        count += max(1, (int)((first[row + 1] - first[row] + FEW_ENTRIES - 1) / FEW_ENTRIES));
-    }
     few_steps(
         count ? team + (count - 1) * FEW_STAGES + 1 : 0, ring, a.g.head,
         [&](int step, uint32_t to, uint32_t bar) {
-            const Step s = step < FEW_STAGES ? now : after(now);
+            const Step s = at(step);
             const unsigned bytes = (unsigned)min(each, width - s.d) * inner * sizeof(T);
             bar_expect(bar, (unsigned)(s.hi - s.lo) * bytes);
             for (int64_t e = s.lo; e < s.hi; e++) {
@@ -775,7 +765,7 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
             }
         },
         [&](int step, const unsigned char *stage) {
-            if (step >= FEW_STAGES) now = after(now);
+            const Step now = at(step);
             const int rows = min(each, width - now.d);
             const unsigned next = (unsigned)inner * sizeof(T);
             auto give = [&](auto batch, int r) {
@@ -802,15 +792,16 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
             int r = 0;
             for (; r + 2 <= rows; r += 2) give(std::integral_constant<int, 2>(), r);
             if (r < rows) give(std::integral_constant<int, 1>(), r);
-            if (now.hi < first[now.row + 1]) return;
+            if (now.hi < last) return;
             team_sync(team);
             for (int r = tid % TEAM; r < rows; r += TEAM)
-                ((T *)a.out)[(int64_t)now.row * width + now.d + r] = from_float<T>((sums[team][0][r] + sums[team][1][r]) + (sums[team][2][r] + sums[team][3][r]));
+                ((T *)a.out)[now.d + r] = from_float<T>((sums[team][0][r] + sums[team][1][r]) + (sums[team][2][r] + sums[team][3][r]));
         });
 }
 
-// wide or narrow tiles for products of tokens' rows
-static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) < sm_count(); }
+// Narrow tiles where wide ones would leave most SMs without any (one expert of 1024 columns: @NARROWED@); at 64 wide tiles both take the same time, at
+// 144 wide ones 17 us and narrow ones 24.
+static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) * 4 < sm_count(); }
 
 template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
 static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, ProductArgs a, int64_t columns, cudaStream_t st)
@@ -930,7 +921,7 @@ static int gated_experts(const Sizes &s, int32_t gelu, int32_t *plan, const void
     a.cols = (int)s.inner;
     a.gelu = gelu != 0;
     a.out = h;
-    if (s.nrows <= FEW_ROWS && s.width * 2 * (int64_t)sizeof(T) <= FEW_BYTES) {
+    if (s.nrows == 1 && s.width * 2 * (int64_t)sizeof(T) <= FEW_BYTES) {
         // no fewer steps than SMs, if there are rows enough
         const int64_t fit = FEW_BYTES / (s.width * 2 * (int64_t)sizeof(T)), most = group_tiles(s.nnz, s.nexperts) - 1, share = ceil_div(most * s.inner, sm_count());
         const int each = (int)(fit < share ? fit : share);
@@ -1006,17 +997,16 @@ static int combine_experts(const Sizes &s, const int64_t *pos, const int64_t *cr
         CB_CUDA(cudaMemsetAsync(y, 0, s.nrows * s.width * sizeof(T), st));
         return 0;
     }
-    if (s.nrows <= FEW_SUMS && s.inner * (int64_t)sizeof(T) <= FEW_BYTES / FEW_ENTRIES) {
-        const int64_t fit = FEW_BYTES / FEW_ENTRIES / (s.inner * (int64_t)sizeof(T)), share = ceil_div(s.nrows * s.width, sm_count());
+    if (s.nrows == 1 && s.inner * (int64_t)sizeof(T) <= FEW_BYTES / FEW_ENTRIES) {
+        const int64_t fit = FEW_BYTES / FEW_ENTRIES / (s.inner * (int64_t)sizeof(T)), share = ceil_div(s.width, sm_count());
         const int each = (int)(fit < share ? fit : share);
-        const int64_t units = s.nrows * ceil_div(s.width, each);
+        const int64_t units = ceil_div(s.width, each);
         ProductArgs a = arguments<T>(s, plan);
         a.numbered = h;
         a.val = val;
         a.out = y;
         a.terms = (int)s.inner;
         a.rows = (int)s.width;
-        a.tiles_m = (int)s.nrows;
         CB_CUDA(cudaFuncSetAttribute(combine_few_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
         CB_CUDA(launch_behind(combine_few_kernel<T>, dim3((unsigned)(units < sm_count() ? units : sm_count())), FEW_THREADS, FEW_SMEM, st, a, pos, crd, (const T *)v, each));
         return 0;

@@ -1,10 +1,12 @@
 // Entries of a CSR matrix grouped by column: a stable counting sort in one launch, by a cluster of up to eight CTAs.
 //
-// A warp has a stretch of rows, a lane a row of 32 of them at a time; it counts its entries by column (lanes with the same column find each
-// other by votes on its bits, so there are no atomics and the order is always the same), the counts are summed over the warps and, through the
+// A warp has a stretch of rows and counts their entries by column (lanes with the same column find each other by votes on its bits, so there
+// are no atomics and the order is always the same), the counts are summed over the warps and, through the
 // cluster's shared memory, over the CTAs, and a second walk over the rows puts each entry where the sums say.
 //
 // Bound: the chains of loads of the two walks.
+#include <type_traits>
+
 #include "groups.cuh"
 #include "logits.cuh"
 #include "stream.cuh"
@@ -31,35 +33,37 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     const int64_t each = (nrows + (int64_t)ranks * GW - 1) / ((int64_t)ranks * GW), from = min((rank * GW + warp) * each, nrows);
     const int64_t to = min(from + each, nrows);
     const int bits = 32 - __clz(n - 1);            // of a column (a vote a bit: match.any takes some 200 clocks, 6 votes 40)
-    // each lane's entries of a row, one after the other, eight on their way at a time; what(entry, its row, its column, the lanes that have the same one)
-    auto walk = [&](auto what) {
+    // The entries of 32 rows after the other, a lane an entry, four loads on their way at a time; what(entry, its row, its column, the lanes that have the
+    // same one).  ROWS: the row is asked for, too; lane i knows where row r + i ends.
+    auto walk = [&](auto rows, auto what) {
         for (int64_t r = from; r < to; r += 32) {
-            int64_t lo = 0, hi = 0;
-            if (r + lane < to) {
-                lo = min(max(pos[r + lane], (int64_t)0), nnz);
-                hi = min(max(pos[r + lane + 1], lo), nnz);
-            }
-            for (; __any_sync(0xffffffffu, lo < hi); lo += 8) {
-                int64_t col[8];
+            const int64_t end = min(max(pos[min(r + lane + 1, to)], (int64_t)0), nnz), begin = min(max(pos[r], (int64_t)0), nnz);
+            const int64_t hi = __shfl_sync(0xffffffffu, end, 31);
+            for (int64_t e0 = begin; e0 < hi; e0 += 128) {
+                int64_t col[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) col[i] = lo + i < hi ? crd[lo + i] : -1;
+                for (int i = 0; i < 4; i++) col[i] = e0 + 32 * i + lane < hi ? crd[e0 + 32 * i + lane] : -1;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const bool on = lo + i < hi;
-                    if (!__any_sync(0xffffffffu, on)) break;
+                for (int i = 0; i < 4; i++) {
+                    const int64_t e = e0 + 32 * i + lane;
+                    if (e0 + 32 * i >= hi) break;
                     const int c = col[i] >= 0 && col[i] < n ? (int)col[i] : -1;
                     unsigned alike = __ballot_sync(0xffffffffu, c >= 0);
                     for (int b = 0; b < bits; b++) {
                         const unsigned set = __ballot_sync(0xffffffffu, c >> b & 1);
                         alike &= c >> b & 1 ? set : ~set;
                     }
-                    if (on) what(lo + i, r + lane, c, alike);
+                    int row = 0;                   // the first one that ends behind the entry
+                    if (decltype(rows)::value)
+#pragma unroll
+                        for (int step = 16; step > 0; step /= 2) row += __shfl_sync(0xffffffffu, end, row + step - 1) <= e ? step : 0;
+                    if (e < hi) what(e, r + row, c, alike);
                     __syncwarp();
                 }
             }
         }
     };
-    walk([&](int64_t, int64_t, int col, unsigned alike) {
+    walk(std::false_type(), [&](int64_t, int64_t, int col, unsigned alike) {
         if (col >= 0 && lane == __ffs(alike) - 1) own[col] += __popc(alike);
     });
     __syncthreads();
@@ -136,7 +140,7 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     int2 *sorted = (int2 *)(warps + (size_t)GW * n);
     unsigned short *of = (unsigned short *)(sorted + sortable);
     const bool staged = here <= sortable;
-    walk([&](int64_t e, int64_t row, int col, unsigned alike) {
+    walk(std::true_type(), [&](int64_t e, int64_t row, int col, unsigned alike) {
         if (col < 0) {
             g.order[g.slots - 1 - atomicAdd(&g.head[1], 1)] = (int)e;
             return;
