@@ -59,8 +59,7 @@ int make_box_map(const char *what, const void *base, bool bf16, int64_t depth, i
 enum Form { ROWS, BACK, OUTER };
 enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 
-// A tile has 128 rows and W columns.  W = 256 where there are tiles enough for the chip; else 64, two CTAs on an SM: the weights of few tokens' experts
-// are read by all SMs then (one token, 8 experts of 1024 x 2048 gates and ups: @GATED_ONE@ us against 21).
+// A tile has 128 rows and W columns: 256, or, where those are few for the chip, 64, two CTAs on an SM (launch_shape).
 static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64;
 static const int A_BYTES = TM * TK * 2;
 static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 64;
@@ -799,7 +798,7 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
         });
 }
 
-// Narrow tiles where wide ones would leave most SMs without any (one expert of 1024 columns: @NARROWED@); at 64 wide tiles both take the same time, at
+// Narrow tiles where wide ones would leave most SMs without any (launch_shape's rule); at 64 wide tiles both take the same time, at
 // 144 wide ones 17 us and narrow ones 24.
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) * 4 < sm_count(); }
 

@@ -337,7 +337,7 @@ def log_probs(S, X, temperature=1.0, entropy=False, top=0):
 
 
 def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperature=1.0, grad=True):
-    """The gradient with respect to X of what log_probs gives, from d_values (float32, one for each of S's entries; columns of a row ascending) and, with the
+    """The gradient with respect to X of what log_probs gives, from d_values (float32, one for each of S's entries) and, with the
     entropies, d_entropy (float32, one for each row).  sums and entropy: of log_probs at the same temperature.  grad: True (a new tensor), or a tensor to write
     it to, such as X.  The alternatives have no gradient here: as S of a second call they have."""
     n, m, ld = shape = _check_logits("log_probs_grad", X)

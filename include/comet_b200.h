@@ -700,7 +700,7 @@ COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_f32_i64(
     float *values, float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, void *stream);
 
 /* Their gradient: grad = d loss / d x in x's type, from d_values[nnz] and (with the entropies; both may be NULL) d_entropy[nrows], and the sums of the forward
-   call at the same temperature.  May be x itself (same ldx).  Columns of a row ascend, repeated ones are next to each other and add up; one outside
+   call at the same temperature.  May be x itself (same ldx).  Columns in any order, repeated ones add up; one outside
    the matrix only adds to the row's sum.  A row whose d_values add up to 0, with a d_entropy of 0, is 0 but at its entries, and so is all of a row of -inf. */
 COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_bf16_i64(
     int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,

@@ -183,3 +183,279 @@ def test_many_entries_an_expert(rows, experts, chosen, width, inner, kind):
     weight = np.linspace(3, 0.2, experts) if experts < 4 else np.array([5, 0, 0.02, 2])
     columns = [np.sort(rng.choice(experts, chosen, replace=False, p=weight / weight.sum())) for _ in range(rows)]
     run_block(rng, rows, experts, np.full(rows, chosen), width, inner, "silu", kind, columns)
+
+
+def listed_slots(G):
+    """(column, entry, token) of each filled slot in order, and the numbers of entries without a column, from a plan as csrc/groups.cuh lays it out."""
+    p, n, nnz = G.plan.cpu().numpy(), G.S.ncols, G.S.nnz
+    tiles = nnz // 128 + min(nnz, n) + 1
+    counts = p[16:16 + n]
+    first = p[16 + (n + 3) // 4 * 4:][:n + 1]
+    column = p[16 + (n + 3) // 4 * 4 + (n + 4) // 4 * 4:][:tiles]
+    slots = tiles * 128
+    order, token = p[-2 * slots:-slots], p[-slots:]
+    assert p[0] == first[n] and p[2] == 0
+    used = np.arange(p[0] * 128)
+    got = order[used] >= 0
+    assert (column[:p[0]] == np.repeat(np.arange(n), np.diff(first))).all() and (np.diff(first) == -(-counts // 128)).all()
+    assert (token[used][~got] == -1).all()
+    return column[used[got] // 128], order[used[got]], token[used[got]], sorted(order[slots - p[1]:])
+
+
+@pytest.mark.parametrize("rows,experts,most,bad", [(1, 64, 8, 0), (1, 1, 1, 0), (3, 1024, 60, 2), (40, 5, 5, 0), (256, 3, 1, 0), (257, 3, 1, 3), (1000, 700, 3, 0), (1025, 64, 8, 5),
+                                                   (9000, 64, 8, 0), (9000, 1024, 8, 7), (40000, 16, 8, 0), (30000, 1000, 9, 1)])
+def test_groups(rows, experts, most, bad):
+    """Entries in the order of columns, and inside a column in their own; by one CTA, by clusters, with and without room to sort in."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows + experts)
+    counts = rng.integers(0, most + 1, rows)
+    counts[rng.integers(rows)] = most
+    pos = np.concatenate([[0], np.cumsum(counts)]).astype(np.int64)
+    # some columns are asked for much more often; repeated ones in a row, and those in any order, are allowed
+    crd = np.minimum((rng.random(pos[-1]) ** 2 * experts).astype(np.int64), experts - 1)
+    wrong = rng.choice(pos[-1], min(bad, int(pos[-1])), replace=False)
+    crd[wrong] = rng.choice([-1, experts, 1 << 40], len(wrong))
+    up = lambda a: torch.from_numpy(a).cuda()                                                  # noqa: E731
+    column, order, token, left = listed_slots(device.group_entries(device.DeviceCSR(rows, experts, up(pos), up(crd), None)))
+    good = np.flatnonzero((crd >= 0) & (crd < experts))
+    want = good[np.argsort(crd[good], kind="stable")]
+    assert (order == want).all() and (column == crd[want]).all() and (token == np.repeat(np.arange(rows), counts)[want]).all()
+    assert left == sorted(wrong)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [1, 5, 700])
+def test_repeated_columns(rows, kind):
+    """A token that has an expert more than once, and columns in any order."""
+    rng = np.random.default_rng(rows)
+    columns = [rng.integers(0, 3, 5) for _ in range(rows)]
+    run_block(rng, rows, 3, np.full(rows, 5), 136, 72, "gelu", kind, columns)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 900])
+def test_columns_outside(rows):
+    """An entry whose column is no expert's makes its own results NaN, and those of its token; the experts' gradients leave it out."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows)
+    S, pos, crd, row = routes(rng, rows, 4, np.full(rows, 2))
+    bad = [0, len(crd) - 1] if rows > 1 else [1]
+    S.crd[bad[0]] = -1
+    S.crd[bad[-1]] = 4
+    O = Oracle(S, pos, S.crd.cpu().numpy(), row, "bf16")
+    X, W, V = matrix(rng, "bf16", rows, 64), matrix(rng, "bf16", 4, 96, 64, scale=0.1), matrix(rng, "bf16", 4, 64, 48, scale=0.1)
+    G = device.group_entries(S)
+    fine = torch.ones(len(crd), dtype=torch.bool, device="cuda")
+    fine[bad] = False
+    tokens = torch.ones(rows, dtype=torch.bool, device="cuda")
+    tokens[row[bad]] = False
+    H = device.gated_experts(G, X, W)
+    assert torch.isnan(H[~fine]).all()
+    want, off = O.gated(X, W)
+    close(H[fine], want[fine], off[fine], "bf16")
+    H = matrix(rng, "bf16", len(crd), 48)
+    Y = device.combine_experts(G, H, V)
+    want, off = O.combine(H, V)
+    assert torch.isnan(Y[~tokens]).all()
+    close(Y[tokens], want[tokens], off[tokens], "bf16")
+    dX, dW = device.gated_experts_grad(G, X, W, H)
+    dx, ox, dw, ow = O.gated_grad(X, W, H)
+    assert torch.isnan(dX[~tokens]).all()
+    close(dX[tokens], dx[tokens], ox[tokens], "bf16")
+    close(dW, dw, ow, "bf16")
+    dH, dV, dval = device.combine_experts_grad(G, H, V, X)
+    dh, oh, dv, ov, dvalue, oval = O.combine_grad(H, V, X)
+    assert torch.isnan(dH[~fine]).all() and torch.isnan(dval[~fine]).all()
+    close(dH[fine], dh[fine], oh[fine], "bf16")
+    close(dV, dv, ov, "bf16")
+    close(dval[fine], dvalue[fine], oval[fine] + 1e-7 * dvalue[fine].abs(), "bf16")
+
+
+@pytest.mark.parametrize("rows", [0, 3])
+def test_nothing_stored(rows):
+    import torch
+    from comet_b200 import device
+    S = device.DeviceCSR(rows, 4, torch.zeros(rows + 1, dtype=torch.int64).cuda(), torch.zeros(0, dtype=torch.int64).cuda(), torch.zeros(0).cuda())
+    G = device.group_entries(S)
+    new = lambda *shape: torch.randn(shape, device="cuda").bfloat16()                           # noqa: E731
+    X, W, H, V = new(rows, 16), new(4, 32, 16), new(0, 16), new(4, 16, 16)
+    assert device.gated_experts(G, X, W).shape == (0, 16)
+    dX, dW = device.gated_experts_grad(G, X, W, H)
+    assert dX.shape == X.shape and not dX.any() and not dW.any()
+    assert torch.equal(device.combine_experts(G, H, V), torch.zeros_like(X))
+    dH, dV, dval = device.combine_experts_grad(G, H, V, X)
+    assert dH.shape == (0, 16) and not dV.any() and dval.shape == (0,)
+    G.check()
+
+
+@pytest.mark.parametrize("rows", [1, 6, 500])
+def test_rows_with_a_stride(rows):
+    """Tokens' rows in a wider matrix, and no more gradients than are asked for."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows)
+    S, pos, crd, row = routes(rng, rows, 5, np.full(rows, 2))
+    wide, W = matrix(rng, "f16", rows, 200), matrix(rng, "f16", 5, 160, 104, scale=0.1)
+    X, V, dY = wide[:, 16:120], matrix(rng, "f16", 5, 104, 80, scale=0.1), wide[:, 88:192]
+    G = device.group_entries(S)
+    H = device.gated_experts(G, X, W)
+    assert torch.equal(H, device.gated_experts(G, X.contiguous(), W))
+    dH = matrix(rng, "f16", len(crd), 80)
+    dX, dW = device.gated_experts_grad(G, X.contiguous(), W, dH)
+    for x, w in [(True, True), (True, False), (False, True)]:
+        got = device.gated_experts_grad(G, X, W, dH, grad_x=x, grad_w=w)
+        assert (got[0] is None) == (not x) and (got[1] is None) == (not w)
+        assert not x or torch.equal(got[0], dX)
+        assert not w or torch.equal(got[1], dW)
+    want = device.combine_experts_grad(G, H, V, dY.contiguous())
+    for a, b in zip(device.combine_experts_grad(G, H, V, dY), want):
+        assert torch.equal(a, b)
+    got = device.combine_experts_grad(G, H, V, dY, grad_v=False)
+    assert torch.equal(got[0], want[0]) and got[1] is None and torch.equal(got[2], want[2])
+
+
+def test_infinities_stay_with_their_expert():
+    """A token of infinities and a weight of NaN: other tokens' and experts' results are what they were."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(4)
+    S, pos, crd, row = routes(rng, 300, 6, np.full(300, 2))
+    X, W, V = matrix(rng, "bf16", 300, 64), matrix(rng, "bf16", 6, 64, 64, scale=0.1), matrix(rng, "bf16", 6, 64, 32, scale=0.1)
+    G = device.group_entries(S)
+    d = matrix(rng, "bf16", len(crd), 32)
+    H, dW, Y, dV = device.gated_experts(G, X, W), device.gated_experts_grad(G, X, W, d)[1], device.combine_experts(G, d, V), device.combine_experts_grad(G, d, V, X)[1]
+    X[7], W[2], V[2] = math.inf, math.nan, math.nan
+    entry = torch.from_numpy((row != 7) & (crd != 2)).cuda()
+    token = torch.tensor([t != 7 and 2 not in crd[pos[t]:pos[t + 1]] for t in range(300)]).cuda()
+    expert = torch.tensor([j != 2 and j not in crd[pos[7]:pos[8]] for j in range(6)]).cuda()
+    without = torch.tensor([2 not in crd[pos[t]:pos[t + 1]] for t in range(300)]).cuda()
+    assert torch.equal(device.gated_experts(G, X, W)[entry], H[entry])
+    assert torch.equal(device.gated_experts_grad(G, X, W, d)[1][expert], dW[expert])
+    assert torch.equal(device.combine_experts(G, d, V)[without], Y[without]) and token.any()
+    assert torch.equal(device.combine_experts_grad(G, d, V, X)[1][expert], dV[expert])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,chosen", [(60, 2), (900, 2)])
+def test_gradients_by_differences(rows, chosen, kind):
+    """Along a direction: the difference quotient of the block in 64 bits against the kernels' gradients times the direction."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows)
+    S, pos, crd, row = routes(rng, rows, 3, np.full(rows, chosen))
+    O = Oracle(S, pos, crd, row, kind, "gelu")
+    X, W = matrix(rng, kind, rows, 40), matrix(rng, kind, 3, 48, 40, scale=0.3)
+    H, V = matrix(rng, kind, len(crd), 24), matrix(rng, kind, 3, 40, 24, scale=0.3)
+    dH, dY = matrix(rng, kind, len(crd), 24), matrix(rng, kind, rows, 40)
+    G = device.group_entries(S)
+    to = lambda t: torch.from_numpy(rng.standard_normal(t.shape)).cuda()                         # noqa: E731
+    vx, vw, vh, vv, vs = to(X), to(W), to(H), to(V), to(S.val)
+
+    def gated(s):
+        return float((O.gated(X.double() + s * vx, W.double() + s * vw)[0] * dH.double()).sum())
+
+    def combine(s):
+        O.S = device.DeviceCSR(S.nrows, S.ncols, S.pos, S.crd, S.val.double() + s * vs)
+        y = O.combine(H.double() + s * vh, V.double() + s * vv)[0]
+        O.S = S
+        return float((y * dY.double()).sum())
+
+    step = 1e-4
+    dX, dW = device.gated_experts_grad(G, X, W, dH, activation="gelu")
+    _, ox, _, ow = O.gated_grad(X, W, dH)
+    got = float((dX.double() * vx).sum() + (dW.double() * vw).sum())
+    off = float((ox * vx.abs()).sum() + (ow * vw.abs()).sum())
+    # the quotient's own error, step^2 times a third derivative, is that of the same quotient with twice the step, divided by three
+    quotient = lambda f, s: (f(s) - f(-s)) / (2 * s)                                             # noqa: E731
+    own = abs(quotient(gated, 2 * step) - quotient(gated, step)) + 1e-6
+    assert abs(got - quotient(gated, step)) <= off + own and off < 0.2 * float((dX.double() * vx).abs().sum())
+    dh, dV, dval = device.combine_experts_grad(G, H, V, dY)
+    _, oh, _, ov, _, oval = O.combine_grad(H, V, dY)
+    got = float((dh.double() * vh).sum() + (dV.double() * vv).sum() + (dval.double() * vs).sum())
+    off = float((oh * vh.abs()).sum() + (ov * vv.abs()).sum() + (oval * vs.abs()).sum())
+    own = abs(quotient(combine, 2 * step) - quotient(combine, step)) + 1e-6
+    assert abs(got - quotient(combine, step)) <= off + own
+
+
+@pytest.mark.parametrize("rows", [1, 30, 2000])
+def test_same_bits_streams_and_graphs(rows):
+    """Calls on another stream, two at once, and captured ones give an eager call's bits, and follow their inputs; so does a graph that holds all of them."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows)
+    S, pos, crd, row = routes(rng, rows, 4, np.full(rows, 2))
+    X, W, V = matrix(rng, "bf16", rows, 264), matrix(rng, "bf16", 4, 400, 264, scale=0.1), matrix(rng, "bf16", 4, 264, 200, scale=0.1)
+    d = matrix(rng, "bf16", len(crd), 200)
+
+    def everything():
+        G = device.group_entries(S)
+        H = device.gated_experts(G, X, W)
+        return [H, device.combine_experts(G, H, V), *device.gated_experts_grad(G, X, W, d), *device.combine_experts_grad(G, H, V, X), G.plan[2:3]]
+
+    want = everything()
+    for a, b in zip(want, everything()):
+        assert torch.equal(a, b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(everything())
+    torch.cuda.synchronize()
+    for g in got:
+        for a, b in zip(want, g):
+            assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        held = everything()
+    other = np.concatenate([np.sort(rng.choice(4, 2, replace=False)) for _ in range(rows)])
+    S.crd.copy_(torch.from_numpy(other))
+    X.copy_(matrix(rng, "bf16", rows, 264))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(everything(), held):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    import torch
+    from comet_b200 import _lib, device
+    rng = np.random.default_rng(0)
+    S, pos, crd, row = routes(rng, 6, 4, np.full(6, 2))
+    G = device.group_entries(S)
+    X, W, H, V = matrix(rng, "bf16", 6, 64), matrix(rng, "bf16", 4, 96, 64), matrix(rng, "bf16", 12, 48), matrix(rng, "bf16", 4, 64, 48)
+    wide = matrix(rng, "bf16", 6, 80)
+    csr = lambda **k: device.DeviceCSR(**{**dict(nrows=6, ncols=4, pos=S.pos, crd=S.crd, val=S.val), **k})          # noqa: E731
+    no_values, doubles = device.group_entries(csr(val=None)), device.group_entries(csr(val=S.val.double()))
+    for call in (lambda: device.group_entries(csr(ncols=0)), lambda: device.group_entries(csr(ncols=1025)), lambda: device.group_entries(csr(pos=S.pos.int())),
+                 lambda: device.group_entries(csr(crd=S.crd.int())), lambda: device.group_entries(csr(nrows=7)), lambda: device.group_entries(csr(pos=S.pos.cpu())),
+                 lambda: device.group_entries(csr(row_ids=S.pos[:6])),
+                 lambda: device.gated_experts(G, X.float(), W.float()), lambda: device.gated_experts(G, X.half(), W), lambda: device.gated_experts(G, X[:5], W),
+                 lambda: device.gated_experts(G, X, W[:3]), lambda: device.gated_experts(G, X, W[:, :, :32]), lambda: device.gated_experts(G, X, W[:, :88].contiguous()),
+                 lambda: device.gated_experts(G, X, W, activation="relu"), lambda: device.gated_experts(G, wide[:, 1:65], W), lambda: device.gated_experts(G, X.t(), W),
+                 lambda: device.gated_experts(G, X.cpu(), W), lambda: device.gated_experts(G, X, W.transpose(1, 2)),
+                 lambda: device.gated_experts(G, wide[:, :68], matrix(rng, "bf16", 4, 96, 68)),
+                 lambda: device.gated_experts_grad(G, X, W, H[:11]), lambda: device.gated_experts_grad(G, X, W, H.half()), lambda: device.gated_experts_grad(G, X, W, H[:, :40]),
+                 lambda: device.combine_experts(G, H, V.half()), lambda: device.combine_experts(G, H[:11], V), lambda: device.combine_experts(G, H, V[:, :60].contiguous()),
+                 lambda: device.combine_experts(no_values, H, V), lambda: device.combine_experts(doubles, H, V),
+                 lambda: device.combine_experts_grad(G, H, V, X.half()), lambda: device.combine_experts_grad(G, H, V, wide), lambda: device.combine_experts_grad(G, H, V, X[:3])):
+        with pytest.raises(ValueError):
+            call()
+    # the C entries themselves
+    at = [t.data_ptr() for t in (G.plan, X, W, H)]
+    for sizes, ldx, plan in [((6, 4, 12, 60, 48), 64, at[0]), ((6, 4, 12, 64, 44), 64, at[0]), ((6, 4, 12, 64, 48), 60, at[0]), ((6, 4, 12, 64, 48), 68, at[0]),
+                             ((6, 0, 12, 64, 48), 64, at[0]), ((6, 1025, 12, 64, 48), 64, at[0]), ((-1, 4, 12, 64, 48), 64, at[0]), ((6, 4, -1, 64, 48), 64, at[0])]:
+        with pytest.raises(_lib.CometB200Error, match="gated_experts"):
+            device._call("comet_b200_dev_gated_experts_bf16_i64", *sizes, 0, plan, at[1], ldx, at[2], at[3], device._stream())
+    with pytest.raises(_lib.CometB200Error, match="16 bytes"):
+        device._call("comet_b200_dev_gated_experts_bf16_i64", 6, 4, 12, 64, 48, 0, at[0], at[1] + 2, 64, at[2], at[3], device._stream())
+    torch.cuda.synchronize()
+    G.check()
+    G.plan[2] = 1                                                          # what a kernel leaves that gave up waiting
+    with pytest.raises(_lib.CometB200Error, match="wait"):
+        G.check()
