@@ -646,10 +646,10 @@ __device__ __forceinline__ void dots(const unsigned char *row, unsigned next, co
 
 __device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory"); }
 
-// What both kernels do: steps, which the teams take in turn.  issue(step, stage's address, barrier) copies a step's rows, by one thread; take(step, stage) works
-// on them.
-template <typename Issue, typename Take>
-__device__ __forceinline__ void few_steps(int steps, unsigned char *ring, int *head, Issue issue, Take take)
+// What both kernels do: steps, which the teams take in turn.  issue(step, stage's address, barrier) copies a step's rows, by one thread; prepare(step) looks up
+// what else they are worked on with, while they are under way; take(stage) works on them.
+template <typename Issue, typename Prepare, typename Take>
+__device__ __forceinline__ void few_steps(int steps, unsigned char *ring, int *head, Issue issue, Prepare prepare, Take take)
 {
     __shared__ __align__(8) uint64_t bars[FEW_STAGES];
     __shared__ int broken_word;
@@ -667,8 +667,9 @@ __device__ __forceinline__ void few_steps(int steps, unsigned char *ring, int *h
     __syncthreads();
     unsigned parity = 0;
     for (int step = team; step < steps; step += FEW_STAGES, parity ^= 1) {
+        prepare(step);
         if (!bar_wait(bar, parity, broken)) break;
-        take(step, stage);
+        take(stage);
         team_sync(team);
         if (first && step + FEW_STAGES < steps) issue(step + FEW_STAGES, smem_at(stage), bar);
     }
@@ -692,6 +693,8 @@ gated_few_kernel(const ProductArgs a, const T *__restrict__ w, int each)
     const int steps = units > blockIdx.x ? (int)((units - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
     auto unit = [&](int step) { return blockIdx.x + (int64_t)step * gridDim.x; };
     const unsigned second = (unsigned)each * width * sizeof(T);
+    int f = 0, slot = 0, count = 0, entry = 0;     // of the step: its first column, its tile's slots, entries, the first one's number and row
+    const T *x0 = nullptr;
     few_steps(
         steps, ring, a.g.head,
         [&](int step, uint32_t to, uint32_t bar) {
@@ -702,22 +705,29 @@ gated_few_kernel(const ProductArgs a, const T *__restrict__ w, int each)
             load_bytes(to, gate, bytes, bar);
             load_bytes(to + second, gate + (int64_t)inner * width, bytes, bar);
         },
-        [&](int step, const unsigned char *stage) {
-            const int m = (int)(unit(step) / pieces), f = (int)(unit(step) % pieces) * each, group = a.g.column[m], slot = m * GROUP_TILE;
-            const int count = min(GROUP_TILE, a.g.counts[group] - (m - a.g.first[group]) * GROUP_TILE), rows = min(each, inner - f), parts = width / 8;
+        [&](int step) {
+            const int m = (int)(unit(step) / pieces), group = a.g.column[m];
+            f = (int)(unit(step) % pieces) * each;
+            slot = m * GROUP_TILE;
+            entry = a.g.order[slot];
+            x0 = (const T *)a.numbered + a.numbers[slot] * a.ld;
+            count = min(GROUP_TILE, a.g.counts[group] - (m - a.g.first[group]) * GROUP_TILE);
+        },
+        [&](const unsigned char *stage) {
+            const int rows = min(each, inner - f), parts = width / 8;
             for (int r = warp; r < rows; r += TEAM / 32) {
                 auto give = [&](auto batch, int e0) {
                     constexpr int B = decltype(batch)::value;
                     const uint4 *x[B];
 #pragma unroll
-                    for (int i = 0; i < B; i++) x[i] = (const uint4 *)((const T *)a.numbered + a.numbers[slot + e0 + i] * a.ld);
+                    for (int i = 0; i < B; i++) x[i] = (const uint4 *)(B == 1 && e0 == 0 ? x0 : (const T *)a.numbered + a.numbers[slot + e0 + i] * a.ld);
                     float2 sum[2][B];
                     dots<T, 2, B>(stage + (size_t)r * width * sizeof(T), second, x, parts, lane, sum);
 #pragma unroll
                     for (int i = 0; i < B; i++) {
                         const float g = warp_sum(sum[0][i].x + sum[0][i].y), u = warp_sum(sum[1][i].x + sum[1][i].y);
                         if (lane == 0)
-                            ((T *)a.out)[(int64_t)a.g.order[slot + e0 + i] * inner + f + r] = from_float<T>(g * logistic(gate_of(g, a.gelu).x) * u);
+                            ((T *)a.out)[(int64_t)(B == 1 && e0 == 0 ? entry : a.g.order[slot + e0 + i]) * inner + f + r] = from_float<T>(g * logistic(gate_of(g, a.gelu).x) * u);
                     }
                 };
                 int e = 0;
@@ -752,6 +762,8 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
         return s;
     };
     const unsigned room = FEW_BYTES / FEW_ENTRIES;
+    Step now = {0, 0, 0, 0};
+    float by[FEW_ENTRIES / (TEAM / 32)] = {};      // the values of the warp's entries
     few_steps(
         count ? team + (count - 1) * FEW_STAGES + 1 : 0, ring, a.g.head,
         [&](int step, uint32_t to, uint32_t bar) {
@@ -763,8 +775,17 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
                 load_bytes(to + (unsigned)(e - s.lo) * room, v + ((col >= 0 && col < a.g.ngroups ? col : 0) * width + s.d) * inner, bytes, bar);
             }
         },
-        [&](int step, const unsigned char *stage) {
-            const Step now = at(step);
+        [&](int step) {
+            now = at(step);
+#pragma unroll
+            for (int i = 0; i < FEW_ENTRIES / (TEAM / 32); i++) {
+                const int64_t e = now.lo + i * (TEAM / 32) + warp;
+                if (e >= now.hi) break;
+                const int64_t col = crd[e];
+                by[i] = col >= 0 && col < a.g.ngroups ? a.val[e] : __int_as_float(0x7fffffff);
+            }
+        },
+        [&](const unsigned char *stage) {
             const int rows = min(each, width - now.d);
             const unsigned next = (unsigned)inner * sizeof(T);
             auto give = [&](auto batch, int r) {
@@ -774,13 +795,11 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
                 for (int i = 0; i < FEW_ENTRIES; i += TEAM / 32) {
                     const int64_t e = now.lo + i + warp;
                     if (e >= now.hi) break;
-                    const int64_t col = crd[e];
-                    const float by = col >= 0 && col < a.g.ngroups ? a.val[e] : __int_as_float(0x7fffffff);
                     const uint4 *const x[1] = {(const uint4 *)((const T *)a.numbered + e * inner)};
                     float2 d[R][1];
                     dots<T, R, 1>(stage + (i + warp) * room + r * next, next, x, inner / 8, lane, d);
 #pragma unroll
-                    for (int j = 0; j < R; j++) sum[j] = fmaf(by, d[j][0].x + d[j][0].y, sum[j]);
+                    for (int j = 0; j < R; j++) sum[j] = fmaf(by[i / (TEAM / 32)], d[j][0].x + d[j][0].y, sum[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < R; j++) {
