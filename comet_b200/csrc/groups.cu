@@ -27,6 +27,7 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     int *own = warps + (size_t)warp * n;
     let_next_start();                              // it waits for this one's end before it reads
+    wait_for_previous();
     for (int i = tid; i < GW * n; i += GT) warps[i] = 0;
     if (rank == 0 && tid < GROUP_HEAD) g.head[tid] = 0;
     __syncthreads();
@@ -177,6 +178,7 @@ group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int6
     __shared__ int rows[FEW_ROWS + 1], cols[FEW], count[MOST_GROUPS], first[MOST_GROUPS], sums[FEW / 32], bad;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     let_next_start();
+    wait_for_previous();
     const int64_t mine = tid < nnz ? crd[tid] : -1;
     for (int i = tid; i <= nrows; i += FEW) rows[i] = (int)min(max(pos[i], (int64_t)0), (int64_t)nnz);
     const int col = mine >= 0 && mine < n ? (int)mine : -1;
@@ -239,14 +241,28 @@ static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_
     if (nrows > 0x7fffffffLL || nnz > 0x70000000LL) return fail("group_entries: more than 2^31 rows, or 1.8e9 entries");
     // one token's 8 entries: 4.9 us, 7.1 by the cluster's kernel
     if (nnz <= FEW && nrows <= FEW_ROWS) {
-        group_few_kernel<<<1, FEW, 0, st>>>((int)nrows, (int)nnz, pos, crd, groups_in(plan, nnz, ncols));
-        CB_LAUNCH_CHECK();
+        CB_CUDA(launch_behind(group_few_kernel, dim3(1), FEW, 0, st, (int)nrows, (int)nnz, pos, crd, groups_in(plan, nnz, ncols)));
         return 0;
     }
     int ranks = 1;                                 // a CTA has 1024 rows under way at a time
     while (ranks < MOST_CLUSTER && nrows > (int64_t)ranks * GT) ranks *= 2;
-    return launch_cluster(group_kernel, (unsigned)ranks, ranks, GT, room_for(ncols), room_for(MOST_GROUPS), st, nrows, nnz, pos, crd,
-                          groups_in(plan, nnz, ncols));
+    // the limit of shared memory is that of the largest call, in every call
+    CB_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room_for(MOST_GROUPS)));
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ranks);
+    cfg.blockDim = dim3(GT);
+    cfg.dynamicSmemBytes = room_for(ncols);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CB_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, nrows, nnz, pos, crd, groups_in(plan, nnz, ncols)));
+    return 0;
 }
 
 }  // namespace cb200
