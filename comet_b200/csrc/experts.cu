@@ -5,10 +5,15 @@
 //   combine   y_t = sum_e val_e v h_e                        dval_e = h_e (v' dy_t),  dh_e = val_e v' dy_t,  dv_j = sum_e val_e dy_t h_e'
 // act(g) = g s(u) with the logistic function s, u = g for silu and 2 sqrt(2 / pi) (g + 0.044715 g^3) for gelu (its tanh form).
 //
-// All of these are one kernel: tiles of 128 x 256 sums in tensor memory, 64 terms a step, with the operands' tiles in a ring of four in shared
-// memory.  Four warps fetch, a thread issues the products, four warps take the sums of the tile before out of tensor memory.  Weights, and what a kernel
-// before has left in the order of the slots (dz, val h), come by tensor copies; rows of x, h and dy by their number, 16 bytes a copy, so that nothing is
-// sorted first (a tensor copy of four numbered rows takes about 70 clocks whatever their width: gated_batch, 65536 entries, 1200 us with them).
+// All of these are one kernel: tiles of 128 x 256 sums in tensor memory, 64 terms a step, with the operands' tiles in a ring in shared memory.  One warp
+// fetches by tensor copies, four by row numbers, one issues the products, eight take the sums of the tile before out of tensor memory.  Weights, and what a
+// kernel before has left in the order of the slots (dz, val h), come by tensor copies; rows of x, h and dy by their number, 16 bytes a copy, so that
+// nothing is sorted first.  (A tensor copy of four numbered rows takes about 70 clocks whatever their width: 65536 entries of width 2048 by 64 experts of
+// inner 1024, the gated product, 1200 us with them, 438 without.)
+//
+// Bound: for that product, 550 GFLOP, 440 to 470 us when the chip is cool and 530 in a row of passes, where the power cap leaves 1.5 GHz (a library's plain product of the
+// same size: 370 and 430).  Tensor cores are busy 62 % of the clocks: a step of 64 terms is 512 clocks of theirs, and 768 of the shared memory's, which the
+// operands are written to and read from (48 KB each).  Where sums are short (dw: 7 steps a tile) or their results f32 (combine), the results' bytes.
 // Three forms:
 //   ROWS   rows of a tile's tokens, times a weight whose rows are outputs                (forward passes, dz)
 //   BACK   the same, times a weight whose rows are the sum's index                       (dx, v' dy)
@@ -607,7 +612,8 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
 // A single token: products of a weight's rows with its vectors, by the ordinary cores.  Neighbouring rows of an expert's weight are one piece of
 // memory, so a CTA's share comes in copies of up to 32 KB.  Six teams of four warps have a stage each: while one of them works on its stage, the others'
 // copies are under way, what an SM has to have in flight for the memory's full rate.  The vectors come through the L1 cache.
-// 8 experts of 64, in L2, us: 14.1 and 11.8 (gated, combine); by the tensor cores 17.5 and 13.3, and with two tokens 25 and 14 where this takes 32 and 18.
+// 8 experts of 64, in L2, us: 13.3 and 10.7 (gated, combine); by the tensor cores 17.5 and 13.3, and with two tokens 25 and 14 where this takes 32 and 18.
+// From memory: 20.0 and 14.0; the copies alone 14.4 and 9.5 (67 and 34 MB, and 4 us of start-up).
 static const int FEW_STAGES = 6, FEW_BYTES = 32 * 1024, FEW_SMEM = FEW_STAGES * FEW_BYTES, FEW_ENTRIES = 8, TEAM = 128, FEW_THREADS = FEW_STAGES * TEAM;
 
 // Of R rows in shared memory, `next` bytes apart, and B vectors: a lane's part of their products.  A vector is loaded once for all the rows.
@@ -817,8 +823,8 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
         });
 }
 
-// Narrow tiles where wide ones would leave most SMs without any (launch_shape's rule); at 64 wide tiles both take the same time, at
-// 144 wide ones 17 us and narrow ones 24.
+// Narrow tiles where wide ones would leave most SMs without any.  Gated products, us, wide and narrow: 64 wide tiles of 32 steps 21 and 20, 144 of 16 steps 17 and
+// 24.
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) * 4 < sm_count(); }
 
 template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
@@ -861,7 +867,7 @@ static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, Pr
     return 0;
 }
 
-// The shape that a product of `columns` columns takes: pairs for sums over an expert's tokens; narrow tiles where wide ones are fewer than SMs.
+// The shape that a product of `columns` columns takes: pairs for sums over an expert's tokens; else narrow tiles where wide ones are fewer than a quarter of the SMs.
 template <typename T, int FORM, int NUMBERED, int SUMS, typename Maps>
 static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, Maps maps)
 {

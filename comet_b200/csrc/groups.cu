@@ -4,7 +4,8 @@
 // are no atomics and the order is always the same), the counts are summed over the warps and, through the
 // cluster's shared memory, over the CTAs, and a second walk over the rows puts each entry where the sums say.
 //
-// Bound: the chains of loads of the two walks.
+// Bound: the chains of loads, votes and sums: 8192 rows of 8 among 64 columns 24 us (33 with a lane a row, whose loads of neighbouring entries are 64 bytes
+// apart), 777 rows 10 us, one row 5.
 #include <type_traits>
 
 #include "groups.cuh"

@@ -8,6 +8,9 @@
 //
 // Forward: one pass; each thread has a maximum and sums of its own (rows.cuh), joined over the CTA and, where there are few rows, over a cluster that
 // has cut the row.  Backward: one pass over pieces of rows, which no other CTA reads, so the gradient may take the place of the logits.
+//
+// Bound: HBM, and the exponential unit under the power cap: 4096 x 131072 bf16 with entropies 172 us alone, 190 in a row of passes (164 by the bytes; the unit is busy
+// 77 % of the time at 1.86 GHz).  The gradient 390 (328 by the bytes).
 #include "rows.cuh"
 
 namespace cb200 {

@@ -2,8 +2,9 @@
 torch CUDA tensors.  torch supplies device memory and streams only; every
 computation is done by the kernels of ``libcomet_b200``.
 
-Beside the sparse operations: the largest entries of rows of logits as a CSR matrix, and two losses of such a matrix beside
-logits (``top_entries``, ``distill_loss``, ``balance_loss``).
+Beside the sparse operations: the largest entries of rows of logits as a CSR matrix, two losses of such a matrix beside
+logits (``top_entries``, ``distill_loss``, ``balance_loss``), log probabilities at such a matrix (``log_probs``), and the products of a router's
+experts, whose choices are one (``group_entries``, ``gated_experts``, ``combine_experts``).
 
 Used by the benchmark (inputs already in HBM when the clock starts), by the
 multi-GPU sharding layer and by the device-level parity tests.

@@ -163,6 +163,8 @@ SHAPES = [
     # rows, experts, chosen, width, inner
     (1, 1, 1, 8, 8), (1, 8, 2, 64, 64), (1, 64, 8, 256, 128), (2, 3, 3, 72, 40), (5, 4, 1, 136, 264), (128, 1, 1, 64, 128), (129, 2, 1, 200, 136),
     (300, 5, 2, 256, 512), (777, 10, 3, 1000, 712), (1500, 64, 6, 128, 96), (4099, 7, 2, 64, 72), (64, 1000, 5, 72, 24),
+    # one token with many experts, and with rows too long for the kernels of one token
+    (1, 64, 20, 264, 136), (1, 1000, 300, 72, 40), (1, 3, 2, 8200, 40), (1, 2, 2, 64, 2056),
 ]
 
 
