@@ -1,11 +1,11 @@
-// Entries of a CSR matrix grouped by column: a stable counting sort in one launch, by a cluster of up to eight CTAs.
+// Entries of a CSR matrix grouped by column: a stable counting sort in one launch, by a cluster of up to sixteen CTAs.
 //
 // A warp has a stretch of rows and counts their entries by column (lanes with the same column find each other by votes on its bits, so there
 // are no atomics and the order is always the same), the counts are summed over the warps and, through the
 // cluster's shared memory, over the CTAs, and a second walk over the rows puts each entry where the sums say.
 //
-// Bound: the chains of loads, votes and sums: 8192 rows of 8 among 64 columns 24 us (33 with a lane a row, whose loads of neighbouring entries are 64 bytes
-// apart), 777 rows 10 us, one row 5.
+// Bound: instructions of the walks (votes, the search for a row), and the chains of loads and sums around them: 8192 rows of 8 among 64 columns 20 us, 777 rows 12, one row 5.
+#include <atomic>
 #include <type_traits>
 
 #include "groups.cuh"
@@ -36,11 +36,12 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     const int64_t to = min(from + each, nrows);
     const int bits = 32 - __clz(n - 1);            // of a column (a vote a bit: match.any takes some 200 clocks, 6 votes 40)
     // The entries of 32 rows after the other, a lane an entry, four loads on their way at a time; what(entry, its row, its column, the lanes that have the
-    // same one).  ROWS: the row is asked for, too; lane i knows where row r + i ends.
+    // same one, whether there is one) by all lanes.  ROWS: the row is asked for, too; lane i knows where row r + i ends.
     auto walk = [&](auto rows, auto what) {
         for (int64_t r = from; r < to; r += 32) {
             const int64_t end = min(max(pos[min(r + lane + 1, to)], (int64_t)0), nnz), begin = min(max(pos[r], (int64_t)0), nnz);
             const int64_t hi = __shfl_sync(0xffffffffu, end, 31);
+            const int ends_at = (int)(end - begin);
             for (int64_t e0 = begin; e0 < hi; e0 += 128) {
                 int64_t col[4];
 #pragma unroll
@@ -51,21 +52,23 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
                     if (e0 + 32 * i >= hi) break;
                     const int c = col[i] >= 0 && col[i] < n ? (int)col[i] : -1;
                     unsigned alike = __ballot_sync(0xffffffffu, c >= 0);
-                    for (int b = 0; b < bits; b++) {
-                        const unsigned set = __ballot_sync(0xffffffffu, c >> b & 1);
-                        alike &= c >> b & 1 ? set : ~set;
+#pragma unroll
+                    for (int b = 0; b < 10; b++) {
+                        if (b >= bits) break;
+                        const bool set = c & 1 << b;
+                        alike &= __ballot_sync(0xffffffffu, set) ^ (set ? 0u : ~0u);
                     }
                     int row = 0;                   // the first one that ends behind the entry
                     if (decltype(rows)::value)
 #pragma unroll
-                        for (int step = 16; step > 0; step /= 2) row += __shfl_sync(0xffffffffu, end, row + step - 1) <= e ? step : 0;
-                    if (e < hi) what(e, r + row, c, alike);
+                        for (int step = 16; step > 0; step /= 2) row += __shfl_sync(0xffffffffu, ends_at, row + step - 1) <= (int)(e - begin) ? step : 0;
+                    what(e, r + row, c, alike, e < hi);
                     __syncwarp();
                 }
             }
         }
     };
-    walk(std::false_type(), [&](int64_t, int64_t, int col, unsigned alike) {
+    walk(std::false_type(), [&](int64_t, int64_t, int col, unsigned alike, bool) {
         if (col >= 0 && lane == __ffs(alike) - 1) own[col] += __popc(alike);
     });
     __syncthreads();
@@ -142,20 +145,20 @@ group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const 
     int2 *sorted = (int2 *)(warps + (size_t)GW * n);
     unsigned short *of = (unsigned short *)(sorted + sortable);
     const bool staged = here <= sortable;
-    walk(std::true_type(), [&](int64_t e, int64_t row, int col, unsigned alike) {
-        if (col < 0) {
+    walk(std::true_type(), [&](int64_t e, int64_t row, int col, unsigned alike, bool on) {
+        const int at = col >= 0 ? own[col] + __popc(alike & ((1u << lane) - 1)) : 0;
+        __syncwarp();                              // all lanes at once: a wait for those alike would be one after the other
+        if (col >= 0) {
+            if (lane == 31 - __clz(alike)) own[col] = at + 1;
+            if (staged) {
+                sorted[at] = make_int2((int)e, (int)row);
+                of[at] = (unsigned short)col;
+            } else {
+                g.order[at] = (int)e;
+                g.token[at] = (int)row;
+            }
+        } else if (on) {
             g.order[g.slots - 1 - atomicAdd(&g.head[1], 1)] = (int)e;
-            return;
-        }
-        const int at = own[col] + __popc(alike & ((1u << lane) - 1));
-        __syncwarp(alike);
-        if (lane == 31 - __clz(alike)) own[col] = at + 1;
-        if (staged) {
-            sorted[at] = make_int2((int)e, (int)row);
-            of[at] = (unsigned short)col;
-        } else {
-            g.order[at] = (int)e;
-            g.token[at] = (int)row;
         }
     });
     if (staged) {
@@ -245,23 +248,39 @@ static int group_entries(int64_t nrows, int64_t ncols, int64_t nnz, const int64_
         CB_CUDA(launch_behind(group_few_kernel, dim3(1), FEW, 0, st, (int)nrows, (int)nnz, pos, crd, groups_in(plan, nnz, ncols)));
         return 0;
     }
-    int ranks = 1;                                 // a CTA has 1024 rows under way at a time
-    while (ranks < MOST_CLUSTER && nrows > (int64_t)ranks * GT) ranks *= 2;
+    static std::atomic<int> most_ranks[64];        // of a device: 16, if it has room for a cluster of so many, else what every device takes
+    int device = 0;
+    CB_CUDA(cudaGetDevice(&device));
     // the limit of shared memory is that of the largest call, in every call
     CB_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room_for(MOST_GROUPS)));
+    CB_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ranks;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ranks);
     cfg.blockDim = dim3(GT);
-    cfg.dynamicSmemBytes = room_for(ncols);
+    cfg.dynamicSmemBytes = room_for(MOST_GROUPS);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
+    int most = device < 64 ? most_ranks[device].load() : MOST_CLUSTER;
+    if (!most) {
+        cfg.gridDim = dim3(16);
+        attr[1].val.clusterDim.x = 16;
+        int clusters = 0;
+        most = cudaOccupancyMaxActiveClusters(&clusters, group_kernel, &cfg) == cudaSuccess && clusters > 0 ? 16 : MOST_CLUSTER;
+        cudaGetLastError();                        // a refusal is an answer
+        most_ranks[device].store(most);
+    }
+    // A share of 256 rows and more clusters pay, 8 entries a row, us: 777 rows 12 by four CTAs, 19 by one; 4096 rows 13 by 16, 22 by four; 8192 rows 20 by 16, 27 by
+    // eight.
+    int ranks = 1;
+    while (ranks < most && nrows > (int64_t)ranks * GT / 4) ranks *= 2;
+    cfg.gridDim = dim3((unsigned)ranks);
+    attr[1].val.clusterDim.x = ranks;
+    cfg.dynamicSmemBytes = room_for(ncols);
     CB_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, nrows, nnz, pos, crd, groups_in(plan, nnz, ncols)));
     return 0;
 }

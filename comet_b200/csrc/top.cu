@@ -507,17 +507,18 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
     // by column, ascending: the complement of the column, descending
     if (n <= TT) {
         u64 it = tid < n ? sh.cand[tid] : 0;
-        if (n > k) {
+        if (n > k) {                               // those with fewer than k above them, to that place
             int above = 0;
-            for (int i = 0; i < n; i++) above += sh.cand[i] > it;
+            if ((tid & ~31) < n)
+                for (int i = 0; i < n; i++) above += sh.cand[i] > it;
             __syncthreads();
-            if (above >= k) it = 0;
-            if (tid < n) sh.cand[tid] = it;
+            if (it && above < k) sh.cand[above] = it;
             __syncthreads();
+            it = tid < k ? sh.cand[tid] : 0;
         }
         if (it) {
             int at = 0;
-            for (int i = 0; i < n; i++) at += (sh.cand[i] & low) > (it & low);
+            for (int i = 0; i < min(n, k); i++) at += (sh.cand[i] & low) > (it & low);
             crd[t * k + at] = (int64_t)(low - (it & low));
             val[t * k + at] = value((uint32_t)(it >> colbits));
         }
