@@ -461,3 +461,35 @@ def test_refusals():
     G.plan[2] = 1                                                          # what a kernel leaves that gave up waiting
     with pytest.raises(_lib.CometB200Error, match="wait"):
         G.check()
+
+
+@pytest.mark.parametrize("width,inner", [(64, 1024), (1024, 64)])
+def test_offsets_beyond_32_bits(width, inner):
+    """2.4 million entries: more than 2^31 elements of H, of dz and of the rows that are summed.  The last tokens are what they are alone."""
+    import torch
+    from comet_b200 import device
+    rows, experts, chosen, last = 300000, 8, 8, 200
+    g = torch.Generator("cuda")
+    g.manual_seed(3)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda").bfloat16()           # noqa: E731
+    pos = torch.arange(rows + 1, device="cuda") * chosen
+    crd = torch.arange(experts, device="cuda").repeat(rows)
+    val = torch.rand(rows * chosen, generator=g, device="cuda")
+    X, W, V = normal(rows, width), normal(experts, 2 * inner, width) * width ** -0.5, normal(experts, width, inner) * inner ** -0.5
+    S = device.DeviceCSR(rows, experts, pos, crd, val)
+    G = device.group_entries(S)
+    H = device.gated_experts(G, X, W)
+    assert H.numel() * (1 if inner > width else width // inner) > 2 ** 31
+    Y = device.combine_experts(G, H, V)
+    dH, _, dval = device.combine_experts_grad(G, H, V, X, grad_v=False)
+    dX, _ = device.gated_experts_grad(G, X, W, H, grad_w=False)
+    torch.cuda.synchronize()
+    G.check()
+    few = slice(-last * chosen, None)
+    g2 = device.group_entries(device.DeviceCSR(last, experts, pos[:last + 1], crd[few], val[few]))
+    x, h = X[-last:].contiguous(), H[few].contiguous()
+    assert torch.equal(device.gated_experts(g2, x, W), h)
+    assert torch.equal(device.combine_experts(g2, h, V), Y[-last:])
+    dh, _, dv = device.combine_experts_grad(g2, h, V, x, grad_v=False)
+    assert torch.equal(dh, dH[few]) and float((dv - dval[few]).abs().max()) <= 1e-5 * float(dv.abs().max())
+    assert torch.equal(device.gated_experts_grad(g2, x, W, h, grad_w=False)[0], dX[-last:])

@@ -87,6 +87,10 @@ def within(got, want, off):
 def rounded(got, want, off):
     import torch
     info = torch.finfo(got.dtype)
+    # What rounds beyond the type's largest number, max (1 + eps / 4) being half a step above it, is infinite.
+    over = want.abs() - off > info.max * (1 + info.eps / 4)
+    assert torch.equal(got[over].double(), torch.sign(want[over]) * math.inf)
+    got, want, off = got[~over], want[~over], off[~over]
     # f32 results below the least normal number are 0
     least = info.smallest_normal * (1 if got.dtype == torch.float32 else info.eps / 2)
     within(got, want, off + (want.abs() + off) * info.eps / 2 + least)
@@ -315,3 +319,45 @@ def test_refusals():
             device.log_probs(S, x, temperature=tau)
         with pytest.raises(RuntimeError, match="temperature"):
             device.log_probs_grad(S, x, sums, d, temperature=tau)
+
+
+@pytest.mark.parametrize("kind,cols", [("bf16", 131072), ("f32", 1201)])
+def test_offsets_beyond_32_bits(kind, cols):
+    """More than 2^31 logits: the last rows are what they are alone, the gradient in the logits' place too."""
+    import torch
+    from comet_b200 import device
+    rows, last = (1 << 31) // cols + 100, 50
+    x = torch.empty((rows, cols), dtype=torch_type(kind), device="cuda")
+    x[-2 * last:] = torch.randn((2 * last, cols), device="cuda").to(x.dtype)
+    x[:-2 * last] = 0
+    S = device.DeviceCSR(rows, cols, torch.arange(rows + 1, device="cuda"), torch.arange(rows, device="cuda") % cols, None)
+    part = device.DeviceCSR(last, cols, torch.arange(last + 1, device="cuda"), S.crd[-last:].clone(), None)
+    d, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    own = x[-last:].clone()
+    want = device.log_probs(part, own, entropy=True, top=3)
+    for top in (0, 3):
+        values, sums, entropy, best = device.log_probs(S, x, entropy=True, top=top)
+        # alone the rows may be cut into parts: the same but for the order of sums
+        assert float((values[-last:] - want[0]).abs().max()) < 1e-5 and float((entropy[-last:] - want[2]).abs().max()) < 1e-5
+        assert float((sums[-last:] - want[1]).abs().max()) < 1e-5
+        if top:
+            assert torch.equal(best.crd[-3 * last:], want[3].crd) and float((best.val[-3 * last:] - want[3].val).abs().max()) < 1e-5
+    want = device.log_probs_grad(part, own, sums[-last:].clone(), d[-last:].clone(), entropy=entropy[-last:].clone(), d_entropy=h[-last:].clone())
+    device.log_probs_grad(S, x, sums, d, entropy=entropy, d_entropy=h, grad=x)
+    assert torch.equal(x[-last:], want)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_products_beyond_what_is_exact(kind):
+    """Logits over the temperature beyond 2^22: differences to the largest one are taken first."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(8)
+    x = logits(rng, 5, 4500, kind, spread=1.0) + 300
+    x[1:3] += 1000
+    x[2, 7] = 2000
+    S, row = given(rng, 5, 4500, 4, ragged=False)
+    for tau in (1e-5, 3e-4):
+        o, sums, entropy = check(S, row, x, tau, 4)
+        d, h = torch.randn(S.nnz, device="cuda"), torch.randn(5, device="cuda")
+        rounded(device.log_probs_grad(S, x, sums, d, entropy=entropy, d_entropy=h, temperature=tau), *o.grad(S, row, d, h))
