@@ -463,27 +463,53 @@ top_kernel(int64_t nrows, int ncols, int slice, const T *__restrict__ xs, int64_
         cluster_arrive();
         cluster_wait();
         if (rank == 0) {
-            const int most = max(k, ROOM / MOST_CLUSTER);        // candidates of a CTA
-            for (unsigned r = 1; r < ranks; r++) {
-                const int n = peer_load(&sh.count, r), have = sh.count;
-                for (int i = tid; i < n; i += TT) sh.cand[have + i] = peer_load(&sh.cand[i], r);
+            // what the others have, all at once: lane r of each warp asks CTA r, and warp r copies its candidates
+            static_assert(TW >= MOST_CLUSTER, "a warp for each CTA");
+            const int lane = tid & 31, from = tid >> 5;
+            const bool other = lane > 0 && lane < (int)ranks;
+            const int theirs = other ? peer_load(&sh.count, lane) : 0, have = sh.count;
+            float om = MINUS_INF, os = 0.0f, oe = 0.0f;
+            if (SUM && other) {
+                om = peer_load(&sh.m, lane);
+                os = peer_load(&sh.s, lane);
+                if (PROB) oe = peer_load(&sh.e, lane);
+            }
+            int upto = theirs;
+#pragma unroll
+            for (int o = 1; o < MOST_CLUSTER; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int all = have + __shfl_sync(0xffffffffu, upto, MOST_CLUSTER - 1);
+            if (all <= ROOM) {
+                const int n = __shfl_sync(0xffffffffu, theirs, from), at = have + __shfl_sync(0xffffffffu, upto, from) - n;
+                for (int i = lane; i < n; i += 32) sh.cand[at + i] = peer_load(&sh.cand[i], from);
                 __syncthreads();
-                if (tid == 0) sh.count = have + n;
+                if (tid == 0) sh.count = all;
                 __syncthreads();
-                if (sh.count > ROOM - most) keep_largest(sh, sh.count, k);
-                if (PROB) {
-                    const float om = peer_load(&sh.m, r), nm = max_nan(m, om);
-                    float os = peer_load(&sh.s, r), oe = peer_load(&sh.e, r);
-                    shift_to(nm, m, c, s, ent);
-                    shift_to(nm, om, c, os, oe);
-                    m = nm;
-                    s += os;
-                    ent += oe;
-                } else if (SUM) {
-                    const float om = peer_load(&sh.m, r), os = peer_load(&sh.s, r), nm = max_nan(m, om);
-                    s = (m == MINUS_INF ? 0.0f : s * exp2_fast((m - nm) * c)) + (om == MINUS_INF ? 0.0f : os * exp2_fast((om - nm) * c));
-                    m = nm;
+            } else {
+                const int most = max(k, ROOM / MOST_CLUSTER);    // candidates of a CTA
+                for (unsigned r = 1; r < ranks; r++) {
+                    const int n = peer_load(&sh.count, r), have = sh.count;
+                    for (int i = tid; i < n; i += TT) sh.cand[have + i] = peer_load(&sh.cand[i], r);
+                    __syncthreads();
+                    if (tid == 0) sh.count = have + n;
+                    __syncthreads();
+                    if (sh.count > ROOM - most) keep_largest(sh, sh.count, k);
                 }
+            }
+            for (unsigned r = 1; SUM && r < ranks; r++) {
+                const float rm = __shfl_sync(0xffffffffu, om, r), nm = max_nan(m, rm);
+                float rs = __shfl_sync(0xffffffffu, os, r), re = __shfl_sync(0xffffffffu, oe, r);
+                if (PROB) {
+                    shift_to(nm, m, c, s, ent);
+                    shift_to(nm, rm, c, rs, re);
+                    s += rs;
+                    ent += re;
+                } else {
+                    s = (m == MINUS_INF ? 0.0f : s * exp2_fast((m - nm) * c)) + (rm == MINUS_INF ? 0.0f : rs * exp2_fast((rm - nm) * c));
+                }
+                m = nm;
             }
         }
         __syncwarp();
