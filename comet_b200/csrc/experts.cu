@@ -105,6 +105,7 @@ struct ProductArgs {
 
 struct Tile {
     int m, n, group, steps, slot;    // slot: the first one
+    int half;                        // 0: all of the tile's columns, 1 or 2: the first or the second half of them
 };
 
 __device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + exp2_fast(-LOG2E * u)); }
@@ -381,9 +382,17 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     wait_for_previous();
 
     const int mine = blockIdx.x / CTAS, all = gridDim.x / CTAS;
-    const int tiles = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
+    // Tiles of a last round that would leave half of the CTAs idle are cut into two (v'dy of combine_grad_step, 3.3 rounds: 86 us, 90 with whole ones; dx of gated_grad_step 110, 114).
+    constexpr bool HALVES = W == WIDE && (SUMS == ENTRY_ROWS || SUMS == COMBINE_GRAD);
+    const int entire = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
+    const int whole = HALVES && entire % all * 2 <= all ? entire / all * all : entire, tiles = whole + 2 * (entire - whole);
     auto tile_of = [&](int id) {
         Tile t;
+        t.half = 0;
+        if (HALVES && id >= whole) {
+            t.half = 1 + (id - whole) % 2;
+            id = whole + (id - whole) / 2;
+        }
         if (FORM == OUTER) {
             t.group = id / (a.tiles_m * a.tiles_n);
             const int rest = id % (a.tiles_m * a.tiles_n);
@@ -419,8 +428,17 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
                 if (!on) break;
                 if (elect()) {
-                    bar_expect(bar, TENSOR_BYTES);
-                    if (FORM == ROWS) {
+                    bar_expect(bar, TENSOR_BYTES - (HALVES && t.half ? B_BYTES / 2 : 0));
+                    if (HALVES && t.half) {
+                        const int n = n0 + (t.half - 1) * (W / 2);
+                        if (FORM == ROWS) {
+                            load_box(to + A_BYTES, &map_b, k * TK, n, t.group, bar);
+                        } else {
+                            if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
+#pragma unroll
+                            for (int i = 0; i < BLOCKS / 2; i++) load_box(to + A_BYTES + i * 8192, &map_b, n + i * 64, k * TK, t.group, bar);
+                        }
+                    } else if (FORM == ROWS) {
                         // an expert's gate rows, and as many up rows; or rows of the one weight
                         constexpr bool GATES = SUMS != ENTRY_ROWS;
                         load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
@@ -499,6 +517,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         bool on = true;
         int after = mine < tiles ? tile_of(mine).steps : 0;
         for (int id = mine; on && id < tiles; id += all) {
+            const bool half = HALVES && id >= whole;
             const int steps = (int)__reduce_max_sync(0xffffffffu, (unsigned)after);  // the same in all, which the compiler does not know
             if (id + all < tiles) after = tile_of(id + all).steps;
             if (steps == 0) continue;
@@ -525,7 +544,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
                 // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
                 constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
-                constexpr uint32_t kind = product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
+                const uint32_t kind = half ? product_descriptor(BF16, CTAS * TM, W / 2, FORM == OUTER, FORM != ROWS)
+                                           : product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
                 if (elect()) {
 #pragma unroll
                     for (int i = 0; i < TK / 16; i++) product<PAIR>(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
@@ -555,7 +575,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (!__all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken))) break;
                 tmem_fence_after();
             }
-            take_sums<T, W, SUMS>(a, tmem + b * W + ((uint32_t)(warp & 3) << 21), t.steps == 0, t, warp >> 2, row, entry, room);
+            const uint32_t at = tmem + b * W + ((uint32_t)(warp & 3) << 21);
+            if (!HALVES || !t.half) take_sums<T, W, SUMS>(a, at, t.steps == 0, t, warp >> 2, row, entry, room);
+            else if (warp < 4) take_sums<T, W, SUMS>(a, at - (t.half - 1) * (W / 2), false, t, t.half - 1, row, entry, room);
             if (t.steps > 0) {
                 tmem_fence_before();
                 __syncwarp();

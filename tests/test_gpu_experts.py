@@ -493,3 +493,10 @@ def test_offsets_beyond_32_bits(width, inner):
     dh, _, dv = device.combine_experts_grad(g2, h, V, x, grad_v=False)
     assert torch.equal(dh, dH[few]) and float((dv - dval[few]).abs().max()) <= 1e-5 * float(dv.abs().max())
     assert torch.equal(device.gated_experts_grad(g2, x, W, h, grad_w=False)[0], dX[-last:])
+
+
+@pytest.mark.parametrize("rows,experts,width,inner", [(128 * 74, 1, 264, 264), (128 * 149, 1, 256, 200), (128 * 100, 2, 1032, 520), (128 * 30 + 1, 1, 2568, 1288)])
+def test_last_rounds(rows, experts, width, inner):
+    """Numbers of tiles around the number of SMs: rounds that end with few tiles, whose columns are halved."""
+    rng = np.random.default_rng(width)
+    run_block(rng, rows, experts, np.full(rows, 1), width, inner, "silu", "bf16")
