@@ -22,7 +22,7 @@ static size_t room_for(int64_t ngroups) { return (size_t)ngroups * GW * sizeof(i
 __global__ void __launch_bounds__(GT)
 group_kernel(int64_t nrows, int64_t nnz, const int64_t *__restrict__ pos, const int64_t *__restrict__ crd, const Groups g)
 {
-    extern __shared__ int warps[];                 // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
+    extern __shared__ __align__(16) int warps[];   // [GW][ngroups]: a warp's entries of a column, then the slot of its next one
     __shared__ int mine[MOST_GROUPS], start[MOST_GROUPS], whole[MOST_GROUPS], ends[MOST_GROUPS], local[MOST_GROUPS], sums[GW + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.ngroups;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
