@@ -190,7 +190,8 @@ _numbers = {}
 
 
 def _floats(*v):
-    """The address of host doubles, and what keeps them alive (the calls take integers and addresses)."""
+    """The address of host doubles, and what keeps them alive, which a caller holds until its call has returned: another thread may clear the
+    dictionary meanwhile (the calls take integers and addresses, and read without the interpreter's lock)."""
     got = _numbers.get(v)
     if got is None:
         if len(_numbers) >= 256:
@@ -333,7 +334,8 @@ def log_probs(S, X, temperature=1.0, entropy=False, top=0):
     if top:
         best = DeviceCSR(n, m, new(n + 1, dtype=torch.int64), new(n * top, dtype=torch.int64), new(n * top, dtype=f32))
         at = best.pos.data_ptr(), best.crd.data_ptr(), best.val.data_ptr()
-    _call(_PROBS[X.dtype], n, m, pos, crd, X.data_ptr(), ld, _floats(float(temperature))[0], values.data_ptr(), sums.data_ptr(), _p(ent), top, *at, _stream())
+    options = _floats(float(temperature))
+    _call(_PROBS[X.dtype], n, m, pos, crd, X.data_ptr(), ld, options[0], values.data_ptr(), sums.data_ptr(), _p(ent), top, *at, _stream())
     return values, sums, ent, best
 
 
@@ -356,7 +358,8 @@ def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperatu
     if grad is None or grad is False:
         raise ValueError("log_probs_grad: grad is True, or a tensor to write to")
     out, to, ldg = _gradient("log_probs_grad", X, shape[:2], grad)
-    _call(_PROBS_GRAD[X.dtype], n, m, pos, crd, X.data_ptr(), ld, _floats(float(temperature))[0], kept, d_val, ent, d_ent, to, ldg, _stream())
+    options = _floats(float(temperature))
+    _call(_PROBS_GRAD[X.dtype], n, m, pos, crd, X.data_ptr(), ld, options[0], kept, d_val, ent, d_ent, to, ldg, _stream())
     return out
 
 
