@@ -673,6 +673,14 @@ __device__ __forceinline__ void dots(const unsigned char *row, unsigned next, co
 }
 
 __device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory"); }
+// whether all threads of the team say so; a barrier of the team, too
+__device__ __forceinline__ bool team_all(int team, bool v)
+{
+    unsigned all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((unsigned)v), "r"(team + 1), "n"(TEAM) : "memory");
+    return all != 0;
+}
 
 // What both kernels do: steps, which the teams take in turn.  issue(step, stage's address, barrier) copies a step's rows, by one thread; prepare(step) looks up
 // what else they are worked on with, while they are under way; take(stage) works on them.
@@ -696,15 +704,18 @@ __device__ __forceinline__ void few_steps(int steps, unsigned char *ring, int *h
     unsigned parity = 0;
     for (int step = team; step < steps; step += FEW_STAGES, parity ^= 1) {
         prepare(step);
-        if (!bar_wait(bar, parity, broken)) break;
+        // A wait that runs out does so for the whole team: threads that went on alone would wait for the others at its next barrier.
+        if (!team_all(team, bar_wait(bar, parity, broken))) {
+            if (first) {                           // what is under way lands first
+                volatile int late = 0;
+                bar_wait(bar, parity, &late);
+                head[2] = 1;
+            }
+            return;
+        }
         take(stage);
         team_sync(team);
         if (first && step + FEW_STAGES < steps) issue(step + FEW_STAGES, smem_at(stage), bar);
-    }
-    if (*broken && first) {                        // gave up: what is under way lands first
-        volatile int late = 0;
-        bar_wait(bar, parity, &late);
-        head[2] = 1;
     }
 }
 
