@@ -68,12 +68,9 @@ enum Sums { GATED, GATED_GRAD, ENTRY_ROWS, COMBINE_GRAD, WEIGHT };
 static const int TM = 128, WIDE = 256, NARROW = 64, TK = 64;
 static const int A_BYTES = TM * TK * 2;
 static const int TAKERS = 256, FETCHERS = 128, PRODUCT_THREADS = TAKERS + FETCHERS + 64;
-// PAIR: two CTAs of a cluster share a product of 256 x 256, with 128 rows of either operand each: two thirds of the bytes that two tiles of their own
-// take from the L2.  The sums over an expert's tokens go that way (dw of gated_grad_step 129 us, 139 by single CTAs; dv of combine_grad_step 76, 78).  Products
-// of tokens' rows do not: where an expert has an odd number of tiles one of a pair is empty (dz 145 against 135, dx 116, 114; gated_batch 483, 470).
-template <int W, bool PAIR>
+template <int W>
 struct Shape {
-    static constexpr int B_ROWS = PAIR ? W / 2 : W, B_BYTES = B_ROWS * TK * 2, STEP = A_BYTES + B_BYTES, RING = PAIR ? 6 : 4;
+    static constexpr int B_BYTES = W * TK * 2, STEP = A_BYTES + B_BYTES, RING = 4;
     static constexpr int TAKEN = W == WIDE ? 128 : 32;         // bytes of a row that a warp takes out at a time
     static constexpr int SMEM = RING * STEP + TAKERS * TAKEN + 1024;
 };
@@ -193,7 +190,7 @@ struct Stage {
 template <typename T, int W, int SUMS>
 __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, bool none, const Tile &t, int half, int row, int64_t entry, unsigned char *room)
 {
-    constexpr int BYTES = Shape<W, false>::TAKEN;
+    constexpr int BYTES = Shape<W>::TAKEN;
     const Stage<T, BYTES> st = {room, (int)threadIdx.x & 31};
     if constexpr (SUMS == GATED || SUMS == GATED_GRAD) {
         constexpr int MINE = W / 4, PART = MINE < 32 ? MINE : 32;                    // columns of the warp, at a time
@@ -337,35 +334,32 @@ __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 // NUMBERED: the operand whose rows come by their number: A (the tile's rows), B (its columns, OUTER), or none
 enum Numbered { NUMBERED_A, NUMBERED_B, NUMBERED_NONE };
 
-template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
+template <typename T, int W, int FORM, int NUMBERED, int SUMS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, W == WIDE ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
 {
     constexpr bool BF16 = !__is_same(T, __half);
-    typedef Shape<W, PAIR> S;
-    constexpr int B_BYTES = S::B_BYTES, STEP_BYTES = S::STEP, RING = S::RING, CTAS = PAIR ? 2 : 1;
+    typedef Shape<W> S;
+    constexpr int B_BYTES = S::B_BYTES, STEP_BYTES = S::STEP, RING = S::RING;
     constexpr unsigned TENSOR_BYTES = (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + (NUMBERED == NUMBERED_B ? 0 : B_BYTES);
-    static_assert(!PAIR || FORM == OUTER, "tiles of tokens have no pairs");
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[3 * RING + 4 + 1];
+    __shared__ __align__(8) uint64_t bars[2 * RING + 4 + 1];
     __shared__ uint32_t tmem_room;
     __shared__ int broken_word;
     volatile int *broken = &broken_word;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int ISSUER = (TAKERS + FETCHERS) / 32, BOXES = ISSUER + 1;
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
-                   last = taken + 16, ready = last + 8;
-    const int rank = PAIR ? (int)cluster_rank() : 0;
-    if (warp == ISSUER) tmem_alloc<PAIR>(smem_at(&tmem_room), 2 * W);
+                   last = taken + 16;
+    if (warp == ISSUER) tmem_alloc(smem_at(&tmem_room), 2 * W);
     if (tid == 0) {
         for (int i = 0; i < RING; i++) {
             bar_init(full + 8 * i, NUMBERED == NUMBERED_NONE ? 1 : 1 + FETCHERS);
             bar_init(empty + 8 * i, 1);
-            bar_init(ready + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
             bar_init(done + 8 * i, 1);
-            bar_init(taken + 8 * i, CTAS * TAKERS / 32);
+            bar_init(taken + 8 * i, TAKERS / 32);
         }
         bar_init(last, 1);
         broken_word = 0;
@@ -373,15 +367,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     tmem_fence_before();
     __syncthreads();
-    if (PAIR) {                                    // the other one's barriers are there
-        cluster_arrive();
-        cluster_wait();
-    }
     tmem_fence_after();
     const uint32_t tmem = tmem_room;
     wait_for_previous();
 
-    const int mine = blockIdx.x / CTAS, all = gridDim.x / CTAS;
+    const int mine = blockIdx.x, all = gridDim.x;
     // Tiles of a last round that would leave half of the CTAs idle are cut into two (v'dy of combine_grad_step, 3.3 rounds: 86 us, 90 with whole ones; dx of gated_grad_step 110, 114).
     constexpr bool HALVES = W == WIDE && (SUMS == ENTRY_ROWS || SUMS == COMBINE_GRAD);
     const int entire = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
@@ -396,7 +386,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (FORM == OUTER) {
             t.group = id / (a.tiles_m * a.tiles_n);
             const int rest = id % (a.tiles_m * a.tiles_n);
-            t.m = rest / a.tiles_n * CTAS + rank;
+            t.m = rest / a.tiles_n;
             t.n = rest % a.tiles_n;
             t.steps = (a.g.counts[t.group] + TK - 1) / TK;
             t.slot = a.g.first[t.group] * GROUP_TILE;
@@ -420,8 +410,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         bool on = true;
         for (int id = mine; on && id < tiles; id += all) {
             const Tile t = tile_of(id);
-            constexpr int BLOCKS = S::B_ROWS / 64;
-            const int n0 = t.n * W + (PAIR ? rank * (W / 2) : 0);                    // of the operand's rows, this CTA's first
+            constexpr int BLOCKS = W / 64;
+            const int n0 = t.n * W;
             for (int k = 0; k < t.steps; k++, step++) {
                 const unsigned s = step % RING;
                 const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
@@ -493,9 +483,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
                 } else {
-                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : S::B_ROWS / 64;
+                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : W / 64;
                     const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
-                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W + (PAIR ? rank * (W / 2) : 0);
+                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const char *src = base + max(next[i], 0) * stride;
@@ -522,43 +512,33 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (id + all < tiles) after = tile_of(id + all).steps;
             if (steps == 0) continue;
             const unsigned b = tile & 1;
-            if (rank == 0) {
-                on = __all_sync(0xffffffffu, bar_wait<PAIR>(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
-                tmem_fence_after();
-            }
+            on = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
+            tmem_fence_after();
             for (int k = 0; on && k < steps; k++, step++) {
                 const unsigned s = step % RING;
                 on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
                 if (!on) break;
                 if (NUMBERED != NUMBERED_NONE) shared_to_products();
-                if (PAIR && rank == 1) {           // tells the first CTA what has landed here
-                    if (elect()) bar_arrive_first(ready + 8 * s);
-                    continue;
-                }
-                if (PAIR) {
-                    on = __all_sync(0xffffffffu, bar_wait<true>(ready + 8 * s, step / RING & 1, broken));
-                    if (!on) break;
-                }
                 tmem_fence_after();
                 const uint32_t at = ring + s * STEP_BYTES;
                 const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
                 // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
                 constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
-                const uint32_t kind = half ? product_descriptor(BF16, CTAS * TM, W / 2, FORM == OUTER, FORM != ROWS)
-                                           : product_descriptor(BF16, CTAS * TM, W, FORM == OUTER, FORM != ROWS);
+                const uint32_t kind = half ? product_descriptor(BF16, TM, W / 2, FORM == OUTER, FORM != ROWS)
+                                           : product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
                 if (elect()) {
 #pragma unroll
-                    for (int i = 0; i < TK / 16; i++) product<PAIR>(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
-                    products_to<PAIR>(empty + 8 * s);
-                    if (k + 1 == steps) products_to<PAIR>(done + 8 * b);
+                    for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
+                    products_to(empty + 8 * s);
+                    if (k + 1 == steps) products_to(done + 8 * b);
                 }
                 __syncwarp();
             }
             tile++;
         }
-        if (*broken && rank == 0) {                // products under way end before tensor memory is given back
+        if (*broken) {                             // products under way end before tensor memory is given back
             volatile int late = 0;
-            if (elect()) products_to<PAIR>(last);
+            if (elect()) products_to(last);
             bar_wait(last, 0, &late);
         }
         __syncwarp();
@@ -581,22 +561,15 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (t.steps > 0) {
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    if (PAIR) bar_arrive_first(taken + 8 * b);
-                    else bar_arrive(taken + 8 * b);
-                }
+                if (lane == 0) bar_arrive(taken + 8 * b);
                 tile++;
             }
         }
     }
     tmem_fence_before();
     __syncthreads();
-    if (PAIR) {                                    // nothing of this CTA is used by the other one any more
-        cluster_arrive();
-        cluster_wait();
-    }
     tmem_fence_after();
-    if (warp == ISSUER) tmem_free<PAIR>(tmem, 2 * W);
+    if (warp == ISSUER) tmem_free(tmem, 2 * W);
     if (tid == 0 && *broken) a.g.head[2] = 1;
 }
 
@@ -860,47 +833,22 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
 // 24.
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) * 4 < sm_count(); }
 
-template <typename T, int W, bool PAIR, int FORM, int NUMBERED, int SUMS>
+template <typename T, int W, int FORM, int NUMBERED, int SUMS>
 static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, ProductArgs a, int64_t columns, cudaStream_t st)
 {
-    typedef Shape<W, PAIR> S;
-    auto kernel = product_kernel<T, W, PAIR, FORM, NUMBERED, SUMS>;
+    typedef Shape<W> S;
+    auto kernel = product_kernel<T, W, FORM, NUMBERED, SUMS>;
     CB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     a.tiles_n = (int)ceil_div(columns, W);
-    if (FORM == OUTER) a.tiles_m = (int)ceil_div(a.rows, PAIR ? 2 * TM : TM);
+    if (FORM == OUTER) a.tiles_m = (int)ceil_div(a.rows, TM);
     const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
     if (tiles > 0x3fffffffLL) return fail("experts: more than 2^30 tiles");
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = PAIR ? 2 : 1;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(PRODUCT_THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 2 : 1;
-    int64_t most = sm_count() * (W == WIDE ? 1 : 2);           // CTAs that run at the same time: each goes from tile to tile
-    if (PAIR) {
-        static std::atomic<int> fit{0};
-        int n = fit.load();
-        if (!n) {
-            cfg.gridDim = dim3((unsigned)(most / 2 * 2));
-            CB_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-            if (n < 1) return fail("experts: no room for a pair of CTAs");
-            fit.store(n);
-        }
-        most = 2 * (n < most / 2 ? n : most / 2);
-    }
-    const int64_t ctas = PAIR ? 2 * tiles : tiles;
-    cfg.gridDim = dim3((unsigned)(ctas < most ? ctas : most));
-    CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, a));
+    const int64_t most = sm_count() * (W == WIDE ? 1 : 2);     // CTAs that run at the same time: each goes from tile to tile
+    CB_CUDA(launch_behind(kernel, dim3((unsigned)(tiles < most ? tiles : most)), PRODUCT_THREADS, S::SMEM, st, map_a, map_b, a));
     return 0;
 }
 
-// The shape that a product of `columns` columns takes: pairs for sums over an expert's tokens; else narrow tiles where wide ones are fewer than a quarter of the SMs.
+// The shape that a product of `columns` columns takes: wide tiles for sums over an expert's tokens; else narrow ones where wide ones are fewer than a quarter of the SMs.
 template <typename T, int FORM, int NUMBERED, int SUMS, typename Maps>
 static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, Maps maps)
 {
@@ -909,14 +857,14 @@ static int launch_shape(const ProductArgs &a, int64_t columns, cudaStream_t st, 
     memset(&mb, 0, sizeof(mb));
     if constexpr (FORM == OUTER) {
         CB_TRY(maps(ma, mb, WIDE));
-        return launch_product<T, WIDE, true, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+        return launch_product<T, WIDE, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
     } else {
         if (narrow(a.g, a.nnz, columns)) {
             CB_TRY(maps(ma, mb, NARROW));
-            return launch_product<T, NARROW, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+            return launch_product<T, NARROW, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
         }
         CB_TRY(maps(ma, mb, WIDE));
-        return launch_product<T, WIDE, false, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
+        return launch_product<T, WIDE, FORM, NUMBERED, SUMS>(ma, mb, a, columns, st);
     }
 }
 

@@ -1,6 +1,5 @@
 // The fifth-generation tensor cores: tensor copies into shared memory, the matrix instruction with its accumulators in tensor memory,
-// and bounded waits for both.  PAIR: products of two CTAs of a cluster (cta_group::2), which have half of the rows of both operands each; the first one
-// issues them.
+// and bounded waits for both.
 #pragma once
 #include <cuda.h>
 
@@ -31,29 +30,14 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity)
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// what the other CTA of the cluster has written before it arrived is seen too
-__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, unsigned parity)
-{
-    unsigned ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-// Arrives at the same barrier of the cluster's first CTA.  What it tells is that copies into this CTA's shared memory have landed, which the thread has seen; a
-// release for the whole cluster waits for every access under way, 1000 clocks a step.
-__device__ __forceinline__ void bar_arrive_first(uint32_t bar)
-{
-    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar) : "memory");
-}
 // Waits for a phase; false after two seconds, or once another wait of the CTA has run out (*broken).
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int *broken)
 {
     unsigned long long began = 0;
     for (;;) {
         // unrolled by the compiler: a loop of one look at a time let the products of gated_batch wait 2 % longer
         for (int i = 0; i < 64; i++)
-            if (CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity)) return true;
+            if (bar_try(bar, parity)) return true;
         if (*broken) return false;
         unsigned long long now;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
@@ -95,23 +79,15 @@ __device__ __forceinline__ void copies_to(uint32_t bar)
 // what threads have written to shared memory, and this thread knows of, is seen by products issued from here on
 __device__ __forceinline__ void shared_to_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// by a warp; of a pair, by a warp of each CTA
-template <bool PAIR>
+// by a warp
 __device__ __forceinline__ void tmem_alloc(uint32_t at, unsigned columns)
 {
-    if (PAIR) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t tmem, unsigned columns)
 {
-    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -128,24 +104,15 @@ constexpr uint32_t product_descriptor(bool bf16, int m, int n, bool rows_a, bool
     return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (rows_a ? 1u : 0u) << 15 | (rows_b ? 1u : 0u) << 16 | (uint32_t)(n / 8) << 17 |
            (uint32_t)(m / 16) << 24;
 }
-template <bool PAIR>
 __device__ __forceinline__ void product(uint32_t tmem, uint64_t a, uint64_t b, uint32_t kind, bool add)
 {
-    if (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(tmem), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(tmem), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
 }
-// the barrier's phase ends when the products issued so far are done; of a pair, in both CTAs
-template <bool PAIR>
+// the barrier's phase ends when the products issued so far are done
 __device__ __forceinline__ void products_to(uint32_t bar)
 {
-    if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 16 or 32 columns of the warp's 32 rows, a row a thread.  The wait is part of it: only so does the compiler know that nothing may use the values before.
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16])

@@ -27,3 +27,10 @@ def test_a_team_leaves_together(tmp_path, thread, step, both):
     """Threads that go on alone would wait for ever for those that have left."""
     text = source("experts.cu")
     run(tmp_path, "few_steps_check.cpp", constant("FEW_STAGES", text) + without_asm(function("few_steps", text)), thread, step, both)
+
+
+@pytest.mark.parametrize("name", ["tensor.cuh", "experts.cu", "logits.cuh", "rows.cuh", "groups.cu"])
+def test_arrivals_at_another_cta_order_what_it_reads(name):
+    """An mbarrier's arrival is a release for the CTA alone unless it says more: what another CTA of the cluster reads after it is not ordered by that."""
+    for arrival in re.findall(r"mbarrier\.arrive[a-z_.:0-9]*", source(name)):
+        assert "shared::cluster" not in arrival or ".release.cluster" in arrival, arrival
