@@ -552,7 +552,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             const unsigned b = tile & 1;
             const int64_t entry = FORM == OUTER ? -1 : a.g.order[t.slot + row];
             if (t.steps > 0) {
-                if (!__all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken))) break;
+                if (!__all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken, t.steps))) break;
                 tmem_fence_after();
             }
             const uint32_t at = tmem + b * W + ((uint32_t)(warp & 3) << 21);
