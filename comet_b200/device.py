@@ -429,7 +429,15 @@ def _check_weights(what, G, name, W, dtype, rows, cols):
     return r, c
 
 
+def _check_groups(what, G):
+    """Kernels read them by their addresses, whatever device those are of."""
+    here = torch._C._cuda_getDevice()
+    if G.plan.get_device() != here or G.S.pos.get_device() != here or G.S.crd.get_device() != here:
+        raise ValueError(what + ": the groups must be of the current CUDA device")
+
+
 def _check_gated(what, G, X, W, activation):
+    _check_groups(what, G)
     width, ld = _check_experts(what, G, "X", X, False)
     rows, _ = _check_weights(what, G, "W", W, X.dtype, None, width)
     if rows % 16 or rows < 16:
@@ -466,6 +474,7 @@ def gated_experts_grad(G, X, W, d_H, activation="silu", grad_x=True, grad_w=True
 
 
 def _check_combine(what, G, H, V):
+    _check_groups(what, G)
     inner, _ = _check_experts(what, G, "H", H, True)
     width, _ = _check_weights(what, G, "V", V, H.dtype, None, inner)
     if width % 8:

@@ -57,3 +57,62 @@ def test_a_temperature_lives_until_its_call_returns(calls, which):
     calls.inside = others
     log_probs_calls()[which](0.749)
     assert alive == [True]
+
+
+class Elsewhere:
+    """A tensor as another one, but on another device."""
+
+    def __init__(self, like):
+        self._like = like
+
+    def get_device(self):
+        return 1
+
+    def __getattr__(self, name):
+        return getattr(self._like, name)
+
+
+def experts_calls(G):
+    """Each of the four operations on 6 tokens with 2 of 4 experts, width 64 and inner 48."""
+    from comet_b200 import device
+    new = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16)                   # noqa: E731
+    X, W, H, V = new(6, 64), new(4, 96, 64), new(12, 48), new(4, 64, 48)
+    return [lambda: device.gated_experts(G, X, W), lambda: device.gated_experts_grad(G, X, W, H), lambda: device.combine_experts(G, H, V),
+            lambda: device.combine_experts_grad(G, H, V, X)]
+
+
+def choices():
+    from comet_b200 import device
+    S = device.DeviceCSR(6, 4, torch.arange(0, 13, 2), torch.arange(12) % 4, torch.ones(12))
+    return S, device.group_entries
+
+
+@pytest.fixture
+def groups(calls):
+    """group_entries asks for a CUDA matrix: EntryGroups as it makes them."""
+    from comet_b200 import device
+    S, _ = choices()
+    plan = torch.zeros(16 + 4 + 8 + 8 + 256 * 5, dtype=torch.int32)
+    return device.EntryGroups(S, plan, 128 * 5)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_groups_of_the_current_device_go_through(calls, groups, which):
+    experts_calls(groups)[which]()
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("part", ["plan", "pos", "crd", "val"])
+def test_groups_of_another_device_are_refused(calls, groups, part, which):
+    """Their addresses are of another device's memory."""
+    if part == "plan":
+        groups.plan = Elsewhere(groups.plan)
+    else:
+        setattr(groups.S, part, Elsewhere(getattr(groups.S, part)))
+    if part == "val" and which < 2:                                                 # not looked at
+        experts_calls(groups)[which]()
+        return
+    with pytest.raises(ValueError, match="device"):
+        experts_calls(groups)[which]()
+    assert not calls
