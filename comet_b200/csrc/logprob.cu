@@ -311,13 +311,14 @@ prob_grad_short_kernel(const ProbGrad p, const T *xs, T *grad)
 }
 
 template <typename T>
-static int check_logits(const char *what, int64_t nrows, int64_t ncols, const void *x, int64_t ldx, const double *temperature)
+static int check_logits(const char *what, int64_t nrows, int64_t ncols, const void *x, int64_t ldx, const double *temperature, const float *sums)
 {
     if (nrows < 0 || ncols <= 0 || ncols >= 1LL << 30) return fail("%s: %lld rows of %lld columns", what, (long long)nrows, (long long)ncols);
     if (ldx < ncols) return fail("%s: leading dimension smaller than the number of columns", what);
     if (nrows > 0x7fffffffLL / MOST_CLUSTER) return fail("%s: more than 2^28 rows", what);
     if (!temperature_fits(*temperature)) return fail("%s: temperature %g is not a number of 1e-38 to 1e30", what, *temperature);
     if ((uintptr_t)x % sizeof(T)) return fail("%s: an address that is not a multiple of the element's size", what);
+    if ((uintptr_t)sums % sizeof(float2)) return fail("%s: sums at an address that is not a multiple of 8 bytes", what);
     return 0;
 }
 
@@ -355,7 +356,7 @@ static int log_probs(int64_t nrows, int64_t ncols, const int64_t *pos, const int
                      float *sums, float *entropy, int64_t k, int64_t *best_pos, int64_t *best_crd, float *best_val, cudaStream_t st)
 {
     clear_error();
-    CB_TRY(check_logits<T>("log_probs", nrows, ncols, x, ldx, temperature));
+    CB_TRY(check_logits<T>("log_probs", nrows, ncols, x, ldx, temperature, sums));
     if (k < 0 || k > ncols || k > 1024) return fail("log_probs: %lld alternatives a row; 0 to 1024, and no more than a row has columns", (long long)k);
     if (nrows == 0) {
         if (k) CB_CUDA(cudaMemsetAsync(best_pos, 0, sizeof(int64_t), st));
@@ -392,7 +393,7 @@ static int log_probs_grad(int64_t nrows, int64_t ncols, const int64_t *pos, cons
                           const float *sums, const float *values, const float *entropy, const float *by_entropy, void *grad, int64_t ldg, cudaStream_t st)
 {
     clear_error();
-    CB_TRY(check_logits<T>("log_probs_grad", nrows, ncols, x, ldx, temperature));
+    CB_TRY(check_logits<T>("log_probs_grad", nrows, ncols, x, ldx, temperature, sums));
     if (ldg < ncols) return fail("log_probs_grad: leading dimension smaller than the number of columns");
     if ((uintptr_t)grad % sizeof(T)) return fail("log_probs_grad: an address that is not a multiple of the element's size");
     if (by_entropy && !entropy) return fail("log_probs_grad: the entropies' gradients need the entropies");

@@ -346,9 +346,9 @@ def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperatu
     n, m, ld = shape = _check_logits("log_probs_grad", X)
     pos, crd = _check_beside("log_probs_grad", S, n, m)
     d_val = _check_vector("log_probs_grad", d_values, torch.float32, S.nnz)
-    if sums.shape != (n, 2):
-        raise ValueError("log_probs_grad: sums must be what log_probs gives, [%d, 2]" % n)
-    kept = _check_vector("log_probs_grad", sums.view(-1), torch.float32, 2 * n)
+    kept = sums.data_ptr()
+    if sums.shape != (n, 2) or sums.dtype is not torch.float32 or not sums.is_contiguous() or kept % 8 or sums.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("log_probs_grad: sums must be what log_probs gives, [%d, 2] contiguous float32 values on the logits' device, at a multiple of 8 bytes" % n)
     ent = d_ent = 0
     if d_entropy is not None:
         if entropy is None:

@@ -684,7 +684,7 @@ COMET_B200_EXPORT int32_t comet_b200_dev_balance_loss_f32_i64(
 
 /* Log probabilities of given columns.  pos/crd: a CSR matrix of x's shape (ncols < 2^30) whose columns are asked for; in any order, repeated or not.
      values[nnz]   = (x_j - m) / *temperature - log s   with m the row's largest logit, s = sum_j exp((x_j - m) / *temperature)
-     sums[2 nrows] = m, log s of each row (m / *temperature + log s is what top_entries gives as lse)
+     sums[2 nrows] = m, log s of each row (m / *temperature + log s is what top_entries gives as lse), at a multiple of 8 bytes
      entropy[nrows] = -sum_j q_j log q_j (may be NULL)
      best_pos/best_crd/best_val: with k > 0 the row's k largest entries as top_entries gives them, with their log probabilities.
    A row of -inf has log probabilities of -inf, sums of -inf and 0 and an entropy of 0; a row with NaN or +inf has NaN.  A logit of -inf adds

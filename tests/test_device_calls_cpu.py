@@ -116,3 +116,21 @@ def test_groups_of_another_device_are_refused(calls, groups, part, which):
     with pytest.raises(ValueError, match="device"):
         experts_calls(groups)[which]()
     assert not calls
+
+
+def sums_of(buffer):
+    from comet_b200 import device
+    return lambda: device.log_probs_grad(pattern(), torch.zeros(3, 40), buffer, torch.zeros(3))
+
+
+def test_sums_at_an_odd_address_are_refused(calls):
+    """Kernels read both numbers of a row at once.  So are sums that are not contiguous, whatever their strides."""
+    room = torch.zeros(32)
+    assert room.data_ptr() % 8 == 0
+    for bad in (room[1:7].view(3, 2), room[:6].view(2, 3).t(), room[:12].view(3, 4)[:, :2], room[:6].double().view(3, 2), room[:6]):
+        with pytest.raises(ValueError, match="sums"):
+            sums_of(bad)()
+    assert not calls
+    for good in (room[2:8].view(3, 2), room[:6].view(3, 2)):
+        sums_of(good)()
+    assert len(calls) == 2

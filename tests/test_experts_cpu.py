@@ -96,3 +96,14 @@ def test_log_probs(kind, room):
         one[0] = bad
         assert "temperature" in call(forward, 4, 8, p, p, p, 8, t, p, p, 0, 0, 0, 0, 0, 0)
         assert "temperature" in call(back, 4, 8, p, p, p, 8, t, p, p, 0, 0, p, 8, 0)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("k", [0, 2])
+def test_address_of_sums(kind, k, room):
+    """Both numbers of a row are read and written at once."""
+    p, one = room, (ctypes.c_double * 1)(1.0)
+    t = ctypes.addressof(one)
+    for ncols in (8, 5000):
+        assert "8 bytes" in call("comet_b200_dev_log_probs_%s_i64" % kind, 4, ncols, p, p, p, ncols, t, p, p + 4, 0, k, p, p, p, 0)
+        assert "8 bytes" in call("comet_b200_dev_log_probs_grad_%s_i64" % kind, 4, ncols, p, p, p, ncols, t, p + 4, p, 0, 0, p, ncols, 0)
