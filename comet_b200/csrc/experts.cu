@@ -39,13 +39,15 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 static int make_map(const char *what, const void *base, bool bf16, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
                     CUtensorMap *map)
 {
-    static EncodeTiled encode = nullptr;
+    static std::atomic<EncodeTiled> found{nullptr};            // the driver's, the same for every device; two threads may look for it at once
+    EncodeTiled encode = found.load();
     if (!encode) {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn || q != cudaDriverEntryPointSuccess)
             return fail("%s: cuTensorMapEncodeTiled is not available from this driver", what);
         encode = (EncodeTiled)fn;
+        found.store(encode);
     }
     const cuuint32_t ones[3] = {1, 1, 1};
     const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, (void *)base, dims, strides, box, ones,

@@ -1,4 +1,4 @@
-"""Waits inside the experts' kernels that run out, with the kernels' own text compiled by g++: no GPU has to wait for anything."""
+"""Waits inside the experts' kernels that run out, and what host threads share, with the sources' own text compiled by g++: no GPU has to wait for anything."""
 import os
 import re
 import subprocess
@@ -67,3 +67,15 @@ def limit_check(tmp_path, steps, ns):
 def test_takers_wait_for_all_of_a_tiles_steps():
     """The sums of a tile are waited for once: with the limit of its steps."""
     assert re.findall(r"bar_wait\(done [^;]*?broken, ([^)]*)\)", source("experts.cu")) == ["t.steps"]
+
+
+def test_first_tensor_maps_by_several_threads(tmp_path):
+    text = source("experts.cu")
+    code = text[text.index("typedef CUresult (*EncodeTiled)"):text.index("enum Form")]
+    with open(str(tmp_path / "kernels.inc"), "w") as f:
+        f.write(code)
+    exe = str(tmp_path / "check")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=thread", "-pthread", "-I" + str(tmp_path), "-I/usr/local/cuda/include",
+                           os.path.join(CHECKS, "tensor_map_check.cpp"), "-o", exe])
+    out = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=60)
+    assert out.returncode == 0 and out.stdout == "ok\n", out.stdout[:3000]
