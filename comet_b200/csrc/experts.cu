@@ -228,7 +228,8 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
                     const float g = gate[i];
                     const float2 u = gate_of(g, a.gelu);
                     const float s = logistic(u.x);
-                    gate[i] = d[i] * up[i] * fmaf(g * s * (1.0f - s), u.y, s);
+                    const float curve = g * s * (1.0f - s);                          // 0 where gelu's u, and u's slope, may be infinite
+                    gate[i] = d[i] * up[i] * (curve == 0.0f ? s : fmaf(curve, u.y, s));
                     up[i] = d[i] * g * s;
                 }
                 const int64_t to = (int64_t)(t.slot + row) * 2 * inner + f0 + c;

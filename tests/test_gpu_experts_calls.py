@@ -27,3 +27,40 @@ def test_one_expert_with_half_a_billion_entries():
     close(dW, dw, ow, "bf16")
     del X, dH, S, G
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_gates_whose_square_is_infinite(act, rows):
+    """Gates of 1e20 and -1e20: the activation's slope is 1 and 0 there, though the cube inside gelu is infinite in f32."""
+    import torch
+    from comet_b200 import device
+    width, inner = 64, 16
+    crd = torch.arange(rows, device="cuda") % 2
+    S = device.DeviceCSR(rows, 2, torch.arange(rows + 1, device="cuda"), crd, None)
+    X = torch.zeros((rows, width), device="cuda")
+    X[:, 0] = 1e10
+    X[:, 1] = 1.0
+    W = torch.zeros((2, 2 * inner, width), device="cuda")
+    W[0, :inner, 0], W[1, :inner, 0] = 1e10, -1e10
+    W[:, inner:, 1] = 2.0
+    X, W = X.bfloat16(), W.bfloat16()
+    G = device.group_entries(S)
+    H = device.gated_experts(G, X, W, activation=act)
+    big = X[0, 0].double() * W[0, 0, 0].double()
+    want = torch.where(crd == 0, 2 * big, 0.0)[:, None].expand(-1, inner)
+    assert float((H.double() - want).abs().max()) <= 2.0 ** -8 * 2 * float(big)
+    d = torch.full((rows, inner), 0.5, device="cuda").bfloat16()
+    dX, dW = device.gated_experts_grad(G, X, W, d, activation=act)
+    # d_gate = 0.5 * 2 * slope, d_up = 0.5 * act(gate); the products of 0 with other columns' weights are 0
+    assert not torch.isnan(dX).any() and not torch.isnan(dW).any()
+    n0, n1 = (rows + 1) // 2, rows // 2
+    x0 = X[0, 0].double()
+    want = torch.stack([torch.full((inner,), float(n0 * x0), device="cuda"), torch.zeros(inner, device="cuda")])
+    off = (dW[:, :inner, 0].double() - want).abs()
+    assert n1 <= n0 and float(off.max()) <= 2.0 ** -7 * n0 * float(x0)
+    assert float(dW[1, :inner].abs().max()) == 0
+    # column 0: 16 gate rows of weight 1e10 with a gradient of 1 each, and nothing from up rows
+    want = torch.where(crd == 0, inner * W[0, 0, 0].double(), 0.0)
+    assert float((dX[:, 0].double() - want).abs().max()) <= 2.0 ** -8 * inner * float(W[0, 0, 0])
+    G.check()
