@@ -76,6 +76,16 @@ struct Shape {
     static constexpr int TAKEN = W == WIDE ? 128 : 32;         // bytes of a row that a warp takes out at a time
     static constexpr int SMEM = RING * STEP + TAKERS * TAKEN + 1024;
 };
+// The tensor cores cut off what does not fit into an f32 sum, each time that they add, so long sums are off by more than f32 sums are.  In results of 16 bits that is
+// nothing; d_values is f32, and was off by 2.0e-6 of its norm at a width of 2048, 9.1e-6 at 8192.  There a tile's sums are taken out after so many steps and added up,
+// rounded to the nearest, in the takers' registers (0: not at all): 4.8e-7 at any width after 8 steps, 1.0e-6 after 16, 2.6e-7 after 4; f32 products 2e-7 to 4e-7.
+// While the takers are at a tile's results, products for two such segments can go on: v'dy of combine_grad_step 95 us after 8 steps, 89 after 16, 106 after 4.
+constexpr int segment(int sums) { return sums == COMBINE_GRAD ? 8 : 0; }
+// In a wide tile that is 128 sums a thread.  The takers get the registers that the other warps do not use: of the 128 that each of 512 threads starts with, theirs then
+// have 192 and the others' 64, by warpgroups of 128 threads.
+constexpr bool many_registers(int w, int sums) { return w == WIDE && segment(sums); }
+constexpr int product_threads(int w, int sums) { return many_registers(w, sums) ? 512 : PRODUCT_THREADS; }
+static_assert(TAKERS * 192 + (512 - TAKERS) * 64 <= 512 * 128 && TAKERS % 128 == 0, "registers that are given were there");
 
 struct ProductArgs {
     Groups g;
@@ -185,6 +195,37 @@ struct Stage {
         }
         __syncwarp();
     }
+    // in two steps: on their way, and there
+    __device__ __forceinline__ void fetch(const E *base, int64_t first, int cols) const
+    {
+#pragma unroll
+        for (int i = 0; i < LANES; i++) {
+            const int row = i * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+            const int64_t from = __shfl_sync(0xffffffffu, first, row);
+            const bool there = from >= 0 && chunk * N < cols;
+            copy_or_zero(smem_at(&at(row, chunk)), base + (there ? from + chunk * N : 0), there);
+        }
+    }
+    __device__ __forceinline__ void fetched() const
+    {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+    }
+    // the same by way of registers
+    __device__ __forceinline__ void load(uint4 (&v)[LANES], const E *base, int64_t first, int cols) const
+    {
+#pragma unroll
+        for (int i = 0; i < LANES; i++) {
+            const int64_t from = __shfl_sync(0xffffffffu, first, i * (32 / LANES) + lane / LANES);
+            v[i] = from >= 0 && lane % LANES * N < cols ? *(const uint4 *)(base + from + lane % LANES * N) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void loaded(const uint4 (&v)[LANES]) const
+    {
+#pragma unroll
+        for (int i = 0; i < LANES; i++) at(i * (32 / LANES) + lane / LANES, lane % LANES) = v[i];
+        __syncwarp();
+    }
 };
 
 // A tile's sums, by two warps for each 32 rows, a half of the columns each; tmem: tensor memory of the rows.  entry: that of the thread's row,
@@ -261,37 +302,6 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
                 rows.out(a.sums, entry < 0 ? -1 : entry * a.cols + c0 + c + p, a.cols - c0 - c - p);
             }
         }
-    } else if constexpr (SUMS == COMBINE_GRAD) {
-        constexpr int MINE = W / 2, PART = st.COLS < 32 ? st.COLS : 32;
-        const Stage<T, PART * 2> part = {room, (int)threadIdx.x & 31};
-        const int c0 = t.n * W + half * MINE;
-        const float by = entry >= 0 ? a.val[entry] : 0.0f;
-        float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-        for (int c = 0; c < MINE; c += PART) {
-            const int left = a.cols - c0 - c;
-            if (left <= 0) break;
-            const int64_t first = entry < 0 ? -1 : entry * a.cols + c0 + c;
-            float h[PART], v[PART];
-            part.in((const T *)a.other, first, left);
-#pragma unroll
-            for (int i = 0; i < PART; i += 8) part.get(i / 8, h + i);
-            tmem_load(tmem + half * MINE + c, v);
-#pragma unroll
-            for (int i = 0; i < PART; i++) {
-                if (entry >= 0) sum[i % 8] = fmaf(v[i], h[i], sum[i % 8]);
-                v[i] *= by;
-                h[i] *= by;
-            }
-#pragma unroll
-            for (int i = 0; i < PART; i += 8) part.put(i / 8, v + i);
-            part.out((T *)a.out, first, left);
-            // a row of zeros adds nothing to the sums over an expert's tokens
-#pragma unroll
-            for (int i = 0; i < PART; i += 8) part.put(i / 8, h + i);
-            part.out((T *)a.scaled, (int64_t)(t.slot + row) * a.cols + c0 + c, left);
-        }
-        if (entry >= 0) a.sums[(t.n * 2 + half) * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     } else {
         constexpr int MINE = W / 2, PART = st.COLS < 32 ? st.COLS : 32;
         const int c0 = t.n * W + half * MINE, r = t.m * TM + row;
@@ -317,6 +327,44 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
     }
 }
 
+// The same for dh, val h and dval, from sums that the thread holds, of columns c0 to c0 + left (or W / 2).  The first part of h's rows is on its way to the stage.
+template <typename T, int W>
+__device__ __forceinline__ void take_held(const ProductArgs &a, const float (&held)[W / 2], const Stage<T, Shape<W>::TAKEN> &st, int64_t first, int64_t slot, int c0, int left,
+                                          int part_of_sums, int64_t entry, float by)
+{
+    constexpr int PART = st.COLS;
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    st.fetched();
+#pragma unroll
+    for (int c = 0; c < W / 2; c += PART) {
+        uint4 scaled[PART / 8], next[st.LANES];
+#pragma unroll
+        for (int i = 0; i < PART; i += 8) {
+            float h[8], v[8];
+            st.get(i / 8, h);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (entry >= 0) sum[j] = fmaf(held[c + i + j], h[j], sum[j]);
+                v[j] = held[c + i + j] * by;
+                h[j] *= by;                        // rounded to its type, as dz is, for the product with dy
+            }
+            Granule<T> packed;
+            packed.pack(h);
+            scaled[i / 8] = packed.w;
+            st.put(i / 8, v);
+        }
+        st.out((T *)a.out, first < 0 ? -1 : first + c, left - c);
+        const bool more = c + PART < W / 2;
+        if (more) st.load(next, (const T *)a.other, first < 0 ? -1 : first + c + PART, left - c - PART);
+        // a row of zeros adds nothing to the sums over an expert's tokens
+#pragma unroll
+        for (int i = 0; i < PART / 8; i++) st.at(st.lane, i) = scaled[i];
+        st.out((T *)a.scaled, slot * a.cols + c0 + c, left - c);
+        if (more) st.loaded(next);
+    }
+    if (entry >= 0) a.sums[part_of_sums * a.nnz + entry] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+}
+
 // An entry whose column is no expert's: NaN.
 template <typename T, int SUMS>
 __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
@@ -338,7 +386,7 @@ __device__ __forceinline__ void spoil(const ProductArgs &a, int thread)
 enum Numbered { NUMBERED_A, NUMBERED_B, NUMBERED_NONE };
 
 template <typename T, int W, int FORM, int NUMBERED, int SUMS>
-__global__ void __launch_bounds__(PRODUCT_THREADS, W == WIDE ? 1 : 2)
+__global__ void __launch_bounds__(product_threads(W, SUMS), W == WIDE || segment(SUMS) ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a)
 {
     constexpr bool BF16 = !__is_same(T, __half);
@@ -351,7 +399,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     __shared__ int broken_word;
     volatile int *broken = &broken_word;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int ISSUER = (TAKERS + FETCHERS) / 32, BOXES = ISSUER + 1;
+    constexpr int ISSUER = (TAKERS + FETCHERS) / 32, BOXES = ISSUER + 1, SEGMENT = segment(SUMS);
     const uint32_t ring = (smem_at(raw) + 1023) & ~1023u, full = smem_at(bars), empty = full + 8 * RING, done = empty + 8 * RING, taken = done + 16,
                    last = taken + 16;
     if (warp == ISSUER) tmem_alloc(smem_at(&tmem_room), 2 * W);
@@ -375,7 +423,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     wait_for_previous();
 
     const int mine = blockIdx.x, all = gridDim.x;
-    // Tiles of a last round that would leave half of the CTAs idle are cut into two (v'dy of combine_grad_step, 3.3 rounds: 86 us, 90 with whole ones; dx of gated_grad_step 110, 114).
+    // Tiles of a last round that would leave half of the CTAs idle are cut into two (dx of gated_grad_step 110 us, 114 with whole ones; v'dy of combine_grad_step, 3.3 rounds, gains 4, too).
     constexpr bool HALVES = W == WIDE && (SUMS == ENTRY_ROWS || SUMS == COMBINE_GRAD);
     const int entire = FORM == OUTER ? a.g.ngroups * a.tiles_m * a.tiles_n : a.g.head[0] * a.tiles_n;
     const int whole = HALVES && entire % all * 2 <= all ? entire / all * all : entire, tiles = whole + 2 * (entire - whole);
@@ -408,152 +456,191 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         volatile int late = 0;
         for (unsigned i = step < RING ? 0 : step - RING; i < step; i++) bar_wait(full + 8 * (i % RING), i / RING & 1, &late);
     };
-    if (warp == BOXES) {                           // fetches by tensor copies
-        unsigned step = 0;                         // steps so far; stage = step % RING
-        bool on = true;
-        for (int id = mine; on && id < tiles; id += all) {
-            const Tile t = tile_of(id);
-            constexpr int BLOCKS = W / 64;
-            const int n0 = t.n * W;
-            for (int k = 0; k < t.steps; k++, step++) {
-                const unsigned s = step % RING;
-                const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
-                on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
-                if (!on) break;
-                if (elect()) {
-                    bar_expect(bar, TENSOR_BYTES - (HALVES && t.half ? B_BYTES / 2 : 0));
-                    if (HALVES && t.half) {
-                        const int n = n0 + (t.half - 1) * (W / 2);
-                        if (FORM == ROWS) {
-                            load_box(to + A_BYTES, &map_b, k * TK, n, t.group, bar);
-                        } else {
+    if (warp >= TAKERS / 32) {
+        if (many_registers(W, SUMS)) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == BOXES) {                           // fetches by tensor copies
+            unsigned step = 0;                         // steps so far; stage = step % RING
+            bool on = true;
+            for (int id = mine; on && id < tiles; id += all) {
+                const Tile t = tile_of(id);
+                constexpr int BLOCKS = W / 64;
+                const int n0 = t.n * W;
+                for (int k = 0; k < t.steps; k++, step++) {
+                    const unsigned s = step % RING;
+                    const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
+                    on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
+                    if (!on) break;
+                    if (elect()) {
+                        bar_expect(bar, TENSOR_BYTES - (HALVES && t.half ? B_BYTES / 2 : 0));
+                        if (HALVES && t.half) {
+                            const int n = n0 + (t.half - 1) * (W / 2);
+                            if (FORM == ROWS) {
+                                load_box(to + A_BYTES, &map_b, k * TK, n, t.group, bar);
+                            } else {
+                                if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
+#pragma unroll
+                                for (int i = 0; i < BLOCKS / 2; i++) load_box(to + A_BYTES + i * 8192, &map_b, n + i * 64, k * TK, t.group, bar);
+                            }
+                        } else if (FORM == ROWS) {
+                            // an expert's gate rows, and as many up rows; or rows of the one weight
+                            constexpr bool GATES = SUMS != ENTRY_ROWS;
+                            load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
+                            load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, GATES ? t.n * (W / 2) : n0 + W / 2, GATES ? 2 * t.group + 1 : t.group, bar);
+                        } else if (FORM == BACK) {
                             if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
 #pragma unroll
-                            for (int i = 0; i < BLOCKS / 2; i++) load_box(to + A_BYTES + i * 8192, &map_b, n + i * 64, k * TK, t.group, bar);
+                            for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, k * TK, t.group, bar);
+                        } else if (NUMBERED == NUMBERED_A) {
+#pragma unroll
+                            for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, t.slot + k * TK, 0, bar);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
                         }
-                    } else if (FORM == ROWS) {
-                        // an expert's gate rows, and as many up rows; or rows of the one weight
-                        constexpr bool GATES = SUMS != ENTRY_ROWS;
-                        load_box(to + A_BYTES, &map_b, k * TK, GATES ? t.n * (W / 2) : n0, GATES ? 2 * t.group : t.group, bar);
-                        load_box(to + A_BYTES + B_BYTES / 2, &map_b, k * TK, GATES ? t.n * (W / 2) : n0 + W / 2, GATES ? 2 * t.group + 1 : t.group, bar);
-                    } else if (FORM == BACK) {
-                        if (NUMBERED == NUMBERED_NONE) load_box(to, &map_a, k * TK, t.slot, 0, bar);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (*broken) land(step);
+        } else if (warp < ISSUER) {                    // fetches rows by their number
+            unsigned step = 0;
+            bool on = NUMBERED != NUMBERED_NONE;
+            const int me = tid - TAKERS, chunk = me & 7, row = me >> 3;
+            // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
+            const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
+            const char *base = (const char *)a.numbered + chunk * 16;
+            const int64_t stride = a.ld * 2;
+            for (int id = mine; on && id < tiles; id += all) {
+                const Tile t = tile_of(id);
+                const char *from[8];
+                unsigned there = 0;
+                if (NUMBERED == NUMBERED_A && FORM != OUTER) {
 #pragma unroll
-                        for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, k * TK, t.group, bar);
-                    } else if (NUMBERED == NUMBERED_A) {
+                    for (int i = 0; i < 8; i++) {
+                        const int n = a.numbers[t.slot + row + 16 * i];
+                        from[i] = base + max(n, 0) * stride;
+                        there |= (n >= 0 ? 1u : 0u) << i;
+                    }
+                }
+                int next[4];
+                if (FORM == OUTER && t.steps)
 #pragma unroll
-                        for (int i = 0; i < BLOCKS; i++) load_box(to + A_BYTES + i * 8192, &map_b, n0 + i * 64, t.slot + k * TK, 0, bar);
+                    for (int i = 0; i < 4; i++) next[i] = a.numbers[t.slot + row + 16 * i];
+                for (int k = 0; k < t.steps; k++, step++) {
+                    const unsigned s = step % RING;
+                    const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
+                    on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
+                    if (!on) break;
+                    if (FORM != OUTER) {
+                        const bool in = k * TK + chunk * 8 < a.numbered_cols;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
                     } else {
+                        constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : W / 64;
+                        const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
+                        const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W;
 #pragma unroll
-                        for (int i = 0; i < 2; i++) load_box(to + i * 8192, &map_a, t.m * TM + i * 64, t.slot + k * TK, 0, bar);
-                    }
-                }
-                __syncwarp();
-            }
-        }
-        if (*broken) land(step);
-    } else if (warp >= TAKERS / 32 && warp < ISSUER) {         // fetches rows by their number
-        unsigned step = 0;
-        bool on = NUMBERED != NUMBERED_NONE;
-        const int me = tid - TAKERS, chunk = me & 7, row = me >> 3;
-        // a tile's row i is 128 bytes, of which chunk c lies at c ^ (i & 7): what tensor copies do, and the products undo
-        const uint32_t at = row * 128 + ((chunk ^ (row & 7)) << 4);
-        const char *base = (const char *)a.numbered + chunk * 16;
-        const int64_t stride = a.ld * 2;
-        for (int id = mine; on && id < tiles; id += all) {
-            const Tile t = tile_of(id);
-            const char *from[8];
-            unsigned there = 0;
-            if (NUMBERED == NUMBERED_A && FORM != OUTER) {
+                        for (int i = 0; i < 4; i++) {
+                            const char *src = base + max(next[i], 0) * stride;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int n = a.numbers[t.slot + row + 16 * i];
-                    from[i] = base + max(n, 0) * stride;
-                    there |= (n >= 0 ? 1u : 0u) << i;
-                }
-            }
-            int next[4];
-            if (FORM == OUTER && t.steps)
-#pragma unroll
-                for (int i = 0; i < 4; i++) next[i] = a.numbers[t.slot + row + 16 * i];
-            for (int k = 0; k < t.steps; k++, step++) {
-                const unsigned s = step % RING;
-                const uint32_t to = ring + s * STEP_BYTES, bar = full + 8 * s;
-                on = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, (step / RING & 1) ^ 1, broken));
-                if (!on) break;
-                if (FORM != OUTER) {
-                    const bool in = k * TK + chunk * 8 < a.numbered_cols;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) copy_or_zero(to + at + i * 2048, from[i] + (in ? k * TK * 2 : 0), in && (there >> i & 1));
-                } else {
-                    constexpr int BLOCKS = NUMBERED == NUMBERED_A ? 2 : W / 64;
-                    const uint32_t first = to + (NUMBERED == NUMBERED_A ? 0 : A_BYTES) + at;
-                    const int col0 = NUMBERED == NUMBERED_A ? t.m * TM : t.n * W;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const char *src = base + max(next[i], 0) * stride;
-#pragma unroll
-                        for (int b = 0; b < BLOCKS; b++) {
-                            const bool in = col0 + b * 64 + chunk * 8 < a.numbered_cols;
-                            copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && next[i] >= 0);
+                            for (int b = 0; b < BLOCKS; b++) {
+                                const bool in = col0 + b * 64 + chunk * 8 < a.numbered_cols;
+                                copy_or_zero(first + b * 8192 + i * 2048, src + (in ? (col0 + b * 64) * 2 : 0), in && next[i] >= 0);
+                            }
+                            if (k + 1 < t.steps) next[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
                         }
-                        if (k + 1 < t.steps) next[i] = a.numbers[t.slot + (k + 1) * TK + row + 16 * i];
                     }
+                    copies_to(bar);
                 }
-                copies_to(bar);
             }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == ISSUER) {                   // issues the products
-        // the whole warp goes along, and one thread of it issues: operands are the warp's then, not a thread's
-        unsigned tile = 0, step = 0;
-        bool on = true;
-        int after = mine < tiles ? tile_of(mine).steps : 0;
-        for (int id = mine; on && id < tiles; id += all) {
-            const bool half = HALVES && id >= whole;
-            const int steps = (int)__reduce_max_sync(0xffffffffu, (unsigned)after);  // the same in all, which the compiler does not know
-            if (id + all < tiles) after = tile_of(id + all).steps;
-            if (steps == 0) continue;
-            const unsigned b = tile & 1;
-            on = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
-            tmem_fence_after();
-            for (int k = 0; on && k < steps; k++, step++) {
-                const unsigned s = step % RING;
-                on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
-                if (!on) break;
-                if (NUMBERED != NUMBERED_NONE) shared_to_products();
-                tmem_fence_after();
-                const uint32_t at = ring + s * STEP_BYTES;
-                const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
-                // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
-                constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
-                const uint32_t kind = half ? product_descriptor(BF16, TM, W / 2, FORM == OUTER, FORM != ROWS)
-                                           : product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
-                if (elect()) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else if (warp == ISSUER) {                   // issues the products
+            // the whole warp goes along, and one thread of it issues: operands are the warp's then, not a thread's
+            unsigned tile = 0, step = 0;
+            bool on = true;
+            int after = mine < tiles ? tile_of(mine).steps : 0;
+            for (int id = mine; on && id < tiles; id += all) {
+                const bool half = HALVES && id >= whole;
+                const int steps = (int)__reduce_max_sync(0xffffffffu, (unsigned)after);  // the same in all, which the compiler does not know
+                if (id + all < tiles) after = tile_of(id + all).steps;
+                for (int k = 0; k < steps; k++, step++) {
+                    const unsigned s = step % RING, b = tile & 1;
+                    const int done_so_far = SEGMENT ? k % (SEGMENT ? SEGMENT : 1) : k;           // of the sums that are taken out at once
+                    const bool all_done = k + 1 == steps || done_so_far + 1 == SEGMENT;
+                    if (done_so_far == 0) {
+                        on = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
+                        if (!on) break;
+                        tmem_fence_after();
+                    }
+                    on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
+                    if (!on) break;
+                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
+                    tmem_fence_after();
+                    const uint32_t at = ring + s * STEP_BYTES;
+                    const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
+                    // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
+                    constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
+                    const uint32_t kind = half ? product_descriptor(BF16, TM, W / 2, FORM == OUTER, FORM != ROWS)
+                                               : product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
+                    if (elect()) {
 #pragma unroll
-                    for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, k + i > 0);
-                    products_to(empty + 8 * s);
-                    if (k + 1 == steps) products_to(done + 8 * b);
+                        for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, done_so_far + i > 0);
+                        products_to(empty + 8 * s);
+                        if (all_done) products_to(done + 8 * b);
+                    }
+                    __syncwarp();
+                    tile += all_done;
                 }
-                __syncwarp();
             }
-            tile++;
+            if (*broken) {                             // products under way end before tensor memory is given back
+                volatile int late = 0;
+                if (elect()) products_to(last);
+                bar_wait(last, 0, &late);
+            }
+            __syncwarp();
         }
-        if (*broken) {                             // products under way end before tensor memory is given back
-            volatile int late = 0;
-            if (elect()) products_to(last);
-            bar_wait(last, 0, &late);
-        }
-        __syncwarp();
     } else {                                       // takes the sums
+        if (many_registers(W, SUMS)) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         spoil<T, SUMS>(a, tid);
         const int row = (warp & 3) * 32 + lane;
         unsigned char *room = raw + (ring - smem_at(raw)) + RING * STEP_BYTES + warp * 32 * S::TAKEN;
         unsigned tile = 0;
         for (int id = mine; id < tiles; id += all) {
             const Tile t = tile_of(id);
-            const unsigned b = tile & 1;
             const int64_t entry = FORM == OUTER ? -1 : a.g.order[t.slot + row];
+            if constexpr (SEGMENT > 0) {
+                const bool has = !t.half || warp < 4;
+                const int half = t.half ? t.half - 1 : warp >> 2, c0 = t.n * W + half * (W / 2);
+                const int64_t first = entry < 0 ? -1 : entry * a.cols + c0;
+                const float by = entry >= 0 ? a.val[entry] : 0.0f;
+                const Stage<T, S::TAKEN> st = {room, lane};
+                if (has) st.fetch((const T *)a.other, first, a.cols - c0);
+                float held[W / 2] = {};
+                bool on = true;
+                for (int k = 0; k < t.steps; k += SEGMENT, tile++) {
+                    const unsigned b = tile & 1;
+                    on = __all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken));
+                    if (!on) break;
+                    tmem_fence_after();
+                    if (has) {
+                        const uint32_t at = tmem + b * W + ((uint32_t)(warp & 3) << 21) + (t.half ? 0 : (warp >> 2) * (W / 2));
+#pragma unroll
+                        for (int c = 0; c < W / 2; c += 16) {
+                            float v[16];
+                            tmem_load(at + c, v);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) held[c + i] += v[i];
+                        }
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(taken + 8 * b);
+                }
+                if (!on) break;
+                if (has) take_held<T, W>(a, held, st, first, t.slot + row, c0, a.cols - c0, t.n * 2 + half, entry, by);
+                continue;
+            }
+            const unsigned b = tile & 1;
             if (t.steps > 0) {
                 if (!__all_sync(0xffffffffu, bar_wait(done + 8 * b, tile / 2 & 1, broken, t.steps))) break;
                 tmem_fence_after();
@@ -568,6 +655,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 tile++;
             }
         }
+        if (SEGMENT) asm volatile("cp.async.wait_all;" ::: "memory");
     }
     tmem_fence_before();
     __syncthreads();
@@ -847,7 +935,7 @@ static int launch_product(const CUtensorMap &map_a, const CUtensorMap &map_b, Pr
     const int64_t tiles = FORM == OUTER ? (int64_t)a.g.ngroups * a.tiles_m * a.tiles_n : (group_tiles(a.nnz, a.g.ngroups) - 1) * a.tiles_n;
     if (tiles > 0x3fffffffLL) return fail("experts: more than 2^30 tiles");
     const int64_t most = sm_count() * (W == WIDE ? 1 : 2);     // CTAs that run at the same time: each goes from tile to tile
-    CB_CUDA(launch_behind(kernel, dim3((unsigned)(tiles < most ? tiles : most)), PRODUCT_THREADS, S::SMEM, st, map_a, map_b, a));
+    CB_CUDA(launch_behind(kernel, dim3((unsigned)(tiles < most ? tiles : most)), product_threads(W, SUMS), S::SMEM, st, map_a, map_b, a));
     return 0;
 }
 

@@ -64,3 +64,24 @@ def test_gates_whose_square_is_infinite(act, rows):
     want = torch.where(crd == 0, inner * W[0, 0, 0].double(), 0.0)
     assert float((dX[:, 0].double() - want).abs().max()) <= 2.0 ** -8 * inner * float(W[0, 0, 0])
     G.check()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,width,inner", [(40, 2048, 64), (700, 2048, 1024), (700, 8192, 512), (60, 32768, 128)])
+def test_gradients_of_values_have_f32s_digits(rows, width, inner, kind):
+    """However long the sums are.  The tensor cores cut off what is below a unit in the last place of the sum so far, 32 times in the 512 terms that they add up.  A unit is
+    0.72 x 2^-23 of a sum on average, half of it is lost: 4.3e-8 of the sum, always towards zero.  Of sums of random signs, which grow with the root of the number of their terms,
+    the 32 losses are 32 / sqrt(3) of that: 8e-7 of the norm.  Beyond 512 terms sums are rounded to the nearest: 2^-24 of the sum, of random signs, 64 times for the
+    longest here, and as often in the sum with h: 4e-7 at most."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(width)
+    S = device.DeviceCSR(rows, 2, torch.arange(rows + 1, device="cuda"), torch.arange(rows, device="cuda") % 2, torch.ones(rows, device="cuda"))
+    H, V, dY = matrix(rng, kind, rows, inner), matrix(rng, kind, 2, width, inner, scale=inner ** -0.5), matrix(rng, kind, rows, width)
+    G = device.group_entries(S)
+    got = device.combine_experts_grad(G, H, V, dY, grad_v=False)[2].double()
+    want = torch.cat([((dY[j::2].double() @ V[j].double()) * H[j::2].double()).sum(1, keepdim=True) for j in range(2)])
+    order = torch.argsort(torch.cat([torch.arange(j, rows, 2) for j in range(2)])).cuda()
+    want = want.reshape(-1)[order]
+    assert float((got - want).norm() / want.norm()) < 1.2e-6
+    G.check()
