@@ -12,8 +12,10 @@
 // inner 1024, the gated product, 1200 us with them, 438 without.)
 //
 // Bound: for that product, 550 GFLOP, 440 to 470 us when the chip is cool and 530 in a row of passes, where the power cap leaves 1.5 GHz (a library's plain product of the
-// same size: 370 and 430).  Tensor cores are busy 62 % of the clocks: a step of 64 terms is 512 clocks of theirs, and 768 of the shared memory's, which the
-// operands are written to and read from (48 KB each).  Where sums are short (dw: 7 steps a tile) or their results f32 (combine), the results' bytes.
+// same size: 370 and 430).  Tensor cores are active 65 to 72 % of the clocks: a step of 64 terms is 512 clocks of theirs and takes some 708, start and end of the launch
+// included.  The operands' 48 KB a step come into an SM at 61 to 66 bytes a clock over the whole launch (dx 60, dz 55), so the way from the L2 to an SM is the
+// likely bound; shared memory's banks are read in 28 % of the clocks and written in 27 %, the L2 is busy 36 %.  Where sums are short (dw: 7 steps a
+// tile, active 44 %; dv 45 %) or their results f32 (combine, 52 %), the results' bytes.
 // Three forms:
 //   ROWS   rows of a tile's tokens, times a weight whose rows are outputs                (forward passes, dz)
 //   BACK   the same, times a weight whose rows are the sum's index                       (dx, v' dy)
@@ -273,6 +275,8 @@ __device__ __forceinline__ void take_sums(const ProductArgs &a, uint32_t tmem, b
                     gate[i] = d[i] * up[i] * (curve == 0.0f ? s : fmaf(curve, u.y, s));
                     up[i] = d[i] * g * s;
                 }
+                // Rounded to the operands' type, as the tensor cores take them: a step of that type in dx and dw beside the last one (2.3e-3 of a bf16 result's norm
+                // instead of 1.7e-3).  In two parts of that type each they would be multiplied with W and X twice: dx and dw are more than half of the call.
                 const int64_t to = (int64_t)(t.slot + row) * 2 * inner + f0 + c;
 #pragma unroll
                 for (int i = 0; i < PART; i += 8) part.put(i / 8, gate + i);
@@ -664,7 +668,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (tid == 0 && *broken) a.g.head[2] = 1;
 }
 
-// A token's f32 rows, added in order: 4 columns a thread.
+// A token's f32 rows, added in order: 8 columns a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
 add_rows_kernel(int64_t nrows, int cols, const int64_t *__restrict__ pos, const float *__restrict__ sums, T *__restrict__ out)
@@ -698,8 +702,10 @@ add_parts_kernel(int64_t n, int parts, const float *__restrict__ sums, float *__
 // A single token: products of a weight's rows with its vectors, by the ordinary cores.  Neighbouring rows of an expert's weight are one piece of
 // memory, so a CTA's share comes in copies of up to 32 KB.  Six teams of four warps have a stage each: while one of them works on its stage, the others'
 // copies are under way, what an SM has to have in flight for the memory's full rate.  The vectors come through the L1 cache.
-// 8 experts of 64, in L2, us: 13.3 and 10.7 (gated, combine); by the tensor cores 17.5 and 13.3, and with two tokens 25 and 14 where this takes 32 and 18.
-// From memory: 20.0 and 14.0; the copies alone 14.4 and 9.5 (67 and 34 MB, and 4 us of start-up).
+// 8 experts of 64, width 2048, inner 1024, gated and combine, us (and by the tensor cores): weights in L2 12.2 and 10.1 (16.6, 13.1), other experts' each time 16.5 and
+// 11.8 (18.4, 14.5); with two tokens 32 and 18 (25, 14), so one is the limit.  2 of 8, 4096, 2048: 15.3 and 15.7 (22.8, 15.1); 4 of 32, 1024, 512: 4.7 and 4.7 (8.1, 7.7);
+// 8 of 128, 2048, 768: 9.6 and 9.6 (16.6, 11.7); one of 16, 2048, 2048: 5.1 and 9.2 (13.0, 14.5); 8 of 64, 512, 256: 5.9 and 5.7 (5.7, 6.7).
+// From memory, once in a while: 20.0 and 14.0 for the first; the copies alone 14.4 and 9.5 (67 and 34 MB, and 4 us of start-up).
 static const int FEW_STAGES = 6, FEW_BYTES = 32 * 1024, FEW_SMEM = FEW_STAGES * FEW_BYTES, FEW_ENTRIES = 8, TEAM = 128, FEW_THREADS = FEW_STAGES * TEAM;
 
 // Of R rows in shared memory, `next` bytes apart, and B vectors: a lane's part of their products.  A vector is loaded once for all the rows.
@@ -920,8 +926,9 @@ combine_few_kernel(const ProductArgs a, const int64_t *__restrict__ pos, const i
         });
 }
 
-// Narrow tiles where wide ones would leave most SMs without any.  Gated products, us, wide and narrow: 64 wide tiles of 32 steps 21 and 20, 144 of 16 steps 17 and
-// 24.
+// Narrow tiles where wide ones would leave most SMs without any.  The number of tiles is on the device; its limit by the numbers of entries and experts decides.
+// Gated products, us, wide and narrow: 16 to 40 wide tiles of 32 steps 16.7 and 13.4, 64 of them 16.8 and 17.2; 32 and 48 of 16 steps 10.9 and 8.5, 64 of them 10.9
+// and 11.0, 145 11.1 and 15.6.  Sums of experts' outputs: 32 of 16 steps 12.5 and 10.4, 64 of them 12.7 and 12.8; 64 of 4 steps 8.1 and 7.5, 128 of them 8.4 and 10.4.
 static bool narrow(const Groups &g, int64_t nnz, int64_t columns) { return (group_tiles(nnz, g.ngroups) - 1) * ceil_div(columns, WIDE) * 4 < sm_count(); }
 
 template <typename T, int W, int FORM, int NUMBERED, int SUMS>

@@ -342,7 +342,8 @@ def log_probs(S, X, temperature=1.0, entropy=False, top=0):
 def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperature=1.0, grad=True):
     """The gradient with respect to X of what log_probs gives, from d_values (float32, one for each of S's entries) and, with the
     entropies, d_entropy (float32, one for each row).  sums and entropy: of log_probs at the same temperature.  grad: True (a new tensor), or a tensor to write
-    it to, such as X.  The alternatives have no gradient here: as S of a second call they have."""
+    it to, such as X.  The alternatives have no gradient here: as S of a second call they have.  Made for rows of few entries: every warp that works on a row looks
+    at all of its entries, so the time grows with their number times the row's length beyond some hundred."""
     n, m, ld = shape = _check_logits("log_probs_grad", X)
     pos, crd = _check_beside("log_probs_grad", S, n, m)
     d_val = _check_vector("log_probs_grad", d_values, torch.float32, S.nnz)
@@ -364,7 +365,9 @@ def log_probs_grad(S, X, sums, d_values, entropy=None, d_entropy=None, temperatu
 
 
 # A router's experts: products of the rows that a CSR matrix (rows tokens, columns experts) sends to each of them.  The operands are contiguous CUDA
-# tensors in bf16 or f16, but for rows of tokens, whose stride may be any multiple of 8 elements; sums are in f32 and results rounded once.
+# tensors in bf16 or f16 on the current device, where the groups were made, but for rows of tokens, whose stride may be any multiple of 8 elements; sums are in f32
+# and results rounded once.  Results are new tensors without a graph (the gradients are for torch.autograd.backward), complete in the current stream's order; groups used on
+# another stream than the one they were made on have to be complete, and recorded there (torch.Tensor.record_stream of `plan`), as any tensor has.
 _EXPERTS = {torch.bfloat16: "bf16", torch.float16: "f16"}
 _GATED, _GATED_GRAD, _COMBINE, _COMBINE_GRAD = ({t: "comet_b200_dev_%s_%s_i64" % (op, name) for t, name in _EXPERTS.items()}
                                                 for op in ("gated_experts", "gated_experts_grad", "combine_experts", "combine_experts_grad"))
@@ -459,7 +462,9 @@ def gated_experts(G, X, W, activation="silu"):
 
 def gated_experts_grad(G, X, W, d_H, activation="silu", grad_x=True, grad_w=True):
     """The gradients of gated_experts with respect to X and W, from d_H, the one with respect to H (None where grad_x or grad_w is False).  The products of the
-    forward pass are computed again; their gradients are rounded to X's type before they are multiplied with W and X."""
+    forward pass are computed again; their gradients are rounded to X's type before they are multiplied with W and X.  Works in memory for 2 inner values of
+    that type for each slot and, for grad_x, width float32 values for each entry.  The sums over an expert's tokens are one CTA's a tile of 128 x 256 of W: few
+    experts of small sizes with many tokens leave most of the device idle."""
     sizes, ld = _check_gated("gated_experts_grad", G, X, W, activation)
     if d_H.dtype is not X.dtype:
         raise ValueError("gated_experts_grad: d_H must have X's type")
@@ -486,7 +491,7 @@ def _check_combine(what, G, H, V):
 
 def combine_experts(G, H, V):
     """The second half: Y [rows of S, width], for each row the sum over its entries (t, j) of S's value (float32) times V_j h, h the entry's row of H
-    [entries, inner]; V [experts, width, inner].  A row that stores nothing gives zeros."""
+    [entries, inner]; V [experts, width, inner].  A row that stores nothing gives zeros.  Works in memory for width float32 values for each entry."""
     sizes, val = _check_combine("combine_experts", G, H, V)
     Y, sums = H.new_empty((sizes[0], sizes[3])), H.new_empty((sizes[2], sizes[3]), dtype=torch.float32)
     _call(_COMBINE[H.dtype], *sizes, G.S.pos.data_ptr(), G.S.crd.data_ptr(), G.plan.data_ptr(), H.data_ptr(), val, V.data_ptr(), sums.data_ptr(), Y.data_ptr(), _stream())
@@ -495,7 +500,7 @@ def combine_experts(G, H, V):
 
 def combine_experts_grad(G, H, V, d_Y, grad_v=True):
     """The gradients of combine_experts with respect to H, V (None where grad_v is False) and S's values (float32), from d_Y, the one with respect to Y.  For V's,
-    the products of values and rows of H are rounded to H's type first."""
+    the products of values and rows of H are rounded to H's type first.  Works in memory for inner values of that type for each slot."""
     sizes, val = _check_combine("combine_experts_grad", G, H, V)
     if d_Y.dtype is not H.dtype:
         raise ValueError("combine_experts_grad: d_Y must have H's type")

@@ -701,7 +701,7 @@ COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_f32_i64(
 
 /* Their gradient: grad = d loss / d x in x's type, from d_values[nnz] and (with the entropies; both may be NULL) d_entropy[nrows], and the sums of the forward
    call at the same temperature.  May be x itself (same ldx).  Columns in any order, repeated ones add up; one outside
-   the matrix only adds to the row's sum.  A row whose d_values add up to 0, with a d_entropy of 0, is 0 but at its entries, and so is all of a row of -inf. */
+   the matrix only adds to the row's sum.  Every warp of a row looks at all of its entries: made for few.  A row whose d_values add up to 0, with a d_entropy of 0, is 0 but at its entries, and so is all of a row of -inf. */
 COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_bf16_i64(
     int64_t nrows, int64_t ncols, const int64_t *pos, const int64_t *crd, const void *x, int64_t ldx, const double *temperature,
     const float *sums, const float *d_values, const float *entropy, const float *d_entropy, void *grad, int64_t ldg, void *stream);

@@ -85,3 +85,49 @@ def test_gradients_of_values_have_f32s_digits(rows, width, inner, kind):
     want = want.reshape(-1)[order]
     assert float((got - want).norm() / want.norm()) < 1.2e-6
     G.check()
+
+
+def test_two_host_threads():
+    """Calls from two threads at once, on a stream each and at temperatures of their own, give what each of them gives alone."""
+    import threading
+
+    import torch
+    from comet_b200 import device
+    torch.cuda.init()
+    wrong, work = [], []
+    for t, (rows, kind) in enumerate([(1, "bf16"), (300, "f16")]):
+        rng = np.random.default_rng(t)
+        crd = torch.from_numpy(np.concatenate([np.sort(rng.choice(6, 2, replace=False)) for _ in range(rows)])).cuda()
+        S = device.DeviceCSR(rows, 6, torch.arange(0, 2 * rows + 1, 2, device="cuda"), crd, torch.rand(2 * rows, device="cuda"))
+        X, W, V = matrix(rng, kind, rows, 136), matrix(rng, kind, 6, 80, 136, scale=0.1), matrix(rng, kind, 6, 136, 40, scale=0.1)
+        L = torch.randn(rows, 5000, device="cuda")
+        given = device.DeviceCSR(rows, 5000, torch.arange(rows + 1, device="cuda"), torch.arange(rows, device="cuda") * 7, None)
+
+        def everything(tau, S=S, X=X, W=W, V=V, L=L, given=given):
+            G = device.group_entries(S)
+            H = device.gated_experts(G, X, W)
+            values, sums, entropy, best = device.log_probs(given, L, temperature=tau, entropy=True, top=3)
+            return [H, device.combine_experts(G, H, V), *device.gated_experts_grad(G, X, W, H), *device.combine_experts_grad(G, H, V, X), values, entropy, best.val,
+                    device.log_probs_grad(given, L, sums, values, temperature=tau), G.plan[2:3]]
+
+        taus = [0.5 + 0.01 * i + 10 * t for i in range(200)]
+        work.append((everything, taus, [everything(tau) for tau in taus[::40]]))
+    torch.cuda.synchronize()
+
+    def go(everything, taus, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i, tau in enumerate(taus):
+                    got = everything(tau)
+                    if i % 40 == 0 and not all(torch.equal(a, b) for a, b in zip(got, want[i // 40])):
+                        wrong.append((tau, [k for k, (a, b) in enumerate(zip(got, want[i // 40])) if not torch.equal(a, b)]))
+        except Exception as e:                                             # noqa: BLE001 - told by the main thread
+            wrong.append(e)
+
+    threads = [threading.Thread(target=go, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
