@@ -185,13 +185,16 @@ group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int6
     wait_for_previous();
     const int64_t mine = tid < nnz ? crd[tid] : -1;
     for (int i = tid; i <= nrows; i += FEW) rows[i] = (int)min(max(pos[i], (int64_t)0), (int64_t)nnz);
-    const int col = mine >= 0 && mine < n ? (int)mine : -1;
-    cols[tid] = col;
+    int col = mine >= 0 && mine < n ? (int)mine : -1;
     for (int i = tid; i < n; i += FEW) count[i] = 0;
     if (tid == 0) bad = 0;
     __syncthreads();
+    const bool there = tid >= rows[0] && tid < rows[nrows];    // pos may be that of some rows of a larger matrix: the other rows' entries are none here
+    if (!there) col = -1;
+    cols[tid] = col;
+    __syncthreads();
     int before = 0, row = 0;
-    if (tid < nnz) {
+    if (there) {
         if (col >= 0) atomicAdd(&count[col], 1);
         for (int i = 0; i < tid; i++) before += cols[i] == col;
         for (int step = FEW_ROWS / 2; step > 0; step /= 2)                           // the last row that begins at or before the entry
@@ -225,7 +228,7 @@ group_few_kernel(int nrows, int nnz, const int64_t *__restrict__ pos, const int6
         const int sum = count[c], end = (sum + GROUP_TILE - 1) / GROUP_TILE * GROUP_TILE;
         for (int i = sum + lane; i < end; i += 32) g.order[first[c] * GROUP_TILE + i] = g.token[first[c] * GROUP_TILE + i] = -1;
     }
-    if (tid < nnz) {
+    if (there) {
         if (col >= 0) {
             g.order[first[col] * GROUP_TILE + before] = tid;
             g.token[first[col] * GROUP_TILE + before] = row;

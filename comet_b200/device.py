@@ -389,7 +389,8 @@ class EntryGroups:
 
 def group_entries(S):
     """The entries of S (DeviceCSR, at most 1024 columns; rows tokens, columns experts) grouped by column, for gated_experts and combine_experts and their
-    gradients: once for a router's choices, whatever is computed with them.  An entry whose column lies outside makes its results NaN."""
+    gradients: once for a router's choices, whatever is computed with them.  An entry whose column lies outside makes its results NaN.  Where pos is that of some
+    rows of a larger matrix, with crd and values of all, the other rows' entries take no part, and what belongs to them in results has no meaning."""
     if S.row_ids is not None:
         raise ValueError("group_entries: the matrix must be CSR (a row that stores nothing is empty there)")
     if not 1 <= S.ncols <= 1024:

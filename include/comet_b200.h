@@ -719,7 +719,8 @@ COMET_B200_EXPORT int32_t comet_b200_dev_log_probs_grad_f32_i64(
 
 /* The entries grouped by column, for the calls below: `plan` is int32 memory of comet_b200_dev_group_entries_size(nnz, ncols)
    elements at a multiple of 16 bytes, which they read.  1 <= ncols <= 1024.  Element 2 becomes 1 if a later call that works with the plan gave up
-   waiting inside a kernel (its results are incomplete then).  An entry whose column is outside makes its results NaN. */
+   waiting inside a kernel (its results are incomplete then).  An entry whose column is outside makes its results NaN.  One outside pos[0] to pos[nrows]
+   takes no part: what belongs to it in results has no meaning. */
 COMET_B200_EXPORT int64_t comet_b200_dev_group_entries_size(int64_t nnz, int64_t ncols);
 COMET_B200_EXPORT int32_t comet_b200_dev_group_entries_i64(
     int64_t nrows, int64_t ncols, int64_t nnz, const int64_t *pos, const int64_t *crd, int32_t *plan, void *stream);

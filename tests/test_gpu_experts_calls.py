@@ -131,3 +131,32 @@ def test_two_host_threads():
         t.join()
     torch.cuda.synchronize()
     assert not wrong
+
+
+@pytest.mark.parametrize("rows,part", [(40, slice(7, 8)), (40, slice(3, 30)), (100, slice(0, 99)), (3000, slice(100, 101)), (3000, slice(100, 140)), (3000, slice(500, 2500))])
+def test_some_rows_of_a_larger_matrix(rows, part):
+    """pos of some rows beside crd and values of all: the other rows' entries are no token's here.  What belongs to the rows is what it is without them, and the experts'
+    gradients leave them out."""
+    import torch
+    from comet_b200 import device
+    rng = np.random.default_rng(rows)
+    crd = np.concatenate([np.sort(rng.choice(5, 2, replace=False)) for _ in range(rows)])
+    crd[[0, -1]] = [-1, 5]                                                 # of rows that are left out, or not
+    crd, val, pos = torch.from_numpy(crd).cuda(), torch.rand(2 * rows, device="cuda"), torch.arange(0, 2 * rows + 1, 2, device="cuda")
+    n, of = part.stop - part.start, slice(2 * part.start, 2 * part.stop)
+    X, W, V = matrix(rng, "bf16", n, 72), matrix(rng, "bf16", 5, 80, 72, scale=0.1), matrix(rng, "bf16", 5, 72, 40, scale=0.1)
+    d = torch.full((2 * rows, 40), float("nan"), device="cuda").bfloat16()
+    d[of] = matrix(rng, "bf16", 2 * n, 40)
+    S, alone = device.DeviceCSR(n, 5, pos[part.start:part.stop + 1], crd, val), device.DeviceCSR(n, 5, pos[:n + 1].clone(), crd[of].clone(), val[of].clone())
+    G, A = device.group_entries(S), device.group_entries(alone)
+    equal = lambda a, b: torch.equal(a.float().nan_to_num(7.0), b.float().nan_to_num(7.0))        # noqa: E731
+    assert equal(device.gated_experts(G, X, W)[of], device.gated_experts(A, X, W))
+    assert equal(device.combine_experts(G, d, V), device.combine_experts(A, d[of].clone(), V))
+    for a, b in zip(device.gated_experts_grad(G, X, W, d), device.gated_experts_grad(A, X, W, d[of].clone())):
+        assert equal(a, b)
+    a, b = device.combine_experts_grad(G, d, V, X), device.combine_experts_grad(A, d[of].clone(), V, X)
+    assert equal(a[0][of], b[0]) and equal(a[1], b[1]) and not torch.isnan(a[1]).any()
+    # the sums of parts of a row of h, whose width goes by the number of all entries, in f32
+    values, want = a[2][of], b[2]
+    assert torch.equal(torch.isnan(values), torch.isnan(want)) and float((values - want).nan_to_num(0.0).abs().max()) <= 1e-5 * float(want.nan_to_num(0.0).abs().max())
+    G.check()
