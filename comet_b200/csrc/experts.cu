@@ -12,8 +12,8 @@
 // inner 1024, the gated product, 1200 us with them, 438 without.)
 //
 // Bound: for that product, 550 GFLOP, 440 to 470 us when the chip is cool and 530 in a row of passes, where the power cap leaves 1.5 GHz (a library's plain product of the
-// same size: 370 and 430).  Tensor cores are active 65 to 72 % of the clocks: a step of 64 terms is 512 clocks of theirs and takes some 708, start and end of the launch
-// included.  The operands' 48 KB a step come into an SM at 61 to 66 bytes a clock over the whole launch (dx 60, dz 55), so the way from the L2 to an SM is the
+// same size: 370 and 430).  Tensor cores are active 70 to 72 % of the clocks: a step of 64 terms is 512 clocks of theirs and takes some 708, start and end of the launch
+// included.  The operands' 48 KB a step come into an SM at 65.5 bytes a clock over the whole launch (dx 60, dz 56), so the way from the L2 to an SM is the
 // likely bound; shared memory's banks are read in 28 % of the clocks and written in 27 %, the L2 is busy 36 %.  Where sums are short (dw: 7 steps a
 // tile, active 44 %; dv 45 %) or their results f32 (combine, 52 %), the results' bytes.
 // Three forms:
@@ -81,7 +81,7 @@ struct Shape {
 // The tensor cores cut off what does not fit into an f32 sum, each time that they add, so long sums are off by more than f32 sums are.  In results of 16 bits that is
 // nothing; d_values is f32, and was off by 2.0e-6 of its norm at a width of 2048, 9.1e-6 at 8192.  There a tile's sums are taken out after so many steps and added up,
 // rounded to the nearest, in the takers' registers (0: not at all): 4.8e-7 at any width after 8 steps, 1.0e-6 after 16, 2.6e-7 after 4; f32 products 2e-7 to 4e-7.
-// While the takers are at a tile's results, products for two such segments can go on: v'dy of combine_grad_step 95 us after 8 steps, 89 after 16, 106 after 4.
+// While the takers are at a tile's results, products for two such segments can go on: v'dy of combine_grad_step 97 us after 8 steps, 89 after 16, 106 after 4, 86 not at all.
 constexpr int segment(int sums) { return sums == COMBINE_GRAD ? 8 : 0; }
 // In a wide tile that is 128 sums a thread.  The takers get the registers that the other warps do not use: of the 128 that each of 512 threads starts with, theirs then
 // have 192 and the others' 64, by warpgroups of 128 threads.
@@ -567,33 +567,38 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const bool half = HALVES && id >= whole;
                 const int steps = (int)__reduce_max_sync(0xffffffffu, (unsigned)after);  // the same in all, which the compiler does not know
                 if (id + all < tiles) after = tile_of(id + all).steps;
-                for (int k = 0; k < steps; k++, step++) {
-                    const unsigned s = step % RING, b = tile & 1;
-                    const int done_so_far = SEGMENT ? k % (SEGMENT ? SEGMENT : 1) : k;           // of the sums that are taken out at once
-                    const bool all_done = k + 1 == steps || done_so_far + 1 == SEGMENT;
-                    if (done_so_far == 0) {
-                        on = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
-                        if (!on) break;
-                        tmem_fence_after();
-                    }
-                    on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
-                    if (!on) break;
-                    if (NUMBERED != NUMBERED_NONE) shared_to_products();
+                // steps from k0 to k1 of the tile, whose sums are taken out at once
+                auto issue = [&](int k0, int k1) {
+                    const unsigned b = tile & 1;
+                    on = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, (tile / 2 & 1) ^ 1, broken));
                     tmem_fence_after();
-                    const uint32_t at = ring + s * STEP_BYTES;
-                    const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
-                    // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
-                    constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
-                    const uint32_t kind = half ? product_descriptor(BF16, TM, W / 2, FORM == OUTER, FORM != ROWS)
-                                               : product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
-                    if (elect()) {
+                    for (int k = k0; on && k < k1; k++, step++) {
+                        const unsigned s = step % RING;
+                        on = __all_sync(0xffffffffu, bar_wait(full + 8 * s, step / RING & 1, broken));
+                        if (!on) break;
+                        if (NUMBERED != NUMBERED_NONE) shared_to_products();
+                        tmem_fence_after();
+                        const uint32_t at = ring + s * STEP_BYTES;
+                        const uint64_t da = tile_descriptor(at, 8192, 1024), db = tile_descriptor(at + A_BYTES, 8192, 1024);
+                        // 16 terms: 32 bytes along a tile's rows, or 16 rows of 128 bytes
+                        constexpr int next_a = FORM == OUTER ? 2048 / 16 : 32 / 16, next_b = FORM == ROWS ? 32 / 16 : 2048 / 16;
+                        const uint32_t kind = half ? product_descriptor(BF16, TM, W / 2, FORM == OUTER, FORM != ROWS)
+                                                   : product_descriptor(BF16, TM, W, FORM == OUTER, FORM != ROWS);
+                        if (elect()) {
 #pragma unroll
-                        for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, done_so_far + i > 0);
-                        products_to(empty + 8 * s);
-                        if (all_done) products_to(done + 8 * b);
+                            for (int i = 0; i < TK / 16; i++) product(tmem + b * W, da + i * next_a, db + i * next_b, kind, k - k0 + i > 0);
+                            products_to(empty + 8 * s);
+                            if (k + 1 == k1) products_to(done + 8 * b);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    tile += all_done;
+                    tile++;
+                };
+                if (steps == 0) continue;
+                if constexpr (SEGMENT == 0) {
+                    issue(0, steps);
+                } else {
+                    for (int k = 0; on && k < steps; k += SEGMENT) issue(k, min(k + SEGMENT, steps));
                 }
             }
             if (*broken) {                             // products under way end before tensor memory is given back
